@@ -40,9 +40,24 @@ EXPORTS = ("fusedMM_csr", "fusedMM_csr_stream", "fusedMM_csr_stream_noalloc", "f
            "fusedMM_amd_set_validate", "fusedMM_amd_set_cache", "fusedMM_amd_invalidate",
            "fusedMM_amd_last_host_phases", "fusedMM_amd_set_split", "fusedMM_amd_get_split", "fusedMM_amd_set_pack_rows", "fusedMM_amd_set_store_tick", "fusedMM_amd_timing",
            "fusedMM_amd_timing_summary", "fusedMM_amd_timing_call", "fusedMM_amd_last_split",
-           "fusedMM_amd_last_row_order", "fusedMM_amd_finalize")
+           "fusedMM_amd_last_row_order", "fusedMM_amd_finalize",
+           "fusedMM_attn_plan_create", "fusedMM_attn_plan_destroy", "fusedMM_attn_workspace", "fusedMM_attn_forward",
+           "fusedMM_attn_backward", "fusedMM_attn_rows_workspace", "fusedMM_attn_rows", "fusedMM_attn_rows_kv4",
+           "fusedMM_kv4_record_bytes", "fusedMM_kv4_write", "fusedMM_kv4_read")
 # the measuring aids of libfusedmm_amd_probes.so (csrc/fusedmm_probes.h): not part of the product's ABI
 PROBE_EXPORTS = ("fusedMM_amd_copy_probe", "fusedMM_amd_read_probe", "fusedMM_amd_gather_probe")
+
+# element types of the attention operators (include/fusedmm_amd.h)
+TYPE_F32, TYPE_F16, TYPE_BF16 = 0, 1, 2
+TYPES = {"f32": TYPE_F32, "f16": TYPE_F16, "bf16": TYPE_BF16}
+
+
+class AttnDesc(C.Structure):
+    """fusedMM_attn_desc: sizes and strides (in elements) of the attention operators."""
+    _fields_ = [("type", C.c_int32), ("maps", C.c_int32), ("m", C.c_int64), ("n", C.c_int64), ("heads", C.c_int32),
+                ("kv_heads", C.c_int32), ("d", C.c_int32), ("dv", C.c_int32), ("scale", C.c_float)] + \
+               [(s, C.c_int64) for s in ("ldq", "hdq", "ldk", "hdk", "ldv", "hdv", "ldo", "hdo")]
+
 
 _libs = {}
 
@@ -113,6 +128,21 @@ def load(index_bits=32, value_bits=32):
     lib.fusedMM_amd_invalidate.restype = None
     lib.fusedMM_amd_last_host_phases.argtypes = [C.POINTER(C.c_double)] * 3
     lib.fusedMM_amd_last_host_phases.restype = C.c_int
+    dp, i64 = C.POINTER(AttnDesc), C.c_int64
+    for name, res, args in (
+            ("fusedMM_attn_plan_create", C.c_int, [it, it, it, vp, vp, vp, vp, C.POINTER(vp)]),
+            ("fusedMM_attn_plan_destroy", C.c_int, [vp]),
+            ("fusedMM_attn_workspace", i64, [dp, vp, vp]),
+            ("fusedMM_attn_forward", C.c_int, [dp] + [vp] * 9 + [i64, vp]),
+            ("fusedMM_attn_backward", C.c_int, [dp] + [vp] * 15 + [i64, vp]),
+            ("fusedMM_attn_rows_workspace", i64, [dp, it]),
+            ("fusedMM_attn_rows", C.c_int, [dp, it] + [vp] * 9 + [i64, vp]),
+            ("fusedMM_kv4_record_bytes", i64, [C.c_int] * 3),
+            ("fusedMM_kv4_write", C.c_int, [dp, it, vp, vp, vp, vp, i64, i64, vp]),
+            ("fusedMM_kv4_read", C.c_int, [dp, it, vp, vp, i64, i64, vp, vp, vp]),
+            ("fusedMM_attn_rows_kv4", C.c_int, [dp, it] + [vp] * 5 + [i64, i64] + [vp] * 3 + [i64, vp])):
+        f = getattr(lib, name)
+        f.restype, f.argtypes = res, args
     assert lib.fusedMM_amd_index_bytes() * 8 == index_bits
     assert lib.fusedMM_amd_value_bytes() * 8 == value_bits
     _libs[key] = lib
@@ -172,3 +202,84 @@ def fusedMM_csr(imessage, m, n, k, alpha, nnz, rows, cols, val, indx, pntrb, pnt
     if stream is None:
         return lib.fusedMM_csr(*args)
     return lib.fusedMM_csr_stream(*args, stream)
+
+
+class AttnPlan:
+    """Owner of a plan of fusedMM_attn_plan_create (same arguments); destroyed with the object.  A call that the library
+    refuses raises OSError with its status."""
+
+    def __init__(self, m, n, nnz, indx, pntrb, pntre, index_bits=32, stream=None):
+        self.lib, self.handle = load(index_bits), None
+        h = C.c_void_p()
+        rc = self.lib.fusedMM_attn_plan_create(m, n, nnz, _addr(indx), _addr(pntrb), _addr(pntre), _stream(stream), C.byref(h))
+        if rc:
+            raise OSError("fusedMM_attn_plan_create returned %d" % rc)
+        self.handle = h.value
+
+    def destroy(self):
+        handle, self.handle = self.handle, None
+        return self.lib.fusedMM_attn_plan_destroy(handle) if handle else SUCCESS
+
+    def __del__(self):
+        if getattr(self, "handle", None):
+            self.destroy()
+
+
+def _stream(stream):
+    """The HIP stream to enqueue on: `stream`, or PyTorch's current one."""
+    if stream is not None:
+        return stream
+    import torch
+    return torch.cuda.current_stream().cuda_stream if torch.cuda.is_available() else None
+
+
+def _handle(plan):
+    return plan.handle if isinstance(plan, AttnPlan) else plan
+
+
+# The attention operators: the argument lists of include/fusedmm_amd.h, device tensors or addresses for pointers, an AttnPlan
+# or a raw handle for plans; without `stream`, PyTorch's current stream.
+
+def fusedMM_attn_workspace(desc, plan, plan_t=None, index_bits=32):
+    return load(index_bits).fusedMM_attn_workspace(C.byref(desc), _handle(plan), _handle(plan_t))
+
+
+def fusedMM_attn_forward(desc, plan, q, k, v, lam, o, o2, lse, work, work_bytes, stream=None, index_bits=32):
+    return load(index_bits).fusedMM_attn_forward(C.byref(desc), _handle(plan), _addr(q), _addr(k), _addr(v), _addr(lam), _addr(o),
+                                                 _addr(o2), _addr(lse), _addr(work), work_bytes, _stream(stream))
+
+
+def fusedMM_attn_backward(desc, plan, plan_t, q, k, v, lam, o, o2, lse, dout, dq, dk, dv, dlam, work, work_bytes, stream=None,
+                          index_bits=32):
+    return load(index_bits).fusedMM_attn_backward(C.byref(desc), _handle(plan), _handle(plan_t), _addr(q), _addr(k), _addr(v),
+                                                  _addr(lam), _addr(o), _addr(o2), _addr(lse), _addr(dout), _addr(dq), _addr(dk),
+                                                  _addr(dv), _addr(dlam), _addr(work), work_bytes, _stream(stream))
+
+
+def fusedMM_attn_rows_workspace(desc, nnz, index_bits=32):
+    return load(index_bits).fusedMM_attn_rows_workspace(C.byref(desc), nnz)
+
+
+def fusedMM_attn_rows(desc, nnz, indx, pntrb, pntre, q, k, v, lam, o, work, work_bytes, stream=None, index_bits=32):
+    return load(index_bits).fusedMM_attn_rows(C.byref(desc), nnz, _addr(indx), _addr(pntrb), _addr(pntre), _addr(q), _addr(k),
+                                              _addr(v), _addr(lam), _addr(o), _addr(work), work_bytes, _stream(stream))
+
+
+def fusedMM_attn_rows_kv4(desc, nnz, indx, pntrb, pntre, q, cache, ldc, hdc, lam, o, work, work_bytes, stream=None, index_bits=32):
+    return load(index_bits).fusedMM_attn_rows_kv4(C.byref(desc), nnz, _addr(indx), _addr(pntrb), _addr(pntre), _addr(q),
+                                                  _addr(cache), ldc, hdc, _addr(lam), _addr(o), _addr(work), work_bytes,
+                                                  _stream(stream))
+
+
+def fusedMM_kv4_record_bytes(maps, d, dv, index_bits=32):
+    return load(index_bits).fusedMM_kv4_record_bytes(maps, d, dv)
+
+
+def fusedMM_kv4_write(desc, tokens, slots, k, v, cache, ldc, hdc, stream=None, index_bits=32):
+    return load(index_bits).fusedMM_kv4_write(C.byref(desc), tokens, _addr(slots), _addr(k), _addr(v), _addr(cache), ldc, hdc,
+                                              _stream(stream))
+
+
+def fusedMM_kv4_read(desc, tokens, slots, cache, ldc, hdc, k, v, stream=None, index_bits=32):
+    return load(index_bits).fusedMM_kv4_read(C.byref(desc), tokens, _addr(slots), _addr(cache), ldc, hdc, _addr(k), _addr(v),
+                                             _stream(stream))

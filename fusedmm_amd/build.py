@@ -4,8 +4,8 @@
     python -m fusedmm_amd.build --force    # recompile everything
 
 libfusedmm_amd_i32.so / _i64.so (float) and libfusedmm_amd_d_i32.so / _d_i64.so (double) are
-linked from a dozen objects each (csrc/*.hip; the fused kernel's instances are spread over
-eight of them, one per op), libfusedmm_amd_probes.so holds the benchmark's yardsticks.  The
+linked from some thirty objects each (csrc/*.hip; the fused kernel's instances are spread over
+eight of them, one per op, the attention kernels' over fourteen that all libraries share), libfusedmm_amd_probes.so holds the benchmark's yardsticks.  The
 libraries are written next to this file so that they travel with the source tree; nothing is
 installed.  Objects go to fusedmm_amd/obj/.
 """
@@ -46,6 +46,11 @@ UNITS = [("fusedmm_state.hip", [], "state"), ("fusedmm_dispatch.hip", [], "dispa
          ("fusedmm_staging.hip", [], "staging"), ("fusedmm_host_stages.hip", [], "host_stages"),
          ("fusedmm_exports.hip", [], "exports")] + \
         [("fusedmm_launch.hip", ["-DFMM_LAUNCH_UNIT=%d" % u], "launch%d" % u) for u in range(LAUNCH_UNITS)]
+# the attention family: its entry points once per library, the plan and the kernels once for all of them
+ATTN_UNITS = 13
+UNITS.append(("fusedmm_attn_exports.hip", [], "attn_exports"))
+SHARED_UNITS = [("fusedmm_attn_plan.hip", [], "attn_plan")] + \
+    [("fusedmm_attn_launch.hip", ["-DFMM_ATTN_UNIT=%d" % u], "attn_launch%d" % u) for u in range(ATTN_UNITS)]
 VARIANTS = ((32, 32), (64, 32), (32, 64), (64, 64))     # (index bits, value bits)
 JOBS = int(os.environ.get("FUSEDMM_BUILD_JOBS", "0")) or min(16, os.cpu_count() or 4)
 
@@ -109,6 +114,10 @@ def _objects(index_bits, value_bits):
             for src, defs, name in UNITS]
 
 
+def _shared_objects():
+    return [(src, os.path.join(OBJ, name + ".o"), defs) for src, defs, name in SHARED_UNITS]
+
+
 def _link(out, objs, verbose, extra=()):
     _run([HIPCC, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", out] + objs + list(extra), verbose)
     return out
@@ -117,7 +126,7 @@ def _link(out, objs, verbose, extra=()):
 def build_libs(variants=VARIANTS, force=False, verbose=False, probes=True):
     """Compile the objects of the requested libraries side by side, then link each library."""
     os.makedirs(OBJ, exist_ok=True)
-    jobs = []
+    jobs = _shared_objects()
     for ib, vb in variants:
         jobs += _objects(ib, vb)
     if probes:
@@ -128,7 +137,8 @@ def build_libs(variants=VARIANTS, force=False, verbose=False, probes=True):
         list(ex.map(lambda j: _compile(j[0], j[1], j[2], force, verbose), jobs))
     libs = []
     for ib, vb in variants:
-        libs.append(_link(os.path.join(OUT, lib_name(ib, vb)), [o for _, o, _ in _objects(ib, vb)], verbose, ["-ldl"]))
+        objs = [o for _, o, _ in _objects(ib, vb) + _shared_objects()]
+        libs.append(_link(os.path.join(OUT, lib_name(ib, vb)), objs, verbose, ["-ldl"]))
     if probes:
         libs.append(_link(os.path.join(OUT, "libfusedmm_amd_probes.so"), [os.path.join(OBJ, "probes.o")], verbose))
     return libs

@@ -1,0 +1,272 @@
+// Attention over a CSR pattern: what the kernels of this family share.
+//
+// For row i, head h and map p:  s_j = scale * <q_p[i], k_p[c_j]>,  P_p = softmax of s over the row's edges,
+// o[i] = sum_j (P_1 - lambda_h P_2)_j v[c_j]  (one map: P_1 alone).  Backward, with dP_j = <do[i], v[c_j]> and
+// delta_p = <do[i], O_p[i]>:  dS_p = sign_p P_p (dP - delta_p),  dq_p = scale sum_j dS_p k_p[c_j],
+// dk_p[c] = scale sum_i dS_p q_p[i],  dv[c] = sum_i (P_1 - lambda P_2) do[i],  dlambda_h = - sum_i sum_j P_2 dP.
+//
+// All of it is small dense products between rows that stay in registers ("resident": 16 per wave) and tiles of 32
+// gathered rows in LDS, on the matrix cores.  Every product is formed transposed, gathered x resident: a lane then
+// holds, for ONE resident row (lane % 16), the scores of gathered rows 4g..4g+3 and 16+4g..16+4g+3 (g = lane / 16),
+// which is - up to an order of the contraction index that both operands share - the register layout in which the
+// scores enter the second product.  Scores, weights and their gradients therefore never leave the registers, and the
+// row statistics are one value per lane.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace fmm_attn {
+
+enum : int { kF32 = 0, kF16 = 1, kBF16 = 2 };
+
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef float f8 __attribute__((ext_vector_type(8)));
+typedef short s4 __attribute__((ext_vector_type(4)));
+typedef short s8 __attribute__((ext_vector_type(8)));
+typedef unsigned int u4 __attribute__((ext_vector_type(4)));
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr int kBlockRows = 64;    // resident rows of a workgroup: 4 waves x 16
+constexpr int kTile = 32;         // gathered rows of a tile
+
+__device__ inline float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// 16-bit and 32-bit element types.  A "chunk" is KC features of a row, of which a lane holds EPL (16 bytes).
+template <int T> struct Num;
+
+template <> struct Num<kBF16> {
+   typedef uint16_t E;
+   static constexpr int KC = 32, EPL = 8;
+   typedef s8 TFrag;
+   static constexpr float kPScale = 1.0f;
+   static __device__ inline f4 mma(u4 a, u4 b, f4 c)
+   {
+      return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
+   }
+   static __device__ inline f4 mma_t(s8 a, s8 b, f4 c)
+   {
+      return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
+   }
+   static __device__ inline E from(float x) { return __builtin_bit_cast(E, (__bf16)x); }   // to nearest even
+   static __device__ inline float to(E x) { return __builtin_bit_cast(float, (uint32_t)x << 16); }
+   static __device__ inline bool odd_word(uint32_t w)   // an infinity or a NaN in either half
+   {
+      return (w & 0x7F80u) == 0x7F80u || (w & 0x7F800000u) == 0x7F800000u;
+   }
+};
+
+template <> struct Num<kF16> {
+   typedef uint16_t E;
+   static constexpr int KC = 32, EPL = 8;
+   typedef s8 TFrag;
+   // weights of long rows are small: 2^10 keeps them clear of fp16's subnormals (they are at most 1 + |lambda|)
+   static constexpr float kPScale = 1024.0f;
+   static __device__ inline f4 mma(u4 a, u4 b, f4 c)
+   {
+      return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
+   }
+   static __device__ inline f4 mma_t(s8 a, s8 b, f4 c)
+   {
+      return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
+   }
+   static __device__ inline E from(float x) { return __builtin_bit_cast(E, (_Float16)x); }
+   static __device__ inline float to(E x) { return (float)__builtin_bit_cast(_Float16, x); }
+   static __device__ inline bool odd_word(uint32_t w)
+   {
+      return (w & 0x7C00u) == 0x7C00u || (w & 0x7C000000u) == 0x7C000000u;
+   }
+};
+
+template <> struct Num<kF32> {
+   typedef float E;
+   static constexpr int KC = 16, EPL = 4;
+   typedef f8 TFrag;
+   static constexpr float kPScale = 1.0f;
+   static __device__ inline f4 mma(u4 a, u4 b, f4 c)
+   {
+      const f4 x = __builtin_bit_cast(f4, a), y = __builtin_bit_cast(f4, b);
+#pragma unroll
+      for (int j = 0; j < 4; j++) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[j], y[j], c, 0, 0, 0);
+      return c;
+   }
+   static __device__ inline f4 mma_t(f8 a, f8 b, f4 c)
+   {
+#pragma unroll
+      for (int j = 0; j < 8; j++) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], c, 0, 0, 0);
+      return c;
+   }
+   static __device__ inline E from(float x) { return x; }
+   static __device__ inline float to(E x) { return x; }
+   static __device__ inline bool odd_word(uint32_t w) { return (w & 0x7F800000u) == 0x7F800000u; }
+};
+
+// EPL elements at p, of which the first `valid` exist (the rest read as zero).  vec: p is 16-byte aligned and valid is
+// 0 or EPL.
+template <int T> __device__ inline u4 load_chunk(const typename Num<T>::E *p, int valid, bool vec)
+{
+   typedef typename Num<T>::E E;
+   u4 r = {0, 0, 0, 0};
+   if (valid <= 0) return r;
+   if (vec) return *reinterpret_cast<const u4 *>(p);
+   if constexpr (sizeof(E) == 2)
+   {
+#pragma unroll
+      for (int k = 0; k < 8; k++)
+         if (k < valid) r[k / 2] |= (uint32_t)p[k] << (16 * (k & 1));
+   }
+   else
+   {
+#pragma unroll
+      for (int k = 0; k < 4; k++)
+         if (k < valid) r[k] = __builtin_bit_cast(uint32_t, p[k]);
+   }
+   return r;
+}
+
+template <int T> __device__ inline bool odd_chunk(u4 v)
+{
+   return Num<T>::odd_word(v[0]) || Num<T>::odd_word(v[1]) || Num<T>::odd_word(v[2]) || Num<T>::odd_word(v[3]);
+}
+
+// scores of 32 gathered rows for one resident row, in the layout of the second product
+template <int T> __device__ inline typename Num<T>::TFrag pack_scores(const float (&p)[2][4])
+{
+   typename Num<T>::TFrag r;
+#pragma unroll
+   for (int j = 0; j < 8; j++)
+   {
+      if constexpr (T == kF32) r[j] = p[j / 4][j % 4];
+      else r[j] = (short)Num<T>::from(p[j / 4][j % 4]);
+   }
+   return r;
+}
+
+// features 16t .. 16t+15 of the tile's 32 rows, transposed: lane i of group g gets feature 16t + i of rows 4g..4g+3 and
+// 16+4g..16+4g+3.  16-bit: two transposing LDS reads, in which lane i of a group of 16 names the address of four
+// elements of row i / 4 and receives element i of the four rows.  32-bit: eight plain reads.
+template <int T> __device__ inline typename Num<T>::TFrag load_t(const typename Num<T>::E *tile, int stride, int t, int g, int i)
+{
+   typename Num<T>::TFrag r;
+   if constexpr (T == kF32)
+   {
+#pragma unroll
+      for (int j = 0; j < 8; j++) r[j] = tile[(16 * (j / 4) + 4 * g + j % 4) * stride + 16 * t + i];
+   }
+   else
+   {
+      typedef __attribute__((address_space(3))) s4 lds_s4;
+      const uint16_t *p = tile + (4 * g + i / 4) * stride + 16 * t + (i % 4) * 4;
+      const s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)p);
+      const s4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(p + 16 * stride));
+      r = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+   }
+   return r;
+}
+
+// an infinity or a NaN
+template <int T> __device__ inline bool odd_element(typename Num<T>::E x)
+{
+   if constexpr (T == kF32) return Num<T>::odd_word(__builtin_bit_cast(uint32_t, x));
+   else return Num<T>::odd_word(x);
+}
+
+template <int T> __device__ inline typename Num<T>::TFrag without_odd(typename Num<T>::TFrag v)
+{
+#pragma unroll
+   for (int j = 0; j < 8; j++)
+   {
+      if constexpr (T == kF32) v[j] = odd_element<T>(v[j]) ? 0.0f : v[j];
+      else v[j] = odd_element<T>((uint16_t)v[j]) ? (short)0 : v[j];
+   }
+   return v;
+}
+
+// What the tile's infinities and NaN add: a matrix instruction would multiply them by the zero weights of rows that do not
+// name them, so it runs without them (without_odd) and every row adds those of the gathered rows that it does name.
+// Rows that name none keep the bits they have without them.
+// mine: bit 4a + r says that gathered row 16a + 4g + r is named by this lane's resident row.
+template <int T, int NT> __device__ inline void add_odd(f4 (&acc)[NT], const float (&p)[2][4], unsigned mine,
+                                                        const typename Num<T>::E *tile, int stride, int g, int i)
+{
+   for (int key = 0; key < kTile; key++)
+   {
+      const int src = ((key & 15) >> 2) * 16 + i, a = key >> 4, r = key & 3;
+      float x = 0;
+#pragma unroll
+      for (int j = 0; j < 8; j++)
+         if (j == 4 * a + r) x = p[j / 4][j % 4];
+      const float w = __shfl(x, src);
+      const bool named = (__shfl((int)mine, src) >> (4 * a + r)) & 1;
+      if (!named) continue;
+#pragma unroll
+      for (int t = 0; t < NT; t++)
+#pragma unroll
+         for (int k = 0; k < 4; k++)
+         {
+            const typename Num<T>::E e = tile[key * stride + 16 * t + 4 * g + k];
+            if (odd_element<T>(e)) acc[t][k] = fmaf(w, Num<T>::to(e), acc[t][k]);
+         }
+   }
+}
+
+// acc += (weights of the tile's 32 rows) x (their features); odd: the tile holds infinities or NaN
+template <int T, int NT> __device__ inline void add_weighted(f4 (&acc)[NT], const float (&p)[2][4], unsigned mine,
+                                                             const typename Num<T>::E *tile, int stride, int g, int i, bool odd)
+{
+   const typename Num<T>::TFrag b = pack_scores<T>(p);
+   if (__builtin_expect(odd, 0))
+   {
+#pragma unroll
+      for (int t = 0; t < NT; t++) acc[t] = Num<T>::mma_t(without_odd<T>(load_t<T>(tile, stride, t, g, i)), b, acc[t]);
+      add_odd<T, NT>(acc, p, mine, tile, stride, g, i);
+      return;
+   }
+#pragma unroll
+   for (int t = 0; t < NT; t++) acc[t] = Num<T>::mma_t(load_t<T>(tile, stride, t, g, i), b, acc[t]);
+}
+
+// four consecutive features of an output row, f .. f+3 of `width`
+template <int T> __device__ inline void store4(typename Num<T>::E *row, int f, int width, f4 v, bool vec)
+{
+   typedef typename Num<T>::E E;
+   if (f >= width) return;
+   if (vec && f + 4 <= width)
+   {
+      if constexpr (T == kF32) *reinterpret_cast<f4 *>(row + f) = v;
+      else
+      {
+         s4 s;
+#pragma unroll
+         for (int k = 0; k < 4; k++) s[k] = (short)Num<T>::from(v[k]);
+         *reinterpret_cast<s4 *>(row + f) = s;
+      }
+      return;
+   }
+#pragma unroll
+   for (int k = 0; k < 4; k++)
+      if (f + k < width) row[f + k] = (E)Num<T>::from(v[k]);
+}
+
+__device__ inline float group_max(float x)   // over the four lane groups: the lanes of one resident row
+{
+   x = fmaxf(x, __shfl_xor(x, 16));
+   return fmaxf(x, __shfl_xor(x, 32));
+}
+__device__ inline float group_sum(float x)
+{
+   x += __shfl_xor(x, 16);
+   return x + __shfl_xor(x, 32);
+}
+
+// Workgroups go round-robin to the 8 XCDs.  Work item of workgroup b of n items: every XCD takes a contiguous eighth, so
+// that the items of one head (whose gathered rows overlap) meet in one L2.  Items at or past n have no work.
+__device__ inline int64_t xcd_item(int64_t b, int64_t n)
+{
+   const int64_t per = (n + 7) / 8;
+   return (b & 7) * per + (b >> 3);
+}
+
+}  // namespace fmm_attn

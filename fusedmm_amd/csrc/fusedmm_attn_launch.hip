@@ -1,0 +1,186 @@
+// Instances of the attention kernels, one object per (element type, kernel): -DFMM_ATTN_UNIT=3 * kernel + type, kernels in
+// the order forward, dq, dkv, rows; unit 12 is the 4-bit cache.
+#include <algorithm>
+
+#include "fusedmm_attn.hpp"
+
+#ifndef FMM_ATTN_UNIT
+#error "compile with -DFMM_ATTN_UNIT=0..12"
+#endif
+#define KERNEL (FMM_ATTN_UNIT / 3)
+#define TYPE (FMM_ATTN_UNIT % 3)
+#if TYPE == 0
+#define NAMED(f) f##_f32
+#elif TYPE == 1
+#define NAMED(f) f##_f16
+#else
+#define NAMED(f) f##_bf16
+#endif
+
+namespace fmm_attn {
+
+namespace {
+
+[[maybe_unused]] unsigned eighths(int64_t n) { return (unsigned)((n + 7) / 8 * 8); }
+
+// F<DC, MAPS>()(args) for the instance of (dc, maps)
+template <template <int, int> class F, class... A> int choose(int dc, int maps, A... a)
+{
+   if (maps == 1)
+      switch (dc)
+      {
+         case 32: return F<32, 1>()(a...);
+         case 64: return F<64, 1>()(a...);
+         case 128: return F<128, 1>()(a...);
+         case 256: return F<256, 1>()(a...);
+      }
+   else
+      switch (dc)
+      {
+         case 32: return F<32, 2>()(a...);
+         case 64: return F<64, 2>()(a...);
+         case 128: return F<128, 2>()(a...);
+      }
+   return kNoImpl;
+}
+
+#if KERNEL == 0
+template <int DC, int MAPS> struct Forward {
+   int operator()(const Params &p, hipStream_t s)
+   {
+      const int64_t n = (int64_t)p.plan.n_units * p.heads;
+      hipLaunchKernelGGL((attn_forward<TYPE, DC, MAPS>), dim3(eighths(n)), dim3(256), 0, s, p);
+      ATTN_HIP(hipGetLastError());
+      if (p.plan.n_joins)
+      {
+         hipLaunchKernelGGL((attn_forward_join<TYPE, DC, MAPS>), dim3((unsigned)((int64_t)p.plan.n_joins * p.heads * kBlockRows / 4)), dim3(256), 0, s, p);
+         ATTN_HIP(hipGetLastError());
+      }
+      return kOk;
+   }
+};
+#elif KERNEL == 1
+template <int DC, int MAPS> struct Dq {
+   int operator()(const Params &p, hipStream_t s)
+   {
+      if (p.m)
+      {
+         hipLaunchKernelGGL((attn_delta<TYPE, MAPS>), dim3((unsigned)((p.m * p.heads + 15) / 16)), dim3(256), 0, s, p);
+         ATTN_HIP(hipGetLastError());
+         const int64_t n = (int64_t)p.plan.n_units * p.heads;
+         hipLaunchKernelGGL((attn_dq<TYPE, DC, MAPS>), dim3(eighths(n)), dim3(256), 0, s, p);
+         ATTN_HIP(hipGetLastError());
+         if (p.plan.n_joins)
+         {
+            hipLaunchKernelGGL((attn_dq_join<TYPE, DC, MAPS>), dim3((unsigned)((int64_t)p.plan.n_joins * p.heads * kBlockRows / 4)), dim3(256), 0, s, p);
+            ATTN_HIP(hipGetLastError());
+         }
+      }
+      if (MAPS == 2 && p.dlambda)
+      {
+         hipLaunchKernelGGL((attn_dlambda<TYPE>), dim3((unsigned)p.heads), dim3(256), 0, s, p);
+         ATTN_HIP(hipGetLastError());
+      }
+      return kOk;
+   }
+};
+#elif KERNEL == 2
+template <int DC, int MAPS> struct Dkv {
+   int operator()(const Params &p, hipStream_t s)
+   {
+      const int64_t n = (int64_t)p.plan.n_units * p.kv_heads;
+      hipLaunchKernelGGL((attn_dkv<TYPE, DC, MAPS>), dim3(eighths(n)), dim3(256), 0, s, p);
+      ATTN_HIP(hipGetLastError());
+      if (p.plan.n_joins)
+      {
+         hipLaunchKernelGGL((attn_dkv_join<TYPE, DC, MAPS>), dim3((unsigned)((int64_t)p.plan.n_joins * p.kv_heads * kBlockRows / 4)), dim3(256), 0, s, p);
+         ATTN_HIP(hipGetLastError());
+      }
+      return kOk;
+   }
+};
+#endif
+
+#if KERNEL >= 3
+int make_table(const RowsParams &p, hipStream_t s)
+{
+   if (!p.cap || p.m <= kTableRows) return kOk;
+   hipLaunchKernelGGL((attn_rows_table<FMM_ATTN_UNIT>), dim3(1), dim3(1024), 0, s, p);
+   ATTN_HIP(hipGetLastError());
+   return kOk;
+}
+
+template <int O, int DC, int MAPS> int join(const RowsParams &p, hipStream_t s)
+{
+   if (!p.cap) return kOk;
+   hipLaunchKernelGGL((attn_rows_join<FMM_ATTN_UNIT, O, DC, MAPS>), dim3((unsigned)((p.m * p.heads + 3) / 4)), dim3(256), 0, s, p);
+   ATTN_HIP(hipGetLastError());
+   return kOk;
+}
+
+unsigned rows_grid(const RowsParams &p) { return eighths(p.cap ? p.cap : p.m) * (unsigned)(p.kv_heads * p.passes); }
+#endif
+
+#if KERNEL == 3
+template <int DC, int MAPS> struct Rows {
+   int operator()(const RowsParams &p, hipStream_t s)
+   {
+      int st = make_table(p, s);
+      if (st) return st;
+      hipLaunchKernelGGL((attn_rows<TYPE, DC, MAPS>), dim3(rows_grid(p)), dim3(256), 0, s, p);
+      ATTN_HIP(hipGetLastError());
+      return join<TYPE, DC, MAPS>(p, s);
+   }
+};
+#elif KERNEL == 4
+template <int DC, int MAPS> struct Rows4 {
+   int operator()(const RowsParams &p, hipStream_t s)
+   {
+      int st = make_table(p, s);
+      if (st) return st;
+      if (p.d == DC && p.dv == DC * MAPS)
+         hipLaunchKernelGGL((attn_rows_kv4<DC, MAPS, true>), dim3(rows_grid(p)), dim3(256), 0, s, p);
+      else
+         hipLaunchKernelGGL((attn_rows_kv4<DC, MAPS, false>), dim3(rows_grid(p)), dim3(256), 0, s, p);
+      ATTN_HIP(hipGetLastError());
+      return p.out_type == kF16 ? join<kF16, DC, MAPS>(p, s) : join<kBF16, DC, MAPS>(p, s);
+   }
+};
+#endif
+
+}  // namespace
+
+#if KERNEL == 0
+int NAMED(launch_forward)(const Params &p, int dc, int maps, hipStream_t s) { return choose<Forward>(dc, maps, p, s); }
+#elif KERNEL == 1
+int NAMED(launch_dq)(const Params &p, int dc, int maps, hipStream_t s) { return choose<Dq>(dc, maps, p, s); }
+#elif KERNEL == 2
+int NAMED(launch_dkv)(const Params &p, int dc, int maps, hipStream_t s) { return choose<Dkv>(dc, maps, p, s); }
+#elif KERNEL == 3
+int NAMED(launch_rows)(const RowsParams &p, int dc, int maps, hipStream_t s) { return choose<Rows>(dc, maps, p, s); }
+#else
+int launch_rows_kv4(const RowsParams &p, int dc, int maps, hipStream_t s) { return choose<Rows4>(dc, maps, p, s); }
+
+int launch_kv4_write(const Kv4Params &p, int type, hipStream_t s)
+{
+   const dim3 grid((unsigned)((p.tokens + p.per_group - 1) / p.per_group));
+   if (type == kF32) hipLaunchKernelGGL((kv4_write<kF32>), grid, dim3(256), 0, s, p);
+   else if (type == kF16) hipLaunchKernelGGL((kv4_write<kF16>), grid, dim3(256), 0, s, p);
+   else hipLaunchKernelGGL((kv4_write<kBF16>), grid, dim3(256), 0, s, p);
+   ATTN_HIP(hipGetLastError());
+   return kOk;
+}
+
+int launch_kv4_read(const Kv4Params &p, int type, hipStream_t s)
+{
+   const int64_t words = p.tokens * p.kv_heads * ((p.k_width + p.v_width) / 8);
+   const dim3 grid((unsigned)std::min<int64_t>((words + 255) / 256, 1 << 16));
+   if (type == kF32) hipLaunchKernelGGL((kv4_read<kF32>), grid, dim3(256), 0, s, p);
+   else if (type == kF16) hipLaunchKernelGGL((kv4_read<kF16>), grid, dim3(256), 0, s, p);
+   else hipLaunchKernelGGL((kv4_read<kBF16>), grid, dim3(256), 0, s, p);
+   ATTN_HIP(hipGetLastError());
+   return kOk;
+}
+#endif
+
+}  // namespace fmm_attn

@@ -1,0 +1,832 @@
+// Serving form of attention over a CSR pattern: few query rows, each over its own list of cache slots, with keys and
+// values in the tensors' own type or in 4 bits.
+//
+// The 16 resident columns of the products are the query heads that share a key head (twice, with two maps), so that a
+// cached row is read once for all of them; the call is bound by those reads.  A row's list is cut into pieces of `piece`
+// slots, one workgroup each: its 4 waves take tiles of 32 slots in turn, each on its own - the keys go from memory
+// straight into the operand layout, the values through the wave's own part of LDS, where they are read transposed - and
+// join their sums at the end.  Rows of several pieces are joined by attn_rows_join.
+#pragma once
+#include "fusedmm_attn_core.h"
+
+namespace fmm_attn {
+
+struct RowsParams {
+   int64_t m, n, nnz;
+   int32_t heads, kv_heads, group, d, dv;
+   int32_t passes;                    // runs of 16 / maps query heads within a group
+   float scale;
+   int32_t index_bytes;
+   const void *indx, *pntrb, *pntre;
+   const void *q, *k, *v;
+   int64_t ldq, hdq, ldk, hdk, ldv, hdv, ldo, hdo;
+   int32_t vec_q, vec_kv, vec_o;
+   const uint8_t *cache;              // 4-bit records, instead of k and v
+   int64_t ldc, hdc;
+   const float *lambda;
+   void *out;
+   int32_t out_type;                  // 4-bit cache: element type of q and out
+   int64_t piece;                     // slots of a piece; doubled on the device while the pieces are more than cap
+   int64_t cap;                       // pieces that the workspace has room for; 0: rows are not cut
+   float *part;                       // [piece][kv head][pass][16 columns][W + 2]
+   int64_t *table;                    // m > kTableRows: [0] slots of a piece, [1 + r] pieces of the rows before r
+};
+constexpr int kTableRows = 256;       // up to this many rows, every wave finds its piece from the row pointers itself
+
+struct Kv4Params {
+   int64_t tokens, n;
+   int32_t kv_heads, k_width, v_width;   // maps * d, dv
+   int32_t d;
+   int32_t index_bytes;
+   const void *slots;
+   const void *k, *v;
+   void *to_k, *to_v;
+   int64_t ldk, hdk, ldv, hdv;
+   int32_t vec;
+   uint8_t *cache;
+   int64_t ldc, hdc;
+   int32_t per_group;                    // tokens of a workgroup
+};
+
+__device__ inline int64_t index_of(const void *a, int64_t i, int bytes)
+{
+   return bytes == 4 ? (int64_t)((const int32_t *)a)[i] : ((const int64_t *)a)[i];
+}
+
+__device__ inline int64_t row_length(const RowsParams &p, int64_t row)
+{
+   const int64_t len = index_of(p.pntre, row, p.index_bytes) - index_of(p.pntrb, row, p.index_bytes);
+   return len < 0 ? 0 : len;
+}
+
+__device__ inline int64_t pieces_of(int64_t len, int64_t piece)
+{
+   return len <= piece ? 1 : (len + piece - 1) / piece;
+}
+
+struct Spot {
+   int64_t row, first, count;   // first piece of the row, number of its pieces
+   int64_t piece;               // slots of a piece
+   int64_t total;
+};
+
+// The row that piece `id` belongs to (id < 0: row `want` is asked for).  Called by whole waves; the result is uniform.
+__device__ inline Spot find_piece(const RowsParams &p, int64_t id, int64_t want)
+{
+   Spot s;
+   s.row = -1;
+   if (p.cap == 0)   // one piece per row
+   {
+      s.row = id < 0 ? want : id < p.m ? id : -1;
+      s.first = s.row;
+      s.count = 1;
+      s.piece = INT64_MAX;
+      s.total = p.m;
+      return s;
+   }
+   if (p.m > kTableRows)
+   {
+      const int64_t *t = p.table + 1;
+      s.piece = p.table[0];
+      s.total = t[p.m];
+      int64_t lo = 0;
+      if (id < 0) lo = want;
+      else
+      {
+         if (id >= s.total) return s;
+         int64_t hi = p.m;   // t[lo] <= id < t[hi]
+         while (hi - lo > 1)
+         {
+            const int64_t mid = (lo + hi) / 2;
+            if (t[mid] <= id) lo = mid;
+            else hi = mid;
+         }
+      }
+      s.row = lo;
+      s.first = t[lo];
+      s.count = t[lo + 1] - t[lo];
+      return s;
+   }
+   const int lane = threadIdx.x & 63;
+   constexpr int kBatches = kTableRows / 64;
+   int64_t len[kBatches];
+#pragma unroll
+   for (int b = 0; b < kBatches; b++) len[b] = 64 * b + lane < p.m ? row_length(p, 64 * b + lane) : -1;
+   int64_t piece = p.piece;
+   for (;;)   // ends at the latest where every row is one piece: m <= cap
+   {
+      int64_t total = 0;
+#pragma unroll
+      for (int b = 0; b < kBatches; b++)
+      {
+         if (64 * b >= p.m) break;
+         int64_t x = len[b] < 0 ? 0 : pieces_of(len[b], piece);
+         const int64_t own = x;
+#pragma unroll
+         for (int k = 1; k < 64; k <<= 1)
+         {
+            const int64_t y = __shfl_up((long long)x, k);
+            if (lane >= k) x += y;
+         }
+         const bool here = id < 0 ? 64 * b + lane == want : len[b] >= 0 && total + x - own <= id && id < total + x;
+         const unsigned long long hit = __ballot(here);
+         if (hit)
+         {
+            const int src = __ffsll(hit) - 1;
+            s.row = 64 * b + src;
+            s.count = __shfl((long long)own, src);
+            s.first = total + __shfl((long long)x, src) - s.count;
+         }
+         total += __shfl((long long)x, 63);
+      }
+      s.piece = piece;
+      s.total = total;
+      if (total <= p.cap) return s;
+      piece *= 2;
+      s.row = -1;
+   }
+}
+
+// m > kTableRows: one workgroup of 1024 threads
+template <int UNIT> __global__ __launch_bounds__(1024) void attn_rows_table(RowsParams p)
+{
+   __shared__ int64_t sums[1024];
+   const int tid = threadIdx.x;
+   const int64_t per = (p.m + 1023) / 1024, lo = tid * per, hi = lo + per < p.m ? lo + per : p.m;
+   int64_t piece = p.piece;
+   for (;;)
+   {
+      int64_t x = 0;
+      for (int64_t r = lo; r < hi; r++) x += pieces_of(row_length(p, r), piece);
+      sums[tid] = x;
+      __syncthreads();
+      for (int s = 1; s < 1024; s <<= 1)
+      {
+         const int64_t y = tid >= s ? sums[tid - s] : 0;
+         __syncthreads();
+         sums[tid] += y;
+         __syncthreads();
+      }
+      const int64_t total = sums[1023];
+      if (total <= p.cap)
+      {
+         int64_t at = sums[tid] - x;
+         for (int64_t r = lo; r < hi; r++)
+         {
+            p.table[1 + r] = at;
+            at += pieces_of(row_length(p, r), piece);
+         }
+         if (tid == 0)
+         {
+            p.table[0] = piece;
+            p.table[1 + p.m] = total;
+         }
+         return;
+      }
+      piece *= 2;
+      __syncthreads();
+   }
+}
+
+template <int T, int DC, int MAPS> struct RowGeo {
+   typedef Num<T> N;
+   typedef typename N::E E;
+   static constexpr int W = DC * MAPS, LD = W + N::EPL, CR = W / N::EPL;
+   static constexpr int CQ = DC / N::KC, NT = W / 16;
+   static constexpr int HP = 16 / MAPS;               // query heads of a pass
+   static constexpr int NV = kTile * CR / 64;         // 16-byte chunks of the values that a lane carries
+};
+
+// what a wave keeps of its 16 columns
+template <class G> struct RowSums {
+   f4 acc[G::NT];
+   float top, sum;
+};
+
+__device__ inline void wave_lds_order()   // this wave's LDS writes before its later LDS reads
+{
+   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+   __builtin_amdgcn_wave_barrier();
+}
+
+// scores (already times scale and log2 e) of 32 slots -> running maximum and sum, weights, and the weighted values
+template <class G, int T>
+__device__ inline void row_step(RowSums<G> &r, float (&w)[2][4], unsigned mine, const typename G::E *vs, int g, int i, bool odd)
+{
+   float mx = -INFINITY;
+#pragma unroll
+   for (int j = 0; j < 8; j++)
+   {
+      w[j / 4][j % 4] = ((mine >> j) & 1) ? w[j / 4][j % 4] : -INFINITY;
+      mx = fmaxf(mx, w[j / 4][j % 4]);
+   }
+   mx = fmaxf(r.top, group_max(mx));
+   const float base = mx == -INFINITY ? 0.0f : mx;
+   const float keep = exp2_fast(r.top - base);
+   float add = 0;
+#pragma unroll
+   for (int j = 0; j < 8; j++)
+   {
+      w[j / 4][j % 4] = exp2_fast(w[j / 4][j % 4] - base);
+      add += w[j / 4][j % 4];
+   }
+   if (__any(mx != r.top))
+   {
+#pragma unroll
+      for (int x = 0; x < G::NT; x++) r.acc[x] *= keep;
+   }
+   r.sum = r.sum * keep + add;
+   r.top = mx;
+   add_weighted<T, G::NT>(r.acc, w, mine, vs, G::LD, g, i, odd);
+}
+
+// The four waves' sums -> the row's output, or its piece of the partial sums.  O: element type of the output.
+template <class G, int MAPS, int O>
+__device__ inline void rows_finish(const RowsParams &p, RowSums<G> &r, typename G::E *vs_all, float (*stat)[16][2], const Spot &s, int64_t id, int kvh, int pass)
+{
+   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, g = lane >> 4, i = lane & 15;
+   r.sum = group_sum(r.sum);
+   float *mine = reinterpret_cast<float *>(vs_all + wave * kTile * G::LD) + i * G::W;   // 16 columns x W floats fit 32 rows of values
+   wave_lds_order();
+#pragma unroll
+   for (int x = 0; x < G::NT; x++) *reinterpret_cast<f4 *>(mine + 16 * x + 4 * g) = r.acc[x];
+   if (g == 0)
+   {
+      stat[wave][i][0] = r.top;
+      stat[wave][i][1] = r.sum;
+   }
+   __syncthreads();
+   auto column = [&](int c, int f, float &top, float &sum) {
+      top = fmaxf(fmaxf(stat[0][c][0], stat[1][c][0]), fmaxf(stat[2][c][0], stat[3][c][0]));
+      const float base = top == -INFINITY ? 0.0f : top;
+      sum = 0;
+      float x = 0;
+#pragma unroll
+      for (int w = 0; w < 4; w++)
+      {
+         const float keep = exp2_fast(stat[w][c][0] - base);
+         sum += stat[w][c][1] * keep;
+         x += reinterpret_cast<const float *>(vs_all + w * kTile * G::LD)[c * G::W + f] * keep;
+      }
+      return x;
+   };
+   const int left = p.group - pass * G::HP, heads = left < G::HP ? left : G::HP;
+   if (s.count > 1)
+   {
+      float *to = p.part + ((id * p.kv_heads + kvh) * p.passes + pass) * 16 * (G::W + 2);
+      for (int e = tid; e < 16 * G::W; e += 256)
+      {
+         const int c = e / G::W, f = e % G::W;
+         if (c % G::HP >= heads) continue;
+         float top, sum;
+         to[c * (G::W + 2) + f] = column(c, f, top, sum);
+         if (f == 0)
+         {
+            to[c * (G::W + 2) + G::W] = top;
+            to[c * (G::W + 2) + G::W + 1] = sum;
+         }
+      }
+      return;
+   }
+   typedef typename Num<O>::E EO;
+   for (int e = tid; e < heads * G::W; e += 256)
+   {
+      const int hh = e / G::W, f = e % G::W;
+      if (f >= p.dv) continue;
+      const int head = kvh * p.group + pass * G::HP + hh;
+      float top, sum;
+      float x = column(hh, f, top, sum);
+      x = sum == 0.0f ? 0.0f : x / sum;
+      if constexpr (MAPS == 2)
+      {
+         const float y = column(hh + 8, f, top, sum);
+         x -= p.lambda[head] * (sum == 0.0f ? 0.0f : y / sum);
+      }
+      ((EO *)p.out)[s.row * p.ldo + head * p.hdo + f] = (EO)Num<O>::from(x);
+   }
+}
+
+// rows of several pieces: one wave per (row, head)
+// (UNIT: the object it is compiled into)
+template <int UNIT, int O, int DC, int MAPS> __global__ __launch_bounds__(256) void attn_rows_join(RowsParams p)
+{
+   constexpr int W = DC * MAPS, HP = 16 / MAPS, PER = (W + 63) / 64;
+   typedef typename Num<O>::E EO;
+   const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+   if (id >= p.m * p.heads) return;
+   const int lane = threadIdx.x & 63;
+   const int64_t row = id / p.heads;
+   const int head = (int)(id % p.heads), kvh = head / p.group, hh = head % p.group, pass = hh / HP;
+   const Spot s = find_piece(p, -1, row);
+   if (s.count <= 1) return;
+   float o[MAPS][PER];
+#pragma unroll
+   for (int mp = 0; mp < MAPS; mp++)
+   {
+      const int64_t step = (int64_t)p.kv_heads * p.passes * 16 * (W + 2);
+      const float *from = p.part + ((s.first * p.kv_heads + kvh) * p.passes + pass) * 16 * (W + 2) + (mp * HP + hh % HP) * (W + 2);
+      float top = -INFINITY;
+      for (int64_t u = lane; u < s.count; u += 64) top = fmaxf(top, from[u * step + W]);
+#pragma unroll
+      for (int k = 1; k < 64; k <<= 1) top = fmaxf(top, __shfl_xor(top, k));
+      const float base = top == -INFINITY ? 0.0f : top;
+      float sum = 0;
+#pragma unroll
+      for (int x = 0; x < PER; x++) o[mp][x] = 0;
+#pragma unroll 4
+      for (int64_t u = 0; u < s.count; u++)
+      {
+         const float *f = from + u * step;
+         const float keep = exp2_fast(f[W] - base);
+         sum += f[W + 1] * keep;
+#pragma unroll
+         for (int x = 0; x < PER; x++)
+            if (lane + 64 * x < W) o[mp][x] += f[lane + 64 * x] * keep;
+      }
+      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+      for (int x = 0; x < PER; x++) o[mp][x] *= inv;
+   }
+   EO *out = (EO *)p.out + row * p.ldo + head * p.hdo;
+#pragma unroll
+   for (int x = 0; x < PER; x++)
+   {
+      const int f = lane + 64 * x;
+      if (f >= p.dv) continue;
+      float res = o[0][x];
+      if constexpr (MAPS == 2) res -= p.lambda[head] * o[1][x];
+      out[f] = (EO)Num<O>::from(res);
+   }
+}
+
+// workgroup b of a launch -> (piece, key head, pass): the key heads of a piece run next to each other on one XCD
+struct RowsItem {
+   int64_t id;
+   int kvh, pass;
+};
+__device__ inline RowsItem rows_item(const RowsParams &p)
+{
+   const int64_t b = blockIdx.x, j = b >> 3;
+   const int y = p.kv_heads * p.passes;
+   RowsItem r;
+   r.id = (j / y) * 8 + (b & 7);
+   r.kvh = (int)(j % y) / p.passes;
+   r.pass = (int)(j % y) % p.passes;
+   return r;
+}
+
+// slot of the tile's row lane % 32, -1 where there is none
+__device__ inline int32_t tile_slot(const RowsParams &p, int64_t at, int64_t end, int lane)
+{
+   const int64_t e = at + (lane & 31);
+   if (e >= end) return -1;
+   const int64_t c = index_of(p.indx, e, p.index_bytes);
+   return c >= 0 && c < p.n ? (int32_t)c : -1;
+}
+
+__device__ inline unsigned tile_bits(int32_t slot, int g)
+{
+   const uint32_t live = (uint32_t)__ballot(slot >= 0);
+   return ((live >> (4 * g)) & 15) | (((live >> (16 + 4 * g)) & 15) << 4);
+}
+
+// ---- keys and values in their own type ------------------------------------------------------------------------------------------
+template <int T, int DC, int MAPS>
+__global__ __launch_bounds__(256, (sizeof(typename Num<T>::E) * DC * MAPS >= 512 ? 1 : 2)) void attn_rows(RowsParams p)
+{
+   typedef RowGeo<T, DC, MAPS> G;
+   typedef typename G::E E;
+   __shared__ __align__(16) E vs_all[4 * kTile * G::LD];
+   __shared__ float stat[4][16][2];
+   const RowsItem it = rows_item(p);
+   const Spot s = find_piece(p, it.id, 0);
+   if (s.row < 0) return;
+   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, g = lane >> 4, i = lane & 15;
+   E *vs = vs_all + wave * kTile * G::LD;
+   const int64_t begin = index_of(p.pntrb, s.row, p.index_bytes), len = row_length(p, s.row);
+   const int64_t lo = s.count > 1 ? (it.id - s.first) * s.piece : 0, hi = s.count > 1 && lo + s.piece < len ? lo + s.piece : len;
+   const E *k = (const E *)p.k + it.kvh * p.hdk, *v = (const E *)p.v + it.kvh * p.hdv;
+
+   const int mp_i = i / G::HP, hh = it.pass * G::HP + i % G::HP;
+   const bool col = hh < p.group;
+   u4 q[G::CQ];
+#pragma unroll
+   for (int c = 0; c < G::CQ; c++)
+   {
+      const int f = c * G::N::KC + g * G::N::EPL;
+      const int left = p.d - f;
+      q[c] = load_chunk<T>((const E *)p.q + s.row * p.ldq + (col ? (it.kvh * p.group + hh) * p.hdq + mp_i * p.d + f : 0),
+                           col ? (left < G::N::EPL ? left : G::N::EPL) : 0, p.vec_q);
+   }
+   RowSums<G> r;
+   r.top = -INFINITY;
+   r.sum = 0;
+#pragma unroll
+   for (int x = 0; x < G::NT; x++) r.acc[x] = f4{0, 0, 0, 0};
+   const float c2 = p.scale * kLog2e;
+
+   u4 kf[2][MAPS][G::CQ], vf[G::NV];
+   auto load = [&](int32_t slot) {
+#pragma unroll
+      for (int a = 0; a < 2; a++)
+      {
+         const int32_t c = __shfl(slot, 16 * a + i);
+         const E *row = k + (int64_t)(c < 0 ? 0 : c) * p.ldk;
+#pragma unroll
+         for (int mp = 0; mp < MAPS; mp++)
+#pragma unroll
+            for (int x = 0; x < G::CQ; x++)
+            {
+               const int f = x * G::N::KC + g * G::N::EPL, left = p.d - f;
+               kf[a][mp][x] = load_chunk<T>(row + mp * p.d + f, c < 0 ? 0 : left < G::N::EPL ? left : G::N::EPL, p.vec_kv);
+            }
+      }
+#pragma unroll
+      for (int j = 0; j < G::NV; j++)
+      {
+         const int e = lane + 64 * j, f = (e % G::CR) * G::N::EPL, left = p.dv - f;
+         const int32_t c = __shfl(slot, e / G::CR);
+         vf[j] = load_chunk<T>(v + (int64_t)(c < 0 ? 0 : c) * p.ldv + f, c < 0 ? 0 : left < G::N::EPL ? left : G::N::EPL, p.vec_kv);
+      }
+   };
+   constexpr int64_t kStride = 4 * kTile;
+   const int64_t end = begin + hi;
+   int64_t at = begin + lo + wave * kTile;
+   int32_t slot = tile_slot(p, at, end, lane);
+   int32_t next = tile_slot(p, at + kStride, end, lane);
+   if (at < end) load(slot);
+   for (; at < end; at += kStride)
+   {
+      const unsigned mine = tile_bits(slot, g);
+      bool odd = false;
+#pragma unroll
+      for (int j = 0; j < G::NV; j++)
+      {
+         const int e = lane + 64 * j;
+         *reinterpret_cast<u4 *>(vs + (e / G::CR) * G::LD + (e % G::CR) * G::N::EPL) = vf[j];
+         odd |= odd_chunk<T>(vf[j]);
+      }
+      odd = __any(odd);
+      f4 sc[MAPS][2];
+#pragma unroll
+      for (int mp = 0; mp < MAPS; mp++)
+#pragma unroll
+         for (int a = 0; a < 2; a++)
+         {
+            sc[mp][a] = f4{0, 0, 0, 0};
+#pragma unroll
+            for (int x = 0; x < G::CQ; x++) sc[mp][a] = G::N::mma(kf[a][mp][x], q[x], sc[mp][a]);
+         }
+      slot = next;
+      if (at + kStride < end)
+      {
+         load(slot);
+         next = tile_slot(p, at + 2 * kStride, end, lane);
+      }
+      float w[2][4];
+#pragma unroll
+      for (int j = 0; j < 8; j++)
+      {
+         float x = sc[0][j / 4][j % 4];
+         if constexpr (MAPS == 2) x = mp_i ? sc[1][j / 4][j % 4] : x;
+         w[j / 4][j % 4] = x * c2;
+      }
+      wave_lds_order();
+      row_step<G, T>(r, w, mine, vs, g, i, odd);
+      wave_lds_order();
+   }
+   rows_finish<G, MAPS, T>(p, r, vs_all, stat, s, it.id, it.kvh, it.pass);
+}
+
+// ---- keys and values in 4 bits ----------------------------------------------------------------------------------------------------
+// A record: codes of k (maps * d / 2 bytes), codes of v (dv / 2), one 16-bit word per 32 values of k and then of v.  The
+// word is an fp16 scale with the zero point z in its low four mantissa bits; the value of code c is s (c - z).  s has at
+// most 7 significant bits, c - z at most 4, so the value is exact in fp16 and the products run on fp16 operands.
+// A code becomes 1024 + c with one and-or (0x6400 is fp16 1024), c - z with one packed subtraction, the value with one
+// packed product: 2 operations for 2 values, a third for the shift.
+__device__ inline u4 dequant8(uint32_t codes, uint32_t word)
+{
+   typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+   const uint32_t s = word & 0xFFF0u, z = 0x6400u | (word & 15u);
+   const h2 scale = __builtin_bit_cast(h2, s | (s << 16)), zero = __builtin_bit_cast(h2, z | (z << 16));
+   u4 r;
+#pragma unroll
+   for (int j = 0; j < 4; j++)
+      r[j] = __builtin_bit_cast(uint32_t, (__builtin_bit_cast(h2, ((codes >> (4 * j)) & 0x000F000Fu) | 0x64006400u) - zero) * scale);
+   return r;
+}
+
+// FULL: d == DC and dv == DC * MAPS; a lane then reads a contiguous quarter of a row's codes, otherwise 4 bytes of every
+// 32 codes.  Feature at which word j of lane group g starts:
+template <bool FULL, int WORDS> __device__ inline int code_feature(int j, int g) { return FULL ? g * (WORDS * 8) + 8 * j : 32 * j + 8 * g; }
+
+template <bool FULL, int WORDS> __device__ inline void load_codes(uint32_t (&to)[WORDS], const uint8_t *from, int width, int g)
+{
+   typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+   if constexpr (FULL && WORDS % 4 == 0)
+   {
+#pragma unroll
+      for (int j = 0; j < WORDS / 4; j++)
+      {
+         const u4 x = *reinterpret_cast<const u4 *>(from + g * (WORDS * 4) + 16 * j);
+#pragma unroll
+         for (int e = 0; e < 4; e++) to[4 * j + e] = x[e];
+      }
+   }
+   else if constexpr (FULL && WORDS == 2)
+   {
+      const u2 x = *reinterpret_cast<const u2 *>(from + g * 8);
+      to[0] = x[0];
+      to[1] = x[1];
+   }
+   else
+   {
+#pragma unroll
+      for (int j = 0; j < WORDS; j++) to[j] = 32 * j < width ? *reinterpret_cast<const uint32_t *>(from + 16 * j + 4 * g) : 0;
+   }
+}
+
+template <bool FULL, int WORDS> __device__ inline void load_scales(uint32_t (&to)[WORDS], const uint8_t *from, int width, int g)
+{
+#pragma unroll
+   for (int j = 0; j < WORDS; j++)
+   {
+      const int f = code_feature<FULL, WORDS>(j, g);
+      to[j] = f < width ? *reinterpret_cast<const uint16_t *>(from + f / 32 * 2) : 0;
+   }
+}
+
+template <int DC, int MAPS, bool FULL>
+__global__ __launch_bounds__(256, (DC * MAPS >= 256 ? 1 : 2)) void attn_rows_kv4(RowsParams p)
+{
+   typedef RowGeo<kF16, DC, MAPS> G;
+   typedef uint16_t E;
+   constexpr int WQ = DC / 32, WV = G::W / 32;   // 4-byte words of codes that a lane reads of one map's key, of a value row
+   __shared__ __align__(16) E vs_all[4 * kTile * G::LD];
+   __shared__ float stat[4][16][2];
+   const RowsItem it = rows_item(p);
+   const Spot s = find_piece(p, it.id, 0);
+   if (s.row < 0) return;
+   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, g = lane >> 4, i = lane & 15;
+   E *vs = vs_all + wave * kTile * G::LD;
+   const int64_t begin = index_of(p.pntrb, s.row, p.index_bytes), len = row_length(p, s.row);
+   const int64_t lo = s.count > 1 ? (it.id - s.first) * s.piece : 0, hi = s.count > 1 && lo + s.piece < len ? lo + s.piece : len;
+   const uint8_t *cache = p.cache + it.kvh * p.hdc;
+   const int kw = MAPS * p.d;
+   const int off_v = kw / 2, off_kw = (kw + p.dv) / 2, off_vw = off_kw + kw / 16;   // bytes
+
+   const int mp_i = i / G::HP, hh = it.pass * G::HP + i % G::HP;
+   const bool col = hh < p.group;
+   // The query as fp16, each head scaled by a power of two so that its largest feature is near 1: bf16's range does not
+   // fit fp16's, its 8 bits of significand do.
+   float qf[WQ][8];
+   float top = 0;
+#pragma unroll
+   for (int j = 0; j < WQ; j++)
+#pragma unroll
+      for (int e = 0; e < 8; e++)
+      {
+         const int f = code_feature<FULL, WQ>(j, g) + e;
+         float x = 0;
+         if (col && f < p.d)
+         {
+            const int64_t off = s.row * p.ldq + (it.kvh * p.group + hh) * p.hdq + mp_i * p.d + f;
+            x = p.out_type == kF16 ? Num<kF16>::to(((const uint16_t *)p.q)[off]) : Num<kBF16>::to(((const uint16_t *)p.q)[off]);
+         }
+         qf[j][e] = x;
+         top = fmaxf(top, fabsf(x));
+      }
+   top = group_max(top);
+   int ex = 0;
+   if (top > 0 && top < INFINITY) (void)frexpf(top, &ex);
+   u4 q[WQ];
+#pragma unroll
+   for (int j = 0; j < WQ; j++)
+   {
+#pragma unroll
+      for (int e = 0; e < 4; e++)
+         q[j][e] = (uint32_t)Num<kF16>::from(ldexpf(qf[j][2 * e], -ex)) | (uint32_t)Num<kF16>::from(ldexpf(qf[j][2 * e + 1], -ex)) << 16;
+   }
+   const float c2 = ldexpf(p.scale * kLog2e, ex);
+
+   RowSums<G> r;
+   r.top = -INFINITY;
+   r.sum = 0;
+#pragma unroll
+   for (int x = 0; x < G::NT; x++) r.acc[x] = f4{0, 0, 0, 0};
+
+   uint32_t kc[2][MAPS][WQ], vc[2][WV], ks[2][MAPS][WQ], vw[2][WV];
+   auto load = [&](int32_t slot) {
+#pragma unroll
+      for (int a = 0; a < 2; a++)
+      {
+         const int32_t c = __shfl(slot, 16 * a + i);
+         if (c >= 0)
+         {
+            const uint8_t *rec = cache + (int64_t)c * p.ldc;
+#pragma unroll
+            for (int mp = 0; mp < MAPS; mp++)
+            {
+               load_codes<FULL>(kc[a][mp], rec + mp * p.d / 2, p.d, g);
+               load_scales<FULL>(ks[a][mp], rec + off_kw + mp * p.d / 16, p.d, g);
+            }
+            load_codes<FULL>(vc[a], rec + off_v, p.dv, g);
+            load_scales<FULL>(vw[a], rec + off_vw, p.dv, g);
+         }
+         else
+         {
+#pragma unroll
+            for (int j = 0; j < WQ; j++)
+#pragma unroll
+               for (int mp = 0; mp < MAPS; mp++) kc[a][mp][j] = ks[a][mp][j] = 0;
+#pragma unroll
+            for (int j = 0; j < WV; j++) vc[a][j] = vw[a][j] = 0;
+         }
+      }
+   };
+   constexpr int64_t kStride = 4 * kTile;
+   const int64_t end = begin + hi;
+   int64_t at = begin + lo + wave * kTile;
+   int32_t slot = tile_slot(p, at, end, lane);
+   int32_t next = tile_slot(p, at + kStride, end, lane);
+   if (at < end) load(slot);
+   for (; at < end; at += kStride)
+   {
+      const unsigned mine = tile_bits(slot, g);
+      bool odd = false;
+      f4 sc[MAPS][2];
+#pragma unroll
+      for (int a = 0; a < 2; a++)
+      {
+#pragma unroll
+         for (int mp = 0; mp < MAPS; mp++)
+         {
+            sc[mp][a] = f4{0, 0, 0, 0};
+#pragma unroll
+            for (int j = 0; j < WQ; j++) sc[mp][a] = G::N::mma(dequant8(kc[a][mp][j], ks[a][mp][j]), q[j], sc[mp][a]);
+         }
+#pragma unroll
+         for (int j = 0; j < WV; j++)
+         {
+            *reinterpret_cast<u4 *>(vs + (16 * a + i) * G::LD + code_feature<FULL, WV>(j, g)) = dequant8(vc[a][j], vw[a][j]);
+            odd |= (vw[a][j] & 0x7C00u) == 0x7C00u;   // an infinite or NaN scale
+         }
+      }
+      odd = __any(odd);
+      slot = next;
+      if (at + kStride < end)
+      {
+         load(slot);
+         next = tile_slot(p, at + 2 * kStride, end, lane);
+      }
+      float w[2][4];
+#pragma unroll
+      for (int j = 0; j < 8; j++)
+      {
+         float x = sc[0][j / 4][j % 4];
+         if constexpr (MAPS == 2) x = mp_i ? sc[1][j / 4][j % 4] : x;
+         w[j / 4][j % 4] = x * c2;
+      }
+      wave_lds_order();
+      row_step<G, kF16>(r, w, mine, vs, g, i, odd);
+      wave_lds_order();
+   }
+   if (p.out_type == kF16) rows_finish<G, MAPS, kF16>(p, r, vs_all, stat, s, it.id, it.kvh, it.pass);
+   else rows_finish<G, MAPS, kBF16>(p, r, vs_all, stat, s, it.id, it.kvh, it.pass);
+}
+
+// ---- into the 4-bit cache and back ---------------------------------------------------------------------------------------------------
+// Eight values per lane, four lanes per group of 32.  The step between codes is the group's range (with zero in it) over
+// 15, rounded up to 7 significant bits and to a multiple of 2^-20; code and zero point are rounded to nearest, ties to
+// even.  The borders between codes are decided in 64 bits for 32-bit values; for 16-bit values the quotient in 32 bits,
+// correctly rounded, decides them alike: x has 11 significant bits and a border 12, so a quotient that is not a border is
+// further from it than 2^-24 of its size.
+template <int T> __device__ inline float code_of(float x, float s)
+{
+   if constexpr (T == kF32) return (float)rint((double)x / (double)s);
+   else return rintf(x / s);
+}
+
+template <int T> __global__ __launch_bounds__(256) void kv4_write(Kv4Params p)
+{
+   typedef typename Num<T>::E E;
+   constexpr int kMost = 32;
+   __shared__ int64_t slot[kMost];
+   __shared__ int later[kMost];
+   const int tid = threadIdx.x;
+   const int64_t t0 = (int64_t)blockIdx.x * p.per_group;
+   const int here = (int)(p.tokens - t0 < p.per_group ? p.tokens - t0 : p.per_group);
+   if (tid < kMost)
+   {
+      later[tid] = 0;
+      slot[tid] = tid < here ? index_of(p.slots, t0 + tid, p.index_bytes) : -1;
+   }
+   __syncthreads();
+   // a slot that is named more than once takes the last token that names it
+   for (int64_t t = t0 + 1 + tid; t < p.tokens; t += 256)
+   {
+      const int64_t c = index_of(p.slots, t, p.index_bytes);
+      for (int x = 0; x < here; x++)
+         if (slot[x] == c && t0 + x < t) later[x] = 1;
+   }
+   __syncthreads();
+   const int words = (p.k_width + p.v_width) / 8, per_token = words * p.kv_heads;   // a multiple of 4: groups do not cross items
+   for (int x = tid; x < here * per_token; x += 256)
+   {
+      const int tok = x / per_token, head = x % per_token / words, w = x % words;
+      const int64_t c = slot[tok];
+      const bool is_v = 8 * w >= p.k_width;
+      const int f = is_v ? 8 * w - p.k_width : 8 * w;
+      const E *from = is_v ? (const E *)p.v + (t0 + tok) * p.ldv + head * p.hdv + f : (const E *)p.k + (t0 + tok) * p.ldk + head * p.hdk + f;
+      float v[8];
+      if constexpr (T == kF32)
+      {
+         const u4 a = load_chunk<T>(from, 4, p.vec), b = load_chunk<T>(from + 4, 4, p.vec);
+#pragma unroll
+         for (int e = 0; e < 4; e++)
+         {
+            v[e] = __uint_as_float(a[e]);
+            v[4 + e] = __uint_as_float(b[e]);
+         }
+      }
+      else
+      {
+         const u4 a = load_chunk<T>(from, 8, p.vec);
+#pragma unroll
+         for (int e = 0; e < 8; e++) v[e] = Num<T>::to((E)(a[e / 2] >> (16 * (e & 1))));
+      }
+      float lo = 0, hi = 0;
+      bool nan = false;
+#pragma unroll
+      for (int e = 0; e < 8; e++)
+      {
+         nan |= v[e] != v[e];
+         v[e] = fminf(fmaxf(v[e], -32768.0f), 32768.0f);   // what a step of fp16 reaches; a NaN makes its whole group NaN
+         lo = fminf(lo, v[e]);
+         hi = fmaxf(hi, v[e]);
+      }
+      int any = nan;
+#pragma unroll
+      for (int k = 1; k < 4; k <<= 1)
+      {
+         lo = fminf(lo, __shfl_xor(lo, k));
+         hi = fmaxf(hi, __shfl_xor(hi, k));
+         any |= __shfl_xor(any, k);
+      }
+      const double step = ((double)hi - (double)lo) / 15.0;
+      int e2;
+      (void)frexp(step, &e2);   // step in [2^(e2 - 1), 2^e2)
+      const int unit = step == 0 || e2 - 7 < -20 ? -20 : e2 - 7;
+      const float s = (float)ldexp(ceil(ldexp(step, -unit)), unit);
+      const float z = s > 0 ? (float)rint(-(double)lo / (double)s) : 0.0f;
+      uint32_t codes = 0;
+      if (s > 0 && !any)
+      {
+#pragma unroll
+         for (int e = 0; e < 8; e++)
+         {
+            const float q = fminf(fmaxf(code_of<T>(v[e], s) + z, 0.0f), 15.0f);
+            codes |= (uint32_t)q << (4 * ((e % 2) * 4 + e / 2));
+         }
+      }
+      if (c < 0 || c >= p.n || later[tok]) continue;
+      uint8_t *rec = p.cache + c * p.ldc + head * p.hdc;
+      *reinterpret_cast<uint32_t *>(rec + 4 * w) = codes;
+      if (w % 4 == 0)
+      {
+         const uint32_t word = any ? 0x7E00u : (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)s) | (uint32_t)z;
+         *reinterpret_cast<uint16_t *>(rec + 4 * words + w / 4 * 2) = (uint16_t)word;
+      }
+   }
+}
+
+template <int T> __global__ __launch_bounds__(256) void kv4_read(Kv4Params p)
+{
+   typedef typename Num<T>::E E;
+   const int words = (p.k_width + p.v_width) / 8;
+   const int64_t total = p.tokens * p.kv_heads * words;
+   for (int64_t x = (int64_t)blockIdx.x * 256 + threadIdx.x; x < total; x += (int64_t)gridDim.x * 256)
+   {
+      const int64_t tok = x / (p.kv_heads * words);
+      const int head = (int)(x / words % p.kv_heads), w = (int)(x % words);
+      const int64_t c = index_of(p.slots, tok, p.index_bytes);
+      uint32_t codes = 0, word = 0;
+      if (c >= 0 && c < p.n)
+      {
+         const uint8_t *rec = p.cache + c * p.ldc + head * p.hdc;
+         codes = *reinterpret_cast<const uint32_t *>(rec + 4 * w);
+         word = *reinterpret_cast<const uint16_t *>(rec + 4 * words + w / 4 * 2);
+      }
+      const u4 h = dequant8(codes, word);
+      const bool is_v = 8 * w >= p.k_width;
+      const int f = is_v ? 8 * w - p.k_width : 8 * w;
+      E *to = is_v ? (E *)p.to_v + tok * p.ldv + head * p.hdv + f : (E *)p.to_k + tok * p.ldk + head * p.hdk + f;
+      float v[8];
+#pragma unroll
+      for (int e = 0; e < 8; e++) v[e] = Num<kF16>::to((uint16_t)(h[e / 2] >> (16 * (e & 1))));
+      store4<T>(to, 0, 8, f4{v[0], v[1], v[2], v[3]}, p.vec);
+      store4<T>(to, 4, 8, f4{v[4], v[5], v[6], v[7]}, p.vec);
+   }
+}
+
+}  // namespace fmm_attn

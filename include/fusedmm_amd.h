@@ -277,6 +277,115 @@ int fusedMM_amd_last_split(unsigned int *heavy_rows, unsigned int *segments, uns
  * (read once, at the first call) overrides the choice.  Waits for the GPU. */
 int fusedMM_amd_last_row_order(int *scattered, unsigned int *edges_lower_half, unsigned int *edges_upper_half);
 
+/*
+ * ---- attention over a CSR pattern ----------------------------------------------------------------
+ *
+ * The same gather as fusedMM_csr - row i of X against the rows of Y that its edges name - with a softmax over
+ * the row's edges between the two products, per head, in fp32, fp16 or bf16.  No counterpart in the reference.
+ *
+ *    maps = 1   P = softmax_j(scale <q_i, k_j>),               o_i = sum_j P_j v_j
+ *    maps = 2   P1, P2 from q1, k1 and q2, k2 (d features each), o_i = sum_j (P1_j - lambda_h P2_j) v_j
+ *
+ * An edge that a row names twice counts twice; a row without edges gives o = 0 (and lse = -infinity).  Edge ids
+ * outside [0, n) are masked places: they are skipped.  There are no edge values.  Sums, maxima and softmax
+ * statistics are fp32; fp16/bf16 products run on matrix cores with fp32 accumulation, the softmax weights (and in
+ * the backward pass the scores' gradients) rounded to the tensors' type in between.  Results are the same bits
+ * from run to run.  Infinities and NaN in rows of k and v reach only the rows that name them.
+ *
+ * All pointers are device memory of the current device, all work is enqueued on `stream` (a hipStream_t), nothing
+ * is allocated, no state is kept and nothing waits for the GPU (fusedMM_attn_plan_create and _destroy apart): the
+ * calls may run side by side on different streams and in different threads, and may be captured into graphs,
+ * as long as calls that can overlap have workspaces and outputs of their own.  Rows behind the last
+ * one and columns between the heads are left as they are.  Return values are fusedMM status codes:
+ * FUSEDMM_FAIL_RETURN for arguments that do not fit together (with a line on stderr), FUSEDMM_NOT_ENOUGH_MEM for
+ * a workspace that is too small, FUSEDMM_NO_OPT_IMPL for sizes without a kernel: d <= 256 and dv <= 256 with one
+ * map, d <= 128 and dv <= 256 with two.
+ */
+#define FUSEDMM_TYPE_F32   0
+#define FUSEDMM_TYPE_F16   1
+#define FUSEDMM_TYPE_BF16  2
+
+/* Sizes and layout.  Strides count elements: feature c of map p of head h of row i of q is
+ * q[i * ldq + h * hdq + p * d + c]; k likewise with kv_heads heads, v and o with dv features and no maps.
+ * Packed rows (ld the width of a packed row) and head-major tensors (hd = rows * width) are both described so.
+ * heads is a multiple of kv_heads: query head h reads key head h / (heads / kv_heads). */
+typedef struct fusedMM_attn_desc {
+   int32_t type;               /* FUSEDMM_TYPE_* of q, k, v, o and their gradients */
+   int32_t maps;               /* 1 or 2 */
+   int64_t m, n;               /* rows of q and o; rows (cache slots) of k and v */
+   int32_t heads, kv_heads;
+   int32_t d, dv;              /* features of one map of q and k; of v and o */
+   float scale;
+   int64_t ldq, hdq, ldk, hdk, ldv, hdv, ldo, hdo;
+} fusedMM_attn_desc;
+
+/*
+ * A plan of a pattern that is used many times (a training graph, a prompt's mask): for every block of 64 rows the
+ * columns that any of them names, so that a gathered row is loaded once for all of them.  m, n <= 2^26 - 1; nnz at
+ * least the sum of the row lengths.  Column ids in ascending order within the rows share best; any order is right.
+ * The plan belongs to the current device, holds device memory (12 bytes per distinct (block, column)) and can be used
+ * for any head count, type and feature width.  Waits for the GPU; refused while `stream` is captured.
+ * Destroying waits for the device's work and frees the memory; graphs that were captured with the plan end with it.
+ */
+int fusedMM_attn_plan_create(const INDEXTYPE m, const INDEXTYPE n, const INDEXTYPE nnz, const INDEXTYPE *indx,
+                             const INDEXTYPE *pntrb, const INDEXTYPE *pntre, void *stream, void **plan);
+int fusedMM_attn_plan_destroy(void *plan);
+
+/* Bytes of workspace (16-byte aligned) of a forward call, or, with the plan of the transposed pattern, of a forward and
+ * of a backward call.  -1: the arguments do not fit together. */
+int64_t fusedMM_attn_workspace(const fusedMM_attn_desc *desc, const void *plan, const void *plan_t);
+
+/* lambda: fp32 [heads], NULL with one map.  o2 and lse may be NULL where no backward pass follows: o2 (laid out as o)
+ * receives sum_j P2_j v_j of two maps, lse (fp32 [m][heads][maps]) the logarithms of the softmax sums. */
+int fusedMM_attn_forward(const fusedMM_attn_desc *desc, const void *plan, const void *q, const void *k, const void *v,
+                         const float *lambda, void *o, void *o2, float *lse, void *work, int64_t work_bytes, void *stream);
+
+/* Gradients of the whole: dout is laid out as o; dq, dk, dv as q, k, v; dlambda fp32 [heads] (NULL: not wanted).
+ * plan_t is the plan of the transposed pattern (a call of fusedMM_attn_plan_create with the CSC arrays, m and n
+ * exchanged).  o, o2 and lse are what the forward call wrote.  Gradients are overwritten, not added to; rows of k that
+ * no edge names get zeros. */
+int fusedMM_attn_backward(const fusedMM_attn_desc *desc, const void *plan, const void *plan_t, const void *q, const void *k,
+                          const void *v, const float *lambda, const void *o, const void *o2, const float *lse,
+                          const void *dout, void *dq, void *dk, void *dv, float *dlambda, void *work, int64_t work_bytes,
+                          void *stream);
+
+/*
+ * Serving form: the pattern is given with the call, rows are the new tokens and their edges the slots of a key/value
+ * cache that the token's sequence holds (in any order; -1 for a masked place).  Rows may be as long as the cache and
+ * of any mixture of lengths: long rows are cut and joined.  nnz bounds the sum of the row lengths; it chooses the pieces
+ * and sizes the workspace (rows that turn out longer are still right).  n <= 2^31 - 1.
+ */
+int64_t fusedMM_attn_rows_workspace(const fusedMM_attn_desc *desc, const INDEXTYPE nnz);
+int fusedMM_attn_rows(const fusedMM_attn_desc *desc, const INDEXTYPE nnz, const INDEXTYPE *indx, const INDEXTYPE *pntrb,
+                      const INDEXTYPE *pntre, const void *q, const void *k, const void *v, const float *lambda, void *o,
+                      void *work, int64_t work_bytes, void *stream);
+
+/*
+ * A key/value cache in 4 bits: one record per (slot, key head), at cache + slot * ldc + head * hdc bytes (multiples of 16,
+ * cache 16-byte aligned), of fusedMM_kv4_record_bytes() bytes:
+ *    codes of k (maps * d / 2 bytes), codes of v (dv / 2), one 16-bit word for every 32 values of k, then of v.
+ * Of eight codes, code e is nibble (e % 2) * 4 + e / 2 (low to high) of their 32-bit word.  The 16-bit word is an fp16
+ * scale s with the zero point z (0 ... 15) in its low four bits (the scale has zeros there); the value is s * (code - z),
+ * exact in fp16.  With lo = min(0, values), hi = max(0, values), s is (hi - lo) / 15 rounded up to 7 significant bits
+ * and to a multiple of 2^-20, z = rint(-lo / s), code = clamp(rint(x / s) + z, 0, 15), ties to even.  Magnitudes above
+ * 32768 saturate; a NaN makes its group of 32 NaN.  d and dv are multiples of 32.
+ */
+int64_t fusedMM_kv4_record_bytes(const int maps, const int d, const int dv);
+
+/* Token t of k and v (ldk, hdk, ldv, hdv and the sizes from desc; m, heads and the other strides are not read) goes to
+ * slot slots[t]; tokens whose slot is outside [0, desc->n) are skipped.  Of tokens with the same slot the last one
+ * counts.  At most 2^20 tokens.  Bytes of a record behind the last word are left as they are. */
+int fusedMM_kv4_write(const fusedMM_attn_desc *desc, const INDEXTYPE tokens, const INDEXTYPE *slots, const void *k, const void *v,
+                      void *cache, int64_t ldc, int64_t hdc, void *stream);
+/* The values of the records of slots[0 .. tokens) in desc->type; slots outside [0, desc->n) read as zeros. */
+int fusedMM_kv4_read(const fusedMM_attn_desc *desc, const INDEXTYPE tokens, const INDEXTYPE *slots, const void *cache, int64_t ldc,
+                     int64_t hdc, void *k, void *v, void *stream);
+/* fusedMM_attn_rows over such a cache; desc->type (of q and o) is fp16 or bf16.  Products run on fp16 operands: the
+ * cache's values are exact in it, each head's query is scaled by a power of two into its range. */
+int fusedMM_attn_rows_kv4(const fusedMM_attn_desc *desc, const INDEXTYPE nnz, const INDEXTYPE *indx, const INDEXTYPE *pntrb,
+                          const INDEXTYPE *pntre, const void *q, const void *cache, int64_t ldc, int64_t hdc, const float *lambda,
+                          void *o, void *work, int64_t work_bytes, void *stream);
+
 /* Release every device buffer the library holds (work queues, staging). */
 void fusedMM_amd_finalize(void);
 

@@ -1,0 +1,380 @@
+"""Serving form of the attention (rows over cache slots, in the tensors' type and in 4 bits) and the 4-bit cache itself,
+against dense 64-bit values with derived bounds (tests/attn_reference.py)."""
+import numpy as np
+import pytest
+
+import fusedmm_amd as fa
+from attn_reference import quantise_row, record
+from attn_run import SENTINEL, Case, Tensor, desc, dtype, index_arrays, inside, random_pattern
+
+pytestmark = pytest.mark.gpu
+
+
+def ragged(lengths, n, seed, masked=True):
+    """Rows of the given lengths over distinct slots of n, in any order."""
+    rng = np.random.default_rng(seed)
+    indx, pb, pe = [], [], []
+    for length in lengths:
+        cols = rng.permutation(n)[:length] if length <= n else rng.integers(0, n, length)
+        if masked and length > 3:
+            cols[rng.integers(0, length)] = rng.choice([-1, n, -(2 ** 31)])
+        pb.append(len(indx))
+        indx.extend(cols.tolist())
+        pe.append(len(indx))
+        indx.append(99)
+    return np.array(indx + [0], np.int64), np.array(pb, np.int64), np.array(pe, np.int64)
+
+
+def check_rows(c, e):
+    inside(c.o.numpy(), e["o"], e["tol"]["o"], "o")
+    assert c.o.untouched_outside()
+
+
+# heads, kv, d, dv, maps: groups that fill 16 columns and that need several passes, odd sizes, every width class
+SHAPES = [(1, 1, 1, 1, 1), (2, 1, 32, 32, 1), (6, 2, 40, 24, 1), (20, 1, 64, 64, 1), (4, 4, 100, 128, 1), (2, 1, 256, 256, 1),
+          (4, 2, 32, 64, 2), (9, 1, 40, 72, 2), (4, 1, 64, 128, 2), (3, 3, 128, 256, 2)]
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("shape", SHAPES, ids=lambda s: "-".join(map(str, s)))
+def test_short_rows(kind, shape):
+    import torch
+    heads, kv, d, dv, maps = shape
+    c = Case(kind, maps, 7, 150, heads, kv, d, dv, *ragged([0, 1, 2, 31, 33, 128, 150], 150, seed=1), seed=2)
+    assert c.rows(nnz=256) == 0      # one piece per row
+    torch.cuda.synchronize()
+    assert c.rows_size == 0
+    check_rows(c, c.exact())
+
+
+@pytest.mark.parametrize("bits", [32, 64])
+@pytest.mark.parametrize("kind,maps", [("f32", 1), ("bf16", 2), ("f16", 1)])
+def test_rows_in_pieces(kind, maps, bits):
+    import torch
+    lengths = [2000, 0, 1, 255, 256, 257, 1025, 3, 2500]
+    c = Case(kind, maps, len(lengths), 2600, 4, 2, 32, 32 * maps, *ragged(lengths, 2600, seed=1), seed=2, bits=bits)
+    assert c.rows() == 0
+    torch.cuda.synchronize()
+    assert c.rows_size > 0
+    e = c.exact()
+    check_rows(c, e)
+    # a bound that is too small chooses longer pieces, or none; a generous one shorter ones
+    for nnz in (1, 300, 10 * c.nnz):
+        assert c.rows(nnz=nnz) == 0
+        torch.cuda.synchronize()
+        check_rows(c, e)
+
+
+@pytest.mark.parametrize("m", [64, 65, 256, 257, 700])
+def test_many_rows(m):
+    """Up to 256 rows every wave finds its piece by itself, beyond that from a table."""
+    import torch
+    rng = np.random.default_rng(m)
+    lengths = rng.integers(0, 12, m)
+    lengths[m // 3], lengths[m - 1] = 900, 700
+    c = Case("f32", 1, m, 1000, 2, 1, 16, 16, *ragged(lengths, 1000, seed=1), seed=2)
+    assert c.rows() == 0
+    torch.cuda.synchronize()
+    assert c.rows_size > 0
+    check_rows(c, c.exact())
+    assert c.rows(nnz=300) == 0      # more pieces than the workspace is sized for at first
+    torch.cuda.synchronize()
+    check_rows(c, c.exact())
+
+
+@pytest.mark.parametrize("how", ["heads", "wide", "odd"])
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_layouts(kind, how):
+    import torch
+    c = Case(kind, 2, 5, 400, 4, 2, 32, 64, *ragged([1, 400, 37, 0, 390], 400, seed=3), seed=4, how=how)
+    assert c.rows() == 0
+    torch.cuda.synchronize()
+    check_rows(c, c.exact())
+
+
+def test_agrees_with_the_planned_form():
+    """The same pattern (empty rows, duplicates, masked ids) through a plan and by rows."""
+    import torch
+    c = Case("f32", 2, 90, 70, 4, 2, 32, 64, *random_pattern(90, 70, 20, seed=3), seed=4)
+    e = c.exact()
+    c.make_plans(False)
+    assert c.forward() == 0
+    torch.cuda.synchronize()
+    inside(c.o.numpy(), e["o"], e["tol"]["o"], "planned")
+    assert c.rows() == 0
+    torch.cuda.synchronize()
+    inside(c.o.numpy(), e["o"], e["tol"]["o"], "rows")
+
+
+@pytest.mark.parametrize("what", [float("inf"), float("nan")])
+def test_values_that_are_not_finite(what):
+    """They reach the rows that name them and no others; slots that nobody names may hold anything."""
+    import torch
+    lengths = [60, 60, 1000, 0]
+    indx, pb, pe = ragged(lengths, 1100, seed=3, masked=False)
+    a, b = [Case("bf16", 1, 4, 1100, 2, 1, 32, 32, indx, pb, pe, seed=2) for _ in range(2)]
+    bad = int(indx[pb[0] + 5])
+    unused = np.setdiff1d(np.arange(1100), np.concatenate([indx[pb[i]:pe[i]] for i in range(4)]))
+    b.v.view()[bad, 0, 3] = what
+    b.v.view()[torch.as_tensor(unused).cuda()] = what
+    b.k.view()[torch.as_tensor(unused).cuda()] = what
+    for c in (a, b):
+        assert c.rows() == 0
+    torch.cuda.synchronize()
+    names = np.array([bad in indx[pb[i]:pe[i]] for i in range(4)])
+    x, y = a.o.numpy(), b.o.numpy()
+    assert np.array_equal(x[~names], y[~names])
+    assert not np.isfinite(y[names][:, :, 3]).any()
+    rest = np.arange(32) != 3
+    assert np.isfinite(y[names][:, :, rest]).all()
+
+
+# ---- the 4-bit cache ---------------------------------------------------------------------------------------------------------------
+
+def cache_of(n, kv, rec, how="slots"):
+    """(buffer, ldc, hdc): slots outermost, or heads outermost with room between the records."""
+    import torch
+    if how == "slots":
+        return torch.full((n * kv * rec,), 0xA5, dtype=torch.uint8, device="cuda"), kv * rec, rec
+    return torch.full((n * kv * (rec + 16),), 0xA5, dtype=torch.uint8, device="cuda"), rec + 16, n * (rec + 16)
+
+
+def records(buf, n, kv, ldc, hdc, rec):
+    return buf.as_strided((n, kv, rec), (ldc, hdc, 1)).cpu().numpy()
+
+
+def special_rows(rng, width, kind):
+    """Rows that quantisation can get wrong: zeros, constants, one sign, ties between codes, tiny and huge, one outlier."""
+    rows = [np.zeros(width), np.full(width, 3.25), np.full(width, -0.5), rng.uniform(1, 2, width), -rng.uniform(1, 2, width),
+            np.resize(np.arange(32) * 0.5 - 4, width), np.resize(np.arange(16) - 7.5, width), rng.standard_normal(width) * 1e-7,
+            rng.standard_normal(width) * 1e-4, rng.standard_normal(width) * 2e4, np.r_[100.0, rng.standard_normal(width - 1)],
+            np.r_[1e30 if kind != "f16" else 6e4, np.zeros(width - 1)], np.resize([2.0 ** -20, -2.0 ** -21], width)]
+    return np.array(rows)
+
+
+@pytest.mark.parametrize("how", ["slots", "heads"])
+@pytest.mark.parametrize("maps,d,dv", [(1, 32, 32), (1, 64, 96), (1, 128, 128), (2, 64, 128), (2, 32, 64), (1, 256, 224)])
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+def test_cache_bytes_and_values(kind, maps, d, dv, how):
+    """Every byte of the records and every value read back, against the format's definition."""
+    import torch
+    rng = np.random.default_rng(d + dv)
+    kv = 2
+    special = special_rows(rng, maps * d, kind)
+    t = len(special) + 9
+    k = rng.standard_normal((t, kv, maps * d))
+    v = rng.standard_normal((t, kv, dv)) * 3
+    k[:len(special), 0], v[:len(special), 1] = special, special_rows(rng, dv, kind)
+    K, V = Tensor(t, kv, maps * d, kind, "wide" if how == "heads" else "packed", k), Tensor(t, kv, dv, kind, "odd" if how == "heads" else "packed", v)
+    n = 2 * t
+    slots = rng.permutation(n)[:t]
+    slots[[1, 4]] = [-1, n]                      # tokens that go nowhere
+    rec = fa.fusedMM_kv4_record_bytes(maps, d, dv)
+    assert rec == -(-((maps * d + dv) * 9 // 16) // 16) * 16
+    cache, ldc, hdc = cache_of(n, kv, rec, how)
+    dsc = desc(kind, maps, 0, n, kv, kv, d, dv, 1.0, None, K, V)
+    s = index_arrays(slots, slots, slots, 32)[0]
+    assert fa.fusedMM_kv4_write(dsc, t, s, K.ptr, V.ptr, cache, ldc, hdc) == 0
+    K2, V2 = Tensor(t, kv, maps * d, kind, "wide" if how == "heads" else "packed"), Tensor(t, kv, dv, kind, "odd" if how == "heads" else "packed")
+    assert fa.fusedMM_kv4_read(dsc, t, s, cache, ldc, hdc, K2.ptr, V2.ptr) == 0
+    torch.cuda.synchronize()
+    got, kn, vn = records(cache, n, kv, ldc, hdc, rec), K.numpy(), V.numpy()
+    used = (maps * d + dv) // 2 + (maps * d + dv) // 16
+    written = set()
+    rt = lambda x: torch.as_tensor(x).to(dtype(kind)).double().numpy()
+    for i in range(t):
+        for h in range(kv):
+            if not 0 <= slots[i] < n:
+                assert (K2.numpy()[i, h] == 0).all() and (V2.numpy()[i, h] == 0).all()
+                continue
+            written.add(slots[i])
+            b, kx, vx = record(kn[i, h], vn[i, h])
+            assert np.array_equal(got[slots[i], h][:used], b[:used]), (i, h)
+            assert (got[slots[i], h][used:] == 0xA5).all()
+            assert np.array_equal(K2.numpy()[i, h], rt(kx)) and np.array_equal(V2.numpy()[i, h], rt(vx)), (i, h)
+    rest = np.setdiff1d(np.arange(n), list(written))
+    assert (got[rest] == 0xA5).all()
+    assert K2.untouched_outside() and V2.untouched_outside()
+
+
+def test_nan_and_infinities_in_the_cache():
+    import torch
+    k = np.zeros((1, 1, 64))
+    k[0, 0, 3], k[0, 0, 40] = np.nan, np.inf
+    K, V = Tensor(1, 1, 64, "bf16", values=k), Tensor(1, 1, 32, "bf16", values=np.ones((1, 1, 32)))
+    dsc = desc("bf16", 1, 0, 2, 1, 1, 64, 32, 1.0)
+    cache, ldc, hdc = cache_of(2, 1, fa.fusedMM_kv4_record_bytes(1, 64, 32))
+    s = index_arrays([1], [0], [0], 64)[0]
+    assert fa.fusedMM_kv4_write(dsc, 1, s, K.ptr, V.ptr, cache, ldc, hdc, index_bits=64) == 0
+    assert fa.fusedMM_kv4_read(dsc, 1, s, cache, ldc, hdc, K.ptr, V.ptr, index_bits=64) == 0
+    torch.cuda.synchronize()
+    got = K.numpy()[0, 0]
+    assert np.isnan(got[:32]).all()
+    want = quantise_row(np.where(np.arange(32) == 8, 32768.0, 0.0))[2]
+    assert np.array_equal(got[32:], torch.as_tensor(want).bfloat16().double().numpy())
+
+
+@pytest.mark.parametrize("t", [3, 40, 5000])
+def test_of_tokens_with_one_slot_the_last_counts(t):
+    import torch
+    rng = np.random.default_rng(t)
+    n = max(2, t // 3)
+    slots = rng.integers(-1, n, t)
+    k, v = rng.standard_normal((t, 1, 32)), rng.standard_normal((t, 1, 32))
+    K, V = Tensor(t, 1, 32, "f16", values=k), Tensor(t, 1, 32, "f16", values=v)
+    cache, ldc, hdc = cache_of(n, 1, 48)
+    dsc = desc("f16", 1, 0, n, 1, 1, 32, 32, 1.0)
+    s = index_arrays(slots, [0], [0], 32)[0]
+    assert fa.fusedMM_kv4_write(dsc, t, s, K.ptr, V.ptr, cache, ldc, hdc) == 0
+    torch.cuda.synchronize()
+    got, kn, vn = records(cache, n, 1, ldc, hdc, 48), K.numpy(), V.numpy()
+    last = {int(c): i for i, c in enumerate(slots) if c >= 0}
+    for c in range(n):
+        if c in last:
+            b = record(kn[last[c], 0], vn[last[c], 0])[0]
+            assert np.array_equal(got[c, 0][:36], b[:36]), c
+        else:
+            assert (got[c] == 0xA5).all()
+
+
+class CacheCase(Case):
+    """A Case whose keys and values live in a 4-bit cache."""
+
+    def __init__(self, *a, how_cache="slots", **kw):
+        super().__init__(*a, **kw)
+        self.rec = fa.fusedMM_kv4_record_bytes(self.maps, self.d, self.dv)
+        self.cache, self.ldc, self.hdc = cache_of(self.n, self.kv, self.rec, how_cache)
+        every = index_arrays(np.arange(self.n), [0], [0], self.bits)[0]
+        kx, vx = self.k.numpy(), self.v.numpy()
+        assert fa.fusedMM_kv4_write(self.desc, self.n, every, self.k.ptr, self.v.ptr, self.cache, self.ldc, self.hdc, index_bits=self.bits) == 0
+        self.k_values = np.array([[quantise_row(kx[i, h])[2] for h in range(self.kv)] for i in range(self.n)])
+        self.v_values = np.array([[quantise_row(vx[i, h])[2] for h in range(self.kv)] for i in range(self.n)])
+
+    def rows_again(self, stream=None, nnz=None):
+        return fa.fusedMM_attn_rows_kv4(self.desc, self.nnz if nnz is None else nnz, *self.index, self.q.ptr, self.cache, self.ldc,
+                                        self.hdc, self.lam, self.o.ptr, self.rows_work, self.rows_size, stream=stream, index_bits=self.bits)
+
+    def exact(self):
+        return super().exact(k=self.k_values, v=self.v_values, weight_type="f16")
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("shape", [(1, 1, 32, 32, 1), (8, 2, 128, 128, 1), (20, 1, 64, 64, 1), (6, 3, 96, 64, 1), (2, 1, 256, 256, 1),
+                                   (4, 2, 32, 64, 2), (9, 1, 64, 128, 2), (4, 4, 96, 160, 2), (2, 1, 128, 256, 2)],
+                         ids=lambda s: "-".join(map(str, s)))
+def test_rows_over_the_cache(kind, shape):
+    import torch
+    heads, kv, d, dv, maps = shape
+    lengths = [0, 1, 33, 128, 300, 2]
+    c = CacheCase(kind, maps, len(lengths), 310, heads, kv, d, dv, *ragged(lengths, 310, seed=1), seed=2, how_cache="heads" if kv > 1 else "slots")
+    e = c.exact()
+    for nnz in (256, c.nnz):                     # whole rows, and pieces
+        assert c.rows(nnz=nnz) == 0
+        torch.cuda.synchronize()
+        check_rows(c, e)
+
+
+def test_queries_beyond_fp16_s_range():
+    """bf16 queries of 1e6 and of 1e-9 against cached keys: the score scale makes up for it."""
+    import torch
+    for spread in (1e6, 1e-9):
+        c = CacheCase("bf16", 1, 3, 200, 2, 1, 64, 64, *ragged([50, 200, 7], 200, seed=1), seed=2, scale=0.125 / spread)
+        c.q.view().copy_((c.q.view().float() * spread).bfloat16())
+        assert c.rows() == 0
+        torch.cuda.synchronize()
+        check_rows(c, c.exact())
+
+
+def test_rows_are_captured_and_replayed():
+    """Rows over a cache, the write of new tokens before them, in one graph; new operands and row lengths for each replay."""
+    import torch
+    lengths = [900, 30, 0, 1500]
+    indx, pb, pe = ragged(lengths, 1600, seed=1, masked=False)
+    c = CacheCase("bf16", 2, 4, 1600, 4, 2, 32, 64, indx, pb, pe, seed=2)
+    e = CacheCase("bf16", 2, 4, 1600, 4, 2, 32, 64, indx, pb, pe, seed=2)
+    new_k, new_v = Tensor(4, 2, 64, "bf16", values=np.zeros((4, 2, 64))), Tensor(4, 2, 64, "bf16", values=np.zeros((4, 2, 64)))
+    slots = index_arrays(indx[pb], [0], [0], 32)[0]
+    slots[2] = -1
+    for x in (c, e):
+        assert x.rows() == 0
+    torch.cuda.synchronize()
+    s, g = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        assert fa.fusedMM_kv4_write(c.desc, 4, slots, new_k.ptr, new_v.ptr, c.cache, c.ldc, c.hdc, stream=s.cuda_stream) == 0
+        assert c.rows_again(stream=s.cuda_stream) == 0
+    other = torch.cuda.Stream()
+    for turn in range(4):
+        for t in (new_k, new_v, c.q):
+            t.view().copy_(torch.randn(t.view().shape, device="cuda"))
+        e.q.view().copy_(c.q.view())
+        shorter = torch.as_tensor(np.maximum(pe - turn * 100, pb)).int().cuda()
+        for x in (c, e):
+            x.index[2].copy_(shorter)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(other):
+            assert fa.fusedMM_kv4_write(e.desc, 4, slots, new_k.ptr, new_v.ptr, e.cache, e.ldc, e.hdc, stream=other.cuda_stream) == 0
+            assert e.rows_again(stream=other.cuda_stream) == 0
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(c.o.buf, e.o.buf) and torch.equal(c.cache, e.cache), turn
+        float(torch.randn(1000, device="cuda").sum())
+
+
+def test_a_prompt_then_steps():
+    """The operators as they are used together: a prompt's attention by a plan, its keys and values into the cache, then
+    single tokens that are written and attend to everything before them."""
+    import torch
+    from attn_reference import attention
+    heads, kv, d, dv, maps, prompt, steps = 4, 2, 64, 128, 2, 70, 3
+    n = prompt + steps
+    rng = np.random.default_rng(5)
+    place = rng.permutation(2 * n)[:n]                                   # the slot of every token
+    indx = np.concatenate([np.arange(i + 1) for i in range(prompt)])
+    pe = np.cumsum(np.arange(1, prompt + 1))
+    c = Case("bf16", maps, prompt, prompt, heads, kv, d, dv, indx, pe - np.arange(1, prompt + 1), pe, seed=7)
+    c.make_plans(False)
+    assert c.forward() == 0
+    rec = fa.fusedMM_kv4_record_bytes(maps, d, dv)
+    cache, ldc, hdc = cache_of(2 * n, kv, rec)
+    c.desc.n = 2 * n
+    assert fa.fusedMM_kv4_write(c.desc, prompt, index_arrays(place[:prompt], [0], [0], 32)[0], c.k.ptr, c.v.ptr, cache, ldc, hdc) == 0
+    torch.cuda.synchronize()
+    c.desc.n = prompt
+    e = c.exact()
+    inside(c.o.numpy(), e["o"], e["tol"]["o"], "prompt")
+    ks, vs = list(c.k.numpy()), list(c.v.numpy())
+    lam = c.lam.double().cpu().numpy()
+    for step in range(steps):
+        at = prompt + step
+        q, k, v = [Tensor(1, h, w, "bf16", values=rng.standard_normal((1, h, w))) for h, w in ((heads, maps * d), (kv, maps * d), (kv, dv))]
+        o = Tensor(1, heads, dv, "bf16")
+        dsc = desc("bf16", maps, 1, 2 * n, heads, kv, d, dv, c.scale, q, k, v, o)
+        assert fa.fusedMM_kv4_write(dsc, 1, index_arrays(place[at:at + 1], [0], [0], 32)[0], k.ptr, v.ptr, cache, ldc, hdc) == 0
+        ix = index_arrays(place[:at + 1], [0], [at + 1], 32)
+        assert fa.fusedMM_attn_rows_kv4(dsc, at + 1, *ix, q.ptr, cache, ldc, hdc, c.lam, o.ptr, None, 0) == 0
+        torch.cuda.synchronize()
+        ks.append(k.numpy()[0])
+        vs.append(v.numpy()[0])
+        kx = np.array([[quantise_row(x)[2] for x in t] for t in ks]).reshape(at + 1, kv, maps, d)
+        vx = np.array([[quantise_row(x)[2] for x in t] for t in vs])
+        e = attention(np.ones((1, at + 1)), q.numpy().reshape(1, heads, maps, d), kx, vx, lam, c.scale, "bf16", weight_type="f16")
+        inside(o.numpy(), e["o"], e["tol"]["o"], "step %d" % step)
+
+
+def test_refusals_on_the_device():
+    import torch
+    c = CacheCase("bf16", 1, 2, 900, 2, 1, 32, 32, *ragged([800, 5], 900, seed=1), seed=2)
+    assert c.rows() == 0 and c.rows_size > 0
+    c.rows_size -= 16
+    assert c.rows_again() == fa.NOT_ENOUGH_MEM
+    c.rows_size += 16
+    host = np.zeros(900 * 48, np.uint8)
+    kept, c.cache = c.cache, host
+    assert c.rows_again() == fa.FAIL
+    c.cache = kept.data_ptr() + 8
+    assert c.rows_again() == fa.FAIL
+    c.cache = kept
+    assert Case.rows_again(c) == 0
+    c.desc.type = fa.TYPE_F32
+    assert c.rows_again() == fa.NO_OPT_IMPL
+    torch.cuda.synchronize()
