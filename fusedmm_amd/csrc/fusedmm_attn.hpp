@@ -66,9 +66,9 @@ inline int width_class(int d, int dv, int maps)
 }
 
 // floats of partial sums that one split unit of one head leaves
-inline int64_t forward_part(int dc, int maps) { return (int64_t)maps * kBlockRows * (dc * maps + 2); }
-inline int64_t dq_part(int dc, int maps) { return (int64_t)kBlockRows * (dc * maps + 1); }
-inline int64_t dkv_part(int dc, int maps) { return (int64_t)kBlockRows * (2 * dc * maps); }
+inline int64_t forward_part(int dc, int maps, int br) { return (int64_t)maps * br * (dc * maps + 2); }
+inline int64_t dq_part(int dc, int maps, int br) { return (int64_t)br * (2 * dc * maps + 2); }
+inline int64_t dkv_part(int dc, int maps, int br) { return (int64_t)br * (2 * dc * maps); }
 
 // one function per (type, kernel) object; dc and maps choose the instance
 int launch_forward_f32(const Params &p, int dc, int maps, hipStream_t s);

@@ -29,7 +29,6 @@ typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
-constexpr int kBlockRows = 64;    // resident rows of a workgroup: 4 waves x 16
 constexpr int kTile = 32;         // gathered rows of a tile
 
 __device__ inline float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -121,7 +120,7 @@ template <int T> __device__ inline u4 load_chunk(const typename Num<T>::E *p, in
    {
 #pragma unroll
       for (int k = 0; k < 4; k++)
-         if (k < valid) r[k] = __builtin_bit_cast(uint32_t, p[k]);
+         if (k < valid) r[k] = __float_as_uint(p[k]);
    }
    return r;
 }
@@ -144,32 +143,80 @@ template <int T> __device__ inline typename Num<T>::TFrag pack_scores(const floa
    return r;
 }
 
-// features 16t .. 16t+15 of the tile's 32 rows, transposed: lane i of group g gets feature 16t + i of rows 4g..4g+3 and
-// 16+4g..16+4g+3.  16-bit: two transposing LDS reads, in which lane i of a group of 16 names the address of four
-// elements of row i / 4 and receives element i of the four rows.  32-bit: eight plain reads.
-template <int T> __device__ inline typename Num<T>::TFrag load_t(const typename Num<T>::E *tile, int stride, int t, int g, int i)
-{
-   typename Num<T>::TFrag r;
-   if constexpr (T == kF32)
+// A tile in LDS: 32 rows of W elements.  A row's 16-byte chunks are stored in an order that depends on the row (chunk ^
+// twist(row)): the 16 rows that a matrix operand reads at one chunk, and the 16 that a transposing read touches, then
+// lie in different banks, without padding - loads that go straight to LDS leave no room for any.
+template <int T, int W> struct TileView {
+   typedef typename Num<T>::E E;
+   static constexpr int EPL = Num<T>::EPL;
+   static constexpr int RB = W * (int)sizeof(E);       // bytes of a row
+   static constexpr int CR = RB / 16;                  // chunks of a row
+   static constexpr int kBytes = kTile * RB;
+   static constexpr int kTwistRows = CR >= 16 ? 1 : 16 / CR;
+   static constexpr int kTwistMask = CR >= 16 ? 15 : CR - 1;
+   static __device__ inline int twist(int row) { return (row / kTwistRows) & kTwistMask; }
+
+   // Where this lane's reads of a tile start.  The chunk number enters by exclusive or, which leaves one address for every
+   // chunk; the compiler would keep them all in registers over the loop, so the starts are hidden from it for each tile
+   // and the addresses are formed again, one operation each.
+   struct Lane {
+      int direct;
+      int transposed[T == kF32 ? 4 : 1];
+   };
+   static __device__ inline Lane lane(int g, int i)
    {
+      Lane l;
+      l.direct = i * RB + (g ^ twist(i)) * 16;
+      if constexpr (T == kF32)
+      {
 #pragma unroll
-      for (int j = 0; j < 8; j++) r[j] = tile[(16 * (j / 4) + 4 * g + j % 4) * stride + 16 * t + i];
+         for (int r = 0; r < 4; r++) l.transposed[r] = (4 * g + r) * RB + (((i / 4) ^ twist(4 * g + r)) * 16) + (i % 4) * 4;
+      }
+      else l.transposed[0] = (4 * g + i / 4) * RB + ((((i % 4) / 2) ^ twist(4 * g + i / 4)) * 16) + (i % 2) * 8;
+      asm volatile("" : "+v"(l.direct));
+#pragma unroll
+      for (int r = 0; r < (T == kF32 ? 4 : 1); r++) asm volatile("" : "+v"(l.transposed[r]));
+      return l;
    }
-   else
+
+   // chunk (a multiple of 4) + g of row i: the 16 bytes of a first operand; a is 0 or 1: rows 16a + i
+   static __device__ inline u4 direct(const unsigned char *tile, int chunk, int a, const Lane &l)
    {
-      typedef __attribute__((address_space(3))) s4 lds_s4;
-      const uint16_t *p = tile + (4 * g + i / 4) * stride + 16 * t + (i % 4) * 4;
-      const s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)p);
-      const s4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(p + 16 * stride));
-      r = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+      return *reinterpret_cast<const u4 *>(tile + (l.direct ^ (chunk * 16)) + 16 * a * RB);
    }
-   return r;
-}
+
+   // features 16t .. 16t+15 of the 32 rows, transposed: lane i of group g gets feature 16t + i of rows 4g..4g+3 and
+   // 16+4g..16+4g+3 (which have the same twist).  16-bit: two transposing LDS reads, in which lane i of a group of 16 names
+   // the address of four elements of row i / 4 and receives element i of the four rows.  32-bit: eight plain reads.
+   static __device__ inline typename Num<T>::TFrag transposed(const unsigned char *tile, int t, const Lane &l)
+   {
+      typename Num<T>::TFrag r;
+      if constexpr (T == kF32)
+      {
+#pragma unroll
+         for (int j = 0; j < 8; j++) r[j] = *reinterpret_cast<const float *>(tile + (l.transposed[j % 4] ^ (4 * t * 16)) + 16 * (j / 4) * RB);
+      }
+      else
+      {
+         typedef __attribute__((address_space(3))) s4 lds_s4;
+         const unsigned char *p = tile + (l.transposed[0] ^ (2 * t * 16));
+         const s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)p);
+         const s4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(p + 16 * RB));
+         r = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+      }
+      return r;
+   }
+
+   static __device__ inline E element(const unsigned char *tile, int row, int f)
+   {
+      return *reinterpret_cast<const E *>(tile + row * RB + (((f / EPL) ^ twist(row)) * 16) + (f % EPL) * (int)sizeof(E));
+   }
+};
 
 // an infinity or a NaN
 template <int T> __device__ inline bool odd_element(typename Num<T>::E x)
 {
-   if constexpr (T == kF32) return Num<T>::odd_word(__builtin_bit_cast(uint32_t, x));
+   if constexpr (T == kF32) return Num<T>::odd_word(__float_as_uint(x));
    else return Num<T>::odd_word(x);
 }
 
@@ -188,8 +235,8 @@ template <int T> __device__ inline typename Num<T>::TFrag without_odd(typename N
 // name them, so it runs without them (without_odd) and every row adds those of the gathered rows that it does name.
 // Rows that name none keep the bits they have without them.
 // mine: bit 4a + r says that gathered row 16a + 4g + r is named by this lane's resident row.
-template <int T, int NT> __device__ inline void add_odd(f4 (&acc)[NT], const float (&p)[2][4], unsigned mine,
-                                                        const typename Num<T>::E *tile, int stride, int g, int i)
+template <int T, int W, int NT>
+__device__ inline void add_odd(f4 (&acc)[NT], const float (&p)[2][4], unsigned mine, const unsigned char *tile, int f0, int g, int i)
 {
    for (int key = 0; key < kTile; key++)
    {
@@ -206,26 +253,27 @@ template <int T, int NT> __device__ inline void add_odd(f4 (&acc)[NT], const flo
 #pragma unroll
          for (int k = 0; k < 4; k++)
          {
-            const typename Num<T>::E e = tile[key * stride + 16 * t + 4 * g + k];
+            const typename Num<T>::E e = TileView<T, W>::element(tile, key, f0 + 16 * t + 4 * g + k);
             if (odd_element<T>(e)) acc[t][k] = fmaf(w, Num<T>::to(e), acc[t][k]);
          }
    }
 }
 
-// acc += (weights of the tile's 32 rows) x (their features); odd: the tile holds infinities or NaN
-template <int T, int NT> __device__ inline void add_weighted(f4 (&acc)[NT], const float (&p)[2][4], unsigned mine,
-                                                             const typename Num<T>::E *tile, int stride, int g, int i, bool odd)
+// acc += (weights of the tile's 32 rows) x (their features f0 .. f0 + 16 NT - 1); odd: the tile may hold infinities or NaN
+template <int T, int W, int NT>
+__device__ inline void add_weighted(f4 (&acc)[NT], const float (&p)[2][4], unsigned mine, const unsigned char *tile, int f0, int g, int i, const typename TileView<T, W>::Lane &l, bool odd)
 {
+   typedef TileView<T, W> V;
    const typename Num<T>::TFrag b = pack_scores<T>(p);
    if (__builtin_expect(odd, 0))
    {
 #pragma unroll
-      for (int t = 0; t < NT; t++) acc[t] = Num<T>::mma_t(without_odd<T>(load_t<T>(tile, stride, t, g, i)), b, acc[t]);
-      add_odd<T, NT>(acc, p, mine, tile, stride, g, i);
+      for (int t = 0; t < NT; t++) acc[t] = Num<T>::mma_t(without_odd<T>(V::transposed(tile, f0 / 16 + t, l)), b, acc[t]);
+      add_odd<T, W, NT>(acc, p, mine, tile, f0, g, i);
       return;
    }
 #pragma unroll
-   for (int t = 0; t < NT; t++) acc[t] = Num<T>::mma_t(load_t<T>(tile, stride, t, g, i), b, acc[t]);
+   for (int t = 0; t < NT; t++) acc[t] = Num<T>::mma_t(V::transposed(tile, f0 / 16 + t, l), b, acc[t]);
 }
 
 // four consecutive features of an output row, f .. f+3 of `width`

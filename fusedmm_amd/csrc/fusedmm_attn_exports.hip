@@ -112,8 +112,8 @@ int check_plans(const char *who, const Desc &d, const void *plan, const void *pl
    if (p->rows != d.m || p->cols != d.n) return refuse(who, "the plan is of a pattern of another size");
    if (t && (t->rows != d.n || t->cols != d.m)) return refuse(who, "the second plan is not of the transposed pattern's size");
    if (t && t->device != p->device) return refuse(who, "the plans belong to different devices");
-   if ((int64_t)p->view.n_units * d.heads > kMaxGrid || (int64_t)p->view.n_joins * d.heads * (kBlockRows / 4) > kMaxGrid || d.m * d.heads > kMaxGrid ||
-       (t && ((int64_t)t->view.n_units * d.kv_heads > kMaxGrid || (int64_t)t->view.n_joins * d.kv_heads * (kBlockRows / 4) > kMaxGrid)))
+   if ((int64_t)p->view.n_units * d.heads > kMaxGrid || (int64_t)p->view.n_joins * d.heads * (p->view.block_rows / 4) > kMaxGrid || d.m * d.heads > kMaxGrid ||
+       (t && ((int64_t)t->view.n_units * d.kv_heads > kMaxGrid || (int64_t)t->view.n_joins * d.kv_heads * (t->view.block_rows / 4) > kMaxGrid || t->tiles * (d.heads / d.kv_heads) > INT32_MAX)))
       return refuse(who, "too many rows and heads for one call");
    return kOk;
 }
@@ -132,7 +132,7 @@ struct Layout {   // of a workspace, in bytes
 Layout forward_layout(const Desc &d, const Plan &p, int dc)
 {
    Layout l;
-   l.total = p.parts * d.heads * forward_part(dc, d.maps) * 4;
+   l.total = p.parts * d.heads * forward_part(dc, d.maps, p.view.block_rows) * 4;
    return l;
 }
 
@@ -141,7 +141,7 @@ Layout backward_layout(const Desc &d, const Plan &p, const Plan &t, int dc)
    Layout l;
    l.dlam = align256(d.m * d.heads * d.maps * 4);
    l.part = l.dlam + (d.maps == 2 ? align256(d.m * d.heads * 4) : 0);
-   l.total = l.part + std::max(p.parts * d.heads * dq_part(dc, d.maps), t.parts * d.kv_heads * dkv_part(dc, d.maps)) * 4;
+   l.total = l.part + std::max(p.parts * d.heads * dq_part(dc, d.maps, p.view.block_rows), t.parts * d.kv_heads * dkv_part(dc, d.maps, t.view.block_rows)) * 4;
    return l;
 }
 

@@ -1,17 +1,21 @@
 // Kernels of attention over a planned pattern: forward, delta, the two backward passes, and the joins of split blocks.
 //
-// A plan (fusedmm_attn_plan.hip) lists, for every block of 64 rows, the columns that any of them names, with one bit per
-// row.  A unit is a run of such columns of one block; a block whose rows are long is several units, whose partial sums
-// the join kernels add in order.  A workgroup does one unit for one head: 4 waves of 16 resident rows share the tiles of
-// 32 gathered rows.  What the block size gives: a gathered row is loaded once for 64 rows instead of once for each that
-// names it, and one 16 x 16 product serves 16 rows; a tile that no row of a wave names is skipped by that wave.
+// A plan (fusedmm_attn_plan.hip) lists, for every block of BR = 64 or 16 rows, the columns that any of them names, with
+// one bit per row.  A unit is a run of such columns of one block; a block whose rows are long is several units, whose
+// partial sums the join kernels add in order.  A workgroup does one unit for one head: BR / 16 waves of 16 resident rows
+// share the tiles of 32 gathered rows, and one 16 x 16 product serves 16 rows.  With BR = 64 a gathered row is loaded once
+// for 64 rows (a tile that no row of a wave names is skipped by that wave); with BR = 16 nothing is shared but nothing
+// is multiplied for the rows of other waves either, which is what rows without common neighbours want.
+//
+// The tiles go from memory straight into LDS (no registers in between), S of them in flight: a gather has several tiles'
+// worth of products to arrive in.  Column ids and masks run ahead of them the same way, in groups of 8 tiles.
 #pragma once
 #include "fusedmm_attn_core.h"
 
 namespace fmm_attn {
 
 struct Unit {
-   int32_t block;     // rows 64 * block ...
+   int32_t block;     // rows BR * block ...
    int32_t part;      // slot of its partial sums, -1: the block's only unit
    int32_t tile0;     // first tile of its columns
    int32_t tiles;
@@ -20,13 +24,16 @@ struct Join {         // a block of several units: partial sums part0 .. part0 +
    int32_t block, part0, parts, pad;
 };
 
+constexpr int kAhead = 8;   // tiles of a group of column ids and masks; the arrays of a plan are padded by a group
+
 struct PlanView {
-   const int32_t *cols;    // [tiles * 32], -1: no column
-   const uint16_t *masks;  // [tiles][4 waves][32]: bit r is row 16 * wave + r of the block
+   const int32_t *cols;    // [tiles][32], -1: no column
+   const uint16_t *masks;  // [tiles][BR / 16 waves][32]: bit r is row 16 * wave + r of the block
    const Unit *units;
    const Join *joins;
    int32_t n_units, n_joins;
    int64_t rows, cols_n;
+   int32_t block_rows;     // BR
 };
 
 struct Params {
@@ -48,71 +55,156 @@ struct Params {
    float *part;                       // partial sums of split blocks
 };
 
-template <int T, int DC, int MAPS> struct Geo {
+__device__ u4 zero_chunk;   // what lanes without a column or a feature load
+
+template <int T, int DC, int MAPS, int BR> struct Geo {
    typedef Num<T> N;
    typedef typename N::E E;
    static constexpr int W = DC * MAPS;                // padded width of a gathered row: all maps of q or k; v and do
-   static constexpr int LD = W + N::EPL;              // of a tile row in LDS: 16 bytes more, so that rows start in other banks
-   static constexpr int CR = W / N::EPL;              // 16-byte chunks of a row
-   static constexpr int NCH = (kTile * CR + 255) / 256;   // chunks a thread stages
-   static constexpr int CQ = DC / N::KC;              // chunks of a product over one map's features
+   typedef TileView<T, W> V;
+   static constexpr int CR = V::CR;
+   static constexpr int THREADS = BR * 4, WAVES = BR / 16;
+   static constexpr int NCH = (kTile * CR + THREADS - 1) / THREADS;   // chunks a thread loads of one tensor's tile
+   static constexpr int CQ = DC / N::KC;              // chunk groups of a product over one map's features
    static constexpr int CV = W / N::KC;
+   static constexpr int MC = DC / N::EPL;             // chunks of one map
    static constexpr int NT = W / 16, NTQ = DC / 16;   // 16-feature tiles of v's and of one map's accumulators
-   static constexpr bool kWide = W * sizeof(E) >= 512;
-   static constexpr bool kIdle = kTile * CR < 256;    // the tile has fewer chunks than the workgroup threads
+   // Tiles in flight and being used.  Two tensors' tiles are 4 ... 64 KB; 4 deep as long as two workgroups of four waves
+   // (six of one wave) fit a compute unit's 160 KB.
+   static constexpr int kPair = 2 * V::kBytes;
+   static constexpr int S = BR == 64 ? (kPair <= 16384 ? 4 : 2) : (kPair <= 4096 ? 4 : kPair <= 8192 ? 3 : 2);
+   static constexpr int kMaskBytes = WAVES * kTile * 2;    // of a tile
+   static constexpr int kStat = 2 * MAPS * kTile * 4;      // lse and delta of a tile's rows (dk, dv)
 };
 
-// ---- staging: 32 gathered rows of two tensors, global -> registers -> LDS ----------------------------------------------------
+template <int N> __device__ inline void wait_loads()   // all but the N newest loads have arrived, LDS operations are done
+{
+   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
+}
+template <int BR> __device__ inline void tile_barrier()
+{
+   if constexpr (BR > 16) asm volatile("s_barrier" ::: "memory");
+}
 
-template <class G> struct Stage {
-   u4 a[G::NCH], b[G::NCH];
+// 16 (4) bytes per lane, memory -> LDS at base + 16 (4) * lane.  The address registers are read when the load issues, it
+// writes no register, and the waits are wait_loads(): the compiler's own waits for its own loads count these as later
+// or earlier ones and only get stricter.
+__device__ inline void load_lds16(uint32_t base, const void *from)
+{
+   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(base), "v"(from) : "memory");
+}
+__device__ inline void load_lds4(uint32_t base, const void *from)
+{
+   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(base), "v"(from) : "memory");
+}
+__device__ inline uint32_t lds_address(const void *p)
+{
+   return __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void *)p);
+}
+
+// ---- the stream of tiles ------------------------------------------------------------------------------------------------------------
+
+template <class G, int T, int DC, int BR> struct Stream {
+   typedef typename G::E E;
+   typedef typename G::V V;
+   const unsigned char *tiles;   // LDS: [S][a, b] tiles
+   unsigned char *ids, *bits;    // LDS: two groups of column ids, of masks
+   const int32_t *cols;          // of the unit
+   const uint16_t *masks;
+   int tid, wave;
+   const E *a, *b;
+   int64_t lda, ldb;
+   int d, dv;
+   bool vec;
+
+   // a: rows of maps pieces of d features each; b: rows of dv features
+   __device__ inline void set(const unsigned char *t, unsigned char *i, unsigned char *m, const PlanView &plan, const Unit &u, const E *a_, int64_t lda_, int d_,
+                              const E *b_, int64_t ldb_, int dv_, bool vec_)
+   {
+      tiles = t;
+      ids = i;
+      bits = m;
+      cols = plan.cols + (int64_t)u.tile0 * kTile;
+      masks = plan.masks + (int64_t)u.tile0 * (G::WAVES * kTile);
+      tid = threadIdx.x;
+      wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+      a = a_;
+      b = b_;
+      lda = lda_;
+      ldb = ldb_;
+      d = d_;
+      dv = dv_;
+      vec = vec_;
+   }
+
+   // column ids and masks of tiles 8 g .. 8 g + 7; waves 0 and 1 (the ones that always load tiles) do it
+   __device__ inline void load_ids(int g) const
+   {
+      const uint32_t to_ids = lds_address(ids + (g & 1) * (kAhead * kTile * 4)), to_bits = lds_address(bits + (g & 1) * (kAhead * G::kMaskBytes));
+      const unsigned char *from = (const unsigned char *)masks + (int64_t)g * (kAhead * G::kMaskBytes);
+      const int lane = tid & 63;
+      if (wave == 0) load_lds16(to_ids, (const unsigned char *)cols + (int64_t)g * (kAhead * kTile * 4) + lane * 16);
+      if constexpr (BR == 64)
+      {
+         if (wave < 2) load_lds16(to_bits + 1024 * wave, from + 1024 * wave + lane * 16);
+      }
+      else
+      {
+         if (lane < kAhead * G::kMaskBytes / 16) load_lds16(to_bits, from + lane * 16);
+      }
+   }
+
+   __device__ inline const int32_t *tile_ids(int t) const
+   {
+      return (const int32_t *)(ids + ((t / kAhead) & 1) * (kAhead * kTile * 4) + (t % kAhead) * (kTile * 4));
+   }
+   // this lane's bits: bit 4a + r for gathered row 16a + 4g + r and resident row i; named: of any lane of the wave
+   __device__ inline unsigned my_bits(int t, int g, int i, bool *named) const
+   {
+      const uint16_t *m = (const uint16_t *)(bits + ((t / kAhead) & 1) * (kAhead * G::kMaskBytes) + (t % kAhead) * G::kMaskBytes) + wave * kTile + 4 * g;
+      const uint64_t m0 = *(const uint64_t *)m, m1 = *(const uint64_t *)(m + 16);
+      *named = __any((m0 | m1) != 0);
+      unsigned b = 0;
+#pragma unroll
+      for (int r = 0; r < 4; r++)
+      {
+         b |= ((unsigned)(m0 >> (16 * r)) >> i & 1) << r;
+         b |= ((unsigned)(m1 >> (16 * r)) >> i & 1) << (4 + r);
+      }
+      return b;
+   }
+
+   // tile t -> buffer; a and b may be moved (other heads) between calls
+   __device__ inline void load_tile(int t, int buf, const E *pa, const E *pb) const
+   {
+      const int32_t *c = tile_ids(t);
+      const unsigned char *ta = tiles + buf * G::kPair, *tb = ta + V::kBytes;
+      const uint32_t la = lds_address(ta) + wave * 1024, lb = lds_address(tb) + wave * 1024;
+      int me = tid;
+      asm volatile("" : "+v"(me));   // the places below are formed again for every tile, not kept in registers over the loop
+#pragma unroll
+      for (int j = 0; j < G::NCH; j++)
+      {
+         const int x = me + G::THREADS * j, r = x / G::CR;
+         if (kTile * G::CR < G::THREADS && x >= kTile * G::CR) break;
+         const int32_t col = c[r];
+         const int e = ((x % G::CR) ^ V::twist(r)) * G::N::EPL, f = e % DC;   // this thread's chunk of a gathered row
+         const E *fa = pa + (int64_t)col * lda + (e / DC * d + f), *fb = pb + (int64_t)col * ldb + e;
+         const bool live_a = col >= 0 && f < d, live_b = col >= 0 && e < dv;
+         if (vec)
+         {
+            load_lds16(la + j * (G::THREADS * 16), live_a ? (const void *)fa : (const void *)&zero_chunk);
+            load_lds16(lb + j * (G::THREADS * 16), live_b ? (const void *)fb : (const void *)&zero_chunk);
+         }
+         else
+         {
+            // rows at any place, ends of rows within a chunk: element by element through registers
+            *(u4 *)(ta + x * 16) = load_chunk<T>(fa, live_a ? (d - f < G::N::EPL ? d - f : G::N::EPL) : 0, false);
+            *(u4 *)(tb + x * 16) = load_chunk<T>(fb, live_b ? (dv - e < G::N::EPL ? dv - e : G::N::EPL) : 0, false);
+         }
+      }
+   }
 };
-
-template <class G> __device__ inline void stage_cols(int32_t (&c)[G::NCH], const int32_t *cols, int tid)
-{
-#pragma unroll
-   for (int j = 0; j < G::NCH; j++)
-   {
-      const int q = tid + 256 * j;
-      c[j] = (!G::kIdle || q < kTile * G::CR) ? cols[q / G::CR] : -1;
-   }
-}
-
-// a: rows of `maps` pieces of d features each; b: rows of dv features
-template <class G, int T, int DC>
-__device__ inline void stage_load(Stage<G> &s, const int32_t (&c)[G::NCH], const typename G::E *a, int64_t lda, int d,
-                                  const typename G::E *b, int64_t ldb, int dv, bool vec, int tid)
-{
-#pragma unroll
-   for (int j = 0; j < G::NCH; j++)
-   {
-      const int e = ((tid + 256 * j) % G::CR) * G::N::EPL;
-      const int mp = e / DC, f = e - mp * DC;
-      const bool live = c[j] >= 0;
-      const int64_t row = live ? c[j] : 0;
-      s.a[j] = load_chunk<T>(a + row * lda + mp * d + f, live ? (d - f < G::N::EPL ? d - f : G::N::EPL) : 0, vec);
-      s.b[j] = load_chunk<T>(b + row * ldb + e, live ? (dv - e < G::N::EPL ? dv - e : G::N::EPL) : 0, vec);
-   }
-}
-
-// returns bit 0 / 1: an infinity or NaN among this thread's chunks of a / b
-template <class G, int T>
-__device__ inline int stage_store(const Stage<G> &s, typename G::E *a, typename G::E *b, int tid, bool look_a, bool look_b)
-{
-   int odd = 0;
-#pragma unroll
-   for (int j = 0; j < G::NCH; j++)
-   {
-      const int q = tid + 256 * j;
-      if (G::kIdle && q >= kTile * G::CR) break;
-      const int off = (q / G::CR) * G::LD + (q % G::CR) * G::N::EPL;
-      *reinterpret_cast<u4 *>(a + off) = s.a[j];
-      *reinterpret_cast<u4 *>(b + off) = s.b[j];
-      if (look_a && odd_chunk<T>(s.a[j])) odd |= 1;
-      if (look_b && odd_chunk<T>(s.b[j])) odd |= 2;
-   }
-   return odd;
-}
 
 // the resident rows of a wave as the second operand: lane i holds its 16 bytes of every chunk of row i
 template <int T, int CQ> __device__ inline void load_resident(u4 (&r)[CQ], const typename Num<T>::E *row, bool live, int d, int g, bool vec)
@@ -125,169 +217,180 @@ template <int T, int CQ> __device__ inline void load_resident(u4 (&r)[CQ], const
    }
 }
 
-// scores of the tile's 32 rows against the resident rows: s[a] rows 16a + 4g + r
-template <int T, int CQ>
-__device__ inline void tile_scores(f4 (&s)[2], const typename Num<T>::E *tile, int ld, const u4 (&res)[CQ], int g, int i)
+// scores of the tile's 32 rows, from chunk `chunk` on, against the resident rows: s[a] rows 16a + 4g + r
+template <int T, int W, int CQ> __device__ inline void tile_scores(f4 (&s)[2], const unsigned char *tile, int chunk, const u4 (&res)[CQ], const typename TileView<T, W>::Lane &l)
 {
+   typedef TileView<T, W> V;
    s[0] = f4{0, 0, 0, 0};
    s[1] = f4{0, 0, 0, 0};
 #pragma unroll
    for (int c = 0; c < CQ; c++)
    {
-      const int f = c * Num<T>::KC + g * Num<T>::EPL;
-      s[0] = Num<T>::mma(*reinterpret_cast<const u4 *>(tile + i * ld + f), res[c], s[0]);
-      s[1] = Num<T>::mma(*reinterpret_cast<const u4 *>(tile + (16 + i) * ld + f), res[c], s[1]);
+      s[0] = Num<T>::mma(V::direct(tile, chunk + 4 * c, 0, l), res[c], s[0]);
+      s[1] = Num<T>::mma(V::direct(tile, chunk + 4 * c, 1, l), res[c], s[1]);
    }
 }
 
-// this lane's bits of a tile's masks: bit 4a + r for gathered row 16a + 4g + r and resident row i
-__device__ inline unsigned my_bits(uint64_t m0, uint64_t m1, int i)
+// Sums that are not finite may be the matrix instructions' zero times infinity: the workgroup then runs its unit again
+// with add_odd.  Finite sums cannot be wrong in that way.
+template <int BR> __device__ inline bool any_odd(bool odd)
 {
-   unsigned b = 0;
-#pragma unroll
-   for (int r = 0; r < 4; r++)
-   {
-      b |= (unsigned)((m0 >> (16 * r + i)) & 1) << r;
-      b |= (unsigned)((m1 >> (16 * r + i)) & 1) << (4 + r);
-   }
-   return b;
+   if constexpr (BR == 16) return __any(odd);
+   else return __syncthreads_or(odd);
 }
+template <int NT> __device__ inline bool odd_sums(const f4 (&acc)[NT])
+{
+   bool odd = false;
+#pragma unroll
+   for (int t = 0; t < NT; t++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) odd |= !(fabsf(acc[t][e]) < INFINITY);
+   return odd;
+}
+
+// The loop over a unit's tiles that all kernels share: fill the pipeline, then for every step wait, free the oldest
+// buffer, fill it, and use the current one.  steps = tiles * per_tile; load(step, buffer), use(step, buffer).
+template <class G, int BR, class S, class Load, class Use> __device__ inline void for_tiles(const S &st, int steps, int per_tile, Load load, Use use)
+{
+   if (steps > 0)
+   {
+      st.load_ids(0);
+      wait_loads<0>();
+      tile_barrier<BR>();
+   }
+#pragma unroll
+   for (int s = 0; s < G::S - 1; s++)
+      if (s < steps) load(s, s);
+   int buf = 0;
+   for (int s = 0; s < steps; s++)
+   {
+      // the loads of later steps may still be under way; at the end of the unit there are fewer, and all are waited for
+      if (st.vec && s + G::S - 2 < steps) wait_loads<(G::S - 2) * 2 * G::NCH>();
+      else wait_loads<0>();
+      tile_barrier<BR>();
+      // The ids of the next group are asked for one group ahead: the loads of any tile that a wave waits for before it uses
+      // them were issued later (2 S - 2 <= 8 tiles).
+      const int group = s / (kAhead * per_tile) + 1;
+      if (s % (kAhead * per_tile) == 0 && group * (kAhead * per_tile) < steps) st.load_ids(group);
+      if (s + G::S - 1 < steps) load(s + G::S - 1, buf == 0 ? G::S - 1 : buf - 1);
+      use(s, buf);
+      buf = buf == G::S - 1 ? 0 : buf + 1;
+   }
+   wait_loads<0>();   // nothing is under way into LDS when it is used again
+   tile_barrier<BR>();
+}
+
+#define ATTN_LDS(EXTRA)                                                                                                                        \
+   __shared__ __align__(1024) unsigned char lds[G::S * G::kPair + 2 * kAhead * kTile * 4 + 2 * kAhead * G::kMaskBytes + G::S * (EXTRA)];          \
+   unsigned char *lds_ids = lds + G::S * G::kPair, *lds_bits = lds_ids + 2 * kAhead * kTile * 4;                                                   \
+   [[maybe_unused]] unsigned char *lds_extra = lds_bits + 2 * kAhead * G::kMaskBytes;
 
 // ---- forward ----------------------------------------------------------------------------------------------------------------------
 // One pass over a unit's columns with a running maximum and sum of every row and map.  Scores are kept times log2(e).
-template <int T, int DC, int MAPS>
-__global__ __launch_bounds__(256, (Geo<T, DC, MAPS>::kWide && (T == kF32 || MAPS == 2) ? 1 : 2)) void attn_forward(Params p)
+template <int T, int DC, int MAPS, int BR> __global__ __launch_bounds__(BR * 4, (DC * MAPS >= 256 ? 1 : 2)) void attn_forward(Params p)
 {
-   typedef Geo<T, DC, MAPS> G;
+   typedef Geo<T, DC, MAPS, BR> G;
    typedef typename G::E E;
-   __shared__ __align__(16) E ks[2][kTile * G::LD];
-   __shared__ __align__(16) E vs[2][kTile * G::LD];
-   __shared__ int odd[2];
+   ATTN_LDS(0)
    const int64_t item = xcd_item(blockIdx.x, (int64_t)p.plan.n_units * p.heads);
    if (item >= (int64_t)p.plan.n_units * p.heads) return;
    const int head = (int)(item / p.plan.n_units);
    const Unit u = p.plan.units[item % p.plan.n_units];
    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, g = lane >> 4, i = lane & 15;
    const int kvh = head / p.group;
-   const E *k = (const E *)p.k + kvh * p.hdk, *v = (const E *)p.v + kvh * p.hdv;
-   const int64_t row = (int64_t)u.block * kBlockRows + 16 * wave + i;
+   const int64_t row = (int64_t)u.block * BR + 16 * wave + i;
    const bool live = row < p.m;
-   if (tid < 2) odd[tid] = 0;
+   Stream<G, T, DC, BR> st;
+   st.set(lds, lds_ids, lds_bits, p.plan, u, (const E *)p.k + kvh * p.hdk, p.ldk, p.d, (const E *)p.v + kvh * p.hdv, p.ldv, p.dv, p.vec);
 
    u4 qr[MAPS][G::CQ];
 #pragma unroll
    for (int mp = 0; mp < MAPS; mp++)
       load_resident<T, G::CQ>(qr[mp], (const E *)p.q + (live ? row : 0) * p.ldq + head * p.hdq + mp * p.d, live, p.d, g, p.vec);
-
+   const float c2 = p.scale * kLog2e;
    f4 acc[MAPS][G::NT];
    float top[MAPS], sum[MAPS];
+   for (int careful = 0; careful < 2; careful++)
+   {
 #pragma unroll
-   for (int mp = 0; mp < MAPS; mp++)
-   {
-      top[mp] = -INFINITY;
-      sum[mp] = 0;
-#pragma unroll
-      for (int t = 0; t < G::NT; t++) acc[mp][t] = f4{0, 0, 0, 0};
-   }
-   const float c2 = p.scale * kLog2e;
-
-   const int32_t *cols = p.plan.cols + (int64_t)u.tile0 * kTile;
-   const uint16_t *masks = p.plan.masks + (int64_t)u.tile0 * (4 * kTile) + wave * kTile + 4 * g;
-   int32_t cn[G::NCH];
-   Stage<G> st;
-   uint64_t m0 = 0, m1 = 0;
-   if (u.tiles > 0)
-   {
-      stage_cols<G>(cn, cols, tid);
-      stage_load<G, T, DC>(st, cn, k, p.ldk, p.d, v, p.ldv, p.dv, p.vec, tid);
-      m0 = *(const uint64_t *)masks;
-      m1 = *(const uint64_t *)(masks + 16);
-      if (u.tiles > 1) stage_cols<G>(cn, cols + kTile, tid);
-      __syncthreads();   // the flags are clear
-      if (stage_store<G, T>(st, ks[0], vs[0], tid, false, true)) odd[0] = 1;
-   }
-   __syncthreads();
-   for (int t = 0; t < u.tiles; t++)
-   {
-      const int b = t & 1;
-      const uint64_t n0 = m0, n1 = m1;
-      if (t + 1 < u.tiles)
+      for (int mp = 0; mp < MAPS; mp++)
       {
-         stage_load<G, T, DC>(st, cn, k, p.ldk, p.d, v, p.ldv, p.dv, p.vec, tid);
-         m0 = *(const uint64_t *)(masks + (int64_t)(t + 1) * (4 * kTile));
-         m1 = *(const uint64_t *)(masks + (int64_t)(t + 1) * (4 * kTile) + 16);
-         if (t + 2 < u.tiles) stage_cols<G>(cn, cols + (int64_t)(t + 2) * kTile, tid);
+         top[mp] = -INFINITY;
+         sum[mp] = 0;
+#pragma unroll
+         for (int t = 0; t < G::NT; t++) acc[mp][t] = f4{0, 0, 0, 0};
       }
-      if (__any((n0 | n1) != 0))
-      {
-         const unsigned mine = my_bits(n0, n1, i);
-         float w[MAPS][2][4];
+      for_tiles<G, BR>(
+         st, u.tiles, 1, [&](int t, int buf) { st.load_tile(t, buf, st.a, st.b); },
+         [&](int t, int buf) {
+            bool named;
+            const unsigned mine = st.my_bits(t, g, i, &named);
+            if (!named) return;
+            const typename G::V::Lane l = G::V::lane(g, i);
+            const unsigned char *ks = lds + buf * G::kPair, *vs = ks + G::V::kBytes;
+            float w[MAPS][2][4];
 #pragma unroll
-         for (int mp = 0; mp < MAPS; mp++)
-         {
-            f4 s[2];
-            tile_scores<T, G::CQ>(s, ks[b] + mp * DC, G::LD, qr[mp], g, i);
-            float mx = -INFINITY;
-#pragma unroll
-            for (int j = 0; j < 8; j++)
+            for (int mp = 0; mp < MAPS; mp++)
             {
-               w[mp][j / 4][j % 4] = ((mine >> j) & 1) ? s[j / 4][j % 4] * c2 : -INFINITY;
-               mx = fmaxf(mx, w[mp][j / 4][j % 4]);
-            }
-            mx = fmaxf(top[mp], group_max(mx));
-            const float base = mx == -INFINITY ? 0.0f : mx;   // nothing named so far: every weight below is exp2(-inf)
-            const float keep = exp2_fast(top[mp] - base);
-            float add = 0;
+               f4 s[2];
+               tile_scores<T, G::W, G::CQ>(s, ks, mp * G::MC, qr[mp], l);
+               float mx = -INFINITY;
 #pragma unroll
-            for (int j = 0; j < 8; j++)
+               for (int j = 0; j < 8; j++)
+               {
+                  w[mp][j / 4][j % 4] = ((mine >> j) & 1) ? s[j / 4][j % 4] * c2 : -INFINITY;
+                  mx = fmaxf(mx, w[mp][j / 4][j % 4]);
+               }
+               mx = fmaxf(top[mp], group_max(mx));
+               const float base = mx == -INFINITY ? 0.0f : mx;   // nothing named so far: every weight below is exp2(-inf)
+               const float keep = exp2_fast(top[mp] - base);
+               float add = 0;
+#pragma unroll
+               for (int j = 0; j < 8; j++)
+               {
+                  w[mp][j / 4][j % 4] = exp2_fast(w[mp][j / 4][j % 4] - base);
+                  add += w[mp][j / 4][j % 4];
+               }
+               if (__any(mx != top[mp]))
+               {
+#pragma unroll
+                  for (int x = 0; x < G::NT; x++) acc[mp][x] *= keep;
+               }
+               sum[mp] = sum[mp] * keep + add;   // of this lane's columns: the four groups are added at the end
+               top[mp] = mx;
+            }
+            if (__builtin_expect(careful, 0))
             {
-               w[mp][j / 4][j % 4] = exp2_fast(w[mp][j / 4][j % 4] - base);
-               add += w[mp][j / 4][j % 4];
-            }
-            if (__any(mx != top[mp]))
-            {
 #pragma unroll
-               for (int x = 0; x < G::NT; x++) acc[mp][x] *= keep;
+               for (int mp = 0; mp < MAPS; mp++) add_weighted<T, G::W, G::NT>(acc[mp], w[mp], mine, vs, 0, g, i, l, true);
+               return;
             }
-            sum[mp] = sum[mp] * keep + add;   // of this lane's columns: the four groups are added at the end
-            top[mp] = mx;
-         }
-         if (__builtin_expect(odd[b] == t + 1, 0))
-         {
-#pragma unroll
-            for (int mp = 0; mp < MAPS; mp++) add_weighted<T, G::NT>(acc[mp], w[mp], mine, vs[b], G::LD, g, i, true);
-         }
-         else
-         {
             typename G::N::TFrag wf[MAPS];
 #pragma unroll
             for (int mp = 0; mp < MAPS; mp++) wf[mp] = pack_scores<T>(w[mp]);
 #pragma unroll
             for (int x = 0; x < G::NT; x++)
             {
-               const typename G::N::TFrag vt = load_t<T>(vs[b], G::LD, x, g, i);
+               const typename G::N::TFrag vt = G::V::transposed(vs, x, l);
 #pragma unroll
                for (int mp = 0; mp < MAPS; mp++) acc[mp][x] = G::N::mma_t(vt, wf[mp], acc[mp][x]);
             }
-         }
-      }
-      if (t + 1 < u.tiles)
-      {
-         if (stage_store<G, T>(st, ks[b ^ 1], vs[b ^ 1], tid, false, true)) odd[b ^ 1] = t + 2;
-      }
-      __syncthreads();
+         });
+      bool odd = odd_sums(acc[0]);
+      if constexpr (MAPS == 2) odd |= odd_sums(acc[1]);
+      if (!any_odd<BR>(odd)) break;
    }
 
 #pragma unroll
    for (int mp = 0; mp < MAPS; mp++) sum[mp] = group_sum(sum[mp]);
    if (u.part >= 0)
    {
-      // [part][head][map][64 rows][W + 2]: sums, then the running maximum and sum
-      float *to = p.part + (((int64_t)u.part * p.heads + head) * MAPS * kBlockRows + 16 * wave + i) * (G::W + 2);
+      // [part][head][map][BR rows][W + 2]: sums, then the running maximum and sum
+      float *to = p.part + (((int64_t)u.part * p.heads + head) * MAPS * BR + 16 * wave + i) * (G::W + 2);
 #pragma unroll
       for (int mp = 0; mp < MAPS; mp++)
       {
-         float *r = to + (int64_t)mp * kBlockRows * (G::W + 2);
+         float *r = to + (int64_t)mp * BR * (G::W + 2);
 #pragma unroll
          for (int x = 0; x < G::NT; x++)
 #pragma unroll
@@ -328,16 +431,17 @@ __global__ __launch_bounds__(256, (Geo<T, DC, MAPS>::kWide && (T == kF32 || MAPS
 // Blocks of several units: one wave per (block, head, row).
 template <int T, int DC, int MAPS> __global__ __launch_bounds__(256) void attn_forward_join(Params p)
 {
-   typedef Geo<T, DC, MAPS> G;
+   typedef Geo<T, DC, MAPS, 64> G;
+   const int br = p.plan.block_rows;
    typedef typename G::E E;
    const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
    const int lane = threadIdx.x & 63;
-   const int r = (int)(id % kBlockRows);
-   const int head = (int)((id / kBlockRows) % p.heads);
-   const int64_t jn = id / kBlockRows / p.heads;
+   const int r = (int)(id % br);
+   const int head = (int)((id / br) % p.heads);
+   const int64_t jn = id / br / p.heads;
    if (jn >= p.plan.n_joins) return;
    const Join j = p.plan.joins[jn];
-   const int64_t row = (int64_t)j.block * kBlockRows + r;
+   const int64_t row = (int64_t)j.block * br + r;
    if (row >= p.m) return;
    const float lam = MAPS == 2 ? p.lambda[head] : 0.0f;
    constexpr int PER = (G::W + 63) / 64;
@@ -345,8 +449,8 @@ template <int T, int DC, int MAPS> __global__ __launch_bounds__(256) void attn_f
 #pragma unroll
    for (int mp = 0; mp < MAPS; mp++)
    {
-      const int64_t step = (int64_t)p.heads * MAPS * kBlockRows * (G::W + 2);
-      const float *from = p.part + (((int64_t)j.part0 * p.heads + head) * MAPS + mp) * kBlockRows * (G::W + 2) + (int64_t)r * (G::W + 2);
+      const int64_t step = (int64_t)p.heads * MAPS * br * (G::W + 2);
+      const float *from = p.part + (((int64_t)j.part0 * p.heads + head) * MAPS + mp) * br * (G::W + 2) + (int64_t)r * (G::W + 2);
       float top = -INFINITY;
       for (int u = 0; u < j.parts; u++) top = fmaxf(top, from[u * step + G::W]);
       const float base = top == -INFINITY ? 0.0f : top;
@@ -420,28 +524,30 @@ template <int T, int MAPS> __global__ __launch_bounds__(256) void attn_delta(Par
 }
 
 // dq: resident q and do of 16 rows per wave, gathered k and v; both maps share the gathered v and dP.
-template <int T, int DC, int MAPS>
-__global__ __launch_bounds__(256, (Geo<T, DC, MAPS>::kWide ? 1 : 2)) void attn_dq(Params p)
+//
+// delta comes from o as it was rounded to 16 bits, which a row of few edges feels: with mean = sum_j P dP, formed here in
+// fp32, dq = sum_j P (dP - delta) k + (delta - mean) sum_j P k.  The second sum is small where it counts, so its own rounding
+// does not matter; the exact mean replaces delta for dk.  fp32 needs none of it.
+template <int T, int DC, int MAPS, int BR> __global__ __launch_bounds__(BR * 4, (DC * MAPS >= 256 || T == kF32 ? 1 : 2)) void attn_dq(Params p)
 {
-   typedef Geo<T, DC, MAPS> G;
+   typedef Geo<T, DC, MAPS, BR> G;
    typedef typename G::E E;
-   __shared__ __align__(16) E ks[2][kTile * G::LD];
-   __shared__ __align__(16) E vs[2][kTile * G::LD];
-   __shared__ int odd[2];
+   constexpr bool kMend = T != kF32;
+   ATTN_LDS(0)
    const int64_t item = xcd_item(blockIdx.x, (int64_t)p.plan.n_units * p.heads);
    if (item >= (int64_t)p.plan.n_units * p.heads) return;
    const int head = (int)(item / p.plan.n_units);
    const Unit u = p.plan.units[item % p.plan.n_units];
    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, g = lane >> 4, i = lane & 15;
    const int kvh = head / p.group;
-   const E *k = (const E *)p.k + kvh * p.hdk, *v = (const E *)p.v + kvh * p.hdv;
-   const int64_t row = (int64_t)u.block * kBlockRows + 16 * wave + i;
+   const int64_t row = (int64_t)u.block * BR + 16 * wave + i;
    const bool live = row < p.m;
    const int64_t srow = live ? row : 0;
-   if (tid < 2) odd[tid] = 0;
+   Stream<G, T, DC, BR> st;
+   st.set(lds, lds_ids, lds_bits, p.plan, u, (const E *)p.k + kvh * p.hdk, p.ldk, p.d, (const E *)p.v + kvh * p.hdv, p.ldv, p.dv, p.vec);
 
    u4 qr[MAPS][G::CQ], gr[G::CV];
-   float lse2[MAPS], delta[MAPS], sign[MAPS];
+   float lse2[MAPS], delta[MAPS], sign[MAPS], mean[MAPS];
 #pragma unroll
    for (int mp = 0; mp < MAPS; mp++)
    {
@@ -452,120 +558,158 @@ __global__ __launch_bounds__(256, (Geo<T, DC, MAPS>::kWide ? 1 : 2)) void attn_d
    }
    load_resident<T, G::CV>(gr, (const E *)p.dout + srow * p.ldo + head * p.hdo, live, p.dv, g, p.vec);
 
-   f4 acc[MAPS][G::NTQ];
-#pragma unroll
-   for (int mp = 0; mp < MAPS; mp++)
-#pragma unroll
-      for (int t = 0; t < G::NTQ; t++) acc[mp][t] = f4{0, 0, 0, 0};
-   float mean2 = 0;
    const float c2 = p.scale * kLog2e;
-
-   const int32_t *cols = p.plan.cols + (int64_t)u.tile0 * kTile;
-   const uint16_t *masks = p.plan.masks + (int64_t)u.tile0 * (4 * kTile) + wave * kTile + 4 * g;
-   int32_t cn[G::NCH];
-   Stage<G> st;
-   uint64_t m0 = 0, m1 = 0;
-   if (u.tiles > 0)
+   f4 acc[MAPS][G::NTQ], pk[kMend ? MAPS : 1][kMend ? G::NTQ : 1];
+   for (int careful = 0; careful < 2; careful++)
    {
-      stage_cols<G>(cn, cols, tid);
-      stage_load<G, T, DC>(st, cn, k, p.ldk, p.d, v, p.ldv, p.dv, p.vec, tid);
-      m0 = *(const uint64_t *)masks;
-      m1 = *(const uint64_t *)(masks + 16);
-      if (u.tiles > 1) stage_cols<G>(cn, cols + kTile, tid);
-      __syncthreads();
-      if (stage_store<G, T>(st, ks[0], vs[0], tid, true, false)) odd[0] = 1;
-   }
-   __syncthreads();
-   for (int t = 0; t < u.tiles; t++)
-   {
-      const int b = t & 1;
-      const uint64_t n0 = m0, n1 = m1;
-      if (t + 1 < u.tiles)
-      {
-         stage_load<G, T, DC>(st, cn, k, p.ldk, p.d, v, p.ldv, p.dv, p.vec, tid);
-         m0 = *(const uint64_t *)(masks + (int64_t)(t + 1) * (4 * kTile));
-         m1 = *(const uint64_t *)(masks + (int64_t)(t + 1) * (4 * kTile) + 16);
-         if (t + 2 < u.tiles) stage_cols<G>(cn, cols + (int64_t)(t + 2) * kTile, tid);
-      }
-      if (__any((n0 | n1) != 0))
-      {
-         const unsigned mine = my_bits(n0, n1, i);
-         const bool bad = odd[b] == t + 1;
-         f4 dp[2];
-         tile_scores<T, G::CV>(dp, vs[b], G::LD, gr, g, i);
-#pragma unroll
-         for (int mp = 0; mp < MAPS; mp++)
-         {
-            f4 s[2];
-            tile_scores<T, G::CQ>(s, ks[b] + mp * DC, G::LD, qr[mp], g, i);
-            float w[2][4];
-#pragma unroll
-            for (int j = 0; j < 8; j++)
-            {
-               const bool named = (mine >> j) & 1;
-               const float pr = named ? exp2_fast(s[j / 4][j % 4] * c2 - lse2[mp]) : 0.0f;
-               const float x = named ? dp[j / 4][j % 4] : 0.0f;
-               w[j / 4][j % 4] = pr * sign[mp] * (x - delta[mp]);
-               if (mp == 1) mean2 = fmaf(pr, x, mean2);
-            }
-            add_weighted<T, G::NTQ>(acc[mp], w, mine, ks[b] + mp * DC, G::LD, g, i, bad);
-         }
-      }
-      if (t + 1 < u.tiles)
-      {
-         if (stage_store<G, T>(st, ks[b ^ 1], vs[b ^ 1], tid, true, false)) odd[b ^ 1] = t + 2;
-      }
-      __syncthreads();
-   }
-
-   if (MAPS == 2) mean2 = group_sum(mean2);
-   if (u.part >= 0)
-   {
-      // [part][head][64 rows][W + 1]
-      float *r = p.part + (((int64_t)u.part * p.heads + head) * kBlockRows + 16 * wave + i) * (G::W + 1);
 #pragma unroll
       for (int mp = 0; mp < MAPS; mp++)
+      {
+         mean[mp] = 0;
+#pragma unroll
+         for (int t = 0; t < G::NTQ; t++)
+         {
+            acc[mp][t] = f4{0, 0, 0, 0};
+            if constexpr (kMend) pk[mp][t] = f4{0, 0, 0, 0};
+         }
+      }
+      for_tiles<G, BR>(
+         st, u.tiles, 1, [&](int t, int buf) { st.load_tile(t, buf, st.a, st.b); },
+         [&](int t, int buf) {
+            bool named;
+            const unsigned mine = st.my_bits(t, g, i, &named);
+            if (!named) return;
+            const typename G::V::Lane l = G::V::lane(g, i);
+            const unsigned char *ks = lds + buf * G::kPair, *vs = ks + G::V::kBytes;
+            f4 dp[2];
+            tile_scores<T, G::W, G::CV>(dp, vs, 0, gr, l);
+#pragma unroll
+            for (int mp = 0; mp < MAPS; mp++)
+            {
+               f4 s[2];
+               tile_scores<T, G::W, G::CQ>(s, ks, mp * G::MC, qr[mp], l);
+               float w[2][4], pr[2][4];
+#pragma unroll
+               for (int j = 0; j < 8; j++)
+               {
+                  const bool one = (mine >> j) & 1;
+                  pr[j / 4][j % 4] = one ? exp2_fast(s[j / 4][j % 4] * c2 - lse2[mp]) : 0.0f;
+                  const float x = one ? dp[j / 4][j % 4] : 0.0f;
+                  w[j / 4][j % 4] = pr[j / 4][j % 4] * sign[mp] * (x - delta[mp]);
+                  mean[mp] = fmaf(pr[j / 4][j % 4], x, mean[mp]);
+               }
+               if (__builtin_expect(careful, 0))
+               {
+                  add_weighted<T, G::W, G::NTQ>(acc[mp], w, mine, ks, mp * DC, g, i, l, true);
+                  if constexpr (kMend) add_weighted<T, G::W, G::NTQ>(pk[mp], pr, mine, ks, mp * DC, g, i, l, true);
+                  continue;
+               }
+               const typename G::N::TFrag wf = pack_scores<T>(w);
+               typename G::N::TFrag pf;
+               if constexpr (kMend) pf = pack_scores<T>(pr);
+#pragma unroll
+               for (int x = 0; x < G::NTQ; x++)
+               {
+                  const typename G::N::TFrag kt = G::V::transposed(ks, mp * G::NTQ + x, l);
+                  acc[mp][x] = G::N::mma_t(kt, wf, acc[mp][x]);
+                  if constexpr (kMend) pk[mp][x] = G::N::mma_t(kt, pf, pk[mp][x]);
+               }
+            }
+         });
+      bool odd = false;
+#pragma unroll
+      for (int mp = 0; mp < MAPS; mp++)
+      {
+         odd |= odd_sums(acc[mp]);
+         if constexpr (kMend) odd |= odd_sums(pk[mp]);
+      }
+      if (!any_odd<BR>(odd)) break;
+   }
+
+#pragma unroll
+   for (int mp = 0; mp < MAPS; mp++) mean[mp] = group_sum(mean[mp]);
+   if (u.part >= 0)
+   {
+      // [part][head][BR rows][W + W + 2]: the two sums, the means
+      float *r = p.part + (((int64_t)u.part * p.heads + head) * BR + 16 * wave + i) * (2 * G::W + 2);
+#pragma unroll
+      for (int mp = 0; mp < MAPS; mp++)
+      {
 #pragma unroll
          for (int x = 0; x < G::NTQ; x++)
 #pragma unroll
-            for (int e = 0; e < 4; e++) r[mp * DC + 16 * x + 4 * g + e] = acc[mp][x][e];
-      if (g == 0) r[G::W] = mean2;
+            for (int e = 0; e < 4; e++)
+            {
+               r[mp * DC + 16 * x + 4 * g + e] = acc[mp][x][e];
+               if constexpr (kMend) r[G::W + mp * DC + 16 * x + 4 * g + e] = pk[mp][x][e];
+            }
+         if (g == 0) r[2 * G::W + mp] = mean[mp];
+      }
       return;
    }
    if (!live) return;
-   if (MAPS == 2 && g == 0) p.dlam_rows[row * p.heads + head] = mean2;
+   if (g == 0)
+   {
+      if (MAPS == 2) p.dlam_rows[row * p.heads + head] = mean[MAPS - 1];
+      if constexpr (kMend)
+      {
+#pragma unroll
+         for (int mp = 0; mp < MAPS; mp++) p.delta[(row * p.heads + head) * MAPS + mp] = mean[mp];
+      }
+   }
    E *out = (E *)p.dq + row * p.ldq + head * p.hdq;
 #pragma unroll
    for (int mp = 0; mp < MAPS; mp++)
 #pragma unroll
-      for (int x = 0; x < G::NTQ; x++) store4<T>(out + mp * p.d, 16 * x + 4 * g, p.d, acc[mp][x] * p.scale, p.vec);
+      for (int x = 0; x < G::NTQ; x++)
+      {
+         f4 r = acc[mp][x];
+         if constexpr (kMend) r += (sign[mp] * (delta[mp] - mean[mp])) * pk[mp][x];
+         store4<T>(out + mp * p.d, 16 * x + 4 * g, p.d, r * p.scale, p.vec);
+      }
 }
 
 template <int T, int DC, int MAPS> __global__ __launch_bounds__(256) void attn_dq_join(Params p)
 {
-   typedef Geo<T, DC, MAPS> G;
-   typedef typename G::E E;
+   constexpr int W = DC * MAPS;
+   constexpr bool kMend = T != kF32;
+   typedef typename Num<T>::E E;
+   const int br = p.plan.block_rows;
    const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
    const int lane = threadIdx.x & 63;
-   const int r = (int)(id % kBlockRows);
-   const int head = (int)((id / kBlockRows) % p.heads);
-   const int64_t jn = id / kBlockRows / p.heads;
+   const int r = (int)(id % br);
+   const int head = (int)((id / br) % p.heads);
+   const int64_t jn = id / br / p.heads;
    if (jn >= p.plan.n_joins) return;
    const Join j = p.plan.joins[jn];
-   const int64_t row = (int64_t)j.block * kBlockRows + r;
+   const int64_t row = (int64_t)j.block * br + r;
    if (row >= p.m) return;
-   const int64_t step = (int64_t)p.heads * kBlockRows * (G::W + 1);
-   const float *from = p.part + (((int64_t)j.part0 * p.heads + head) * kBlockRows + r) * (G::W + 1);
-   for (int f = lane; f <= G::W; f += 64)
+   const int64_t step = (int64_t)p.heads * br * (2 * W + 2);
+   const float *from = p.part + (((int64_t)j.part0 * p.heads + head) * br + r) * (2 * W + 2);
+   float mend[MAPS];
+#pragma unroll
+   for (int mp = 0; mp < MAPS; mp++)
    {
-      float s = 0;
-      for (int u = 0; u < j.parts; u++) s += from[u * step + f];
-      if (f == G::W)
+      float mean = 0;
+      for (int u = 0; u < j.parts; u++) mean += from[u * step + 2 * W + mp];
+      float *delta = p.delta + (row * p.heads + head) * MAPS + mp;
+      mend[mp] = (mp == 0 ? 1.0f : -p.lambda[head]) * (*delta - mean);
+      if (lane == 0)
       {
-         if (MAPS == 2) p.dlam_rows[row * p.heads + head] = s;
-         continue;
+         if (mp == 1) p.dlam_rows[row * p.heads + head] = mean;
+         if (kMend) *delta = mean;   // (every lane has read it: one wave, in step)
+      }
+   }
+   for (int f = lane; f < W; f += 64)
+   {
+      float s = 0, s2 = 0;
+      for (int u = 0; u < j.parts; u++)
+      {
+         s += from[u * step + f];
+         if (kMend) s2 += from[u * step + W + f];
       }
       const int mp = f / DC, e = f - mp * DC;
+      if (kMend) s += (mp == 0 ? mend[0] : mend[MAPS - 1]) * s2;
       if (e < p.d) ((E *)p.dq)[row * p.ldq + head * p.hdq + mp * p.d + e] = (E)Num<T>::from(s * p.scale);
    }
 }
@@ -589,133 +733,102 @@ template <int T> __global__ __launch_bounds__(256) void attn_dlambda(Params p)
 
 // dk, dv: resident k and v of 16 key rows per wave, gathered q and do of the query rows that name them, for every query
 // head of the key head in turn.  p.plan is the plan of the transposed pattern.
-template <int T, int DC, int MAPS>
-__global__ __launch_bounds__(256, (Geo<T, DC, MAPS>::kWide ? 1 : 2)) void attn_dkv(Params p)
+template <int T, int DC, int MAPS, int BR> __global__ __launch_bounds__(BR * 4, (DC * MAPS >= 256 || T == kF32 ? 1 : 2)) void attn_dkv(Params p)
 {
-   typedef Geo<T, DC, MAPS> G;
+   typedef Geo<T, DC, MAPS, BR> G;
    typedef typename G::E E;
-   __shared__ __align__(16) E qs[2][kTile * G::LD];
-   __shared__ __align__(16) E gs[2][kTile * G::LD];
-   __shared__ __align__(16) float stat[2][2 * MAPS][kTile];   // lse * log2(e), delta of the gathered rows
-   __shared__ int odd[2];
+   ATTN_LDS(G::kStat)
    const int64_t item = xcd_item(blockIdx.x, (int64_t)p.plan.n_units * p.kv_heads);
    if (item >= (int64_t)p.plan.n_units * p.kv_heads) return;
    const int kvh = (int)(item / p.plan.n_units);
    const Unit u = p.plan.units[item % p.plan.n_units];
    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, g = lane >> 4, i = lane & 15;
-   const int64_t row = (int64_t)u.block * kBlockRows + 16 * wave + i;
+   const int64_t row = (int64_t)u.block * BR + 16 * wave + i;
    const bool live = row < p.n;
    const int64_t srow = live ? row : 0;
-   if (tid < 2) odd[tid] = 0;
+   Stream<G, T, DC, BR> st;
+   st.set(lds, lds_ids, lds_bits, p.plan, u, (const E *)p.q, p.ldq, p.d, (const E *)p.dout, p.ldo, p.dv, p.vec);
 
    u4 kr[MAPS][G::CQ], vr[G::CV];
 #pragma unroll
    for (int mp = 0; mp < MAPS; mp++)
       load_resident<T, G::CQ>(kr[mp], (const E *)p.k + srow * p.ldk + kvh * p.hdk + mp * p.d, live, p.d, g, p.vec);
    load_resident<T, G::CV>(vr, (const E *)p.v + srow * p.ldv + kvh * p.hdv, live, p.dv, g, p.vec);
-
-   f4 dk[MAPS][G::NTQ], dv[G::NT];
-#pragma unroll
-   for (int mp = 0; mp < MAPS; mp++)
-#pragma unroll
-      for (int t = 0; t < G::NTQ; t++) dk[mp][t] = f4{0, 0, 0, 0};
-#pragma unroll
-   for (int t = 0; t < G::NT; t++) dv[t] = f4{0, 0, 0, 0};
    const float c2 = p.scale * kLog2e;
+   f4 dk[MAPS][G::NTQ], dv[G::NT];
 
-   const int32_t *cols = p.plan.cols + (int64_t)u.tile0 * kTile;
-   const uint16_t *masks = p.plan.masks + (int64_t)u.tile0 * (4 * kTile) + wave * kTile + 4 * g;
-   const int steps = u.tiles * p.group;   // tile by tile, the heads of the group within a tile
-   int32_t cn[G::NCH];
-   Stage<G> st;
-   float sv = 0;
-   // thread tid < 64 * MAPS also carries one statistic of the tile's rows: number tid / 32 of row tid % 32
-   const int sk = tid >> 5;
-   auto load_stat = [&](int tile, int head) {
-      float x = 0;
-      if (sk < 2 * MAPS)
-      {
-         const int32_t c = cols[(int64_t)tile * kTile + (tid & 31)];
-         if (c >= 0)
-         {
-            const int64_t at = ((int64_t)c * p.heads + head) * MAPS + (sk % MAPS);
-            x = sk < MAPS ? p.lse_in[at] * kLog2e : p.delta[at];
-         }
-      }
-      return x;
-   };
-   auto load_step = [&](int s) {
-      const int tile = s / p.group, head = kvh * p.group + s % p.group;
-      stage_cols<G>(cn, cols + (int64_t)tile * kTile, tid);
-      stage_load<G, T, DC>(st, cn, (const E *)p.q + head * p.hdq, p.ldq, p.d, (const E *)p.dout + head * p.hdo, p.ldo, p.dv, p.vec, tid);
-      sv = load_stat(tile, head);
-   };
-   auto store_step = [&](int b, int mark) {
-      if (stage_store<G, T>(st, qs[b], gs[b], tid, true, true)) odd[b] = mark;
-      if (sk < 2 * MAPS) stat[b][sk][tid & 31] = sv;
-   };
-   if (steps > 0)
-   {
-      load_step(0);
-      __syncthreads();
-      store_step(0, 1);
-   }
-   __syncthreads();
-   uint64_t m0 = 0, m1 = 0;
-   unsigned mine = 0;
-   for (int s = 0; s < steps; s++)
-   {
-      const int b = s & 1, hh = s % p.group;
-      if (s + 1 < steps) load_step(s + 1);
-      if (hh == 0)
-      {
-         const int64_t off = (int64_t)(s / p.group) * (4 * kTile);
-         m0 = *(const uint64_t *)(masks + off);
-         m1 = *(const uint64_t *)(masks + off + 16);
-         mine = my_bits(m0, m1, i);
-      }
-      if (__any((m0 | m1) != 0))
-      {
-         const bool bad = odd[b] == s + 1;
-         const float lam = MAPS == 2 ? p.lambda[kvh * p.group + hh] : 0.0f;
-         f4 dp[2];
-         tile_scores<T, G::CV>(dp, gs[b], G::LD, vr, g, i);
-         float wv[2][4];
+   auto load = [&](int s, int buf) {
+      const int t = s / p.group, head = kvh * p.group + s % p.group;
+      st.load_tile(t, buf, st.a + head * p.hdq, st.b + head * p.hdo);
+      // [lse of every map, delta of every map][32 rows]: 64 values for each of the first waves, or for the wave twice
 #pragma unroll
-         for (int mp = 0; mp < MAPS; mp++)
-         {
-            f4 sc[2];
-            tile_scores<T, G::CQ>(sc, qs[b] + mp * DC, G::LD, kr[mp], g, i);
-            const float sign = mp == 0 ? 1.0f : -lam;
-            float w[2][4];
+      for (int x = 0; x < (BR == 64 ? 1 : MAPS); x++)
+      {
+         const int sk = (tid >> 5) + 2 * x;
+         if (sk >= 2 * MAPS) break;
+         const int32_t c = st.tile_ids(t)[tid & 31];
+         const float *from = (sk < MAPS ? p.lse_in : p.delta) + ((int64_t)c * p.heads + head) * MAPS + sk % MAPS;
+         load_lds4(lds_address(lds_extra + buf * G::kStat) + 256 * (st.wave + x), c >= 0 ? (const void *)from : (const void *)&zero_chunk);
+      }
+   };
+   auto use = [&](int s, int buf, bool careful) {
+      bool named;
+      const unsigned mine = st.my_bits(s / p.group, g, i, &named);
+      if (!named) return;
+      const typename G::V::Lane l = G::V::lane(g, i);
+      const unsigned char *qs = lds + buf * G::kPair, *gs = qs + G::V::kBytes;
+      const float *stat = (const float *)(lds_extra + buf * G::kStat);
+      const float lam = MAPS == 2 ? p.lambda[kvh * p.group + s % p.group] : 0.0f;
+      f4 dp[2];
+      tile_scores<T, G::W, G::CV>(dp, gs, 0, vr, l);
+      float wv[2][4];
 #pragma unroll
-            for (int a = 0; a < 2; a++)
+      for (int mp = 0; mp < MAPS; mp++)
+      {
+         f4 sc[2];
+         tile_scores<T, G::W, G::CQ>(sc, qs, mp * G::MC, kr[mp], l);
+         const float sign = mp == 0 ? 1.0f : -lam;
+         float w[2][4];
+#pragma unroll
+         for (int a = 0; a < 2; a++)
+         {
+            const f4 ls = *(const f4 *)(stat + mp * kTile + 16 * a + 4 * g), dl = *(const f4 *)(stat + (MAPS + mp) * kTile + 16 * a + 4 * g);
+#pragma unroll
+            for (int r = 0; r < 4; r++)
             {
-               const f4 l = *(const f4 *)&stat[b][mp][16 * a + 4 * g], dl = *(const f4 *)&stat[b][MAPS + mp][16 * a + 4 * g];
-#pragma unroll
-               for (int r = 0; r < 4; r++)
-               {
-                  const bool named = (mine >> (4 * a + r)) & 1;
-                  const float pr = named ? sign * exp2_fast(sc[a][r] * c2 - l[r]) : 0.0f;
-                  w[a][r] = named ? pr * (dp[a][r] - dl[r]) : 0.0f;
-                  wv[a][r] = mp == 0 ? pr : wv[a][r] + pr;
-               }
+               const bool one = (mine >> (4 * a + r)) & 1;
+               const float pr = one ? sign * exp2_fast(sc[a][r] * c2 - ls[r] * kLog2e) : 0.0f;
+               w[a][r] = one ? pr * (dp[a][r] - dl[r]) : 0.0f;
+               wv[a][r] = mp == 0 ? pr : wv[a][r] + pr;
             }
-            add_weighted<T, G::NTQ>(dk[mp], w, mine, qs[b] + mp * DC, G::LD, g, i, bad);
          }
-#pragma unroll
-         for (int j = 0; j < 8; j++) wv[j / 4][j % 4] *= G::N::kPScale;
-         add_weighted<T, G::NT>(dv, wv, mine, gs[b], G::LD, g, i, bad);
+         add_weighted<T, G::W, G::NTQ>(dk[mp], w, mine, qs, mp * DC, g, i, l, careful);
       }
-      if (s + 1 < steps) store_step(b ^ 1, s + 2);
-      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < 8; j++) wv[j / 4][j % 4] *= G::N::kPScale;
+      add_weighted<T, G::W, G::NT>(dv, wv, mine, gs, 0, g, i, l, careful);
+   };
+   for (int careful = 0; careful < 2; careful++)
+   {
+#pragma unroll
+      for (int mp = 0; mp < MAPS; mp++)
+#pragma unroll
+         for (int t = 0; t < G::NTQ; t++) dk[mp][t] = f4{0, 0, 0, 0};
+#pragma unroll
+      for (int t = 0; t < G::NT; t++) dv[t] = f4{0, 0, 0, 0};
+      // (steps of one tile, the heads of the group, follow each other: tiles * group < 2^31 is checked by the host)
+      for_tiles<G, BR>(st, u.tiles * p.group, p.group, load, [&](int s, int buf) { use(s, buf, careful); });
+      bool odd = odd_sums(dv);
+#pragma unroll
+      for (int mp = 0; mp < MAPS; mp++) odd |= odd_sums(dk[mp]);
+      if (!any_odd<BR>(odd)) break;
    }
 
    constexpr float unscale = 1.0f / G::N::kPScale;
    if (u.part >= 0)
    {
-      // [part][kv head][64 rows][2 W]
-      float *r = p.part + (((int64_t)u.part * p.kv_heads + kvh) * kBlockRows + 16 * wave + i) * (2 * G::W);
+      // [part][kv head][BR rows][2 W]
+      float *r = p.part + (((int64_t)u.part * p.kv_heads + kvh) * BR + 16 * wave + i) * (2 * G::W);
 #pragma unroll
       for (int mp = 0; mp < MAPS; mp++)
 #pragma unroll
@@ -741,19 +854,20 @@ __global__ __launch_bounds__(256, (Geo<T, DC, MAPS>::kWide ? 1 : 2)) void attn_d
 
 template <int T, int DC, int MAPS> __global__ __launch_bounds__(256) void attn_dkv_join(Params p)
 {
-   typedef Geo<T, DC, MAPS> G;
+   typedef Geo<T, DC, MAPS, 64> G;
+   const int br = p.plan.block_rows;
    typedef typename G::E E;
    const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
    const int lane = threadIdx.x & 63;
-   const int r = (int)(id % kBlockRows);
-   const int kvh = (int)((id / kBlockRows) % p.kv_heads);
-   const int64_t jn = id / kBlockRows / p.kv_heads;
+   const int r = (int)(id % br);
+   const int kvh = (int)((id / br) % p.kv_heads);
+   const int64_t jn = id / br / p.kv_heads;
    if (jn >= p.plan.n_joins) return;
    const Join j = p.plan.joins[jn];
-   const int64_t row = (int64_t)j.block * kBlockRows + r;
+   const int64_t row = (int64_t)j.block * br + r;
    if (row >= p.n) return;
-   const int64_t step = (int64_t)p.kv_heads * kBlockRows * (2 * G::W);
-   const float *from = p.part + (((int64_t)j.part0 * p.kv_heads + kvh) * kBlockRows + r) * (2 * G::W);
+   const int64_t step = (int64_t)p.kv_heads * br * (2 * G::W);
+   const float *from = p.part + (((int64_t)j.part0 * p.kv_heads + kvh) * br + r) * (2 * G::W);
    for (int f = lane; f < 2 * G::W; f += 64)
    {
       float s = 0;

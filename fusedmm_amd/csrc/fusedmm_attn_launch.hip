@@ -49,11 +49,12 @@ template <int DC, int MAPS> struct Forward {
    int operator()(const Params &p, hipStream_t s)
    {
       const int64_t n = (int64_t)p.plan.n_units * p.heads;
-      hipLaunchKernelGGL((attn_forward<TYPE, DC, MAPS>), dim3(eighths(n)), dim3(256), 0, s, p);
+      if (p.plan.block_rows == 64) hipLaunchKernelGGL((attn_forward<TYPE, DC, MAPS, 64>), dim3(eighths(n)), dim3(256), 0, s, p);
+         else hipLaunchKernelGGL((attn_forward<TYPE, DC, MAPS, 16>), dim3(eighths(n)), dim3(64), 0, s, p);
       ATTN_HIP(hipGetLastError());
       if (p.plan.n_joins)
       {
-         hipLaunchKernelGGL((attn_forward_join<TYPE, DC, MAPS>), dim3((unsigned)((int64_t)p.plan.n_joins * p.heads * kBlockRows / 4)), dim3(256), 0, s, p);
+         hipLaunchKernelGGL((attn_forward_join<TYPE, DC, MAPS>), dim3((unsigned)((int64_t)p.plan.n_joins * p.heads * p.plan.block_rows / 4)), dim3(256), 0, s, p);
          ATTN_HIP(hipGetLastError());
       }
       return kOk;
@@ -68,11 +69,12 @@ template <int DC, int MAPS> struct Dq {
          hipLaunchKernelGGL((attn_delta<TYPE, MAPS>), dim3((unsigned)((p.m * p.heads + 15) / 16)), dim3(256), 0, s, p);
          ATTN_HIP(hipGetLastError());
          const int64_t n = (int64_t)p.plan.n_units * p.heads;
-         hipLaunchKernelGGL((attn_dq<TYPE, DC, MAPS>), dim3(eighths(n)), dim3(256), 0, s, p);
+         if (p.plan.block_rows == 64) hipLaunchKernelGGL((attn_dq<TYPE, DC, MAPS, 64>), dim3(eighths(n)), dim3(256), 0, s, p);
+         else hipLaunchKernelGGL((attn_dq<TYPE, DC, MAPS, 16>), dim3(eighths(n)), dim3(64), 0, s, p);
          ATTN_HIP(hipGetLastError());
          if (p.plan.n_joins)
          {
-            hipLaunchKernelGGL((attn_dq_join<TYPE, DC, MAPS>), dim3((unsigned)((int64_t)p.plan.n_joins * p.heads * kBlockRows / 4)), dim3(256), 0, s, p);
+            hipLaunchKernelGGL((attn_dq_join<TYPE, DC, MAPS>), dim3((unsigned)((int64_t)p.plan.n_joins * p.heads * p.plan.block_rows / 4)), dim3(256), 0, s, p);
             ATTN_HIP(hipGetLastError());
          }
       }
@@ -89,11 +91,12 @@ template <int DC, int MAPS> struct Dkv {
    int operator()(const Params &p, hipStream_t s)
    {
       const int64_t n = (int64_t)p.plan.n_units * p.kv_heads;
-      hipLaunchKernelGGL((attn_dkv<TYPE, DC, MAPS>), dim3(eighths(n)), dim3(256), 0, s, p);
+      if (p.plan.block_rows == 64) hipLaunchKernelGGL((attn_dkv<TYPE, DC, MAPS, 64>), dim3(eighths(n)), dim3(256), 0, s, p);
+         else hipLaunchKernelGGL((attn_dkv<TYPE, DC, MAPS, 16>), dim3(eighths(n)), dim3(64), 0, s, p);
       ATTN_HIP(hipGetLastError());
       if (p.plan.n_joins)
       {
-         hipLaunchKernelGGL((attn_dkv_join<TYPE, DC, MAPS>), dim3((unsigned)((int64_t)p.plan.n_joins * p.kv_heads * kBlockRows / 4)), dim3(256), 0, s, p);
+         hipLaunchKernelGGL((attn_dkv_join<TYPE, DC, MAPS>), dim3((unsigned)((int64_t)p.plan.n_joins * p.kv_heads * p.plan.block_rows / 4)), dim3(256), 0, s, p);
          ATTN_HIP(hipGetLastError());
       }
       return kOk;

@@ -1,6 +1,9 @@
 // The plan of a pattern: for every block of 64 rows, the columns that any of them names, ascending, with one bit per row.
+// Where rows have few neighbours in common - the four runs of 16 rows of a block together name less than kShare times as
+// many columns as the block does - blocks of 16 rows take their place: a gathered row is then loaded once for each run, but
+// multiplied only for the run that names it.
 //
-// The 64 rows' lists are cut into chunks of 512 slots each (at most 32768 edges); a workgroup sorts a chunk's (column, row)
+// The rows' lists are cut into chunks of 512 slots each (at most 32768 edges); a workgroup sorts a chunk's (column, row)
 // keys in LDS and keeps one entry for each column.  Columns that are in ascending order within the rows, as loaders leave
 // them, put the same stretch of columns into one chunk; any other order is as right and only shares less.  A column that a
 // row names twice gets a second entry, so that it counts twice, as it does in every sum over edges.  Sorting costs
@@ -13,6 +16,8 @@ namespace fmm_attn {
 
 namespace {
 
+constexpr int kMostRows = 64;
+constexpr double kShare = 2.0;
 constexpr int kChunkSlots = 512;
 constexpr uint32_t kNoKey = 0xffffffffu;
 
@@ -34,13 +39,14 @@ __device__ inline int64_t index_at(const void *a, int64_t i, int bytes)
 }
 
 // one wave per block: its longest row and all its edges
-__global__ __launch_bounds__(256) void plan_count(int64_t m, int64_t blocks, const void *pb, const void *pe, int ib, int64_t *longest, int64_t *edges, int *bad)
+__global__ __launch_bounds__(256) void plan_count(int64_t m, int br, int64_t blocks, const void *pb, const void *pe, int ib, int64_t *longest, int64_t *edges, int *bad)
 {
    const int64_t b = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
    if (b >= blocks) return;
-   const int64_t row = b * kBlockRows + (threadIdx.x & 63);
+   const int lane = threadIdx.x & 63;
+   const int64_t row = b * br + lane;
    int64_t len = 0;
-   if (row < m)
+   if (lane < br && row < m)
    {
       const int64_t lo = index_at(pb, row, ib), hi = index_at(pe, row, ib);
       if (lo > hi || lo < 0) *bad = 1;
@@ -66,42 +72,44 @@ __device__ inline int64_t chunk_length(int64_t len, int number)
 }
 
 // one wave per chunk: its edges
-__global__ __launch_bounds__(256) void plan_chunk_edges(Chunk *chunks, int64_t n_chunks, int64_t m, const void *pb, const void *pe, int ib)
+__global__ __launch_bounds__(256) void plan_chunk_edges(Chunk *chunks, int64_t n_chunks, int64_t m, int br, const void *pb, const void *pe, int ib)
 {
    const int64_t c = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
    if (c >= n_chunks) return;
-   const int64_t row = (int64_t)chunks[c].block * kBlockRows + (threadIdx.x & 63);
-   int x = row < m ? (int)chunk_length(index_at(pe, row, ib) - index_at(pb, row, ib), chunks[c].number) : 0;
+   const int lane = threadIdx.x & 63;
+   const int64_t row = (int64_t)chunks[c].block * br + lane;
+   int x = lane < br && row < m ? (int)chunk_length(index_at(pe, row, ib) - index_at(pb, row, ib), chunks[c].number) : 0;
    for (int k = 1; k < 64; k <<= 1) x += __shfl_xor(x, k);
    if ((threadIdx.x & 63) == 0) chunks[c].edges = x;
 }
 
 // SIZE: keys that fit; chunks of at most that many edges
 template <int SIZE, int THREADS>
-__global__ __launch_bounds__(THREADS) void plan_fill(const Chunk *chunks, int64_t n_chunks, int64_t m, int64_t n, const void *indx, const void *pb,
-                                                      const void *pe, int ib, int32_t *cols, uint64_t *masks, int32_t *counts)
+__global__ __launch_bounds__(THREADS) void plan_fill(const Chunk *chunks, int64_t n_chunks, int64_t m, int br, int64_t n, const void *indx, const void *pb,
+                                                      const void *pe, int ib, int32_t *cols, uint64_t *masks, int2 *counts)
 {
    __shared__ uint32_t key[SIZE];
-   __shared__ int32_t start[kBlockRows + 1];
+   __shared__ int32_t start[kMostRows + 1];
+   __shared__ int32_t runs;
    __shared__ int32_t sums[THREADS];
    const int tid = threadIdx.x;
    if ((int64_t)blockIdx.x >= n_chunks) return;
    const Chunk c = chunks[blockIdx.x];
    const bool mine = SIZE == 4096 ? c.edges <= 4096 : c.edges > 4096;
    if (!mine) return;   // the other instance's chunk
-   if (tid < kBlockRows)
+   if (tid < kMostRows)
    {
-      const int64_t row = (int64_t)c.block * kBlockRows + tid;
+      const int64_t row = (int64_t)c.block * br + tid;
       int64_t len = 0;
-      if (row < m) len = chunk_length(index_at(pe, row, ib) - index_at(pb, row, ib), c.number);
+      if (tid < br && row < m) len = chunk_length(index_at(pe, row, ib) - index_at(pb, row, ib), c.number);
       start[tid + 1] = (int32_t)len;
-      if (tid == 0) start[0] = 0;
+      if (tid == 0) start[0] = runs = 0;
    }
    __syncthreads();
    if (tid == 0)
-      for (int r = 0; r < kBlockRows; r++) start[r + 1] += start[r];
+      for (int r = 0; r < kMostRows; r++) start[r + 1] += start[r];
    __syncthreads();
-   const int total = start[kBlockRows] < SIZE ? start[kBlockRows] : SIZE;
+   const int total = start[kMostRows] < SIZE ? start[kMostRows] : SIZE;
    int size = 64;
    while (size < total) size <<= 1;
    for (int e = tid; e < size; e += THREADS)
@@ -113,7 +121,7 @@ __global__ __launch_bounds__(THREADS) void plan_fill(const Chunk *chunks, int64_
 #pragma unroll
          for (int s = 32; s; s >>= 1)
             if (start[r + s] <= e) r += s;
-         const int64_t row = (int64_t)c.block * kBlockRows + r;
+         const int64_t row = (int64_t)c.block * br + r;
          const int64_t col = index_at(indx, index_at(pb, row, ib) + (int64_t)c.number * kChunkSlots + (e - start[r]), ib);
          if (col >= 0 && col < n) k = ((uint32_t)col << 6) | (uint32_t)r;   // any other id names no column
       }
@@ -154,6 +162,7 @@ __global__ __launch_bounds__(THREADS) void plan_fill(const Chunk *chunks, int64_
       __syncthreads();
    }
    int64_t to = c.at + sums[tid] - count;
+   int in_runs = 0;   // columns, counted once for every run of 16 rows that names them
    for (int e = lo; e < hi; e++)
       if (starts(e))
       {
@@ -163,11 +172,14 @@ __global__ __launch_bounds__(THREADS) void plan_fill(const Chunk *chunks, int64_
          cols[to] = (int32_t)(k >> 6);
          masks[to] = bits;
          to++;
+         for (int w = 0; w < 4; w++) in_runs += ((bits >> (16 * w)) & 0xffff) != 0;
       }
-   if (tid == THREADS - 1) counts[blockIdx.x] = sums[tid];
+   atomicAdd(&runs, in_runs);   // (whole numbers: the order does not matter)
+   __syncthreads();
+   if (tid == THREADS - 1) counts[blockIdx.x] = make_int2(sums[tid], runs);
 }
 
-__global__ __launch_bounds__(256) void plan_pack(const Piece *pieces, const int32_t *cols, const uint64_t *masks, int32_t *to_cols, uint16_t *to_masks)
+__global__ __launch_bounds__(256) void plan_pack(const Piece *pieces, int waves, const int32_t *cols, const uint64_t *masks, int32_t *to_cols, uint16_t *to_masks)
 {
    const Piece p = pieces[blockIdx.x];
    for (int e = threadIdx.x; e < p.end; e += 256)
@@ -176,8 +188,7 @@ __global__ __launch_bounds__(256) void plan_pack(const Piece *pieces, const int3
       const int64_t to = p.to + e;
       to_cols[to] = live ? cols[p.from + e] : -1;
       const uint64_t bits = live ? masks[p.from + e] : 0;
-#pragma unroll
-      for (int w = 0; w < 4; w++) to_masks[(to / kTile) * (4 * kTile) + w * kTile + to % kTile] = (uint16_t)(bits >> (16 * w));
+      for (int w = 0; w < waves; w++) to_masks[(to / kTile) * (waves * kTile) + w * kTile + to % kTile] = (uint16_t)(bits >> (16 * w));
    }
 }
 
@@ -195,14 +206,14 @@ template <class X> int upload(Memory &to, const std::vector<X> &v)
    return kOk;
 }
 
-}  // namespace
-
-int plan_create(Plan *plan, int64_t m, int64_t n, int64_t nnz, const void *indx, const void *pb, const void *pe, int ib, hipStream_t stream)
+// with blocks of br rows; *shared: false where blocks of 64 rows share too little (nothing is built then)
+int build(Plan *plan, int br, bool *shared, int64_t m, int64_t n, int64_t nnz, const void *indx, const void *pb, const void *pe, int ib, hipStream_t stream)
 {
+   *shared = true;
    ATTN_HIP(hipGetDevice(&plan->device));
    plan->rows = m;
    plan->cols = n;
-   const int64_t blocks = (m + kBlockRows - 1) / kBlockRows;
+   const int64_t blocks = (m + br - 1) / br;
    std::vector<int64_t> longest((size_t)blocks), edges((size_t)blocks);
    if (blocks)
    {
@@ -212,7 +223,7 @@ int plan_create(Plan *plan, int64_t m, int64_t n, int64_t nnz, const void *indx,
       int64_t *d = (int64_t *)scratch.p;
       int *bad = (int *)(d + 2 * blocks);
       ATTN_HIP(hipMemsetAsync(bad, 0, 16, stream));
-      hipLaunchKernelGGL(plan_count, dim3((unsigned)((blocks + 3) / 4)), dim3(256), 0, stream, m, blocks, pb, pe, ib, d, d + blocks, bad);
+      hipLaunchKernelGGL(plan_count, dim3((unsigned)((blocks + 3) / 4)), dim3(256), 0, stream, m, br, blocks, pb, pe, ib, d, d + blocks, bad);
       ATTN_HIP(hipGetLastError());
       int is_bad = 0;
       ATTN_HIP(hipMemcpyAsync(longest.data(), d, (size_t)blocks * 8, hipMemcpyDeviceToHost, stream));
@@ -242,14 +253,14 @@ int plan_create(Plan *plan, int64_t m, int64_t n, int64_t nnz, const void *indx,
       }
    int64_t at = 0;
    bool small = false, large = false;
-   std::vector<int32_t> counts(chunks.size());
+   std::vector<int2> counts(chunks.size());
    Memory d_chunks, d_cols, d_masks, d_counts;
    if (!chunks.empty())
    {
       int st = upload(d_chunks, chunks);
       if (st) return st;
       hipLaunchKernelGGL(plan_chunk_edges, dim3((unsigned)((chunks.size() + 3) / 4)), dim3(256), 0, stream, (Chunk *)d_chunks.p,
-                         (int64_t)chunks.size(), m, pb, pe, ib);
+                         (int64_t)chunks.size(), m, br, pb, pe, ib);
       ATTN_HIP(hipGetLastError());
       ATTN_HIP(hipMemcpyAsync(chunks.data(), d_chunks.p, chunks.size() * sizeof(Chunk), hipMemcpyDeviceToHost, stream));
       ATTN_HIP(hipStreamSynchronize(stream));
@@ -262,18 +273,29 @@ int plan_create(Plan *plan, int64_t m, int64_t n, int64_t nnz, const void *indx,
       ATTN_HIP(hipMemcpy(d_chunks.p, chunks.data(), chunks.size() * sizeof(Chunk), hipMemcpyHostToDevice));
       st = d_cols.get((size_t)at * 4);
       if (!st) st = d_masks.get((size_t)at * 8);
-      if (!st) st = d_counts.get(chunks.size() * 4);
+      if (!st) st = d_counts.get(chunks.size() * sizeof(int2));
       if (st) return st;
       const dim3 grid((unsigned)chunks.size());
       if (small)
-         hipLaunchKernelGGL((plan_fill<4096, 256>), grid, dim3(256), 0, stream, (const Chunk *)d_chunks.p, (int64_t)chunks.size(), m, n, indx, pb, pe, ib,
-                            (int32_t *)d_cols.p, (uint64_t *)d_masks.p, (int32_t *)d_counts.p);
+         hipLaunchKernelGGL((plan_fill<4096, 256>), grid, dim3(256), 0, stream, (const Chunk *)d_chunks.p, (int64_t)chunks.size(), m, br, n, indx, pb, pe, ib,
+                            (int32_t *)d_cols.p, (uint64_t *)d_masks.p, (int2 *)d_counts.p);
       if (large)
-         hipLaunchKernelGGL((plan_fill<kBlockRows * kChunkSlots, 1024>), grid, dim3(1024), 0, stream, (const Chunk *)d_chunks.p,
-                            (int64_t)chunks.size(), m, n, indx, pb, pe, ib, (int32_t *)d_cols.p, (uint64_t *)d_masks.p, (int32_t *)d_counts.p);
+         hipLaunchKernelGGL((plan_fill<kMostRows * kChunkSlots, 1024>), grid, dim3(1024), 0, stream, (const Chunk *)d_chunks.p,
+                            (int64_t)chunks.size(), m, br, n, indx, pb, pe, ib, (int32_t *)d_cols.p, (uint64_t *)d_masks.p, (int2 *)d_counts.p);
       ATTN_HIP(hipGetLastError());
-      ATTN_HIP(hipMemcpyAsync(counts.data(), d_counts.p, chunks.size() * 4, hipMemcpyDeviceToHost, stream));
+      ATTN_HIP(hipMemcpyAsync(counts.data(), d_counts.p, chunks.size() * sizeof(int2), hipMemcpyDeviceToHost, stream));
       ATTN_HIP(hipStreamSynchronize(stream));
+      if (br == 64)
+      {
+         double columns = 0, runs = 0;
+         for (const int2 &c : counts)
+         {
+            columns += c.x;
+            runs += c.y;
+         }
+         *shared = runs >= kShare * columns;
+         if (!*shared) return kOk;
+      }
    }
 
    // Units.  A unit of many chunks has little to join, one of few leaves more workgroups: a chunk of full rows is 16
@@ -295,8 +317,8 @@ int plan_create(Plan *plan, int64_t m, int64_t n, int64_t nnz, const void *indx,
          const int64_t begin = to;
          for (size_t x = lo; x < hi; x++)
          {
-            pieces.push_back(Piece{chunks[x].at, to, counts[x], counts[x]});
-            to += counts[x];
+            pieces.push_back(Piece{chunks[x].at, to, counts[x].x, counts[x].x});
+            to += counts[x].x;
          }
          const int64_t padded = begin + (to - begin + kTile - 1) / kTile * kTile;
          if (padded != to) pieces.back().end += (int32_t)(padded - to);
@@ -317,7 +339,9 @@ int plan_create(Plan *plan, int64_t m, int64_t n, int64_t nnz, const void *indx,
    plan->tiles = to / kTile;
    plan->parts = parts;
    auto up = [](size_t v) { return (v + 255) & ~(size_t)255; };
-   const size_t off_masks = up((size_t)to * 4), off_units = off_masks + up((size_t)to * 8), off_joins = off_units + up(units.size() * sizeof(Unit));
+   const int waves = br / 16;
+   // (a group of column ids and masks is read ahead as a whole: room for one behind the last tile)
+   const size_t off_masks = up((size_t)(to + kAhead * kTile) * 4), off_units = off_masks + up((size_t)(to + kAhead * kTile) * 2 * waves), off_joins = off_units + up(units.size() * sizeof(Unit));
    const size_t bytes = off_joins + up(joins.size() * sizeof(Join)) + 256;
    ATTN_HIP(hipMalloc(&plan->memory, bytes));
    unsigned char *base = (unsigned char *)plan->memory;
@@ -328,14 +352,23 @@ int plan_create(Plan *plan, int64_t m, int64_t n, int64_t nnz, const void *indx,
    {
       const int st = upload(d_pieces, pieces);
       if (st) return st;
-      hipLaunchKernelGGL(plan_pack, dim3((unsigned)pieces.size()), dim3(256), 0, stream, (const Piece *)d_pieces.p, (const int32_t *)d_cols.p,
+      hipLaunchKernelGGL(plan_pack, dim3((unsigned)pieces.size()), dim3(256), 0, stream, (const Piece *)d_pieces.p, waves, (const int32_t *)d_cols.p,
                          (const uint64_t *)d_masks.p, (int32_t *)base, (uint16_t *)(base + off_masks));
       ATTN_HIP(hipGetLastError());
    }
    ATTN_HIP(hipStreamSynchronize(stream));
    plan->view = PlanView{(const int32_t *)base, (const uint16_t *)(base + off_masks), (const Unit *)(base + off_units),
-                         (const Join *)(base + off_joins), (int32_t)units.size(), (int32_t)joins.size(), m, n};
+                         (const Join *)(base + off_joins), (int32_t)units.size(), (int32_t)joins.size(), m, n, br};
    return kOk;
+}
+
+}  // namespace
+
+int plan_create(Plan *plan, int64_t m, int64_t n, int64_t nnz, const void *indx, const void *pb, const void *pe, int ib, hipStream_t stream)
+{
+   bool shared;
+   const int st = build(plan, 64, &shared, m, n, nnz, indx, pb, pe, ib, stream);
+   return st || shared ? st : build(plan, 16, &shared, m, n, nnz, indx, pb, pe, ib, stream);
 }
 
 void plan_release(Plan *p)

@@ -191,7 +191,8 @@ template <int UNIT> __global__ __launch_bounds__(1024) void attn_rows_table(Rows
 template <int T, int DC, int MAPS> struct RowGeo {
    typedef Num<T> N;
    typedef typename N::E E;
-   static constexpr int W = DC * MAPS, LD = W + N::EPL, CR = W / N::EPL;
+   static constexpr int W = DC * MAPS, CR = W / N::EPL;
+   typedef TileView<T, W> V;
    static constexpr int CQ = DC / N::KC, NT = W / 16;
    static constexpr int HP = 16 / MAPS;               // query heads of a pass
    static constexpr int NV = kTile * CR / 64;         // 16-byte chunks of the values that a lane carries
@@ -211,7 +212,7 @@ __device__ inline void wave_lds_order()   // this wave's LDS writes before its l
 
 // scores (already times scale and log2 e) of 32 slots -> running maximum and sum, weights, and the weighted values
 template <class G, int T>
-__device__ inline void row_step(RowSums<G> &r, float (&w)[2][4], unsigned mine, const typename G::E *vs, int g, int i, bool odd)
+__device__ inline void row_step(RowSums<G> &r, float (&w)[2][4], unsigned mine, const unsigned char *vs, int g, int i, bool odd)
 {
    float mx = -INFINITY;
 #pragma unroll
@@ -237,16 +238,16 @@ __device__ inline void row_step(RowSums<G> &r, float (&w)[2][4], unsigned mine, 
    }
    r.sum = r.sum * keep + add;
    r.top = mx;
-   add_weighted<T, G::NT>(r.acc, w, mine, vs, G::LD, g, i, odd);
+   add_weighted<T, G::W, G::NT>(r.acc, w, mine, vs, 0, g, i, G::V::lane(g, i), odd);
 }
 
 // The four waves' sums -> the row's output, or its piece of the partial sums.  O: element type of the output.
 template <class G, int MAPS, int O>
-__device__ inline void rows_finish(const RowsParams &p, RowSums<G> &r, typename G::E *vs_all, float (*stat)[16][2], const Spot &s, int64_t id, int kvh, int pass)
+__device__ inline void rows_finish(const RowsParams &p, RowSums<G> &r, unsigned char *vs_all, float (*stat)[16][2], const Spot &s, int64_t id, int kvh, int pass)
 {
    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, g = lane >> 4, i = lane & 15;
    r.sum = group_sum(r.sum);
-   float *mine = reinterpret_cast<float *>(vs_all + wave * kTile * G::LD) + i * G::W;   // 16 columns x W floats fit 32 rows of values
+   float *mine = reinterpret_cast<float *>(vs_all + wave * G::V::kBytes) + i * G::W;   // 16 columns x W floats fit 32 rows of values
    wave_lds_order();
 #pragma unroll
    for (int x = 0; x < G::NT; x++) *reinterpret_cast<f4 *>(mine + 16 * x + 4 * g) = r.acc[x];
@@ -266,7 +267,7 @@ __device__ inline void rows_finish(const RowsParams &p, RowSums<G> &r, typename 
       {
          const float keep = exp2_fast(stat[w][c][0] - base);
          sum += stat[w][c][1] * keep;
-         x += reinterpret_cast<const float *>(vs_all + w * kTile * G::LD)[c * G::W + f] * keep;
+         x += reinterpret_cast<const float *>(vs_all + w * G::V::kBytes)[c * G::W + f] * keep;
       }
       return x;
    };
@@ -396,13 +397,13 @@ __global__ __launch_bounds__(256, (sizeof(typename Num<T>::E) * DC * MAPS >= 512
 {
    typedef RowGeo<T, DC, MAPS> G;
    typedef typename G::E E;
-   __shared__ __align__(16) E vs_all[4 * kTile * G::LD];
+   __shared__ __align__(16) unsigned char vs_all[4 * G::V::kBytes];
    __shared__ float stat[4][16][2];
    const RowsItem it = rows_item(p);
    const Spot s = find_piece(p, it.id, 0);
    if (s.row < 0) return;
    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, g = lane >> 4, i = lane & 15;
-   E *vs = vs_all + wave * kTile * G::LD;
+   unsigned char *vs = vs_all + wave * G::V::kBytes;
    const int64_t begin = index_of(p.pntrb, s.row, p.index_bytes), len = row_length(p, s.row);
    const int64_t lo = s.count > 1 ? (it.id - s.first) * s.piece : 0, hi = s.count > 1 && lo + s.piece < len ? lo + s.piece : len;
    const E *k = (const E *)p.k + it.kvh * p.hdk, *v = (const E *)p.v + it.kvh * p.hdv;
@@ -463,7 +464,7 @@ __global__ __launch_bounds__(256, (sizeof(typename Num<T>::E) * DC * MAPS >= 512
       for (int j = 0; j < G::NV; j++)
       {
          const int e = lane + 64 * j;
-         *reinterpret_cast<u4 *>(vs + (e / G::CR) * G::LD + (e % G::CR) * G::N::EPL) = vf[j];
+         *reinterpret_cast<u4 *>(vs + (e / G::CR) * G::V::RB + ((e % G::CR) ^ G::V::twist(e / G::CR)) * 16) = vf[j];
          odd |= odd_chunk<T>(vf[j]);
       }
       odd = __any(odd);
@@ -560,15 +561,14 @@ template <int DC, int MAPS, bool FULL>
 __global__ __launch_bounds__(256, (DC * MAPS >= 256 ? 1 : 2)) void attn_rows_kv4(RowsParams p)
 {
    typedef RowGeo<kF16, DC, MAPS> G;
-   typedef uint16_t E;
    constexpr int WQ = DC / 32, WV = G::W / 32;   // 4-byte words of codes that a lane reads of one map's key, of a value row
-   __shared__ __align__(16) E vs_all[4 * kTile * G::LD];
+   __shared__ __align__(16) unsigned char vs_all[4 * G::V::kBytes];
    __shared__ float stat[4][16][2];
    const RowsItem it = rows_item(p);
    const Spot s = find_piece(p, it.id, 0);
    if (s.row < 0) return;
    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, g = lane >> 4, i = lane & 15;
-   E *vs = vs_all + wave * kTile * G::LD;
+   unsigned char *vs = vs_all + wave * G::V::kBytes;
    const int64_t begin = index_of(p.pntrb, s.row, p.index_bytes), len = row_length(p, s.row);
    const int64_t lo = s.count > 1 ? (it.id - s.first) * s.piece : 0, hi = s.count > 1 && lo + s.piece < len ? lo + s.piece : len;
    const uint8_t *cache = p.cache + it.kvh * p.hdc;
@@ -668,7 +668,7 @@ __global__ __launch_bounds__(256, (DC * MAPS >= 256 ? 1 : 2)) void attn_rows_kv4
 #pragma unroll
          for (int j = 0; j < WV; j++)
          {
-            *reinterpret_cast<u4 *>(vs + (16 * a + i) * G::LD + code_feature<FULL, WV>(j, g)) = dequant8(vc[a][j], vw[a][j]);
+            *reinterpret_cast<u4 *>(vs + (16 * a + i) * G::V::RB + ((code_feature<FULL, WV>(j, g) / 8) ^ G::V::twist(i)) * 16) = dequant8(vc[a][j], vw[a][j]);
             odd |= (vw[a][j] & 0x7C00u) == 0x7C00u;   // an infinite or NaN scale
          }
       }
