@@ -231,6 +231,9 @@ template <int T> __device__ inline typename Num<T>::TFrag without_odd(typename N
    return v;
 }
 
+// No load moves over this: the rare path below would otherwise load ahead into registers that set the kernels' occupancy.
+__device__ inline void keep_order() { asm volatile("" ::: "memory"); }
+
 // What the tile's infinities and NaN add: a matrix instruction would multiply them by the zero weights of rows that do not
 // name them, so it runs without them (without_odd) and every row adds those of the gathered rows that it does name.
 // Rows that name none keep the bits they have without them.
@@ -250,31 +253,55 @@ __device__ inline void add_odd(f4 (&acc)[NT], const float (&p)[2][4], unsigned m
       if (!named) continue;
 #pragma unroll
       for (int t = 0; t < NT; t++)
+      {
 #pragma unroll
          for (int k = 0; k < 4; k++)
          {
             const typename Num<T>::E e = TileView<T, W>::element(tile, key, f0 + 16 * t + 4 * g + k);
             if (odd_element<T>(e)) acc[t][k] = fmaf(w, Num<T>::to(e), acc[t][k]);
          }
+         keep_order();
+      }
    }
 }
 
-// acc += (weights of the tile's 32 rows) x (their features f0 .. f0 + 16 NT - 1); odd: the tile may hold infinities or NaN
-template <int T, int W, int NT>
-__device__ inline void add_weighted(f4 (&acc)[NT], const float (&p)[2][4], unsigned mine, const unsigned char *tile, int f0, int g, int i, const typename TileView<T, W>::Lane &l, bool odd)
+// acc += (weights of the tile's 32 rows) x (their features f0 .. f0 + 16 NT - 1); CAREFUL: the tile may hold infinities or NaN
+template <int T, int W, bool CAREFUL, int NT>
+__device__ inline void add_weighted(f4 (&acc)[NT], const float (&p)[2][4], unsigned mine, const unsigned char *tile, int f0, int g, int i, const typename TileView<T, W>::Lane &l)
 {
    typedef TileView<T, W> V;
    const typename Num<T>::TFrag b = pack_scores<T>(p);
-   if (__builtin_expect(odd, 0))
+   if constexpr (CAREFUL)
    {
 #pragma unroll
-      for (int t = 0; t < NT; t++) acc[t] = Num<T>::mma_t(without_odd<T>(V::transposed(tile, f0 / 16 + t, l)), b, acc[t]);
+      for (int t = 0; t < NT; t++)
+      {
+         acc[t] = Num<T>::mma_t(without_odd<T>(V::transposed(tile, f0 / 16 + t, l)), b, acc[t]);
+         keep_order();
+      }
       add_odd<T, W, NT>(acc, p, mine, tile, f0, g, i);
-      return;
    }
+   else
+   {
 #pragma unroll
-   for (int t = 0; t < NT; t++) acc[t] = Num<T>::mma_t(V::transposed(tile, f0 / 16 + t, l), b, acc[t]);
+      for (int t = 0; t < NT; t++) acc[t] = Num<T>::mma_t(V::transposed(tile, f0 / 16 + t, l), b, acc[t]);
+   }
 }
+
+// Sums that are not finite may be the matrix instructions' zero times infinity: the work is then done again with CAREFUL.
+// Finite sums cannot be wrong in that way.
+template <int NT> __device__ inline bool odd_sums(const f4 (&acc)[NT])
+{
+   bool odd = false;
+#pragma unroll
+   for (int t = 0; t < NT; t++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) odd |= !(fabsf(acc[t][e]) < INFINITY);
+   return odd;
+}
+template <bool X> struct Flag {
+   static constexpr bool value = X;
+};
 
 // four consecutive features of an output row, f .. f+3 of `width`
 template <int T> __device__ inline void store4(typename Num<T>::E *row, int f, int width, f4 v, bool vec)
@@ -298,16 +325,76 @@ template <int T> __device__ inline void store4(typename Num<T>::E *row, int f, i
       if (f + k < width) row[f + k] = (E)Num<T>::from(v[k]);
 }
 
-__device__ inline float group_max(float x)   // over the four lane groups: the lanes of one resident row
+// over the four lane groups: the lanes of one resident row
+typedef unsigned int u2 __attribute__((ext_vector_type(2)));
+__device__ inline float group_max(float x)
 {
-   x = fmaxf(x, __shfl_xor(x, 16));
-   return fmaxf(x, __shfl_xor(x, 32));
+   const u2 a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+   x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+   const u2 b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+   return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 __device__ inline float group_sum(float x)
 {
-   x += __shfl_xor(x, 16);
-   return x + __shfl_xor(x, 32);
+   const u2 a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+   x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+   const u2 b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+   return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
+
+// scores whose bit of `mine` is clear -> `other`
+__device__ inline float masked(float x, unsigned mine, int j, float other)
+{
+   const unsigned m = (unsigned)((int)(mine << (31 - j)) >> 31);
+   return __uint_as_float((__float_as_uint(x) & m) | (__float_as_uint(other) & ~m));
+}
+
+// The score factor, times log2(e) and made positive (a negative one changes the sign of the resident queries instead, so
+// that the largest product is the largest score) and not zero (a masked score of minus infinity stays one).
+__device__ inline float score_factor(float scale) { return fmaxf(fabsf(scale) * kLog2e, 1.17549435e-38f); }
+template <int T> __device__ inline u4 negated(u4 v)
+{
+   const uint32_t m = T == kF32 ? 0x80000000u : 0x80008000u;
+   return u4{v[0] ^ m, v[1] ^ m, v[2] ^ m, v[3] ^ m};
+}
+
+// Running softmax of one resident row per lane.  The sums are relative to 2^base; base follows the largest score only when
+// that runs ahead by more than 2^8, so that most tiles rescale nothing: weights are then at most 256, and one of them
+// was 1 when base was set.
+template <int NT> struct Softmax {
+   f4 acc[NT];
+   float base, sum;
+   __device__ inline void clear()
+   {
+      base = -INFINITY;
+      sum = 0;
+#pragma unroll
+      for (int t = 0; t < NT; t++) acc[t] = f4{0, 0, 0, 0};
+   }
+   // products s (masked ones -infinity) -> weights
+   __device__ inline void weights(float (&w)[2][4], const f4 (&s)[2], float c2)
+   {
+      float mx = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < 8; j++) mx = fmaxf(mx, s[j / 4][j % 4]);
+      mx = group_max(mx) * c2;
+      if (__any(mx > base + 8.0f))
+      {
+         const float to = mx > base + 8.0f ? mx : base, keep = to == base ? 1.0f : exp2_fast(base - to);
+#pragma unroll
+         for (int t = 0; t < NT; t++) acc[t] *= keep;
+         sum *= keep;
+         base = to;
+      }
+      const float from = base == -INFINITY ? 0.0f : base;   // nothing named so far: every weight is exp2(-infinity)
+#pragma unroll
+      for (int j = 0; j < 8; j++)
+      {
+         w[j / 4][j % 4] = exp2_fast(fmaf(s[j / 4][j % 4], c2, -from));
+         sum += w[j / 4][j % 4];   // of this lane's columns: the four groups are added at the end
+      }
+   }
+};
 
 // Workgroups go round-robin to the 8 XCDs.  Work item of workgroup b of n items: every XCD takes a contiguous eighth, so
 // that the items of one head (whose gathered rows overlap) meet in one L2.  Items at or past n have no work.

@@ -64,8 +64,7 @@ int check_heads(const char *who, const Desc &d)
 
 bool strides_ok(int64_t ld, int64_t hd)
 {
-   const int64_t most = (int64_t)1 << 48;
-   return ld >= 0 && hd >= 0 && ld < most && hd < most;
+   return ld >= 0 && hd >= 0 && ld < ((int64_t)1 << 29) && hd < ((int64_t)1 << 48);   // a row's bytes fit 32 bits
 }
 
 // (row, head) pieces of `width` elements that do not overlap: packed rows, or whole heads
@@ -126,7 +125,7 @@ int check_device(const char *who, const void *plan)
 }
 
 struct Layout {   // of a workspace, in bytes
-   int64_t delta = 0, dlam = 0, part = 0, total = 0;
+   int64_t stats = 0, dlam = 0, part = 0, total = 0;
 };
 
 Layout forward_layout(const Desc &d, const Plan &p, int dc)
@@ -139,7 +138,7 @@ Layout forward_layout(const Desc &d, const Plan &p, int dc)
 Layout backward_layout(const Desc &d, const Plan &p, const Plan &t, int dc)
 {
    Layout l;
-   l.dlam = align256(d.m * d.heads * d.maps * 4);
+   l.dlam = align256(d.m * d.heads * d.maps * 8);
    l.part = l.dlam + (d.maps == 2 ? align256(d.m * d.heads * 4) : 0);
    l.total = l.part + std::max(p.parts * d.heads * dq_part(dc, d.maps, p.view.block_rows), t.parts * d.kv_heads * dkv_part(dc, d.maps, t.view.block_rows)) * 4;
    return l;
@@ -177,6 +176,13 @@ Params base_params(const Desc &d, const Plan &plan)
    p.hdv = d.hdv;
    p.ldo = d.ldo;
    p.hdo = d.hdo;
+   const int bytes = element_bytes(d);
+   p.ldq_bytes = (int32_t)(d.ldq * bytes);
+   p.ldk_bytes = (int32_t)(d.ldk * bytes);
+   p.ldv_bytes = (int32_t)(d.ldv * bytes);
+   p.ldo_bytes = (int32_t)(d.ldo * bytes);
+   const int dc = width_class(d.d, d.dv, d.maps);
+   p.full = d.d == dc && d.dv == dc * d.maps;
    return p;
 }
 
@@ -476,7 +482,7 @@ int fusedMM_attn_backward(const fusedMM_attn_desc *desc, const void *plan, const
    p.dk = dk;
    p.dvv = dv;
    p.dlambda = d.maps == 2 ? dlambda : nullptr;
-   p.delta = (float *)((unsigned char *)work + l.delta);
+   p.stats = (float *)((unsigned char *)work + l.stats);
    p.dlam_rows = (float *)((unsigned char *)work + l.dlam);
    p.part = (float *)((unsigned char *)work + l.part);
    const hipStream_t s = (hipStream_t)stream;

@@ -27,8 +27,8 @@ struct Join {         // a block of several units: partial sums part0 .. part0 +
 constexpr int kAhead = 8;   // tiles of a group of column ids and masks; the arrays of a plan are padded by a group
 
 struct PlanView {
-   const int32_t *cols;    // [tiles][32], -1: no column
-   const uint16_t *masks;  // [tiles][BR / 16 waves][32]: bit r is row 16 * wave + r of the block
+   const int32_t *cols;    // [tiles][32]; behind a unit's last column that column again, named by no row
+   const uint32_t *masks;  // [tiles][BR]: row r of the block; bit 8g + 4a + r is the tile's column 16a + 4g + r, as the lanes hold them
    const Unit *units;
    const Join *joins;
    int32_t n_units, n_joins;
@@ -42,7 +42,9 @@ struct Params {
    int32_t heads, kv_heads, group, d, dv;
    float scale;
    int64_t ldq, hdq, ldk, hdk, ldv, hdv, ldo, hdo;
+   int32_t ldk_bytes, ldv_bytes, ldq_bytes, ldo_bytes;
    int32_t vec;                       // every row of every tensor is 16-byte aligned and d, dv are multiples of a 16-byte chunk
+   int32_t full;                      // d and dv fill the instance's width
    const void *q, *k, *v, *o, *o2, *dout;
    const float *lambda;
    const float *lse_in;
@@ -50,12 +52,12 @@ struct Params {
    float *lse;                        // may be null
    void *dq, *dk, *dvv;
    float *dlambda;
-   float *delta;                      // [m][heads][maps]
+   float *stats;                      // [m][heads][2 maps]: lse * log2(e) of every map, delta of every map
    float *dlam_rows;                  // [m][heads]: sum_j P_2 dP
    float *part;                       // partial sums of split blocks
 };
 
-__device__ u4 zero_chunk;   // what lanes without a column or a feature load
+__device__ u4 zero_chunk;   // what lanes whose chunk is behind the features load
 
 template <int T, int DC, int MAPS, int BR> struct Geo {
    typedef Num<T> N;
@@ -73,8 +75,8 @@ template <int T, int DC, int MAPS, int BR> struct Geo {
    // (six of one wave) fit a compute unit's 160 KB.
    static constexpr int kPair = 2 * V::kBytes;
    static constexpr int S = BR == 64 ? (kPair <= 16384 ? 4 : 2) : (kPair <= 4096 ? 4 : kPair <= 8192 ? 3 : 2);
-   static constexpr int kMaskBytes = WAVES * kTile * 2;    // of a tile
-   static constexpr int kStat = 2 * MAPS * kTile * 4;      // lse and delta of a tile's rows (dk, dv)
+   static constexpr int kMaskBytes = BR * 4;               // of a tile
+   static constexpr int kStat = 2 * MAPS * kTile * 4;      // statistics of a tile's rows (dk, dv)
 };
 
 template <int N> __device__ inline void wait_loads()   // all but the N newest loads have arrived, LDS operations are done
@@ -91,11 +93,11 @@ template <int BR> __device__ inline void tile_barrier()
 // or earlier ones and only get stricter.
 __device__ inline void load_lds16(uint32_t base, const void *from)
 {
-   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(base), "v"(from) : "memory");
+   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(__builtin_amdgcn_readfirstlane(base)), "v"(from) : "memory");
 }
 __device__ inline void load_lds4(uint32_t base, const void *from)
 {
-   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(base), "v"(from) : "memory");
+   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(__builtin_amdgcn_readfirstlane(base)), "v"(from) : "memory");
 }
 __device__ inline uint32_t lds_address(const void *p)
 {
@@ -110,35 +112,35 @@ template <class G, int T, int DC, int BR> struct Stream {
    const unsigned char *tiles;   // LDS: [S][a, b] tiles
    unsigned char *ids, *bits;    // LDS: two groups of column ids, of masks
    const int32_t *cols;          // of the unit
-   const uint16_t *masks;
+   const uint32_t *masks;
    int tid, wave;
    const E *a, *b;
-   int64_t lda, ldb;
+   uint32_t lda, ldb;            // bytes from row to row
    int d, dv;
-   bool vec;
+   bool vec, full;
 
    // a: rows of maps pieces of d features each; b: rows of dv features
-   __device__ inline void set(const unsigned char *t, unsigned char *i, unsigned char *m, const PlanView &plan, const Unit &u, const E *a_, int64_t lda_, int d_,
-                              const E *b_, int64_t ldb_, int dv_, bool vec_)
+   __device__ inline void set(const unsigned char *t, unsigned char *i, unsigned char *m, const Params &p, const Unit &u, const E *a_, int lda_, const E *b_, int ldb_)
    {
       tiles = t;
       ids = i;
       bits = m;
-      cols = plan.cols + (int64_t)u.tile0 * kTile;
-      masks = plan.masks + (int64_t)u.tile0 * (G::WAVES * kTile);
+      cols = p.plan.cols + (int64_t)u.tile0 * kTile;
+      masks = p.plan.masks + (int64_t)u.tile0 * BR;
       tid = threadIdx.x;
       wave = __builtin_amdgcn_readfirstlane(tid >> 6);
       a = a_;
       b = b_;
       lda = lda_;
       ldb = ldb_;
-      d = d_;
-      dv = dv_;
-      vec = vec_;
+      d = p.d;
+      dv = p.dv;
+      vec = p.vec;
+      full = p.full;
    }
 
    // column ids and masks of tiles 8 g .. 8 g + 7; waves 0 and 1 (the ones that always load tiles) do it
-   __device__ inline void load_ids(int g) const
+   __device__ __forceinline__ void load_ids(int g) const
    {
       const uint32_t to_ids = lds_address(ids + (g & 1) * (kAhead * kTile * 4)), to_bits = lds_address(bits + (g & 1) * (kAhead * G::kMaskBytes));
       const unsigned char *from = (const unsigned char *)masks + (int64_t)g * (kAhead * G::kMaskBytes);
@@ -158,24 +160,14 @@ template <class G, int T, int DC, int BR> struct Stream {
    {
       return (const int32_t *)(ids + ((t / kAhead) & 1) * (kAhead * kTile * 4) + (t % kAhead) * (kTile * 4));
    }
-   // this lane's bits: bit 4a + r for gathered row 16a + 4g + r and resident row i; named: of any lane of the wave
-   __device__ inline unsigned my_bits(int t, int g, int i, bool *named) const
+   // which of the tile's columns resident row i names
+   __device__ inline uint32_t row_mask(int t, int i) const
    {
-      const uint16_t *m = (const uint16_t *)(bits + ((t / kAhead) & 1) * (kAhead * G::kMaskBytes) + (t % kAhead) * G::kMaskBytes) + wave * kTile + 4 * g;
-      const uint64_t m0 = *(const uint64_t *)m, m1 = *(const uint64_t *)(m + 16);
-      *named = __any((m0 | m1) != 0);
-      unsigned b = 0;
-#pragma unroll
-      for (int r = 0; r < 4; r++)
-      {
-         b |= ((unsigned)(m0 >> (16 * r)) >> i & 1) << r;
-         b |= ((unsigned)(m1 >> (16 * r)) >> i & 1) << (4 + r);
-      }
-      return b;
+      return *(const uint32_t *)(bits + ((t / kAhead) & 1) * (kAhead * G::kMaskBytes) + (t % kAhead) * G::kMaskBytes + (wave * 16 + i) * 4);
    }
 
    // tile t -> buffer; a and b may be moved (other heads) between calls
-   __device__ inline void load_tile(int t, int buf, const E *pa, const E *pb) const
+   __device__ __forceinline__ void load_tile(int t, int buf, const E *pa, const E *pb) const
    {
       const int32_t *c = tile_ids(t);
       const unsigned char *ta = tiles + buf * G::kPair, *tb = ta + V::kBytes;
@@ -187,20 +179,28 @@ template <class G, int T, int DC, int BR> struct Stream {
       {
          const int x = me + G::THREADS * j, r = x / G::CR;
          if (kTile * G::CR < G::THREADS && x >= kTile * G::CR) break;
-         const int32_t col = c[r];
+         const uint32_t col = (uint32_t)c[r];
          const int e = ((x % G::CR) ^ V::twist(r)) * G::N::EPL, f = e % DC;   // this thread's chunk of a gathered row
-         const E *fa = pa + (int64_t)col * lda + (e / DC * d + f), *fb = pb + (int64_t)col * ldb + e;
-         const bool live_a = col >= 0 && f < d, live_b = col >= 0 && e < dv;
+         const E *fa = (const E *)((const unsigned char *)pa + (uint64_t)col * lda) + (e / DC * d + f);
+         const E *fb = (const E *)((const unsigned char *)pb + (uint64_t)col * ldb) + e;
          if (vec)
          {
-            load_lds16(la + j * (G::THREADS * 16), live_a ? (const void *)fa : (const void *)&zero_chunk);
-            load_lds16(lb + j * (G::THREADS * 16), live_b ? (const void *)fb : (const void *)&zero_chunk);
+            if (full)
+            {
+               load_lds16(la + j * (G::THREADS * 16), fa);
+               load_lds16(lb + j * (G::THREADS * 16), fb);
+            }
+            else
+            {
+               load_lds16(la + j * (G::THREADS * 16), f < d ? (const void *)fa : (const void *)&zero_chunk);
+               load_lds16(lb + j * (G::THREADS * 16), e < dv ? (const void *)fb : (const void *)&zero_chunk);
+            }
          }
          else
          {
             // rows at any place, ends of rows within a chunk: element by element through registers
-            *(u4 *)(ta + x * 16) = load_chunk<T>(fa, live_a ? (d - f < G::N::EPL ? d - f : G::N::EPL) : 0, false);
-            *(u4 *)(tb + x * 16) = load_chunk<T>(fb, live_b ? (dv - e < G::N::EPL ? dv - e : G::N::EPL) : 0, false);
+            *(u4 *)(ta + x * 16) = load_chunk<T>(fa, d - f < G::N::EPL ? d - f : G::N::EPL, false);
+            *(u4 *)(tb + x * 16) = load_chunk<T>(fb, dv - e < G::N::EPL ? dv - e : G::N::EPL, false);
          }
       }
    }
@@ -231,26 +231,14 @@ template <int T, int W, int CQ> __device__ inline void tile_scores(f4 (&s)[2], c
    }
 }
 
-// Sums that are not finite may be the matrix instructions' zero times infinity: the workgroup then runs its unit again
-// with add_odd.  Finite sums cannot be wrong in that way.
 template <int BR> __device__ inline bool any_odd(bool odd)
 {
    if constexpr (BR == 16) return __any(odd);
    else return __syncthreads_or(odd);
 }
-template <int NT> __device__ inline bool odd_sums(const f4 (&acc)[NT])
-{
-   bool odd = false;
-#pragma unroll
-   for (int t = 0; t < NT; t++)
-#pragma unroll
-      for (int e = 0; e < 4; e++) odd |= !(fabsf(acc[t][e]) < INFINITY);
-   return odd;
-}
-
 // The loop over a unit's tiles that all kernels share: fill the pipeline, then for every step wait, free the oldest
 // buffer, fill it, and use the current one.  steps = tiles * per_tile; load(step, buffer), use(step, buffer).
-template <class G, int BR, class S, class Load, class Use> __device__ inline void for_tiles(const S &st, int steps, int per_tile, Load load, Use use)
+template <class G, int BR, class S, class Load, class Use> __device__ __forceinline__ void for_tiles(const S &st, int steps, int per_tile, Load load, Use use)
 {
    if (steps > 0)
    {
@@ -301,31 +289,32 @@ template <int T, int DC, int MAPS, int BR> __global__ __launch_bounds__(BR * 4, 
    const int64_t row = (int64_t)u.block * BR + 16 * wave + i;
    const bool live = row < p.m;
    Stream<G, T, DC, BR> st;
-   st.set(lds, lds_ids, lds_bits, p.plan, u, (const E *)p.k + kvh * p.hdk, p.ldk, p.d, (const E *)p.v + kvh * p.hdv, p.ldv, p.dv, p.vec);
+   st.set(lds, lds_ids, lds_bits, p, u, (const E *)p.k + kvh * p.hdk, p.ldk_bytes, (const E *)p.v + kvh * p.hdv, p.ldv_bytes);
 
    u4 qr[MAPS][G::CQ];
 #pragma unroll
    for (int mp = 0; mp < MAPS; mp++)
       load_resident<T, G::CQ>(qr[mp], (const E *)p.q + (live ? row : 0) * p.ldq + head * p.hdq + mp * p.d, live, p.d, g, p.vec);
-   const float c2 = p.scale * kLog2e;
-   f4 acc[MAPS][G::NT];
-   float top[MAPS], sum[MAPS];
-   for (int careful = 0; careful < 2; careful++)
+   const float c2 = score_factor(p.scale);
+   if (p.scale < 0)
    {
 #pragma unroll
       for (int mp = 0; mp < MAPS; mp++)
-      {
-         top[mp] = -INFINITY;
-         sum[mp] = 0;
 #pragma unroll
-         for (int t = 0; t < G::NT; t++) acc[mp][t] = f4{0, 0, 0, 0};
-      }
+         for (int c = 0; c < G::CQ; c++) qr[mp][c] = negated<T>(qr[mp][c]);
+   }
+   Softmax<G::NT> soft[MAPS];
+   auto pass = [&](auto careful) {
+      constexpr bool CAREFUL = decltype(careful)::value;
+#pragma unroll
+      for (int mp = 0; mp < MAPS; mp++) soft[mp].clear();
       for_tiles<G, BR>(
-         st, u.tiles, 1, [&](int t, int buf) { st.load_tile(t, buf, st.a, st.b); },
-         [&](int t, int buf) {
-            bool named;
-            const unsigned mine = st.my_bits(t, g, i, &named);
-            if (!named) return;
+         st, u.tiles, 1, [&](int t, int buf) __attribute__((always_inline)) { st.load_tile(t, buf, st.a, st.b); },
+         [&](int t, int buf) __attribute__((always_inline)) {
+            const uint32_t word = st.row_mask(t, i);
+            if (!__any(word != 0)) return;
+            const bool all = __all(word == 0xffffffffu);   // most tiles of a window: nothing to mask
+            const unsigned mine = (word >> (8 * g)) & 255;
             const typename G::V::Lane l = G::V::lane(g, i);
             const unsigned char *ks = lds + buf * G::kPair, *vs = ks + G::V::kBytes;
             float w[MAPS][2][4];
@@ -334,35 +323,17 @@ template <int T, int DC, int MAPS, int BR> __global__ __launch_bounds__(BR * 4, 
             {
                f4 s[2];
                tile_scores<T, G::W, G::CQ>(s, ks, mp * G::MC, qr[mp], l);
-               float mx = -INFINITY;
-#pragma unroll
-               for (int j = 0; j < 8; j++)
-               {
-                  w[mp][j / 4][j % 4] = ((mine >> j) & 1) ? s[j / 4][j % 4] * c2 : -INFINITY;
-                  mx = fmaxf(mx, w[mp][j / 4][j % 4]);
-               }
-               mx = fmaxf(top[mp], group_max(mx));
-               const float base = mx == -INFINITY ? 0.0f : mx;   // nothing named so far: every weight below is exp2(-inf)
-               const float keep = exp2_fast(top[mp] - base);
-               float add = 0;
-#pragma unroll
-               for (int j = 0; j < 8; j++)
-               {
-                  w[mp][j / 4][j % 4] = exp2_fast(w[mp][j / 4][j % 4] - base);
-                  add += w[mp][j / 4][j % 4];
-               }
-               if (__any(mx != top[mp]))
+               if (!all)
                {
 #pragma unroll
-                  for (int x = 0; x < G::NT; x++) acc[mp][x] *= keep;
+                  for (int j = 0; j < 8; j++) s[j / 4][j % 4] = masked(s[j / 4][j % 4], mine, j, -INFINITY);
                }
-               sum[mp] = sum[mp] * keep + add;   // of this lane's columns: the four groups are added at the end
-               top[mp] = mx;
+               soft[mp].weights(w[mp], s, c2);
             }
-            if (__builtin_expect(careful, 0))
+            if constexpr (CAREFUL)
             {
 #pragma unroll
-               for (int mp = 0; mp < MAPS; mp++) add_weighted<T, G::W, G::NT>(acc[mp], w[mp], mine, vs, 0, g, i, l, true);
+               for (int mp = 0; mp < MAPS; mp++) add_weighted<T, G::W, true>(soft[mp].acc, w[mp], mine, vs, 0, g, i, l);
                return;
             }
             typename G::N::TFrag wf[MAPS];
@@ -373,19 +344,20 @@ template <int T, int DC, int MAPS, int BR> __global__ __launch_bounds__(BR * 4, 
             {
                const typename G::N::TFrag vt = G::V::transposed(vs, x, l);
 #pragma unroll
-               for (int mp = 0; mp < MAPS; mp++) acc[mp][x] = G::N::mma_t(vt, wf[mp], acc[mp][x]);
+               for (int mp = 0; mp < MAPS; mp++) soft[mp].acc[x] = G::N::mma_t(vt, wf[mp], soft[mp].acc[x]);
             }
          });
-      bool odd = odd_sums(acc[0]);
-      if constexpr (MAPS == 2) odd |= odd_sums(acc[1]);
-      if (!any_odd<BR>(odd)) break;
-   }
+      bool odd = odd_sums(soft[0].acc);
+      if constexpr (MAPS == 2) odd |= odd_sums(soft[1].acc);
+      return odd;
+   };
+   if (any_odd<BR>(pass(Flag<false>()))) (void)pass(Flag<true>());
 
 #pragma unroll
-   for (int mp = 0; mp < MAPS; mp++) sum[mp] = group_sum(sum[mp]);
+   for (int mp = 0; mp < MAPS; mp++) soft[mp].sum = group_sum(soft[mp].sum);
    if (u.part >= 0)
    {
-      // [part][head][map][BR rows][W + 2]: sums, then the running maximum and sum
+      // [part][head][map][BR rows][W + 2]: sums, then what they are relative to and the sum of weights
       float *to = p.part + (((int64_t)u.part * p.heads + head) * MAPS * BR + 16 * wave + i) * (G::W + 2);
 #pragma unroll
       for (int mp = 0; mp < MAPS; mp++)
@@ -394,11 +366,11 @@ template <int T, int DC, int MAPS, int BR> __global__ __launch_bounds__(BR * 4, 
 #pragma unroll
          for (int x = 0; x < G::NT; x++)
 #pragma unroll
-            for (int e = 0; e < 4; e++) r[16 * x + 4 * g + e] = acc[mp][x][e];
+            for (int e = 0; e < 4; e++) r[16 * x + 4 * g + e] = soft[mp].acc[x][e];
          if (g == 0)
          {
-            r[G::W] = top[mp];
-            r[G::W + 1] = sum[mp];
+            r[G::W] = soft[mp].base;
+            r[G::W + 1] = soft[mp].sum;
          }
       }
       return;
@@ -409,18 +381,18 @@ template <int T, int DC, int MAPS, int BR> __global__ __launch_bounds__(BR * 4, 
 #pragma unroll
    for (int mp = 0; mp < MAPS; mp++)
    {
-      inv[mp] = sum[mp] == 0.0f ? 0.0f : 1.0f / sum[mp];   // a row without edges is zero
-      if (p.lse && g == 0) p.lse[(row * p.heads + head) * MAPS + mp] = sum[mp] == 0.0f ? -INFINITY : (top[mp] + log2f(sum[mp])) * kLn2;
+      inv[mp] = soft[mp].sum == 0.0f ? 0.0f : 1.0f / soft[mp].sum;   // a row without edges is zero
+      if (p.lse && g == 0) p.lse[(row * p.heads + head) * MAPS + mp] = soft[mp].sum == 0.0f ? -INFINITY : (soft[mp].base + log2f(soft[mp].sum)) * kLn2;
    }
    E *out = (E *)p.out + row * p.ldo + head * p.hdo;
    E *out2 = MAPS == 2 && p.out2 ? (E *)p.out2 + row * p.ldo + head * p.hdo : nullptr;
 #pragma unroll
    for (int x = 0; x < G::NT; x++)
    {
-      f4 r = acc[0][x] * inv[0];
+      f4 r = soft[0].acc[x] * inv[0];
       if constexpr (MAPS == 2)
       {
-         const f4 r2 = acc[1][x] * inv[1];
+         const f4 r2 = soft[1].acc[x] * inv[1];
          if (out2) store4<T>(out2, 16 * x + 4 * g, p.dv, r2, p.vec);
          r -= lam * r2;
       }
@@ -488,7 +460,7 @@ template <int T, int DC, int MAPS> __global__ __launch_bounds__(256) void attn_f
 }
 
 // ---- backward ---------------------------------------------------------------------------------------------------------------------
-// delta_p = <do, O_p>: 16 lanes per (row, head).  With O_2 at hand, <do, O_1> = <do, o> + lambda <do, O_2>.
+// The statistics that both passes read, delta_p = <do, O_p> among them: 16 lanes per (row, head).  With O_2 at hand, <do, O_1> = <do, o> + lambda <do, O_2>.
 template <int T, int MAPS> __global__ __launch_bounds__(256) void attn_delta(Params p)
 {
    typedef typename Num<T>::E E;
@@ -514,13 +486,15 @@ template <int T, int MAPS> __global__ __launch_bounds__(256) void attn_delta(Par
       if constexpr (MAPS == 2) s2 += __shfl_xor(s2, k);
    }
    if (!live || lane) return;
-   float *to = p.delta + id * MAPS;
+   float *to = p.stats + id * (2 * MAPS);
+#pragma unroll
+   for (int mp = 0; mp < MAPS; mp++) to[mp] = p.lse_in[id * MAPS + mp] * kLog2e;
    if constexpr (MAPS == 2)
    {
-      to[0] = s + p.lambda[head] * s2;
-      to[1] = s2;
+      to[2] = s + p.lambda[head] * s2;
+      to[3] = s2;
    }
-   else to[0] = s;
+   else to[1] = s;
 }
 
 // dq: resident q and do of 16 rows per wave, gathered k and v; both maps share the gathered v and dP.
@@ -544,7 +518,7 @@ template <int T, int DC, int MAPS, int BR> __global__ __launch_bounds__(BR * 4, 
    const bool live = row < p.m;
    const int64_t srow = live ? row : 0;
    Stream<G, T, DC, BR> st;
-   st.set(lds, lds_ids, lds_bits, p.plan, u, (const E *)p.k + kvh * p.hdk, p.ldk, p.d, (const E *)p.v + kvh * p.hdv, p.ldv, p.dv, p.vec);
+   st.set(lds, lds_ids, lds_bits, p, u, (const E *)p.k + kvh * p.hdk, p.ldk_bytes, (const E *)p.v + kvh * p.hdv, p.ldv_bytes);
 
    u4 qr[MAPS][G::CQ], gr[G::CV];
    float lse2[MAPS], delta[MAPS], sign[MAPS], mean[MAPS];
@@ -552,16 +526,16 @@ template <int T, int DC, int MAPS, int BR> __global__ __launch_bounds__(BR * 4, 
    for (int mp = 0; mp < MAPS; mp++)
    {
       load_resident<T, G::CQ>(qr[mp], (const E *)p.q + srow * p.ldq + head * p.hdq + mp * p.d, live, p.d, g, p.vec);
-      lse2[mp] = p.lse_in[(srow * p.heads + head) * MAPS + mp] * kLog2e;
-      delta[mp] = p.delta[(srow * p.heads + head) * MAPS + mp];
+      lse2[mp] = p.stats[(srow * p.heads + head) * (2 * MAPS) + mp];
+      delta[mp] = p.stats[(srow * p.heads + head) * (2 * MAPS) + MAPS + mp];
       sign[mp] = mp == 0 ? 1.0f : -p.lambda[head];
    }
    load_resident<T, G::CV>(gr, (const E *)p.dout + srow * p.ldo + head * p.hdo, live, p.dv, g, p.vec);
 
    const float c2 = p.scale * kLog2e;
    f4 acc[MAPS][G::NTQ], pk[kMend ? MAPS : 1][kMend ? G::NTQ : 1];
-   for (int careful = 0; careful < 2; careful++)
-   {
+   auto pass = [&](auto careful) {
+      constexpr bool CAREFUL = decltype(careful)::value;
 #pragma unroll
       for (int mp = 0; mp < MAPS; mp++)
       {
@@ -574,15 +548,21 @@ template <int T, int DC, int MAPS, int BR> __global__ __launch_bounds__(BR * 4, 
          }
       }
       for_tiles<G, BR>(
-         st, u.tiles, 1, [&](int t, int buf) { st.load_tile(t, buf, st.a, st.b); },
-         [&](int t, int buf) {
-            bool named;
-            const unsigned mine = st.my_bits(t, g, i, &named);
-            if (!named) return;
+         st, u.tiles, 1, [&](int t, int buf) __attribute__((always_inline)) { st.load_tile(t, buf, st.a, st.b); },
+         [&](int t, int buf) __attribute__((always_inline)) {
+            const uint32_t word = st.row_mask(t, i);
+            if (!__any(word != 0)) return;
+            const bool all = __all(word == 0xffffffffu);   // most tiles of a window: nothing to mask
+            const unsigned mine = (word >> (8 * g)) & 255;
             const typename G::V::Lane l = G::V::lane(g, i);
             const unsigned char *ks = lds + buf * G::kPair, *vs = ks + G::V::kBytes;
             f4 dp[2];
             tile_scores<T, G::W, G::CV>(dp, vs, 0, gr, l);
+            if (!all)   // (zero times what is masked has to be zero)
+            {
+#pragma unroll
+               for (int j = 0; j < 8; j++) dp[j / 4][j % 4] = masked(dp[j / 4][j % 4], mine, j, 0.0f);
+            }
 #pragma unroll
             for (int mp = 0; mp < MAPS; mp++)
             {
@@ -590,18 +570,22 @@ template <int T, int DC, int MAPS, int BR> __global__ __launch_bounds__(BR * 4, 
                tile_scores<T, G::W, G::CQ>(s, ks, mp * G::MC, qr[mp], l);
                float w[2][4], pr[2][4];
 #pragma unroll
+               for (int j = 0; j < 8; j++) pr[j / 4][j % 4] = exp2_fast(fmaf(s[j / 4][j % 4], c2, -lse2[mp]));
+               if (!all)
+               {
+#pragma unroll
+                  for (int j = 0; j < 8; j++) pr[j / 4][j % 4] = masked(pr[j / 4][j % 4], mine, j, 0.0f);
+               }
+#pragma unroll
                for (int j = 0; j < 8; j++)
                {
-                  const bool one = (mine >> j) & 1;
-                  pr[j / 4][j % 4] = one ? exp2_fast(s[j / 4][j % 4] * c2 - lse2[mp]) : 0.0f;
-                  const float x = one ? dp[j / 4][j % 4] : 0.0f;
-                  w[j / 4][j % 4] = pr[j / 4][j % 4] * sign[mp] * (x - delta[mp]);
-                  mean[mp] = fmaf(pr[j / 4][j % 4], x, mean[mp]);
+                  w[j / 4][j % 4] = pr[j / 4][j % 4] * (dp[j / 4][j % 4] - delta[mp]);   // sign: at the end
+                  mean[mp] = fmaf(pr[j / 4][j % 4], dp[j / 4][j % 4], mean[mp]);
                }
-               if (__builtin_expect(careful, 0))
+               if constexpr (CAREFUL)
                {
-                  add_weighted<T, G::W, G::NTQ>(acc[mp], w, mine, ks, mp * DC, g, i, l, true);
-                  if constexpr (kMend) add_weighted<T, G::W, G::NTQ>(pk[mp], pr, mine, ks, mp * DC, g, i, l, true);
+                  add_weighted<T, G::W, true>(acc[mp], w, mine, ks, mp * DC, g, i, l);
+                  if constexpr (kMend) add_weighted<T, G::W, true>(pk[mp], pr, mine, ks, mp * DC, g, i, l);
                   continue;
                }
                const typename G::N::TFrag wf = pack_scores<T>(w);
@@ -623,8 +607,9 @@ template <int T, int DC, int MAPS, int BR> __global__ __launch_bounds__(BR * 4, 
          odd |= odd_sums(acc[mp]);
          if constexpr (kMend) odd |= odd_sums(pk[mp]);
       }
-      if (!any_odd<BR>(odd)) break;
-   }
+      return odd;
+   };
+   if (any_odd<BR>(pass(Flag<false>()))) (void)pass(Flag<true>());
 
 #pragma unroll
    for (int mp = 0; mp < MAPS; mp++) mean[mp] = group_sum(mean[mp]);
@@ -654,7 +639,7 @@ template <int T, int DC, int MAPS, int BR> __global__ __launch_bounds__(BR * 4, 
       if constexpr (kMend)
       {
 #pragma unroll
-         for (int mp = 0; mp < MAPS; mp++) p.delta[(row * p.heads + head) * MAPS + mp] = mean[mp];
+         for (int mp = 0; mp < MAPS; mp++) p.stats[(row * p.heads + head) * (2 * MAPS) + MAPS + mp] = mean[mp];
       }
    }
    E *out = (E *)p.dq + row * p.ldq + head * p.hdq;
@@ -664,8 +649,8 @@ template <int T, int DC, int MAPS, int BR> __global__ __launch_bounds__(BR * 4, 
       for (int x = 0; x < G::NTQ; x++)
       {
          f4 r = acc[mp][x];
-         if constexpr (kMend) r += (sign[mp] * (delta[mp] - mean[mp])) * pk[mp][x];
-         store4<T>(out + mp * p.d, 16 * x + 4 * g, p.d, r * p.scale, p.vec);
+         if constexpr (kMend) r += (delta[mp] - mean[mp]) * pk[mp][x];
+         store4<T>(out + mp * p.d, 16 * x + 4 * g, p.d, r * (sign[mp] * p.scale), p.vec);
       }
 }
 
@@ -692,8 +677,8 @@ template <int T, int DC, int MAPS> __global__ __launch_bounds__(256) void attn_d
    {
       float mean = 0;
       for (int u = 0; u < j.parts; u++) mean += from[u * step + 2 * W + mp];
-      float *delta = p.delta + (row * p.heads + head) * MAPS + mp;
-      mend[mp] = (mp == 0 ? 1.0f : -p.lambda[head]) * (*delta - mean);
+      float *delta = p.stats + (row * p.heads + head) * (2 * MAPS) + MAPS + mp;
+      mend[mp] = *delta - mean;
       if (lane == 0)
       {
          if (mp == 1) p.dlam_rows[row * p.heads + head] = mean;
@@ -710,7 +695,7 @@ template <int T, int DC, int MAPS> __global__ __launch_bounds__(256) void attn_d
       }
       const int mp = f / DC, e = f - mp * DC;
       if (kMend) s += (mp == 0 ? mend[0] : mend[MAPS - 1]) * s2;
-      if (e < p.d) ((E *)p.dq)[row * p.ldq + head * p.hdq + mp * p.d + e] = (E)Num<T>::from(s * p.scale);
+      if (e < p.d) ((E *)p.dq)[row * p.ldq + head * p.hdq + mp * p.d + e] = (E)Num<T>::from(s * ((mp == 0 ? 1.0f : -p.lambda[head]) * p.scale));
    }
 }
 
@@ -747,7 +732,7 @@ template <int T, int DC, int MAPS, int BR> __global__ __launch_bounds__(BR * 4, 
    const bool live = row < p.n;
    const int64_t srow = live ? row : 0;
    Stream<G, T, DC, BR> st;
-   st.set(lds, lds_ids, lds_bits, p.plan, u, (const E *)p.q, p.ldq, p.d, (const E *)p.dout, p.ldo, p.dv, p.vec);
+   st.set(lds, lds_ids, lds_bits, p, u, (const E *)p.q, p.ldq_bytes, (const E *)p.dout, p.ldo_bytes);
 
    u4 kr[MAPS][G::CQ], vr[G::CV];
 #pragma unroll
@@ -757,59 +742,72 @@ template <int T, int DC, int MAPS, int BR> __global__ __launch_bounds__(BR * 4, 
    const float c2 = p.scale * kLog2e;
    f4 dk[MAPS][G::NTQ], dv[G::NT];
 
-   auto load = [&](int s, int buf) {
+   auto load = [&](int s, int buf) __attribute__((always_inline)) {
       const int t = s / p.group, head = kvh * p.group + s % p.group;
       st.load_tile(t, buf, st.a + head * p.hdq, st.b + head * p.hdo);
-      // [lse of every map, delta of every map][32 rows]: 64 values for each of the first waves, or for the wave twice
-#pragma unroll
-      for (int x = 0; x < (BR == 64 ? 1 : MAPS); x++)
+      // the statistics of the tile's rows: [32 rows][2 maps], 8 or 16 bytes of a row each
+      if (tid < (MAPS == 2 ? 32 : 64))
       {
-         const int sk = (tid >> 5) + 2 * x;
-         if (sk >= 2 * MAPS) break;
-         const int32_t c = st.tile_ids(t)[tid & 31];
-         const float *from = (sk < MAPS ? p.lse_in : p.delta) + ((int64_t)c * p.heads + head) * MAPS + sk % MAPS;
-         load_lds4(lds_address(lds_extra + buf * G::kStat) + 256 * (st.wave + x), c >= 0 ? (const void *)from : (const void *)&zero_chunk);
+         const int32_t c = st.tile_ids(t)[MAPS == 2 ? tid : tid >> 1];
+         const float *from = p.stats + ((int64_t)c * p.heads + head) * (2 * MAPS);
+         if constexpr (MAPS == 2) load_lds16(lds_address(lds_extra + buf * G::kStat), from);
+         else load_lds4(lds_address(lds_extra + buf * G::kStat), from + (tid & 1));
       }
    };
-   auto use = [&](int s, int buf, bool careful) {
-      bool named;
-      const unsigned mine = st.my_bits(s / p.group, g, i, &named);
-      if (!named) return;
+   auto use = [&](int s, int buf, auto careful) __attribute__((always_inline)) {
+      constexpr bool CAREFUL = decltype(careful)::value;
+      const uint32_t word = st.row_mask(s / p.group, i);
+      if (!__any(word != 0)) return;
+      const bool all = __all(word == 0xffffffffu);
+      const unsigned mine = (word >> (8 * g)) & 255;
       const typename G::V::Lane l = G::V::lane(g, i);
       const unsigned char *qs = lds + buf * G::kPair, *gs = qs + G::V::kBytes;
       const float *stat = (const float *)(lds_extra + buf * G::kStat);
       const float lam = MAPS == 2 ? p.lambda[kvh * p.group + s % p.group] : 0.0f;
       f4 dp[2];
       tile_scores<T, G::W, G::CV>(dp, gs, 0, vr, l);
+      float rs[8][2 * MAPS];   // statistics of this lane's gathered rows
+#pragma unroll
+      for (int j = 0; j < 8; j++)
+#pragma unroll
+         for (int k = 0; k < 2 * MAPS; k++) rs[j][k] = stat[(16 * (j / 4) + 4 * g + j % 4) * (2 * MAPS) + k];
       float wv[2][4];
 #pragma unroll
       for (int mp = 0; mp < MAPS; mp++)
       {
          f4 sc[2];
          tile_scores<T, G::W, G::CQ>(sc, qs, mp * G::MC, kr[mp], l);
-         const float sign = mp == 0 ? 1.0f : -lam;
          float w[2][4];
 #pragma unroll
-         for (int a = 0; a < 2; a++)
+         for (int j = 0; j < 8; j++) w[j / 4][j % 4] = exp2_fast(fmaf(sc[j / 4][j % 4], c2, -rs[j][mp]));
+         if (!all)
          {
-            const f4 ls = *(const f4 *)(stat + mp * kTile + 16 * a + 4 * g), dl = *(const f4 *)(stat + (MAPS + mp) * kTile + 16 * a + 4 * g);
 #pragma unroll
-            for (int r = 0; r < 4; r++)
-            {
-               const bool one = (mine >> (4 * a + r)) & 1;
-               const float pr = one ? sign * exp2_fast(sc[a][r] * c2 - ls[r] * kLog2e) : 0.0f;
-               w[a][r] = one ? pr * (dp[a][r] - dl[r]) : 0.0f;
-               wv[a][r] = mp == 0 ? pr : wv[a][r] + pr;
-            }
+            for (int j = 0; j < 8; j++) w[j / 4][j % 4] = masked(w[j / 4][j % 4], mine, j, 0.0f);
          }
-         add_weighted<T, G::W, G::NTQ>(dk[mp], w, mine, qs, mp * DC, g, i, l, careful);
-      }
 #pragma unroll
-      for (int j = 0; j < 8; j++) wv[j / 4][j % 4] *= G::N::kPScale;
-      add_weighted<T, G::W, G::NT>(dv, wv, mine, gs, 0, g, i, l, careful);
+         for (int j = 0; j < 8; j++)
+         {
+            float pr = w[j / 4][j % 4];
+            if (mp == 1) pr *= -lam;
+            w[j / 4][j % 4] = pr * (dp[j / 4][j % 4] - rs[j][MAPS + mp]);
+            wv[j / 4][j % 4] = mp == 0 ? pr : wv[j / 4][j % 4] + pr;
+         }
+         if (!all)   // (zero times the products and statistics of a row that is masked has to be zero)
+         {
+#pragma unroll
+            for (int j = 0; j < 8; j++) w[j / 4][j % 4] = masked(w[j / 4][j % 4], mine, j, 0.0f);
+         }
+         add_weighted<T, G::W, CAREFUL>(dk[mp], w, mine, qs, mp * DC, g, i, l);
+      }
+      if constexpr (G::N::kPScale != 1.0f)
+      {
+#pragma unroll
+         for (int j = 0; j < 8; j++) wv[j / 4][j % 4] *= G::N::kPScale;
+      }
+      add_weighted<T, G::W, CAREFUL>(dv, wv, mine, gs, 0, g, i, l);
    };
-   for (int careful = 0; careful < 2; careful++)
-   {
+   auto pass = [&](auto careful) {
 #pragma unroll
       for (int mp = 0; mp < MAPS; mp++)
 #pragma unroll
@@ -817,12 +815,13 @@ template <int T, int DC, int MAPS, int BR> __global__ __launch_bounds__(BR * 4, 
 #pragma unroll
       for (int t = 0; t < G::NT; t++) dv[t] = f4{0, 0, 0, 0};
       // (steps of one tile, the heads of the group, follow each other: tiles * group < 2^31 is checked by the host)
-      for_tiles<G, BR>(st, u.tiles * p.group, p.group, load, [&](int s, int buf) { use(s, buf, careful); });
+      for_tiles<G, BR>(st, u.tiles * p.group, p.group, load, [&](int s, int buf) __attribute__((always_inline)) { use(s, buf, careful); });
       bool odd = odd_sums(dv);
 #pragma unroll
       for (int mp = 0; mp < MAPS; mp++) odd |= odd_sums(dk[mp]);
-      if (!any_odd<BR>(odd)) break;
-   }
+      return odd;
+   };
+   if (any_odd<BR>(pass(Flag<false>()))) (void)pass(Flag<true>());
 
    constexpr float unscale = 1.0f / G::N::kPScale;
    if (u.part >= 0)

@@ -30,7 +30,7 @@ struct Chunk {
 
 struct Piece {        // a chunk's entries, in their place in the plan
    int64_t from, to;
-   int32_t count, end;   // entries at to + count .. to + end - 1 are filled with "no column"
+   int32_t count, end;   // entries at to + count .. to + end - 1 fill the unit's last tile
 };
 
 __device__ inline int64_t index_at(const void *a, int64_t i, int bytes)
@@ -179,16 +179,27 @@ __global__ __launch_bounds__(THREADS) void plan_fill(const Chunk *chunks, int64_
    if (tid == THREADS - 1) counts[blockIdx.x] = make_int2(sums[tid], runs);
 }
 
-__global__ __launch_bounds__(256) void plan_pack(const Piece *pieces, int waves, const int32_t *cols, const uint64_t *masks, int32_t *to_cols, uint16_t *to_masks)
+__global__ __launch_bounds__(256) void plan_pack(const Piece *pieces, const int32_t *cols, const uint64_t *masks, int32_t *to_cols, uint64_t *to_masks)
 {
    const Piece p = pieces[blockIdx.x];
    for (int e = threadIdx.x; e < p.end; e += 256)
    {
-      const bool live = e < p.count;
-      const int64_t to = p.to + e;
-      to_cols[to] = live ? cols[p.from + e] : -1;
-      const uint64_t bits = live ? masks[p.from + e] : 0;
-      for (int w = 0; w < waves; w++) to_masks[(to / kTile) * (waves * kTile) + w * kTile + to % kTile] = (uint16_t)(bits >> (16 * w));
+      // behind the last column: that column again, named by no row
+      to_cols[p.to + e] = cols[p.from + (e < p.count ? e : p.count - 1)];
+      to_masks[p.to + e] = e < p.count ? masks[p.from + e] : 0;
+   }
+}
+
+// per column a bit for each row -> per row a bit for each of the tile's 32 columns, in the order in which lanes hold scores
+__global__ __launch_bounds__(256) void plan_masks(const uint64_t *masks, int64_t tiles, int br, uint32_t *to)
+{
+   for (int64_t x = (int64_t)blockIdx.x * 256 + threadIdx.x; x < tiles * br; x += (int64_t)gridDim.x * 256)
+   {
+      const int64_t tile = x / br;
+      const int row = (int)(x % br);
+      uint32_t word = 0;
+      for (int c = 0; c < kTile; c++) word |= (uint32_t)((masks[tile * kTile + c] >> row) & 1) << (8 * (c % 16 / 4) + 4 * (c / 16) + c % 4);
+      to[x] = word;
    }
 }
 
@@ -317,6 +328,7 @@ int build(Plan *plan, int br, bool *shared, int64_t m, int64_t n, int64_t nnz, c
          const int64_t begin = to;
          for (size_t x = lo; x < hi; x++)
          {
+            if (!counts[x].x) continue;
             pieces.push_back(Piece{chunks[x].at, to, counts[x].x, counts[x].x});
             to += counts[x].x;
          }
@@ -339,9 +351,8 @@ int build(Plan *plan, int br, bool *shared, int64_t m, int64_t n, int64_t nnz, c
    plan->tiles = to / kTile;
    plan->parts = parts;
    auto up = [](size_t v) { return (v + 255) & ~(size_t)255; };
-   const int waves = br / 16;
    // (a group of column ids and masks is read ahead as a whole: room for one behind the last tile)
-   const size_t off_masks = up((size_t)(to + kAhead * kTile) * 4), off_units = off_masks + up((size_t)(to + kAhead * kTile) * 2 * waves), off_joins = off_units + up(units.size() * sizeof(Unit));
+   const size_t off_masks = up((size_t)(to + kAhead * kTile) * 4), off_units = off_masks + up((size_t)(to / kTile + kAhead) * br * 4), off_joins = off_units + up(units.size() * sizeof(Unit));
    const size_t bytes = off_joins + up(joins.size() * sizeof(Join)) + 256;
    ATTN_HIP(hipMalloc(&plan->memory, bytes));
    unsigned char *base = (unsigned char *)plan->memory;
@@ -350,14 +361,20 @@ int build(Plan *plan, int br, bool *shared, int64_t m, int64_t n, int64_t nnz, c
    Memory d_pieces;
    if (!pieces.empty())
    {
-      const int st = upload(d_pieces, pieces);
+      int st = upload(d_pieces, pieces);
       if (st) return st;
-      hipLaunchKernelGGL(plan_pack, dim3((unsigned)pieces.size()), dim3(256), 0, stream, (const Piece *)d_pieces.p, waves, (const int32_t *)d_cols.p,
-                         (const uint64_t *)d_masks.p, (int32_t *)base, (uint16_t *)(base + off_masks));
+      Memory by_column;
+      st = by_column.get((size_t)to * 8);
+      if (st) return st;
+      hipLaunchKernelGGL(plan_pack, dim3((unsigned)pieces.size()), dim3(256), 0, stream, (const Piece *)d_pieces.p, (const int32_t *)d_cols.p,
+                         (const uint64_t *)d_masks.p, (int32_t *)base, (uint64_t *)by_column.p);
+      hipLaunchKernelGGL(plan_masks, dim3((unsigned)std::min<int64_t>((to / kTile * br + 255) / 256, 1 << 16)), dim3(256), 0, stream,
+                         (const uint64_t *)by_column.p, to / kTile, br, (uint32_t *)(base + off_masks));
       ATTN_HIP(hipGetLastError());
+      ATTN_HIP(hipStreamSynchronize(stream));
    }
    ATTN_HIP(hipStreamSynchronize(stream));
-   plan->view = PlanView{(const int32_t *)base, (const uint16_t *)(base + off_masks), (const Unit *)(base + off_units),
+   plan->view = PlanView{(const int32_t *)base, (const uint32_t *)(base + off_masks), (const Unit *)(base + off_units),
                          (const Join *)(base + off_joins), (int32_t)units.size(), (int32_t)joins.size(), m, n, br};
    return kOk;
 }

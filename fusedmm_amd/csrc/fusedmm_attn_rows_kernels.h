@@ -198,52 +198,29 @@ template <int T, int DC, int MAPS> struct RowGeo {
    static constexpr int NV = kTile * CR / 64;         // 16-byte chunks of the values that a lane carries
 };
 
-// what a wave keeps of its 16 columns
-template <class G> struct RowSums {
-   f4 acc[G::NT];
-   float top, sum;
-};
-
 __device__ inline void wave_lds_order()   // this wave's LDS writes before its later LDS reads
 {
    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
    __builtin_amdgcn_wave_barrier();
 }
 
-// scores (already times scale and log2 e) of 32 slots -> running maximum and sum, weights, and the weighted values
-template <class G, int T>
-__device__ inline void row_step(RowSums<G> &r, float (&w)[2][4], unsigned mine, const unsigned char *vs, int g, int i, bool odd)
+// products of 32 slots with the columns -> weights, and the weighted values
+template <class G, int T, bool CAREFUL>
+__device__ inline void row_step(Softmax<G::NT> &r, f4 (&sc)[2], float c2, unsigned mine, bool all, const unsigned char *vs, int g, int i)
 {
-   float mx = -INFINITY;
-#pragma unroll
-   for (int j = 0; j < 8; j++)
-   {
-      w[j / 4][j % 4] = ((mine >> j) & 1) ? w[j / 4][j % 4] : -INFINITY;
-      mx = fmaxf(mx, w[j / 4][j % 4]);
-   }
-   mx = fmaxf(r.top, group_max(mx));
-   const float base = mx == -INFINITY ? 0.0f : mx;
-   const float keep = exp2_fast(r.top - base);
-   float add = 0;
-#pragma unroll
-   for (int j = 0; j < 8; j++)
-   {
-      w[j / 4][j % 4] = exp2_fast(w[j / 4][j % 4] - base);
-      add += w[j / 4][j % 4];
-   }
-   if (__any(mx != r.top))
+   if (!all)
    {
 #pragma unroll
-      for (int x = 0; x < G::NT; x++) r.acc[x] *= keep;
+      for (int j = 0; j < 8; j++) sc[j / 4][j % 4] = masked(sc[j / 4][j % 4], mine, j, -INFINITY);
    }
-   r.sum = r.sum * keep + add;
-   r.top = mx;
-   add_weighted<T, G::W, G::NT>(r.acc, w, mine, vs, 0, g, i, G::V::lane(g, i), odd);
+   float w[2][4];
+   r.weights(w, sc, c2);
+   add_weighted<T, G::W, CAREFUL>(r.acc, w, mine, vs, 0, g, i, G::V::lane(g, i));
 }
 
 // The four waves' sums -> the row's output, or its piece of the partial sums.  O: element type of the output.
 template <class G, int MAPS, int O>
-__device__ inline void rows_finish(const RowsParams &p, RowSums<G> &r, unsigned char *vs_all, float (*stat)[16][2], const Spot &s, int64_t id, int kvh, int pass)
+__device__ inline void rows_finish(const RowsParams &p, Softmax<G::NT> &r, unsigned char *vs_all, float (*stat)[16][2], const Spot &s, int64_t id, int kvh, int pass)
 {
    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, g = lane >> 4, i = lane & 15;
    r.sum = group_sum(r.sum);
@@ -253,7 +230,7 @@ __device__ inline void rows_finish(const RowsParams &p, RowSums<G> &r, unsigned 
    for (int x = 0; x < G::NT; x++) *reinterpret_cast<f4 *>(mine + 16 * x + 4 * g) = r.acc[x];
    if (g == 0)
    {
-      stat[wave][i][0] = r.top;
+      stat[wave][i][0] = r.base;
       stat[wave][i][1] = r.sum;
    }
    __syncthreads();
@@ -385,9 +362,10 @@ __device__ inline int32_t tile_slot(const RowsParams &p, int64_t at, int64_t end
    return c >= 0 && c < p.n ? (int32_t)c : -1;
 }
 
-__device__ inline unsigned tile_bits(int32_t slot, int g)
+__device__ inline unsigned tile_bits(int32_t slot, int g, bool *all)
 {
    const uint32_t live = (uint32_t)__ballot(slot >= 0);
+   *all = live == 0xffffffffu;
    return ((live >> (4 * g)) & 15) | (((live >> (16 + 4 * g)) & 15) << 4);
 }
 
@@ -418,16 +396,13 @@ __global__ __launch_bounds__(256, (sizeof(typename Num<T>::E) * DC * MAPS >= 512
       const int left = p.d - f;
       q[c] = load_chunk<T>((const E *)p.q + s.row * p.ldq + (col ? (it.kvh * p.group + hh) * p.hdq + mp_i * p.d + f : 0),
                            col ? (left < G::N::EPL ? left : G::N::EPL) : 0, p.vec_q);
+      if (p.scale < 0) q[c] = negated<T>(q[c]);
    }
-   RowSums<G> r;
-   r.top = -INFINITY;
-   r.sum = 0;
-#pragma unroll
-   for (int x = 0; x < G::NT; x++) r.acc[x] = f4{0, 0, 0, 0};
-   const float c2 = p.scale * kLog2e;
+   Softmax<G::NT> r;
+   const float c2 = score_factor(p.scale);
 
    u4 kf[2][MAPS][G::CQ], vf[G::NV];
-   auto load = [&](int32_t slot) {
+   auto load = [&](int32_t slot) __attribute__((always_inline)) {
 #pragma unroll
       for (int a = 0; a < 2; a++)
       {
@@ -452,50 +427,51 @@ __global__ __launch_bounds__(256, (sizeof(typename Num<T>::E) * DC * MAPS >= 512
    };
    constexpr int64_t kStride = 4 * kTile;
    const int64_t end = begin + hi;
-   int64_t at = begin + lo + wave * kTile;
-   int32_t slot = tile_slot(p, at, end, lane);
-   int32_t next = tile_slot(p, at + kStride, end, lane);
-   if (at < end) load(slot);
-   for (; at < end; at += kStride)
-   {
-      const unsigned mine = tile_bits(slot, g);
-      bool odd = false;
-#pragma unroll
-      for (int j = 0; j < G::NV; j++)
+   auto pass = [&](auto careful) {
+      constexpr bool CAREFUL = decltype(careful)::value;
+      r.clear();
+      int64_t at = begin + lo + wave * kTile;
+      int32_t slot = tile_slot(p, at, end, lane);
+      int32_t next = tile_slot(p, at + kStride, end, lane);
+      if (at < end) load(slot);
+      for (; at < end; at += kStride)
       {
-         const int e = lane + 64 * j;
-         *reinterpret_cast<u4 *>(vs + (e / G::CR) * G::V::RB + ((e % G::CR) ^ G::V::twist(e / G::CR)) * 16) = vf[j];
-         odd |= odd_chunk<T>(vf[j]);
-      }
-      odd = __any(odd);
-      f4 sc[MAPS][2];
+         bool all;
+         const unsigned mine = tile_bits(slot, g, &all);
 #pragma unroll
-      for (int mp = 0; mp < MAPS; mp++)
-#pragma unroll
-         for (int a = 0; a < 2; a++)
+         for (int j = 0; j < G::NV; j++)
          {
-            sc[mp][a] = f4{0, 0, 0, 0};
-#pragma unroll
-            for (int x = 0; x < G::CQ; x++) sc[mp][a] = G::N::mma(kf[a][mp][x], q[x], sc[mp][a]);
+            const int e = lane + 64 * j;
+            *reinterpret_cast<u4 *>(vs + (e / G::CR) * G::V::RB + ((e % G::CR) ^ G::V::twist(e / G::CR)) * 16) = vf[j];
          }
-      slot = next;
-      if (at + kStride < end)
-      {
-         load(slot);
-         next = tile_slot(p, at + 2 * kStride, end, lane);
-      }
-      float w[2][4];
+         f4 sc[MAPS][2];
 #pragma unroll
-      for (int j = 0; j < 8; j++)
-      {
-         float x = sc[0][j / 4][j % 4];
-         if constexpr (MAPS == 2) x = mp_i ? sc[1][j / 4][j % 4] : x;
-         w[j / 4][j % 4] = x * c2;
+         for (int mp = 0; mp < MAPS; mp++)
+#pragma unroll
+            for (int a = 0; a < 2; a++)
+            {
+               sc[mp][a] = f4{0, 0, 0, 0};
+#pragma unroll
+               for (int x = 0; x < G::CQ; x++) sc[mp][a] = G::N::mma(kf[a][mp][x], q[x], sc[mp][a]);
+            }
+         slot = next;
+         if (at + kStride < end)
+         {
+            load(slot);
+            next = tile_slot(p, at + 2 * kStride, end, lane);
+         }
+         if constexpr (MAPS == 2)
+         {
+            sc[0][0] = mp_i ? sc[1][0] : sc[0][0];
+            sc[0][1] = mp_i ? sc[1][1] : sc[0][1];
+         }
+         wave_lds_order();
+         row_step<G, T, CAREFUL>(r, sc[0], c2, mine, all, vs, g, i);
+         wave_lds_order();
       }
-      wave_lds_order();
-      row_step<G, T>(r, w, mine, vs, g, i, odd);
-      wave_lds_order();
-   }
+      return odd_sums(r.acc);
+   };
+   if (__any(pass(Flag<false>()))) (void)pass(Flag<true>());
    rows_finish<G, MAPS, T>(p, r, vs_all, stat, s, it.id, it.kvh, it.pass);
 }
 
@@ -523,7 +499,6 @@ template <bool FULL, int WORDS> __device__ inline int code_feature(int j, int g)
 
 template <bool FULL, int WORDS> __device__ inline void load_codes(uint32_t (&to)[WORDS], const uint8_t *from, int width, int g)
 {
-   typedef uint32_t u2 __attribute__((ext_vector_type(2)));
    if constexpr (FULL && WORDS % 4 == 0)
    {
 #pragma unroll
@@ -593,12 +568,11 @@ __global__ __launch_bounds__(256, (DC * MAPS >= 256 ? 1 : 2)) void attn_rows_kv4
             const int64_t off = s.row * p.ldq + (it.kvh * p.group + hh) * p.hdq + mp_i * p.d + f;
             x = p.out_type == kF16 ? Num<kF16>::to(((const uint16_t *)p.q)[off]) : Num<kBF16>::to(((const uint16_t *)p.q)[off]);
          }
-         qf[j][e] = x;
+         qf[j][e] = p.scale < 0 ? -x : x;
          top = fmaxf(top, fabsf(x));
       }
    top = group_max(top);
-   int ex = 0;
-   if (top > 0 && top < INFINITY) (void)frexpf(top, &ex);
+   const int ex = top > 0 && top < INFINITY ? __builtin_amdgcn_frexp_expf(top) : 0;
    u4 q[WQ];
 #pragma unroll
    for (int j = 0; j < WQ; j++)
@@ -607,16 +581,12 @@ __global__ __launch_bounds__(256, (DC * MAPS >= 256 ? 1 : 2)) void attn_rows_kv4
       for (int e = 0; e < 4; e++)
          q[j][e] = (uint32_t)Num<kF16>::from(ldexpf(qf[j][2 * e], -ex)) | (uint32_t)Num<kF16>::from(ldexpf(qf[j][2 * e + 1], -ex)) << 16;
    }
-   const float c2 = ldexpf(p.scale * kLog2e, ex);
+   const float c2 = score_factor(ldexpf(p.scale, ex));
 
-   RowSums<G> r;
-   r.top = -INFINITY;
-   r.sum = 0;
-#pragma unroll
-   for (int x = 0; x < G::NT; x++) r.acc[x] = f4{0, 0, 0, 0};
+   Softmax<G::NT> r;
 
    uint32_t kc[2][MAPS][WQ], vc[2][WV], ks[2][MAPS][WQ], vw[2][WV];
-   auto load = [&](int32_t slot) {
+   auto load = [&](int32_t slot) __attribute__((always_inline)) {
 #pragma unroll
       for (int a = 0; a < 2; a++)
       {
@@ -646,51 +616,52 @@ __global__ __launch_bounds__(256, (DC * MAPS >= 256 ? 1 : 2)) void attn_rows_kv4
    };
    constexpr int64_t kStride = 4 * kTile;
    const int64_t end = begin + hi;
-   int64_t at = begin + lo + wave * kTile;
-   int32_t slot = tile_slot(p, at, end, lane);
-   int32_t next = tile_slot(p, at + kStride, end, lane);
-   if (at < end) load(slot);
-   for (; at < end; at += kStride)
-   {
-      const unsigned mine = tile_bits(slot, g);
-      bool odd = false;
-      f4 sc[MAPS][2];
-#pragma unroll
-      for (int a = 0; a < 2; a++)
+   auto pass = [&](auto careful) {
+      constexpr bool CAREFUL = decltype(careful)::value;
+      r.clear();
+      int64_t at = begin + lo + wave * kTile;
+      int32_t slot = tile_slot(p, at, end, lane);
+      int32_t next = tile_slot(p, at + kStride, end, lane);
+      if (at < end) load(slot);
+      for (; at < end; at += kStride)
       {
+         bool all;
+         const unsigned mine = tile_bits(slot, g, &all);
+         f4 sc[MAPS][2];
 #pragma unroll
-         for (int mp = 0; mp < MAPS; mp++)
+         for (int a = 0; a < 2; a++)
          {
-            sc[mp][a] = f4{0, 0, 0, 0};
 #pragma unroll
-            for (int j = 0; j < WQ; j++) sc[mp][a] = G::N::mma(dequant8(kc[a][mp][j], ks[a][mp][j]), q[j], sc[mp][a]);
+            for (int mp = 0; mp < MAPS; mp++)
+            {
+               sc[mp][a] = f4{0, 0, 0, 0};
+#pragma unroll
+               for (int j = 0; j < WQ; j++) sc[mp][a] = G::N::mma(dequant8(kc[a][mp][j], ks[a][mp][j]), q[j], sc[mp][a]);
+            }
+#pragma unroll
+            for (int j = 0; j < WV; j++)
+            {
+               *reinterpret_cast<u4 *>(vs + (16 * a + i) * G::V::RB + ((code_feature<FULL, WV>(j, g) / 8) ^ G::V::twist(i)) * 16) = dequant8(vc[a][j], vw[a][j]);
+            }
          }
-#pragma unroll
-         for (int j = 0; j < WV; j++)
+         slot = next;
+         if (at + kStride < end)
          {
-            *reinterpret_cast<u4 *>(vs + (16 * a + i) * G::V::RB + ((code_feature<FULL, WV>(j, g) / 8) ^ G::V::twist(i)) * 16) = dequant8(vc[a][j], vw[a][j]);
-            odd |= (vw[a][j] & 0x7C00u) == 0x7C00u;   // an infinite or NaN scale
+            load(slot);
+            next = tile_slot(p, at + 2 * kStride, end, lane);
          }
+         if constexpr (MAPS == 2)
+         {
+            sc[0][0] = mp_i ? sc[1][0] : sc[0][0];
+            sc[0][1] = mp_i ? sc[1][1] : sc[0][1];
+         }
+         wave_lds_order();
+         row_step<G, kF16, CAREFUL>(r, sc[0], c2, mine, all, vs, g, i);
+         wave_lds_order();
       }
-      odd = __any(odd);
-      slot = next;
-      if (at + kStride < end)
-      {
-         load(slot);
-         next = tile_slot(p, at + 2 * kStride, end, lane);
-      }
-      float w[2][4];
-#pragma unroll
-      for (int j = 0; j < 8; j++)
-      {
-         float x = sc[0][j / 4][j % 4];
-         if constexpr (MAPS == 2) x = mp_i ? sc[1][j / 4][j % 4] : x;
-         w[j / 4][j % 4] = x * c2;
-      }
-      wave_lds_order();
-      row_step<G, kF16>(r, w, mine, vs, g, i, odd);
-      wave_lds_order();
-   }
+      return odd_sums(r.acc);
+   };
+   if (__any(pass(Flag<false>()))) (void)pass(Flag<true>());
    if (p.out_type == kF16) rows_finish<G, MAPS, kF16>(p, r, vs_all, stat, s, it.id, it.kvh, it.pass);
    else rows_finish<G, MAPS, kBF16>(p, r, vs_all, stat, s, it.id, it.kvh, it.pass);
 }
