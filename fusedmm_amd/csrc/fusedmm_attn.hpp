@@ -67,14 +67,14 @@ inline int width_class(int d, int dv, int maps)
 
 // floats of partial sums that one split unit of one head leaves
 inline int64_t forward_part(int dc, int maps, int br) { return (int64_t)maps * br * (dc * maps + 2); }
-inline int64_t dq_part(int dc, int maps, int br) { return (int64_t)br * (2 * dc * maps + 2); }
+inline int64_t dq_part(int dc, int maps, int br) { return (int64_t)br * (2 * dc * maps + 4); }
 inline int64_t dkv_part(int dc, int maps, int br) { return (int64_t)br * (2 * dc * maps); }
 
 // one function per (type, kernel) object; dc and maps choose the instance
 int launch_forward_f32(const Params &p, int dc, int maps, hipStream_t s);
 int launch_forward_f16(const Params &p, int dc, int maps, hipStream_t s);
 int launch_forward_bf16(const Params &p, int dc, int maps, hipStream_t s);
-int launch_dq_f32(const Params &p, int dc, int maps, hipStream_t s);      // delta, dq and the head sums of dlambda
+int launch_dq_f32(const Params &p, int dc, int maps, hipStream_t s);      // dq and dlambda, and the statistics that dkv reads
 int launch_dq_f16(const Params &p, int dc, int maps, hipStream_t s);
 int launch_dq_bf16(const Params &p, int dc, int maps, hipStream_t s);
 int launch_dkv_f32(const Params &p, int dc, int maps, hipStream_t s);

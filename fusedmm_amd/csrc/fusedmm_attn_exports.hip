@@ -111,8 +111,8 @@ int check_plans(const char *who, const Desc &d, const void *plan, const void *pl
    if (p->rows != d.m || p->cols != d.n) return refuse(who, "the plan is of a pattern of another size");
    if (t && (t->rows != d.n || t->cols != d.m)) return refuse(who, "the second plan is not of the transposed pattern's size");
    if (t && t->device != p->device) return refuse(who, "the plans belong to different devices");
-   if ((int64_t)p->view.n_units * d.heads > kMaxGrid || (int64_t)p->view.n_joins * d.heads * (p->view.block_rows / 4) > kMaxGrid || d.m * d.heads > kMaxGrid ||
-       (t && ((int64_t)t->view.n_units * d.kv_heads > kMaxGrid || (int64_t)t->view.n_joins * d.kv_heads * (t->view.block_rows / 4) > kMaxGrid || t->tiles * (d.heads / d.kv_heads) > INT32_MAX)))
+   if ((int64_t)p->view.n_units * d.heads > kMaxGrid || (int64_t)p->view.n_joins * d.heads * (p->view.block_rows / 4) * 8 > kMaxGrid || d.m * d.heads > kMaxGrid ||
+       (t && ((int64_t)t->view.n_units * d.kv_heads > kMaxGrid || (int64_t)t->view.n_joins * d.kv_heads * (t->view.block_rows / 4) * 8 > kMaxGrid || t->tiles * (d.heads / d.kv_heads) > INT32_MAX)))
       return refuse(who, "too many rows and heads for one call");
    return kOk;
 }
@@ -139,7 +139,7 @@ Layout backward_layout(const Desc &d, const Plan &p, const Plan &t, int dc)
 {
    Layout l;
    l.dlam = align256(d.m * d.heads * d.maps * 8);
-   l.part = l.dlam + (d.maps == 2 ? align256(d.m * d.heads * 4) : 0);
+   l.part = l.dlam + (d.maps == 2 ? align256((int64_t)p.view.n_units * (p.view.block_rows / 16) * d.heads * 4) : 0);
    l.total = l.part + std::max(p.parts * d.heads * dq_part(dc, d.maps, p.view.block_rows), t.parts * d.kv_heads * dkv_part(dc, d.maps, t.view.block_rows)) * 4;
    return l;
 }
@@ -483,7 +483,7 @@ int fusedMM_attn_backward(const fusedMM_attn_desc *desc, const void *plan, const
    p.dvv = dv;
    p.dlambda = d.maps == 2 ? dlambda : nullptr;
    p.stats = (float *)((unsigned char *)work + l.stats);
-   p.dlam_rows = (float *)((unsigned char *)work + l.dlam);
+   p.dlam_units = (float *)((unsigned char *)work + l.dlam);
    p.part = (float *)((unsigned char *)work + l.part);
    const hipStream_t s = (hipStream_t)stream;
    if (d.m > 0 || p.dlambda)

@@ -53,7 +53,7 @@ struct Params {
    void *dq, *dk, *dvv;
    float *dlambda;
    float *stats;                      // [m][heads][2 maps]: lse * log2(e) of every map, delta of every map
-   float *dlam_rows;                  // [m][heads]: sum_j P_2 dP
+   float *dlam_units;                 // [unit][wave][heads]: sum over a wave's rows of sum_j P_2 dP
    float *part;                       // partial sums of split blocks
 };
 
@@ -71,10 +71,10 @@ template <int T, int DC, int MAPS, int BR> struct Geo {
    static constexpr int CV = W / N::KC;
    static constexpr int MC = DC / N::EPL;             // chunks of one map
    static constexpr int NT = W / 16, NTQ = DC / 16;   // 16-feature tiles of v's and of one map's accumulators
-   // Tiles in flight and being used.  Two tensors' tiles are 4 ... 64 KB; 4 deep as long as two workgroups of four waves
-   // (six of one wave) fit a compute unit's 160 KB.
+   // Tiles in flight and being used.  More than two cost residency (two tensors' tiles are 4 ... 64 KB of 160): a window
+   // of 512 at 128 bf16 features 55 us with 3 or 4, 44 with 2; a graph's training pass 438 us with 3, 320 with 2.
    static constexpr int kPair = 2 * V::kBytes;
-   static constexpr int S = BR == 64 ? (kPair <= 16384 ? 4 : 2) : (kPair <= 4096 ? 4 : kPair <= 8192 ? 3 : 2);
+   static constexpr int S = 2;
    static constexpr int kMaskBytes = BR * 4;               // of a tile
    static constexpr int kStat = 2 * MAPS * kTile * 4;      // statistics of a tile's rows (dk, dv)
 };
@@ -215,6 +215,25 @@ template <int T, int CQ> __device__ inline void load_resident(u4 (&r)[CQ], const
       const int f = c * Num<T>::KC + g * Num<T>::EPL;
       r[c] = load_chunk<T>(row + f, live ? (d - f < Num<T>::EPL ? d - f : Num<T>::EPL) : 0, vec);
    }
+}
+
+// this lane's part of the product of two resident rows
+template <int T, int CQ> __device__ inline float chunk_dot(const u4 (&a)[CQ], const u4 (&b)[CQ])
+{
+   float s = 0;
+#pragma unroll
+   for (int c = 0; c < CQ; c++)
+#pragma unroll
+      for (int e = 0; e < 4; e++)
+      {
+         if constexpr (T == kF32) s = fmaf(__uint_as_float(a[c][e]), __uint_as_float(b[c][e]), s);
+         else
+         {
+            s = fmaf(Num<T>::to((uint16_t)a[c][e]), Num<T>::to((uint16_t)b[c][e]), s);
+            s = fmaf(Num<T>::to((uint16_t)(a[c][e] >> 16)), Num<T>::to((uint16_t)(b[c][e] >> 16)), s);
+         }
+      }
+   return s;
 }
 
 // scores of the tile's 32 rows, from chunk `chunk` on, against the resident rows: s[a] rows 16a + 4g + r
@@ -400,106 +419,61 @@ template <int T, int DC, int MAPS, int BR> __global__ __launch_bounds__(BR * 4, 
    }
 }
 
-// Blocks of several units: one wave per (block, head, row).
+// Blocks of several units: a wave for every 64 features of a (block, head, row); the units' sums in order.
+#define JOIN_WHERE(HEADS, PIECES)                                                        \
+   const int br = p.plan.block_rows, lane = threadIdx.x & 63;                             \
+   const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);                       \
+   const int piece = (int)(id % (PIECES)), r = (int)(id / (PIECES) % br);                 \
+   const int head = (int)(id / (PIECES) / br % (HEADS));                                  \
+   if (id / (PIECES) / br / (HEADS) >= p.plan.n_joins) return;                            \
+   const Join j = p.plan.joins[id / (PIECES) / br / (HEADS)];
+
 template <int T, int DC, int MAPS> __global__ __launch_bounds__(256) void attn_forward_join(Params p)
 {
-   typedef Geo<T, DC, MAPS, 64> G;
-   const int br = p.plan.block_rows;
-   typedef typename G::E E;
-   const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-   const int lane = threadIdx.x & 63;
-   const int r = (int)(id % br);
-   const int head = (int)((id / br) % p.heads);
-   const int64_t jn = id / br / p.heads;
-   if (jn >= p.plan.n_joins) return;
-   const Join j = p.plan.joins[jn];
+   constexpr int W = DC * MAPS;
+   typedef typename Num<T>::E E;
+   JOIN_WHERE(p.heads, (W + 63) / 64)
    const int64_t row = (int64_t)j.block * br + r;
    if (row >= p.m) return;
-   const float lam = MAPS == 2 ? p.lambda[head] : 0.0f;
-   constexpr int PER = (G::W + 63) / 64;
-   float o[MAPS][PER];
+   const int f = 64 * piece + lane;
+   const bool live = f < W;
+   float o[MAPS];
 #pragma unroll
    for (int mp = 0; mp < MAPS; mp++)
    {
-      const int64_t step = (int64_t)p.heads * MAPS * br * (G::W + 2);
-      const float *from = p.part + (((int64_t)j.part0 * p.heads + head) * MAPS + mp) * br * (G::W + 2) + (int64_t)r * (G::W + 2);
+      const int64_t step = (int64_t)p.heads * MAPS * br * (W + 2);
+      const float *from = p.part + (((int64_t)j.part0 * p.heads + head) * MAPS + mp) * br * (W + 2) + (int64_t)r * (W + 2);
       float top = -INFINITY;
-      for (int u = 0; u < j.parts; u++) top = fmaxf(top, from[u * step + G::W]);
+#pragma unroll 8
+      for (int u = 0; u < j.parts; u++) top = fmaxf(top, from[u * step + W]);
       const float base = top == -INFINITY ? 0.0f : top;
-      float sum = 0;
-#pragma unroll
-      for (int x = 0; x < PER; x++) o[mp][x] = 0;
+      float sum = 0, x = 0;
+#pragma unroll 8
       for (int u = 0; u < j.parts; u++)
       {
          const float *s = from + u * step;
-         const float keep = exp2_fast(s[G::W] - base);
-         sum += s[G::W + 1] * keep;
-#pragma unroll
-         for (int x = 0; x < PER; x++)
-            if (lane + 64 * x < G::W) o[mp][x] += s[lane + 64 * x] * keep;
+         const float keep = exp2_fast(s[W] - base);
+         sum += s[W + 1] * keep;
+         if (live) x += s[f] * keep;
       }
-      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-#pragma unroll
-      for (int x = 0; x < PER; x++) o[mp][x] *= inv;
-      if (p.lse && lane == 0) p.lse[(row * p.heads + head) * MAPS + mp] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
+      o[mp] = sum == 0.0f ? 0.0f : x / sum;
+      if (p.lse && lane == 0 && piece == 0) p.lse[(row * p.heads + head) * MAPS + mp] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
    }
-   E *out = (E *)p.out + row * p.ldo + head * p.hdo;
-#pragma unroll
-   for (int x = 0; x < PER; x++)
+   if (f >= p.dv) return;
+   const int64_t at = row * p.ldo + head * p.hdo + f;
+   if constexpr (MAPS == 2)
    {
-      const int f = lane + 64 * x;
-      if (f >= p.dv) continue;
-      float res = o[0][x];
-      if constexpr (MAPS == 2)
-      {
-         if (p.out2) ((E *)p.out2)[row * p.ldo + head * p.hdo + f] = (E)Num<T>::from(o[1][x]);
-         res -= lam * o[1][x];
-      }
-      out[f] = (E)Num<T>::from(res);
+      if (p.out2) ((E *)p.out2)[at] = (E)Num<T>::from(o[1]);
+      o[0] -= p.lambda[head] * o[1];
    }
+   ((E *)p.out)[at] = (E)Num<T>::from(o[0]);
 }
 
 // ---- backward ---------------------------------------------------------------------------------------------------------------------
-// The statistics that both passes read, delta_p = <do, O_p> among them: 16 lanes per (row, head).  With O_2 at hand, <do, O_1> = <do, o> + lambda <do, O_2>.
-template <int T, int MAPS> __global__ __launch_bounds__(256) void attn_delta(Params p)
-{
-   typedef typename Num<T>::E E;
-   const int64_t id = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 4;
-   const int lane = threadIdx.x & 15;
-   const bool live = id < p.m * p.heads;
-   const int64_t row = live ? id / p.heads : 0;
-   const int head = live ? (int)(id % p.heads) : 0;
-   const E *g = (const E *)p.dout + row * p.ldo + head * p.hdo;
-   const E *o = (const E *)p.o + row * p.ldo + head * p.hdo;
-   const E *o2 = MAPS == 2 ? (const E *)p.o2 + row * p.ldo + head * p.hdo : nullptr;
-   float s = 0, s2 = 0;
-   for (int f = lane; f < p.dv; f += 16)
-   {
-      const float x = Num<T>::to(g[f]);
-      s = fmaf(x, Num<T>::to(o[f]), s);
-      if constexpr (MAPS == 2) s2 = fmaf(x, Num<T>::to(o2[f]), s2);
-   }
-#pragma unroll
-   for (int k = 8; k; k >>= 1)
-   {
-      s += __shfl_xor(s, k);
-      if constexpr (MAPS == 2) s2 += __shfl_xor(s2, k);
-   }
-   if (!live || lane) return;
-   float *to = p.stats + id * (2 * MAPS);
-#pragma unroll
-   for (int mp = 0; mp < MAPS; mp++) to[mp] = p.lse_in[id * MAPS + mp] * kLog2e;
-   if constexpr (MAPS == 2)
-   {
-      to[2] = s + p.lambda[head] * s2;
-      to[3] = s2;
-   }
-   else to[1] = s;
-}
-
 // dq: resident q and do of 16 rows per wave, gathered k and v; both maps share the gathered v and dP.
 //
-// delta comes from o as it was rounded to 16 bits, which a row of few edges feels: with mean = sum_j P dP, formed here in
+// delta_p = <do, O_p>: with O_2 at hand, <do, O_1> = <do, o> + lambda <do, O_2>; the rows are resident, so the unit forms it.
+// It comes from o as it was rounded to 16 bits, which a row of few edges feels: with mean = sum_j P dP, formed here in
 // fp32, dq = sum_j P (dP - delta) k + (delta - mean) sum_j P k.  The second sum is small where it counts, so its own rounding
 // does not matter; the exact mean replaces delta for dk.  fp32 needs none of it.
 template <int T, int DC, int MAPS, int BR> __global__ __launch_bounds__(BR * 4, (DC * MAPS >= 256 || T == kF32 ? 1 : 2)) void attn_dq(Params p)
@@ -526,11 +500,21 @@ template <int T, int DC, int MAPS, int BR> __global__ __launch_bounds__(BR * 4, 
    for (int mp = 0; mp < MAPS; mp++)
    {
       load_resident<T, G::CQ>(qr[mp], (const E *)p.q + srow * p.ldq + head * p.hdq + mp * p.d, live, p.d, g, p.vec);
-      lse2[mp] = p.stats[(srow * p.heads + head) * (2 * MAPS) + mp];
-      delta[mp] = p.stats[(srow * p.heads + head) * (2 * MAPS) + MAPS + mp];
+      lse2[mp] = p.lse_in[(srow * p.heads + head) * MAPS + mp] * kLog2e;
       sign[mp] = mp == 0 ? 1.0f : -p.lambda[head];
    }
    load_resident<T, G::CV>(gr, (const E *)p.dout + srow * p.ldo + head * p.hdo, live, p.dv, g, p.vec);
+   {
+      u4 orow[G::CV];
+      load_resident<T, G::CV>(orow, (const E *)p.o + srow * p.ldo + head * p.hdo, live, p.dv, g, p.vec);
+      delta[0] = group_sum(chunk_dot<T>(gr, orow));
+      if constexpr (MAPS == 2)
+      {
+         load_resident<T, G::CV>(orow, (const E *)p.o2 + srow * p.ldo + head * p.hdo, live, p.dv, g, p.vec);
+         delta[1] = group_sum(chunk_dot<T>(gr, orow));
+         delta[0] -= sign[1] * delta[1];
+      }
+   }
 
    const float c2 = p.scale * kLog2e;
    f4 acc[MAPS][G::NTQ], pk[kMend ? MAPS : 1][kMend ? G::NTQ : 1];
@@ -613,10 +597,18 @@ template <int T, int DC, int MAPS, int BR> __global__ __launch_bounds__(BR * 4, 
 
 #pragma unroll
    for (int mp = 0; mp < MAPS; mp++) mean[mp] = group_sum(mean[mp]);
+   if constexpr (MAPS == 2)
+   {
+      // (a row behind the last one names nothing: its mean is zero; the units of a split block add up)
+      float x = mean[1];
+#pragma unroll
+      for (int k = 8; k; k >>= 1) x += __shfl_xor(x, k);
+      if (lane == 0) p.dlam_units[((item % p.plan.n_units) * G::WAVES + wave) * p.heads + head] = x;
+   }
    if (u.part >= 0)
    {
-      // [part][head][BR rows][W + W + 2]: the two sums, the means
-      float *r = p.part + (((int64_t)u.part * p.heads + head) * BR + 16 * wave + i) * (2 * G::W + 2);
+      // [part][head][BR rows][W + W + 4]: the two sums, the means, the deltas
+      float *r = p.part + (((int64_t)u.part * p.heads + head) * BR + 16 * wave + i) * (2 * G::W + 4);
 #pragma unroll
       for (int mp = 0; mp < MAPS; mp++)
       {
@@ -628,18 +620,22 @@ template <int T, int DC, int MAPS, int BR> __global__ __launch_bounds__(BR * 4, 
                r[mp * DC + 16 * x + 4 * g + e] = acc[mp][x][e];
                if constexpr (kMend) r[G::W + mp * DC + 16 * x + 4 * g + e] = pk[mp][x][e];
             }
-         if (g == 0) r[2 * G::W + mp] = mean[mp];
+         if (g == 0)
+         {
+            r[2 * G::W + mp] = mean[mp];
+            r[2 * G::W + 2 + mp] = delta[mp];
+         }
       }
       return;
    }
    if (!live) return;
    if (g == 0)
    {
-      if (MAPS == 2) p.dlam_rows[row * p.heads + head] = mean[MAPS - 1];
-      if constexpr (kMend)
-      {
 #pragma unroll
-         for (int mp = 0; mp < MAPS; mp++) p.stats[(row * p.heads + head) * (2 * MAPS) + MAPS + mp] = mean[mp];
+      for (int mp = 0; mp < MAPS; mp++)
+      {
+         p.stats[(row * p.heads + head) * (2 * MAPS) + mp] = lse2[mp];
+         p.stats[(row * p.heads + head) * (2 * MAPS) + MAPS + mp] = kMend ? mean[mp] : delta[mp];
       }
    }
    E *out = (E *)p.dq + row * p.ldq + head * p.hdq;
@@ -659,53 +655,49 @@ template <int T, int DC, int MAPS> __global__ __launch_bounds__(256) void attn_d
    constexpr int W = DC * MAPS;
    constexpr bool kMend = T != kF32;
    typedef typename Num<T>::E E;
-   const int br = p.plan.block_rows;
-   const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-   const int lane = threadIdx.x & 63;
-   const int r = (int)(id % br);
-   const int head = (int)((id / br) % p.heads);
-   const int64_t jn = id / br / p.heads;
-   if (jn >= p.plan.n_joins) return;
-   const Join j = p.plan.joins[jn];
+   JOIN_WHERE(p.heads, (W + 63) / 64)
    const int64_t row = (int64_t)j.block * br + r;
    if (row >= p.m) return;
-   const int64_t step = (int64_t)p.heads * br * (2 * W + 2);
-   const float *from = p.part + (((int64_t)j.part0 * p.heads + head) * br + r) * (2 * W + 2);
+   const int64_t step = (int64_t)p.heads * br * (2 * W + 4);
+   const float *from = p.part + (((int64_t)j.part0 * p.heads + head) * br + r) * (2 * W + 4);
    float mend[MAPS];
 #pragma unroll
    for (int mp = 0; mp < MAPS; mp++)
    {
       float mean = 0;
+#pragma unroll 8
       for (int u = 0; u < j.parts; u++) mean += from[u * step + 2 * W + mp];
-      float *delta = p.stats + (row * p.heads + head) * (2 * MAPS) + MAPS + mp;
-      mend[mp] = *delta - mean;
-      if (lane == 0)
+      const float delta = from[2 * W + 2 + mp];
+      mend[mp] = delta - mean;
+      if (lane == 0 && piece == 0)
       {
-         if (mp == 1) p.dlam_rows[row * p.heads + head] = mean;
-         if (kMend) *delta = mean;   // (every lane has read it: one wave, in step)
+         p.stats[(row * p.heads + head) * (2 * MAPS) + mp] = p.lse_in[(row * p.heads + head) * MAPS + mp] * kLog2e;
+         p.stats[(row * p.heads + head) * (2 * MAPS) + MAPS + mp] = kMend ? mean : delta;
       }
    }
-   for (int f = lane; f < W; f += 64)
+   const int f = 64 * piece + lane;
+   if (f >= W) return;
+   float s = 0, s2 = 0;
+#pragma unroll 8
+   for (int u = 0; u < j.parts; u++)
    {
-      float s = 0, s2 = 0;
-      for (int u = 0; u < j.parts; u++)
-      {
-         s += from[u * step + f];
-         if (kMend) s2 += from[u * step + W + f];
-      }
-      const int mp = f / DC, e = f - mp * DC;
-      if (kMend) s += (mp == 0 ? mend[0] : mend[MAPS - 1]) * s2;
-      if (e < p.d) ((E *)p.dq)[row * p.ldq + head * p.hdq + mp * p.d + e] = (E)Num<T>::from(s * ((mp == 0 ? 1.0f : -p.lambda[head]) * p.scale));
+      s += from[u * step + f];
+      if (kMend) s2 += from[u * step + W + f];
    }
+   const int mp = f / DC, e = f - mp * DC;
+   if (kMend) s += (mp == 0 ? mend[0] : mend[MAPS - 1]) * s2;
+   if (e < p.d) ((E *)p.dq)[row * p.ldq + head * p.hdq + mp * p.d + e] = (E)Num<T>::from(s * ((mp == 0 ? 1.0f : -p.lambda[head]) * p.scale));
 }
 
-// dlambda_h = - sum of dlam_rows: one workgroup per head, in 64 bits, every thread's rows and then the threads in order
+// dlambda_h = - sum of dlam_units: one workgroup per head, in 64 bits, every thread's units and then the threads in order
 template <int T> __global__ __launch_bounds__(256) void attn_dlambda(Params p)
 {
    __shared__ double s[256];
    const int head = blockIdx.x;
+   const int64_t n = p.m ? (int64_t)p.plan.n_units * (p.plan.block_rows / 16) : 0;
    double x = 0;
-   for (int64_t r = threadIdx.x; r < p.m; r += 256) x += (double)p.dlam_rows[r * p.heads + head];
+#pragma unroll 4
+   for (int64_t u = threadIdx.x; u < n; u += 256) x += (double)p.dlam_units[u * p.heads + head];
    s[threadIdx.x] = x;
    __syncthreads();
    for (int k = 128; k; k >>= 1)
@@ -853,31 +845,24 @@ template <int T, int DC, int MAPS, int BR> __global__ __launch_bounds__(BR * 4, 
 
 template <int T, int DC, int MAPS> __global__ __launch_bounds__(256) void attn_dkv_join(Params p)
 {
-   typedef Geo<T, DC, MAPS, 64> G;
-   const int br = p.plan.block_rows;
-   typedef typename G::E E;
-   const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-   const int lane = threadIdx.x & 63;
-   const int r = (int)(id % br);
-   const int kvh = (int)((id / br) % p.kv_heads);
-   const int64_t jn = id / br / p.kv_heads;
-   if (jn >= p.plan.n_joins) return;
-   const Join j = p.plan.joins[jn];
+   constexpr int W = DC * MAPS;
+   typedef typename Num<T>::E E;
+   JOIN_WHERE(p.kv_heads, (2 * W + 63) / 64)
    const int64_t row = (int64_t)j.block * br + r;
    if (row >= p.n) return;
-   const int64_t step = (int64_t)p.kv_heads * br * (2 * G::W);
-   const float *from = p.part + (((int64_t)j.part0 * p.kv_heads + kvh) * br + r) * (2 * G::W);
-   for (int f = lane; f < 2 * G::W; f += 64)
+   const int64_t step = (int64_t)p.kv_heads * br * (2 * W);
+   const float *from = p.part + (((int64_t)j.part0 * p.kv_heads + head) * br + r) * (2 * W);
+   const int f = 64 * piece + lane;
+   if (f >= 2 * W) return;
+   float s = 0;
+#pragma unroll 8
+   for (int u = 0; u < j.parts; u++) s += from[u * step + f];
+   if (f < W)
    {
-      float s = 0;
-      for (int u = 0; u < j.parts; u++) s += from[u * step + f];
-      if (f < G::W)
-      {
-         const int mp = f / DC, e = f - mp * DC;
-         if (e < p.d) ((E *)p.dk)[row * p.ldk + kvh * p.hdk + mp * p.d + e] = (E)Num<T>::from(s * p.scale);
-      }
-      else if (f - G::W < p.dv) ((E *)p.dvv)[row * p.ldv + kvh * p.hdv + f - G::W] = (E)Num<T>::from(s);
+      const int mp = f / DC, e = f - mp * DC;
+      if (e < p.d) ((E *)p.dk)[row * p.ldk + head * p.hdk + mp * p.d + e] = (E)Num<T>::from(s * p.scale);
    }
+   else if (f - W < p.dv) ((E *)p.dvv)[row * p.ldv + head * p.hdv + f - W] = (E)Num<T>::from(s);
 }
 
 }  // namespace fmm_attn

@@ -54,7 +54,7 @@ template <int DC, int MAPS> struct Forward {
       ATTN_HIP(hipGetLastError());
       if (p.plan.n_joins)
       {
-         hipLaunchKernelGGL((attn_forward_join<TYPE, DC, MAPS>), dim3((unsigned)((int64_t)p.plan.n_joins * p.heads * p.plan.block_rows / 4)), dim3(256), 0, s, p);
+         hipLaunchKernelGGL((attn_forward_join<TYPE, DC, MAPS>), dim3((unsigned)((int64_t)p.plan.n_joins * p.heads * p.plan.block_rows / 4 * ((DC * MAPS + 63) / 64))), dim3(256), 0, s, p);
          ATTN_HIP(hipGetLastError());
       }
       return kOk;
@@ -66,15 +66,13 @@ template <int DC, int MAPS> struct Dq {
    {
       if (p.m)
       {
-         hipLaunchKernelGGL((attn_delta<TYPE, MAPS>), dim3((unsigned)((p.m * p.heads + 15) / 16)), dim3(256), 0, s, p);
-         ATTN_HIP(hipGetLastError());
          const int64_t n = (int64_t)p.plan.n_units * p.heads;
          if (p.plan.block_rows == 64) hipLaunchKernelGGL((attn_dq<TYPE, DC, MAPS, 64>), dim3(eighths(n)), dim3(256), 0, s, p);
          else hipLaunchKernelGGL((attn_dq<TYPE, DC, MAPS, 16>), dim3(eighths(n)), dim3(64), 0, s, p);
          ATTN_HIP(hipGetLastError());
          if (p.plan.n_joins)
          {
-            hipLaunchKernelGGL((attn_dq_join<TYPE, DC, MAPS>), dim3((unsigned)((int64_t)p.plan.n_joins * p.heads * p.plan.block_rows / 4)), dim3(256), 0, s, p);
+            hipLaunchKernelGGL((attn_dq_join<TYPE, DC, MAPS>), dim3((unsigned)((int64_t)p.plan.n_joins * p.heads * p.plan.block_rows / 4 * ((DC * MAPS + 63) / 64))), dim3(256), 0, s, p);
             ATTN_HIP(hipGetLastError());
          }
       }
@@ -96,7 +94,7 @@ template <int DC, int MAPS> struct Dkv {
       ATTN_HIP(hipGetLastError());
       if (p.plan.n_joins)
       {
-         hipLaunchKernelGGL((attn_dkv_join<TYPE, DC, MAPS>), dim3((unsigned)((int64_t)p.plan.n_joins * p.kv_heads * p.plan.block_rows / 4)), dim3(256), 0, s, p);
+         hipLaunchKernelGGL((attn_dkv_join<TYPE, DC, MAPS>), dim3((unsigned)((int64_t)p.plan.n_joins * p.kv_heads * p.plan.block_rows / 4 * ((2 * DC * MAPS + 63) / 64))), dim3(256), 0, s, p);
          ATTN_HIP(hipGetLastError());
       }
       return kOk;
@@ -116,7 +114,7 @@ int make_table(const RowsParams &p, hipStream_t s)
 template <int O, int DC, int MAPS> int join(const RowsParams &p, hipStream_t s)
 {
    if (!p.cap) return kOk;
-   hipLaunchKernelGGL((attn_rows_join<FMM_ATTN_UNIT, O, DC, MAPS>), dim3((unsigned)((p.m * p.heads + 3) / 4)), dim3(256), 0, s, p);
+   hipLaunchKernelGGL((attn_rows_join<FMM_ATTN_UNIT, O, DC, MAPS>), dim3((unsigned)(p.m * p.heads)), dim3(256), 0, s, p);
    ATTN_HIP(hipGetLastError());
    return kOk;
 }

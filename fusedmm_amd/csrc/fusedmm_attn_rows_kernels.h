@@ -67,8 +67,14 @@ __device__ inline int64_t pieces_of(int64_t len, int64_t piece)
 struct Spot {
    int64_t row, first, count;   // first piece of the row, number of its pieces
    int64_t piece;               // slots of a piece
-   int64_t total;
+   int64_t begin, len;          // the row's slots
 };
+
+__device__ inline void row_slots(const RowsParams &p, Spot &s)
+{
+   s.begin = index_of(p.pntrb, s.row, p.index_bytes);
+   s.len = row_length(p, s.row);
+}
 
 // The row that piece `id` belongs to (id < 0: row `want` is asked for).  Called by whole waves; the result is uniform.
 __device__ inline Spot find_piece(const RowsParams &p, int64_t id, int64_t want)
@@ -81,19 +87,18 @@ __device__ inline Spot find_piece(const RowsParams &p, int64_t id, int64_t want)
       s.first = s.row;
       s.count = 1;
       s.piece = INT64_MAX;
-      s.total = p.m;
+      if (s.row >= 0) row_slots(p, s);
       return s;
    }
    if (p.m > kTableRows)
    {
       const int64_t *t = p.table + 1;
       s.piece = p.table[0];
-      s.total = t[p.m];
       int64_t lo = 0;
       if (id < 0) lo = want;
       else
       {
-         if (id >= s.total) return s;
+         if (id >= t[p.m]) return s;
          int64_t hi = p.m;   // t[lo] <= id < t[hi]
          while (hi - lo > 1)
          {
@@ -105,13 +110,24 @@ __device__ inline Spot find_piece(const RowsParams &p, int64_t id, int64_t want)
       s.row = lo;
       s.first = t[lo];
       s.count = t[lo + 1] - t[lo];
+      row_slots(p, s);
       return s;
    }
    const int lane = threadIdx.x & 63;
    constexpr int kBatches = kTableRows / 64;
-   int64_t len[kBatches];
+   int64_t begin[kBatches], len[kBatches];
 #pragma unroll
-   for (int b = 0; b < kBatches; b++) len[b] = 64 * b + lane < p.m ? row_length(p, 64 * b + lane) : -1;
+   for (int b = 0; b < kBatches; b++)
+   {
+      len[b] = -1;
+      begin[b] = 0;
+      if (64 * b + lane < p.m)
+      {
+         begin[b] = index_of(p.pntrb, 64 * b + lane, p.index_bytes);
+         len[b] = index_of(p.pntre, 64 * b + lane, p.index_bytes) - begin[b];
+         if (len[b] < 0) len[b] = 0;
+      }
+   }
    int64_t piece = p.piece;
    for (;;)   // ends at the latest where every row is one piece: m <= cap
    {
@@ -120,12 +136,14 @@ __device__ inline Spot find_piece(const RowsParams &p, int64_t id, int64_t want)
       for (int b = 0; b < kBatches; b++)
       {
          if (64 * b >= p.m) break;
-         int64_t x = len[b] < 0 ? 0 : pieces_of(len[b], piece);
-         const int64_t own = x;
+         // (pieces in all are at most nnz / piece + m of the call's arguments, or more for wrong ones: kept within 32 bits)
+         const int64_t most = len[b] < 0 ? 0 : pieces_of(len[b], piece);
+         const int own = (int)(most < (1 << 24) ? most : 1 << 24);
+         int x = own;
 #pragma unroll
          for (int k = 1; k < 64; k <<= 1)
          {
-            const int64_t y = __shfl_up((long long)x, k);
+            const int y = __shfl_up(x, k);
             if (lane >= k) x += y;
          }
          const bool here = id < 0 ? 64 * b + lane == want : len[b] >= 0 && total + x - own <= id && id < total + x;
@@ -134,13 +152,14 @@ __device__ inline Spot find_piece(const RowsParams &p, int64_t id, int64_t want)
          {
             const int src = __ffsll(hit) - 1;
             s.row = 64 * b + src;
-            s.count = __shfl((long long)own, src);
-            s.first = total + __shfl((long long)x, src) - s.count;
+            s.count = __shfl(own, src);
+            s.first = total + __shfl(x, src) - s.count;
+            s.begin = __shfl((long long)begin[b], src);
+            s.len = __shfl((long long)len[b], src);
          }
-         total += __shfl((long long)x, 63);
+         total += __shfl(x, 63);
       }
       s.piece = piece;
-      s.total = total;
       if (total <= p.cap) return s;
       piece *= 2;
       s.row = -1;
@@ -284,20 +303,18 @@ __device__ inline void rows_finish(const RowsParams &p, Softmax<G::NT> &r, unsig
    }
 }
 
-// rows of several pieces: one wave per (row, head)
+// rows of several pieces: a workgroup per (row, head), its waves take the pieces in turn
 // (UNIT: the object it is compiled into)
 template <int UNIT, int O, int DC, int MAPS> __global__ __launch_bounds__(256) void attn_rows_join(RowsParams p)
 {
    constexpr int W = DC * MAPS, HP = 16 / MAPS, PER = (W + 63) / 64;
    typedef typename Num<O>::E EO;
-   const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-   if (id >= p.m * p.heads) return;
-   const int lane = threadIdx.x & 63;
-   const int64_t row = id / p.heads;
-   const int head = (int)(id % p.heads), kvh = head / p.group, hh = head % p.group, pass = hh / HP;
+   __shared__ float part[4][MAPS][W + 1];
+   const int64_t row = blockIdx.x / p.heads;
+   const int head = (int)(blockIdx.x % p.heads), kvh = head / p.group, hh = head % p.group, pass = hh / HP;
+   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
    const Spot s = find_piece(p, -1, row);
    if (s.count <= 1) return;
-   float o[MAPS][PER];
 #pragma unroll
    for (int mp = 0; mp < MAPS; mp++)
    {
@@ -308,32 +325,38 @@ template <int UNIT, int O, int DC, int MAPS> __global__ __launch_bounds__(256) v
 #pragma unroll
       for (int k = 1; k < 64; k <<= 1) top = fmaxf(top, __shfl_xor(top, k));
       const float base = top == -INFINITY ? 0.0f : top;
-      float sum = 0;
+      float sum = 0, o[PER];
 #pragma unroll
-      for (int x = 0; x < PER; x++) o[mp][x] = 0;
+      for (int x = 0; x < PER; x++) o[x] = 0;
 #pragma unroll 4
-      for (int64_t u = 0; u < s.count; u++)
+      for (int64_t u = wave; u < s.count; u += 4)
       {
          const float *f = from + u * step;
          const float keep = exp2_fast(f[W] - base);
          sum += f[W + 1] * keep;
 #pragma unroll
          for (int x = 0; x < PER; x++)
-            if (lane + 64 * x < W) o[mp][x] += f[lane + 64 * x] * keep;
+            if (lane + 64 * x < W) o[x] += f[lane + 64 * x] * keep;
       }
-      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
-      for (int x = 0; x < PER; x++) o[mp][x] *= inv;
+      for (int x = 0; x < PER; x++)
+         if (lane + 64 * x < W) part[wave][mp][lane + 64 * x] = o[x];
+      if (lane == 0) part[wave][mp][W] = sum;
    }
+   __syncthreads();
    EO *out = (EO *)p.out + row * p.ldo + head * p.hdo;
-#pragma unroll
-   for (int x = 0; x < PER; x++)
+   for (int f = threadIdx.x; f < p.dv; f += 256)
    {
-      const int f = lane + 64 * x;
-      if (f >= p.dv) continue;
-      float res = o[0][x];
-      if constexpr (MAPS == 2) res -= p.lambda[head] * o[1][x];
-      out[f] = (EO)Num<O>::from(res);
+      float r[MAPS];
+#pragma unroll
+      for (int mp = 0; mp < MAPS; mp++)
+      {
+         const float sum = part[0][mp][W] + part[1][mp][W] + part[2][mp][W] + part[3][mp][W];
+         const float x = part[0][mp][f] + part[1][mp][f] + part[2][mp][f] + part[3][mp][f];
+         r[mp] = sum == 0.0f ? 0.0f : x / sum;
+      }
+      if constexpr (MAPS == 2) r[0] -= p.lambda[head] * r[1];
+      out[f] = (EO)Num<O>::from(r[0]);
    }
 }
 
@@ -382,7 +405,7 @@ __global__ __launch_bounds__(256, (sizeof(typename Num<T>::E) * DC * MAPS >= 512
    if (s.row < 0) return;
    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, g = lane >> 4, i = lane & 15;
    unsigned char *vs = vs_all + wave * G::V::kBytes;
-   const int64_t begin = index_of(p.pntrb, s.row, p.index_bytes), len = row_length(p, s.row);
+   const int64_t begin = s.begin, len = s.len;
    const int64_t lo = s.count > 1 ? (it.id - s.first) * s.piece : 0, hi = s.count > 1 && lo + s.piece < len ? lo + s.piece : len;
    const E *k = (const E *)p.k + it.kvh * p.hdk, *v = (const E *)p.v + it.kvh * p.hdv;
 
@@ -481,15 +504,28 @@ __global__ __launch_bounds__(256, (sizeof(typename Num<T>::E) * DC * MAPS >= 512
 // most 7 significant bits, c - z at most 4, so the value is exact in fp16 and the products run on fp16 operands.
 // A code becomes 1024 + c with one and-or (0x6400 is fp16 1024), c - z with one packed subtraction, the value with one
 // packed product: 2 operations for 2 values, a third for the shift.
-__device__ inline u4 dequant8(uint32_t codes, uint32_t word)
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+struct Scale4 {
+   h2 scale, zero;
+};
+__device__ inline Scale4 scale_of(uint32_t word)
 {
-   typedef _Float16 h2 __attribute__((ext_vector_type(2)));
    const uint32_t s = word & 0xFFF0u, z = 0x6400u | (word & 15u);
-   const h2 scale = __builtin_bit_cast(h2, s | (s << 16)), zero = __builtin_bit_cast(h2, z | (z << 16));
+   return Scale4{__builtin_bit_cast(h2, s | (s << 16)), __builtin_bit_cast(h2, z | (z << 16))};
+}
+__device__ inline u4 dequant8(uint32_t codes, Scale4 q)
+{
+   // (one of an and-or's two constants has to be a register: hidden from the compiler, which would split it in two)
+   uint32_t bias = 0x64006400u;
+   asm("" : "+v"(bias));
    u4 r;
 #pragma unroll
    for (int j = 0; j < 4; j++)
-      r[j] = __builtin_bit_cast(uint32_t, (__builtin_bit_cast(h2, ((codes >> (4 * j)) & 0x000F000Fu) | 0x64006400u) - zero) * scale);
+   {
+      const h2 x = __builtin_bit_cast(h2, ((codes >> (4 * j)) & 0x000F000Fu) | bias);
+      const h2 y = (x - q.zero) * q.scale;
+      r[j] = __builtin_bit_cast(uint32_t, y);
+   }
    return r;
 }
 
@@ -522,15 +558,25 @@ template <bool FULL, int WORDS> __device__ inline void load_codes(uint32_t (&to)
    }
 }
 
-template <bool FULL, int WORDS> __device__ inline void load_scales(uint32_t (&to)[WORDS], const uint8_t *from, int width, int g)
+// The 16-bit words of a lane's codes: contiguous codes share one per 32
+template <bool FULL, int WORDS> struct Words4 {
+   static constexpr int N = FULL ? (WORDS + 3) / 4 : WORDS;
+};
+template <bool FULL, int WORDS, int N> __device__ inline void load_scales(uint32_t (&to)[N], const uint8_t *from, int width, int g)
 {
 #pragma unroll
-   for (int j = 0; j < WORDS; j++)
+   for (int j = 0; j < N; j++)
    {
-      const int f = code_feature<FULL, WORDS>(j, g);
+      const int f = code_feature<FULL, WORDS>(FULL ? 4 * j : j, g);
       to[j] = f < width ? *reinterpret_cast<const uint16_t *>(from + f / 32 * 2) : 0;
    }
 }
+
+// one map's key and all of a value row of one slot, as a lane holds them
+template <int DC, int MAPS, bool FULL> struct Record4 {
+   static constexpr int WQ = DC / 32, WV = DC * MAPS / 32;
+   uint32_t kc[MAPS][WQ], ks[MAPS][Words4<FULL, WQ>::N], vc[WV], vs[Words4<FULL, WV>::N];
+};
 
 template <int DC, int MAPS, bool FULL>
 __global__ __launch_bounds__(256, (DC * MAPS >= 256 ? 1 : 2)) void attn_rows_kv4(RowsParams p)
@@ -544,8 +590,9 @@ __global__ __launch_bounds__(256, (DC * MAPS >= 256 ? 1 : 2)) void attn_rows_kv4
    if (s.row < 0) return;
    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, g = lane >> 4, i = lane & 15;
    unsigned char *vs = vs_all + wave * G::V::kBytes;
-   const int64_t begin = index_of(p.pntrb, s.row, p.index_bytes), len = row_length(p, s.row);
-   const int64_t lo = s.count > 1 ? (it.id - s.first) * s.piece : 0, hi = s.count > 1 && lo + s.piece < len ? lo + s.piece : len;
+   const int64_t begin = s.begin, len = s.len;
+   // (a cache without slots: nothing is read)
+   const int64_t lo = s.count > 1 ? (it.id - s.first) * s.piece : 0, hi = p.n == 0 ? lo : s.count > 1 && lo + s.piece < len ? lo + s.piece : len;
    const uint8_t *cache = p.cache + it.kvh * p.hdc;
    const int kw = MAPS * p.d;
    const int off_v = kw / 2, off_kw = (kw + p.dv) / 2, off_vw = off_kw + kw / 16;   // bytes
@@ -585,32 +632,26 @@ __global__ __launch_bounds__(256, (DC * MAPS >= 256 ? 1 : 2)) void attn_rows_kv4
 
    Softmax<G::NT> r;
 
-   uint32_t kc[2][MAPS][WQ], vc[2][WV], ks[2][MAPS][WQ], vw[2][WV];
-   auto load = [&](int32_t slot) __attribute__((always_inline)) {
+   typedef Record4<DC, MAPS, FULL> Rec;
+   auto load = [&](Rec (&to)[2], int32_t slot) __attribute__((always_inline)) {
 #pragma unroll
       for (int a = 0; a < 2; a++)
       {
+         // a place without a slot reads record 0, which is masked
          const int32_t c = __shfl(slot, 16 * a + i);
-         if (c >= 0)
-         {
-            const uint8_t *rec = cache + (int64_t)c * p.ldc;
+         const uint8_t *rec = cache + (int64_t)(c < 0 ? 0 : c) * p.ldc;
 #pragma unroll
-            for (int mp = 0; mp < MAPS; mp++)
-            {
-               load_codes<FULL>(kc[a][mp], rec + mp * p.d / 2, p.d, g);
-               load_scales<FULL>(ks[a][mp], rec + off_kw + mp * p.d / 16, p.d, g);
-            }
-            load_codes<FULL>(vc[a], rec + off_v, p.dv, g);
-            load_scales<FULL>(vw[a], rec + off_vw, p.dv, g);
+         for (int mp = 0; mp < MAPS; mp++)
+         {
+            load_codes<FULL>(to[a].kc[mp], rec + mp * p.d / 2, p.d, g);
+            load_scales<FULL, WQ>(to[a].ks[mp], rec + off_kw + mp * p.d / 16, p.d, g);
          }
-         else
+         load_codes<FULL>(to[a].vc, rec + off_v, p.dv, g);
+         load_scales<FULL, WV>(to[a].vs, rec + off_vw, p.dv, g);
+         if (c < 0)
          {
 #pragma unroll
-            for (int j = 0; j < WQ; j++)
-#pragma unroll
-               for (int mp = 0; mp < MAPS; mp++) kc[a][mp][j] = ks[a][mp][j] = 0;
-#pragma unroll
-            for (int j = 0; j < WV; j++) vc[a][j] = vw[a][j] = 0;
+            for (int j = 0; j < Words4<FULL, WV>::N; j++) to[a].vs[j] = 0;   // values of zero, whatever the record holds
          }
       }
    };
@@ -620,11 +661,8 @@ __global__ __launch_bounds__(256, (DC * MAPS >= 256 ? 1 : 2)) void attn_rows_kv4
       constexpr bool CAREFUL = decltype(careful)::value;
       r.clear();
       int64_t at = begin + lo + wave * kTile;
-      int32_t slot = tile_slot(p, at, end, lane);
-      int32_t next = tile_slot(p, at + kStride, end, lane);
-      if (at < end) load(slot);
-      for (; at < end; at += kStride)
-      {
+      int32_t slot = tile_slot(p, at, end, lane), next = tile_slot(p, at + kStride, end, lane);
+      auto use = [&](const Rec (&rec)[2], int32_t slot) __attribute__((always_inline)) {
          bool all;
          const unsigned mine = tile_bits(slot, g, &all);
          f4 sc[MAPS][2];
@@ -636,19 +674,12 @@ __global__ __launch_bounds__(256, (DC * MAPS >= 256 ? 1 : 2)) void attn_rows_kv4
             {
                sc[mp][a] = f4{0, 0, 0, 0};
 #pragma unroll
-               for (int j = 0; j < WQ; j++) sc[mp][a] = G::N::mma(dequant8(kc[a][mp][j], ks[a][mp][j]), q[j], sc[mp][a]);
+               for (int j = 0; j < WQ; j++) sc[mp][a] = G::N::mma(dequant8(rec[a].kc[mp][j], scale_of(rec[a].ks[mp][FULL ? j / 4 : j])), q[j], sc[mp][a]);
             }
 #pragma unroll
             for (int j = 0; j < WV; j++)
-            {
-               *reinterpret_cast<u4 *>(vs + (16 * a + i) * G::V::RB + ((code_feature<FULL, WV>(j, g) / 8) ^ G::V::twist(i)) * 16) = dequant8(vc[a][j], vw[a][j]);
-            }
-         }
-         slot = next;
-         if (at + kStride < end)
-         {
-            load(slot);
-            next = tile_slot(p, at + 2 * kStride, end, lane);
+               *reinterpret_cast<u4 *>(vs + (16 * a + i) * G::V::RB + ((code_feature<FULL, WV>(j, g) / 8) ^ G::V::twist(i)) * 16) =
+                  dequant8(rec[a].vc[j], scale_of(rec[a].vs[FULL ? j / 4 : j]));
          }
          if constexpr (MAPS == 2)
          {
@@ -658,6 +689,23 @@ __global__ __launch_bounds__(256, (DC * MAPS >= 256 ? 1 : 2)) void attn_rows_kv4
          wave_lds_order();
          row_step<G, kF16, CAREFUL>(r, sc[0], c2, mine, all, vs, g, i);
          wave_lds_order();
+      };
+      // two tiles in turn, so that one is under way while the other is used
+      Rec even[2], odd[2];
+      if (at < end) load(even, slot);
+      while (at < end)
+      {
+         const int32_t after = tile_slot(p, at + 2 * kStride, end, lane);
+         if (at + kStride < end) load(odd, next);
+         use(even, slot);
+         at += kStride;
+         if (at >= end) break;
+         slot = tile_slot(p, at + 2 * kStride, end, lane);
+         if (at + kStride < end) load(even, after);
+         use(odd, next);
+         at += kStride;
+         next = slot;
+         slot = after;
       }
       return odd_sums(r.acc);
    };
@@ -788,7 +836,7 @@ template <int T> __global__ __launch_bounds__(256) void kv4_read(Kv4Params p)
          codes = *reinterpret_cast<const uint32_t *>(rec + 4 * w);
          word = *reinterpret_cast<const uint16_t *>(rec + 4 * words + w / 4 * 2);
       }
-      const u4 h = dequant8(codes, word);
+      const u4 h = dequant8(codes, scale_of(word));
       const bool is_v = 8 * w >= p.k_width;
       const int f = is_v ? 8 * w - p.k_width : 8 * w;
       E *to = is_v ? (E *)p.to_v + tok * p.ldv + head * p.hdv + f : (E *)p.to_k + tok * p.ldk + head * p.hdk + f;

@@ -274,6 +274,22 @@ def test_rows_over_the_cache(kind, shape):
         check_rows(c, e)
 
 
+@pytest.mark.parametrize("maps", [1, 2])
+def test_rows_that_name_nothing(maps):
+    """Empty rows, rows of masked ids only, and a cache without a single slot, in both forms: zeros."""
+    import torch
+    indx = np.array([-1, 40, 77, -5, 41])
+    for n in (40, 0):
+        c = CacheCase("bf16", maps, 3, n, 2, 1, 32, 32 * maps, indx, np.array([0, 0, 2]), np.array([5, 0, 4]), seed=1)
+        assert c.rows() == 0
+        torch.cuda.synchronize()
+        assert (c.o.numpy() == 0).all() and c.o.untouched_outside()
+        c.o.buf.fill_(SENTINEL)
+        assert Case.rows(c) == 0 and Case.rows_again(c) == 0
+        torch.cuda.synchronize()
+        assert (c.o.numpy() == 0).all() and c.o.untouched_outside()
+
+
 def test_queries_beyond_fp16_s_range():
     """bf16 queries of 1e6 and of 1e-9 against cached keys: the score scale makes up for it."""
     import torch
