@@ -179,13 +179,12 @@ def load_probes():
 
 def _addr(a):
     """Raw address of a numpy array, a torch tensor, an int, or None."""
-    if a is None:
-        return None
-    if isinstance(a, int):
+    if a is None or isinstance(a, int):
         return a
-    if hasattr(a, "data_ptr"):
+    try:
         return a.data_ptr()
-    return a.ctypes.data
+    except AttributeError:
+        return a.ctypes.data
 
 
 def fusedMM_csr(imessage, m, n, k, alpha, nnz, rows, cols, val, indx, pntrb, pntre, x, ldx, y, ldy, beta, z, ldz,

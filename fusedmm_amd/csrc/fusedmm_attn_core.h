@@ -342,6 +342,9 @@ __device__ inline float group_sum(float x)
    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
+// what stands behind this in a branch is not done without it (the compiler would rather select than branch)
+__device__ inline void keep_branch() { asm volatile(""); }
+
 // scores whose bit of `mine` is clear -> `other`
 __device__ inline float masked(float x, unsigned mine, int j, float other)
 {

@@ -181,8 +181,6 @@ Params base_params(const Desc &d, const Plan &plan)
    p.ldk_bytes = (int32_t)(d.ldk * bytes);
    p.ldv_bytes = (int32_t)(d.ldv * bytes);
    p.ldo_bytes = (int32_t)(d.ldo * bytes);
-   const int dc = width_class(d.d, d.dv, d.maps);
-   p.full = d.d == dc && d.dv == dc * d.maps;
    return p;
 }
 
@@ -199,12 +197,11 @@ bool whole_chunks(const Desc &d)
 
 // ---- serving form ----
 
-// Slots of a piece: about 2048 workgroups over all key heads, so that 256 compute units of two to four have several
-// turns to even out what rows of different lengths leave; not under 256 (two tiles per wave: below that a join costs more
-// than it spreads), not over 8192.
+// Slots of a piece: about 1024 workgroups over all key heads - a ragged batch is no faster with 2048, two rows of 200k
+// slots are a quarter slower (48 and 62 us with 768 and 2048) - and not under 256 (two tiles per wave), not over 8192.
 int64_t piece_slots(int64_t nnz, int64_t columns)
 {
-   const int64_t want = nnz * columns / 2048;
+   const int64_t want = nnz * columns / 1024;
    return (std::min<int64_t>(std::max<int64_t>(want, 256), 8192) + 127) / 128 * 128;
 }
 
@@ -428,6 +425,7 @@ int fusedMM_attn_forward(const fusedMM_attn_desc *desc, const void *plan, const 
    const int bytes = element_bytes(d);
    p.vec = whole_chunks(d) && lines_up(q, d.ldq, d.hdq, bytes) && lines_up(k, d.ldk, d.hdk, bytes) && lines_up(v, d.ldv, d.hdv, bytes) &&
            lines_up(o, d.ldo, d.hdo, bytes) && lines_up(o2, 0, 0, bytes);
+   p.full = p.vec && d.d == dc && d.dv == dc * d.maps;
    p.q = q;
    p.k = k;
    p.v = v;
@@ -470,6 +468,7 @@ int fusedMM_attn_backward(const fusedMM_attn_desc *desc, const void *plan, const
    p.vec = whole_chunks(d) && lines_up(q, d.ldq, d.hdq, bytes) && lines_up(k, d.ldk, d.hdk, bytes) && lines_up(v, d.ldv, d.hdv, bytes) &&
            lines_up(o, d.ldo, d.hdo, bytes) && lines_up(dout, 0, 0, bytes) && lines_up(dq, 0, 0, bytes) && lines_up(dk, 0, 0, bytes) &&
            lines_up(dv, 0, 0, bytes);
+   p.full = p.vec && d.d == dc && d.dv == dc * d.maps;
    p.q = q;
    p.k = k;
    p.v = v;
@@ -574,6 +573,11 @@ int fusedMM_attn_rows_kv4(const fusedMM_attn_desc *desc, const INDEXTYPE nnz, co
       return kNoImpl;
    }
    st = check_cache(who, *desc, cache, ldc, hdc, false);
+   if (!st && dc * desc->maps == 256 && (desc->d != dc || desc->dv != 256))
+   {
+      ATTN_LOG("%s: over 128 features a key or value, d is %d and dv 256", who, dc);
+      st = kNoImpl;
+   }
    if (st || desc->m == 0) return st;
    if (desc->n > 0 && !cache) return refuse(who, "a pointer is null");
    const void *ptrs[] = {indx, pntrb, pntre, q, cache, lambda, o, work};

@@ -44,7 +44,7 @@ struct Params {
    int64_t ldq, hdq, ldk, hdk, ldv, hdv, ldo, hdo;
    int32_t ldk_bytes, ldv_bytes, ldq_bytes, ldo_bytes;
    int32_t vec;                       // every row of every tensor is 16-byte aligned and d, dv are multiples of a 16-byte chunk
-   int32_t full;                      // d and dv fill the instance's width
+   int32_t full;                      // vec, and d and dv fill the instance's width
    const void *q, *k, *v, *o, *o2, *dout;
    const float *lambda;
    const float *lse_in;
@@ -114,10 +114,12 @@ template <class G, int T, int DC, int BR> struct Stream {
    const int32_t *cols;          // of the unit
    const uint32_t *masks;
    int tid, wave;
-   const E *a, *b;
+   const unsigned char *a, *b;
    uint32_t lda, ldb;            // bytes from row to row
    int d, dv;
-   bool vec, full;
+   bool vec;
+   static constexpr int NB = BR == 64 ? G::NCH : 1;
+   const unsigned char *pa[NB], *pb[NB];   // BR = 64: this thread's chunks of row 0 (more threads would be more registers)
 
    // a: rows of maps pieces of d features each; b: rows of dv features
    __device__ inline void set(const unsigned char *t, unsigned char *i, unsigned char *m, const Params &p, const Unit &u, const E *a_, int lda_, const E *b_, int ldb_)
@@ -129,14 +131,23 @@ template <class G, int T, int DC, int BR> struct Stream {
       masks = p.plan.masks + (int64_t)u.tile0 * BR;
       tid = threadIdx.x;
       wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-      a = a_;
-      b = b_;
+      a = (const unsigned char *)a_;
+      b = (const unsigned char *)b_;
       lda = lda_;
       ldb = ldb_;
       d = p.d;
       dv = p.dv;
       vec = p.vec;
-      full = p.full;
+      if constexpr (BR == 64)
+      {
+#pragma unroll
+         for (int j = 0; j < G::NCH; j++)
+         {
+            const int x = tid + G::THREADS * j, at = ((x % G::CR) ^ V::twist(x / G::CR)) * 16;
+            pa[j] = a + at;
+            pb[j] = b + at;
+         }
+      }
    }
 
    // column ids and masks of tiles 8 g .. 8 g + 7; waves 0 and 1 (the ones that always load tiles) do it
@@ -166,14 +177,45 @@ template <class G, int T, int DC, int BR> struct Stream {
       return *(const uint32_t *)(bits + ((t / kAhead) & 1) * (kAhead * G::kMaskBytes) + (t % kAhead) * G::kMaskBytes + (wave * 16 + i) * 4);
    }
 
-   // tile t -> buffer; a and b may be moved (other heads) between calls
-   __device__ __forceinline__ void load_tile(int t, int buf, const E *pa, const E *pb) const
+   // Tile t -> buffer; the rows start oa and ob bytes behind a and b (other heads).
+   // d and dv fill the width and every chunk is 16-byte aligned: the shortest way.
+   __device__ __forceinline__ void load_full(int t, int buf, int64_t oa, int64_t ob) const
    {
       const int32_t *c = tile_ids(t);
-      const unsigned char *ta = tiles + buf * G::kPair, *tb = ta + V::kBytes;
-      const uint32_t la = lds_address(ta) + wave * 1024, lb = lds_address(tb) + wave * 1024;
+      const uint32_t la = lds_address(tiles + buf * G::kPair) + wave * 1024, lb = la + V::kBytes;
       int me = tid;
-      asm volatile("" : "+v"(me));   // the places below are formed again for every tile, not kept in registers over the loop
+      if constexpr (BR != 64) asm volatile("" : "+v"(me));   // the places are formed again for every tile, not kept in registers
+#pragma unroll
+      for (int j = 0; j < G::NCH; j++)
+      {
+         const int x = me + G::THREADS * j, r = x / G::CR;
+         if (kTile * G::CR < G::THREADS && x >= kTile * G::CR) break;
+         const uint32_t col = (uint32_t)c[r];
+         const unsigned char *fa, *fb;
+         if constexpr (BR == 64)
+         {
+            fa = pa[j];
+            fb = pb[j];
+         }
+         else
+         {
+            const int at = ((x % G::CR) ^ V::twist(r)) * 16;
+            fa = a + at;
+            fb = b + at;
+         }
+         load_lds16(la + j * (G::THREADS * 16), fa + oa + (uint64_t)col * lda);
+         load_lds16(lb + j * (G::THREADS * 16), fb + ob + (uint64_t)col * ldb);
+      }
+   }
+
+   // any sizes and places
+   __device__ __forceinline__ void load_any(int t, int buf, int64_t oa, int64_t ob) const
+   {
+      const int32_t *c = tile_ids(t);
+      unsigned char *ta = const_cast<unsigned char *>(tiles) + buf * G::kPair, *tb = ta + V::kBytes;
+      const uint32_t la = lds_address(ta) + wave * 1024, lb = la + V::kBytes;
+      int me = tid;
+      asm volatile("" : "+v"(me));
 #pragma unroll
       for (int j = 0; j < G::NCH; j++)
       {
@@ -181,20 +223,12 @@ template <class G, int T, int DC, int BR> struct Stream {
          if (kTile * G::CR < G::THREADS && x >= kTile * G::CR) break;
          const uint32_t col = (uint32_t)c[r];
          const int e = ((x % G::CR) ^ V::twist(r)) * G::N::EPL, f = e % DC;   // this thread's chunk of a gathered row
-         const E *fa = (const E *)((const unsigned char *)pa + (uint64_t)col * lda) + (e / DC * d + f);
-         const E *fb = (const E *)((const unsigned char *)pb + (uint64_t)col * ldb) + e;
+         const E *fa = (const E *)(a + oa + (uint64_t)col * lda) + (e / DC * d + f);
+         const E *fb = (const E *)(b + ob + (uint64_t)col * ldb) + e;
          if (vec)
          {
-            if (full)
-            {
-               load_lds16(la + j * (G::THREADS * 16), fa);
-               load_lds16(lb + j * (G::THREADS * 16), fb);
-            }
-            else
-            {
-               load_lds16(la + j * (G::THREADS * 16), f < d ? (const void *)fa : (const void *)&zero_chunk);
-               load_lds16(lb + j * (G::THREADS * 16), e < dv ? (const void *)fb : (const void *)&zero_chunk);
-            }
+            load_lds16(la + j * (G::THREADS * 16), f < d ? (const void *)fa : (const void *)&zero_chunk);
+            load_lds16(lb + j * (G::THREADS * 16), e < dv ? (const void *)fb : (const void *)&zero_chunk);
          }
          else
          {
@@ -203,6 +237,12 @@ template <class G, int T, int DC, int BR> struct Stream {
             *(u4 *)(tb + x * 16) = load_chunk<T>(fb, dv - e < G::N::EPL ? dv - e : G::N::EPL, false);
          }
       }
+   }
+
+   template <bool FULL> __device__ __forceinline__ void load_tile(int t, int buf, int64_t oa, int64_t ob) const
+   {
+      if constexpr (FULL) load_full(t, buf, oa, ob);
+      else load_any(t, buf, oa, ob);
    }
 };
 
@@ -255,6 +295,12 @@ template <int BR> __device__ inline bool any_odd(bool odd)
    if constexpr (BR == 16) return __any(odd);
    else return __syncthreads_or(odd);
 }
+// How a pass over a unit runs: full 16-byte chunks, any sizes, or any sizes with care for infinities and NaN.
+enum : int { kFull, kAny, kCareful };
+template <int M> struct Mode {
+   static constexpr int value = M;
+};
+
 // The loop over a unit's tiles that all kernels share: fill the pipeline, then for every step wait, free the oldest
 // buffer, fill it, and use the current one.  steps = tiles * per_tile; load(step, buffer), use(step, buffer).
 template <class G, int BR, class S, class Load, class Use> __device__ __forceinline__ void for_tiles(const S &st, int steps, int per_tile, Load load, Use use)
@@ -323,12 +369,12 @@ template <int T, int DC, int MAPS, int BR> __global__ __launch_bounds__(BR * 4, 
          for (int c = 0; c < G::CQ; c++) qr[mp][c] = negated<T>(qr[mp][c]);
    }
    Softmax<G::NT> soft[MAPS];
-   auto pass = [&](auto careful) {
-      constexpr bool CAREFUL = decltype(careful)::value;
+   auto pass = [&](auto mode) {
+      constexpr bool CAREFUL = decltype(mode)::value == kCareful, FULL = decltype(mode)::value == kFull;
 #pragma unroll
       for (int mp = 0; mp < MAPS; mp++) soft[mp].clear();
       for_tiles<G, BR>(
-         st, u.tiles, 1, [&](int t, int buf) __attribute__((always_inline)) { st.load_tile(t, buf, st.a, st.b); },
+         st, u.tiles, 1, [&](int t, int buf) __attribute__((always_inline)) { st.template load_tile<FULL>(t, buf, 0, 0); },
          [&](int t, int buf) __attribute__((always_inline)) {
             const uint32_t word = st.row_mask(t, i);
             if (!__any(word != 0)) return;
@@ -344,6 +390,7 @@ template <int T, int DC, int MAPS, int BR> __global__ __launch_bounds__(BR * 4, 
                tile_scores<T, G::W, G::CQ>(s, ks, mp * G::MC, qr[mp], l);
                if (!all)
                {
+                  keep_branch();
 #pragma unroll
                   for (int j = 0; j < 8; j++) s[j / 4][j % 4] = masked(s[j / 4][j % 4], mine, j, -INFINITY);
                }
@@ -370,7 +417,7 @@ template <int T, int DC, int MAPS, int BR> __global__ __launch_bounds__(BR * 4, 
       if constexpr (MAPS == 2) odd |= odd_sums(soft[1].acc);
       return odd;
    };
-   if (any_odd<BR>(pass(Flag<false>()))) (void)pass(Flag<true>());
+   if (any_odd<BR>(p.full ? pass(Mode<kFull>()) : pass(Mode<kAny>()))) (void)pass(Mode<kCareful>());
 
 #pragma unroll
    for (int mp = 0; mp < MAPS; mp++) soft[mp].sum = group_sum(soft[mp].sum);
@@ -518,8 +565,8 @@ template <int T, int DC, int MAPS, int BR> __global__ __launch_bounds__(BR * 4, 
 
    const float c2 = p.scale * kLog2e;
    f4 acc[MAPS][G::NTQ], pk[kMend ? MAPS : 1][kMend ? G::NTQ : 1];
-   auto pass = [&](auto careful) {
-      constexpr bool CAREFUL = decltype(careful)::value;
+   auto pass = [&](auto mode) {
+      constexpr bool CAREFUL = decltype(mode)::value == kCareful, FULL = decltype(mode)::value == kFull;
 #pragma unroll
       for (int mp = 0; mp < MAPS; mp++)
       {
@@ -532,7 +579,7 @@ template <int T, int DC, int MAPS, int BR> __global__ __launch_bounds__(BR * 4, 
          }
       }
       for_tiles<G, BR>(
-         st, u.tiles, 1, [&](int t, int buf) __attribute__((always_inline)) { st.load_tile(t, buf, st.a, st.b); },
+         st, u.tiles, 1, [&](int t, int buf) __attribute__((always_inline)) { st.template load_tile<FULL>(t, buf, 0, 0); },
          [&](int t, int buf) __attribute__((always_inline)) {
             const uint32_t word = st.row_mask(t, i);
             if (!__any(word != 0)) return;
@@ -544,6 +591,7 @@ template <int T, int DC, int MAPS, int BR> __global__ __launch_bounds__(BR * 4, 
             tile_scores<T, G::W, G::CV>(dp, vs, 0, gr, l);
             if (!all)   // (zero times what is masked has to be zero)
             {
+               keep_branch();
 #pragma unroll
                for (int j = 0; j < 8; j++) dp[j / 4][j % 4] = masked(dp[j / 4][j % 4], mine, j, 0.0f);
             }
@@ -557,6 +605,7 @@ template <int T, int DC, int MAPS, int BR> __global__ __launch_bounds__(BR * 4, 
                for (int j = 0; j < 8; j++) pr[j / 4][j % 4] = exp2_fast(fmaf(s[j / 4][j % 4], c2, -lse2[mp]));
                if (!all)
                {
+                  keep_branch();
 #pragma unroll
                   for (int j = 0; j < 8; j++) pr[j / 4][j % 4] = masked(pr[j / 4][j % 4], mine, j, 0.0f);
                }
@@ -593,7 +642,7 @@ template <int T, int DC, int MAPS, int BR> __global__ __launch_bounds__(BR * 4, 
       }
       return odd;
    };
-   if (any_odd<BR>(pass(Flag<false>()))) (void)pass(Flag<true>());
+   if (any_odd<BR>(p.full ? pass(Mode<kFull>()) : pass(Mode<kAny>()))) (void)pass(Mode<kCareful>());
 
 #pragma unroll
    for (int mp = 0; mp < MAPS; mp++) mean[mp] = group_sum(mean[mp]);
@@ -734,9 +783,9 @@ template <int T, int DC, int MAPS, int BR> __global__ __launch_bounds__(BR * 4, 
    const float c2 = p.scale * kLog2e;
    f4 dk[MAPS][G::NTQ], dv[G::NT];
 
-   auto load = [&](int s, int buf) __attribute__((always_inline)) {
+   auto load = [&](int s, int buf, auto full) __attribute__((always_inline)) {
       const int t = s / p.group, head = kvh * p.group + s % p.group;
-      st.load_tile(t, buf, st.a + head * p.hdq, st.b + head * p.hdo);
+      st.template load_tile<decltype(full)::value>(t, buf, head * p.hdq * (int64_t)sizeof(E), head * p.hdo * (int64_t)sizeof(E));
       // the statistics of the tile's rows: [32 rows][2 maps], 8 or 16 bytes of a row each
       if (tid < (MAPS == 2 ? 32 : 64))
       {
@@ -774,6 +823,7 @@ template <int T, int DC, int MAPS, int BR> __global__ __launch_bounds__(BR * 4, 
          for (int j = 0; j < 8; j++) w[j / 4][j % 4] = exp2_fast(fmaf(sc[j / 4][j % 4], c2, -rs[j][mp]));
          if (!all)
          {
+            keep_branch();
 #pragma unroll
             for (int j = 0; j < 8; j++) w[j / 4][j % 4] = masked(w[j / 4][j % 4], mine, j, 0.0f);
          }
@@ -787,6 +837,7 @@ template <int T, int DC, int MAPS, int BR> __global__ __launch_bounds__(BR * 4, 
          }
          if (!all)   // (zero times the products and statistics of a row that is masked has to be zero)
          {
+            keep_branch();
 #pragma unroll
             for (int j = 0; j < 8; j++) w[j / 4][j % 4] = masked(w[j / 4][j % 4], mine, j, 0.0f);
          }
@@ -799,7 +850,8 @@ template <int T, int DC, int MAPS, int BR> __global__ __launch_bounds__(BR * 4, 
       }
       add_weighted<T, G::W, CAREFUL>(dv, wv, mine, gs, 0, g, i, l);
    };
-   auto pass = [&](auto careful) {
+   auto pass = [&](auto mode) {
+      constexpr bool CAREFUL = decltype(mode)::value == kCareful, FULL = decltype(mode)::value == kFull;
 #pragma unroll
       for (int mp = 0; mp < MAPS; mp++)
 #pragma unroll
@@ -807,13 +859,15 @@ template <int T, int DC, int MAPS, int BR> __global__ __launch_bounds__(BR * 4, 
 #pragma unroll
       for (int t = 0; t < G::NT; t++) dv[t] = f4{0, 0, 0, 0};
       // (steps of one tile, the heads of the group, follow each other: tiles * group < 2^31 is checked by the host)
-      for_tiles<G, BR>(st, u.tiles * p.group, p.group, load, [&](int s, int buf) __attribute__((always_inline)) { use(s, buf, careful); });
+      for_tiles<G, BR>(st, u.tiles * p.group, p.group,
+         [&](int s, int buf) __attribute__((always_inline)) { load(s, buf, Flag<FULL>()); },
+         [&](int s, int buf) __attribute__((always_inline)) { use(s, buf, Flag<CAREFUL>()); });
       bool odd = odd_sums(dv);
 #pragma unroll
       for (int mp = 0; mp < MAPS; mp++) odd |= odd_sums(dk[mp]);
       return odd;
    };
-   if (any_odd<BR>(pass(Flag<false>()))) (void)pass(Flag<true>());
+   if (any_odd<BR>(p.full ? pass(Mode<kFull>()) : pass(Mode<kAny>()))) (void)pass(Mode<kCareful>());
 
    constexpr float unscale = 1.0f / G::N::kPScale;
    if (u.part >= 0)

@@ -128,7 +128,8 @@ template <int DC, int MAPS> struct Rows {
    {
       int st = make_table(p, s);
       if (st) return st;
-      hipLaunchKernelGGL((attn_rows<TYPE, DC, MAPS>), dim3(rows_grid(p)), dim3(256), 0, s, p);
+      if (p.vec_kv && p.d == DC && p.dv == DC * MAPS) hipLaunchKernelGGL((attn_rows<TYPE, DC, MAPS, true>), dim3(rows_grid(p)), dim3(256), 0, s, p);
+      else hipLaunchKernelGGL((attn_rows<TYPE, DC, MAPS, false>), dim3(rows_grid(p)), dim3(256), 0, s, p);
       ATTN_HIP(hipGetLastError());
       return join<TYPE, DC, MAPS>(p, s);
    }
@@ -139,10 +140,9 @@ template <int DC, int MAPS> struct Rows4 {
    {
       int st = make_table(p, s);
       if (st) return st;
-      if (p.d == DC && p.dv == DC * MAPS)
-         hipLaunchKernelGGL((attn_rows_kv4<DC, MAPS, true>), dim3(rows_grid(p)), dim3(256), 0, s, p);
-      else
-         hipLaunchKernelGGL((attn_rows_kv4<DC, MAPS, false>), dim3(rows_grid(p)), dim3(256), 0, s, p);
+      if (p.d == DC && p.dv == DC * MAPS) hipLaunchKernelGGL((attn_rows_kv4<DC, MAPS, true>), dim3(rows_grid(p)), dim3(256), 0, s, p);
+      else if constexpr (DC * MAPS < 256) hipLaunchKernelGGL((attn_rows_kv4<DC, MAPS, false>), dim3(rows_grid(p)), dim3(256), 0, s, p);
+      else return kNoImpl;   // refused by the entry point
       ATTN_HIP(hipGetLastError());
       return p.out_type == kF16 ? join<kF16, DC, MAPS>(p, s) : join<kBF16, DC, MAPS>(p, s);
    }

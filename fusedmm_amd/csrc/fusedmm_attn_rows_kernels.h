@@ -229,6 +229,7 @@ __device__ inline void row_step(Softmax<G::NT> &r, f4 (&sc)[2], float c2, unsign
 {
    if (!all)
    {
+      keep_branch();
 #pragma unroll
       for (int j = 0; j < 8; j++) sc[j / 4][j % 4] = masked(sc[j / 4][j % 4], mine, j, -INFINITY);
    }
@@ -376,8 +377,20 @@ __device__ inline RowsItem rows_item(const RowsParams &p)
    return r;
 }
 
-// slot of the tile's row lane % 32, -1 where there is none
+// Slot of the tile's row lane % 32, -1 where there is none.  No branches: a load under a condition leaves the compiler
+// without a count of the loads under way, and it then waits for all of them, the next tile's among them.  So the place is
+// kept within the piece, and the two halves of a 64-bit id are read as such (of a 32-bit id, the same one twice).
 __device__ inline int32_t tile_slot(const RowsParams &p, int64_t at, int64_t end, int lane)
+{
+   const int64_t e = at + (lane & 31), last = end - 1;
+   const unsigned char *from = (const unsigned char *)p.indx + (e < end ? e : last) * p.index_bytes;
+   const int32_t lo = *(const int32_t *)from, hi = *(const int32_t *)(from + p.index_bytes - 4);
+   const bool wide = hi != (p.index_bytes == 8 ? 0 : lo);
+   return e < end && !wide && lo >= 0 && lo < p.n ? lo : -1;
+}
+
+// the same with branches, where the loads are conditional anyhow
+__device__ inline int32_t tile_slot_any(const RowsParams &p, int64_t at, int64_t end, int lane)
 {
    const int64_t e = at + (lane & 31);
    if (e >= end) return -1;
@@ -393,7 +406,10 @@ __device__ inline unsigned tile_bits(int32_t slot, int g, bool *all)
 }
 
 // ---- keys and values in their own type ------------------------------------------------------------------------------------------
-template <int T, int DC, int MAPS>
+// FULL: d and dv fill the width and every chunk is 16-byte aligned.  All loads are then unconditional: a place without a
+// slot reads slot 0, whose scores are masked, and whose values have weight zero (or, if they are not finite, are seen by
+// the pass that takes care of those).
+template <int T, int DC, int MAPS, bool FULL>
 __global__ __launch_bounds__(256, (sizeof(typename Num<T>::E) * DC * MAPS >= 512 ? 1 : 2)) void attn_rows(RowsParams p)
 {
    typedef RowGeo<T, DC, MAPS> G;
@@ -406,7 +422,8 @@ __global__ __launch_bounds__(256, (sizeof(typename Num<T>::E) * DC * MAPS >= 512
    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, g = lane >> 4, i = lane & 15;
    unsigned char *vs = vs_all + wave * G::V::kBytes;
    const int64_t begin = s.begin, len = s.len;
-   const int64_t lo = s.count > 1 ? (it.id - s.first) * s.piece : 0, hi = s.count > 1 && lo + s.piece < len ? lo + s.piece : len;
+   // (a cache without slots: nothing is read)
+   const int64_t lo = s.count > 1 ? (it.id - s.first) * s.piece : 0, hi = p.n == 0 ? lo : s.count > 1 && lo + s.piece < len ? lo + s.piece : len;
    const E *k = (const E *)p.k + it.kvh * p.hdk, *v = (const E *)p.v + it.kvh * p.hdv;
 
    const int mp_i = i / G::HP, hh = it.pass * G::HP + i % G::HP;
@@ -437,7 +454,8 @@ __global__ __launch_bounds__(256, (sizeof(typename Num<T>::E) * DC * MAPS >= 512
             for (int x = 0; x < G::CQ; x++)
             {
                const int f = x * G::N::KC + g * G::N::EPL, left = p.d - f;
-               kf[a][mp][x] = load_chunk<T>(row + mp * p.d + f, c < 0 ? 0 : left < G::N::EPL ? left : G::N::EPL, p.vec_kv);
+               if constexpr (FULL) kf[a][mp][x] = *reinterpret_cast<const u4 *>(row + mp * DC + f);
+               else kf[a][mp][x] = load_chunk<T>(row + mp * p.d + f, c < 0 ? 0 : left < G::N::EPL ? left : G::N::EPL, p.vec_kv);
             }
       }
 #pragma unroll
@@ -445,7 +463,9 @@ __global__ __launch_bounds__(256, (sizeof(typename Num<T>::E) * DC * MAPS >= 512
       {
          const int e = lane + 64 * j, f = (e % G::CR) * G::N::EPL, left = p.dv - f;
          const int32_t c = __shfl(slot, e / G::CR);
-         vf[j] = load_chunk<T>(v + (int64_t)(c < 0 ? 0 : c) * p.ldv + f, c < 0 ? 0 : left < G::N::EPL ? left : G::N::EPL, p.vec_kv);
+         const E *at = v + (int64_t)(c < 0 ? 0 : c) * p.ldv + f;
+         if constexpr (FULL) vf[j] = *reinterpret_cast<const u4 *>(at);
+         else vf[j] = load_chunk<T>(at, c < 0 ? 0 : left < G::N::EPL ? left : G::N::EPL, p.vec_kv);
       }
    };
    constexpr int64_t kStride = 4 * kTile;
@@ -454,9 +474,13 @@ __global__ __launch_bounds__(256, (sizeof(typename Num<T>::E) * DC * MAPS >= 512
       constexpr bool CAREFUL = decltype(careful)::value;
       r.clear();
       int64_t at = begin + lo + wave * kTile;
-      int32_t slot = tile_slot(p, at, end, lane);
-      int32_t next = tile_slot(p, at + kStride, end, lane);
-      if (at < end) load(slot);
+      int32_t slot = -1, next = -1;
+      if (at < end)
+      {
+         slot = tile_slot(p, at, end, lane);
+         next = tile_slot(p, at + kStride, end, lane);
+         load(slot);
+      }
       for (; at < end; at += kStride)
       {
          bool all;
@@ -568,7 +592,8 @@ template <bool FULL, int WORDS, int N> __device__ inline void load_scales(uint32
    for (int j = 0; j < N; j++)
    {
       const int f = code_feature<FULL, WORDS>(FULL ? 4 * j : j, g);
-      to[j] = f < width ? *reinterpret_cast<const uint16_t *>(from + f / 32 * 2) : 0;
+      if constexpr (FULL) to[j] = *reinterpret_cast<const uint16_t *>(from + f / 32 * 2);
+      else to[j] = f < width ? *reinterpret_cast<const uint16_t *>(from + f / 32 * 2) : 0;
    }
 }
 
@@ -579,7 +604,7 @@ template <int DC, int MAPS, bool FULL> struct Record4 {
 };
 
 template <int DC, int MAPS, bool FULL>
-__global__ __launch_bounds__(256, (DC * MAPS >= 256 ? 1 : 2)) void attn_rows_kv4(RowsParams p)
+__global__ __launch_bounds__(256, (DC * MAPS >= 256 ? 1 : DC * MAPS == 128 && FULL ? 3 : 2)) void attn_rows_kv4(RowsParams p)
 {
    typedef RowGeo<kF16, DC, MAPS> G;
    constexpr int WQ = DC / 32, WV = G::W / 32;   // 4-byte words of codes that a lane reads of one map's key, of a value row
@@ -637,7 +662,7 @@ __global__ __launch_bounds__(256, (DC * MAPS >= 256 ? 1 : 2)) void attn_rows_kv4
 #pragma unroll
       for (int a = 0; a < 2; a++)
       {
-         // a place without a slot reads record 0, which is masked
+         // (a place without a slot reads record 0: see attn_rows)
          const int32_t c = __shfl(slot, 16 * a + i);
          const uint8_t *rec = cache + (int64_t)(c < 0 ? 0 : c) * p.ldc;
 #pragma unroll
@@ -648,7 +673,7 @@ __global__ __launch_bounds__(256, (DC * MAPS >= 256 ? 1 : 2)) void attn_rows_kv4
          }
          load_codes<FULL>(to[a].vc, rec + off_v, p.dv, g);
          load_scales<FULL, WV>(to[a].vs, rec + off_vw, p.dv, g);
-         if (c < 0)
+         if (!FULL && c < 0)
          {
 #pragma unroll
             for (int j = 0; j < Words4<FULL, WV>::N; j++) to[a].vs[j] = 0;   // values of zero, whatever the record holds
@@ -661,7 +686,6 @@ __global__ __launch_bounds__(256, (DC * MAPS >= 256 ? 1 : 2)) void attn_rows_kv4
       constexpr bool CAREFUL = decltype(careful)::value;
       r.clear();
       int64_t at = begin + lo + wave * kTile;
-      int32_t slot = tile_slot(p, at, end, lane), next = tile_slot(p, at + kStride, end, lane);
       auto use = [&](const Rec (&rec)[2], int32_t slot) __attribute__((always_inline)) {
          bool all;
          const unsigned mine = tile_bits(slot, g, &all);
@@ -692,16 +716,23 @@ __global__ __launch_bounds__(256, (DC * MAPS >= 256 ? 1 : 2)) void attn_rows_kv4
       };
       // two tiles in turn, so that one is under way while the other is used
       Rec even[2], odd[2];
-      if (at < end) load(even, slot);
+      int32_t slot = -1, next = -1;
+      auto slot_of = [&](int64_t at) __attribute__((always_inline)) { return FULL ? tile_slot(p, at, end, lane) : tile_slot_any(p, at, end, lane); };
+      if (at < end)
+      {
+         slot = slot_of(at);
+         next = slot_of(at + kStride);
+         load(even, slot);
+      }
       while (at < end)
       {
-         const int32_t after = tile_slot(p, at + 2 * kStride, end, lane);
-         if (at + kStride < end) load(odd, next);
+         const int32_t after = slot_of(at + 2 * kStride);
+         if (FULL || at + kStride < end) load(odd, next);   // (behind the end: slot 0, not used)
          use(even, slot);
          at += kStride;
          if (at >= end) break;
-         slot = tile_slot(p, at + 2 * kStride, end, lane);
-         if (at + kStride < end) load(even, after);
+         slot = slot_of(at + 2 * kStride);
+         if (FULL || at + kStride < end) load(even, after);
          use(odd, next);
          at += kStride;
          next = slot;
@@ -715,21 +746,26 @@ __global__ __launch_bounds__(256, (DC * MAPS >= 256 ? 1 : 2)) void attn_rows_kv4
 }
 
 // ---- into the 4-bit cache and back ---------------------------------------------------------------------------------------------------
-// Eight values per lane, four lanes per group of 32.  The step between codes is the group's range (with zero in it) over
-// 15, rounded up to 7 significant bits and to a multiple of 2^-20; code and zero point are rounded to nearest, ties to
-// even.  The borders between codes are decided in 64 bits for 32-bit values; for 16-bit values the quotient in 32 bits,
-// correctly rounded, decides them alike: x has 11 significant bits and a border 12, so a quotient that is not a border is
-// further from it than 2^-24 of its size.
-template <int T> __device__ inline float code_of(float x, float s)
+// The step between codes is the group's range (with zero in it) over 15, rounded up to 7 significant bits and to a multiple
+// of 2^-20; code and zero point are rounded to nearest, ties to even.  The borders between codes are decided by the
+// correctly rounded quotient x / s, in 64 bits for 32-bit values.  For 16-bit values 32 bits decide alike: x has 11
+// significant bits and a border 12, so a quotient that is not a border is further from it than 2^-24 of its size; and
+// with the correctly rounded 1 / s, q + (x - q s) / s is the correctly rounded quotient (Markstein, 1990).
+template <int T> __device__ inline float code_of(float x, float s, float inv)
 {
    if constexpr (T == kF32) return (float)rint((double)x / (double)s);
-   else return rintf(x / s);
+   else
+   {
+      const float q = x * inv;
+      return rintf(fmaf(fmaf(-q, s, x), inv, q));
+   }
 }
 
+// A lane per group of 32 values: the 64-bit arithmetic of the step, once per group, then costs less than the codes.
 template <int T> __global__ __launch_bounds__(256) void kv4_write(Kv4Params p)
 {
    typedef typename Num<T>::E E;
-   constexpr int kMost = 32;
+   constexpr int kMost = 32, EPL = Num<T>::EPL;
    __shared__ int64_t slot[kMost];
    __shared__ int later[kMost];
    const int tid = threadIdx.x;
@@ -749,73 +785,57 @@ template <int T> __global__ __launch_bounds__(256) void kv4_write(Kv4Params p)
          if (slot[x] == c && t0 + x < t) later[x] = 1;
    }
    __syncthreads();
-   const int words = (p.k_width + p.v_width) / 8, per_token = words * p.kv_heads;   // a multiple of 4: groups do not cross items
+   const int groups = (p.k_width + p.v_width) / 32, per_token = groups * p.kv_heads;
    for (int x = tid; x < here * per_token; x += 256)
    {
-      const int tok = x / per_token, head = x % per_token / words, w = x % words;
+      const int tok = x / per_token, head = x % per_token / groups, grp = x % groups;
       const int64_t c = slot[tok];
-      const bool is_v = 8 * w >= p.k_width;
-      const int f = is_v ? 8 * w - p.k_width : 8 * w;
+      if (c < 0 || c >= p.n || later[tok]) continue;
+      const bool is_v = 32 * grp >= p.k_width;
+      const int f = is_v ? 32 * grp - p.k_width : 32 * grp;
       const E *from = is_v ? (const E *)p.v + (t0 + tok) * p.ldv + head * p.hdv + f : (const E *)p.k + (t0 + tok) * p.ldk + head * p.hdk + f;
-      float v[8];
-      if constexpr (T == kF32)
-      {
-         const u4 a = load_chunk<T>(from, 4, p.vec), b = load_chunk<T>(from + 4, 4, p.vec);
+      float v[32];
 #pragma unroll
-         for (int e = 0; e < 4; e++)
+      for (int j = 0; j < 32 / EPL; j++)
+      {
+         const u4 a = load_chunk<T>(from + j * EPL, EPL, p.vec);
+#pragma unroll
+         for (int e = 0; e < EPL; e++)
          {
-            v[e] = __uint_as_float(a[e]);
-            v[4 + e] = __uint_as_float(b[e]);
+            if constexpr (T == kF32) v[4 * j + e] = __uint_as_float(a[e]);
+            else v[8 * j + e] = Num<T>::to((E)(a[e / 2] >> (16 * (e & 1))));
          }
       }
-      else
-      {
-         const u4 a = load_chunk<T>(from, 8, p.vec);
-#pragma unroll
-         for (int e = 0; e < 8; e++) v[e] = Num<T>::to((E)(a[e / 2] >> (16 * (e & 1))));
-      }
       float lo = 0, hi = 0;
-      bool nan = false;
+      bool nan = false;   // makes its whole group NaN
 #pragma unroll
-      for (int e = 0; e < 8; e++)
+      for (int e = 0; e < 32; e++)
       {
          nan |= v[e] != v[e];
-         v[e] = fminf(fmaxf(v[e], -32768.0f), 32768.0f);   // what a step of fp16 reaches; a NaN makes its whole group NaN
+         v[e] = fminf(fmaxf(v[e], -32768.0f), 32768.0f);   // what a step of fp16 reaches
          lo = fminf(lo, v[e]);
          hi = fmaxf(hi, v[e]);
-      }
-      int any = nan;
-#pragma unroll
-      for (int k = 1; k < 4; k <<= 1)
-      {
-         lo = fminf(lo, __shfl_xor(lo, k));
-         hi = fmaxf(hi, __shfl_xor(hi, k));
-         any |= __shfl_xor(any, k);
       }
       const double step = ((double)hi - (double)lo) / 15.0;
       int e2;
       (void)frexp(step, &e2);   // step in [2^(e2 - 1), 2^e2)
       const int unit = step == 0 || e2 - 7 < -20 ? -20 : e2 - 7;
       const float s = (float)ldexp(ceil(ldexp(step, -unit)), unit);
-      const float z = s > 0 ? (float)rint(-(double)lo / (double)s) : 0.0f;
-      uint32_t codes = 0;
-      if (s > 0 && !any)
+      const float z = s > 0 ? (float)rint(-(double)lo / (double)s) : 0.0f, inv = s > 0 ? 1.0f / s : 0.0f;
+      u4 codes = {0, 0, 0, 0};
+      if (s > 0 && !nan)
       {
 #pragma unroll
-         for (int e = 0; e < 8; e++)
+         for (int e = 0; e < 32; e++)
          {
-            const float q = fminf(fmaxf(code_of<T>(v[e], s) + z, 0.0f), 15.0f);
-            codes |= (uint32_t)q << (4 * ((e % 2) * 4 + e / 2));
+            const float q = fminf(fmaxf(code_of<T>(v[e], s, inv) + z, 0.0f), 15.0f);
+            codes[e / 8] |= (uint32_t)q << (4 * ((e % 2) * 4 + e % 8 / 2));
          }
       }
-      if (c < 0 || c >= p.n || later[tok]) continue;
       uint8_t *rec = p.cache + c * p.ldc + head * p.hdc;
-      *reinterpret_cast<uint32_t *>(rec + 4 * w) = codes;
-      if (w % 4 == 0)
-      {
-         const uint32_t word = any ? 0x7E00u : (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)s) | (uint32_t)z;
-         *reinterpret_cast<uint16_t *>(rec + 4 * words + w / 4 * 2) = (uint16_t)word;
-      }
+      *reinterpret_cast<u4 *>(rec + 16 * grp) = codes;
+      const uint32_t word = nan ? 0x7E00u : (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)s) | (uint32_t)z;
+      *reinterpret_cast<uint16_t *>(rec + 16 * groups + 2 * grp) = (uint16_t)word;
    }
 }
 

@@ -380,7 +380,8 @@ int fusedMM_kv4_write(const fusedMM_attn_desc *desc, const INDEXTYPE tokens, con
 /* The values of the records of slots[0 .. tokens) in desc->type; slots outside [0, desc->n) read as zeros. */
 int fusedMM_kv4_read(const fusedMM_attn_desc *desc, const INDEXTYPE tokens, const INDEXTYPE *slots, const void *cache, int64_t ldc,
                      int64_t hdc, void *k, void *v, void *stream);
-/* fusedMM_attn_rows over such a cache; desc->type (of q and o) is fp16 or bf16.  Products run on fp16 operands: the
+/* fusedMM_attn_rows over such a cache; desc->type (of q and o) is fp16 or bf16.  d and dv are any multiples of 32 up
+ * to 128 (d to 64 with two maps), or d = dv = 256 (d = 128, dv = 256 with two maps).  Products run on fp16 operands: the
  * cache's values are exact in it, each head's query is scaled by a power of two into its range. */
 int fusedMM_attn_rows_kv4(const fusedMM_attn_desc *desc, const INDEXTYPE nnz, const INDEXTYPE *indx, const INDEXTYPE *pntrb,
                           const INDEXTYPE *pntre, const void *q, const void *cache, int64_t ldc, int64_t hdc, const float *lambda,

@@ -110,6 +110,8 @@ def test_the_cache_refuses_what_does_not_fit(capfd):
     assert write(desc(), tokens=(1 << 20) + 1) == fa.FAIL and "2^20" in capfd.readouterr().err
     assert read(desc(ldk=64)) == fa.FAIL and "overlap" in capfd.readouterr().err
     assert rows4(desc(type=fa.TYPE_F32)) == fa.NO_OPT_IMPL
+    for sizes in (dict(maps=2, d=96, dv=160, heads=4, kv_heads=4), dict(d=160, dv=160), dict(d=256, dv=128), dict(d=32, dv=160), dict(maps=2, d=32, dv=256)):
+        assert rows4(desc(ldq=1024, hdq=256, ldo=1024, hdo=256, **sizes), ldc=2048, hdc=512, lam=16) == fa.NO_OPT_IMPL
 
 
 def test_record_bytes():
