@@ -311,6 +311,7 @@ int kv4_common(const char *who, const Desc *d, int64_t tokens, const void *slots
    if (!write && (!apart(d->ldk, d->hdk, tokens, d->kv_heads, (int64_t)d->maps * d->d) || !apart(d->ldv, d->hdv, tokens, d->kv_heads, d->dv)))
       return refuse(who, "the rows of k or v overlap");
    const int64_t words = ((int64_t)d->maps * d->d + d->dv) / 8;
+   if (d->n > INT32_MAX) return refuse(who, "n is at most 2^31 - 1");
    if (words * d->kv_heads > INT32_MAX / 32) return refuse(who, "too many key heads");
    if (tokens == 0) return kOk;
    if (!slots || !k || !v || !cache) return refuse(who, "a pointer is null");
@@ -334,8 +335,8 @@ int kv4_common(const char *who, const Desc *d, int64_t tokens, const void *slots
    p->vec = lines_up(k, d->ldk, d->hdk, bytes) && lines_up(v, d->ldv, d->hdv, bytes);
    p->ldc = ldc;
    p->hdc = hdc;
-   // Tokens of a workgroup: it compares its slots with all later ones, so many tokens share that walk.
-   p->per_group = (int)std::min<int64_t>(32, std::max<int64_t>(1, tokens / 2048));
+   // Tokens of a workgroup: it walks over all later slots, so tokens share that walk as soon as there are enough of them.
+   p->per_group = (int)std::min<int64_t>(kKv4Tokens, std::max<int64_t>(1, tokens / 2048));
    return kOk;
 }
 
@@ -481,16 +482,17 @@ int fusedMM_attn_backward(const fusedMM_attn_desc *desc, const void *plan, const
    p.dk = dk;
    p.dvv = dv;
    p.dlambda = d.maps == 2 ? dlambda : nullptr;
+   p.dlam_count = d.m ? (int64_t)pp.view.n_units * (pp.view.block_rows / 16) : 0;
    p.stats = (float *)((unsigned char *)work + l.stats);
    p.dlam_units = (float *)((unsigned char *)work + l.dlam);
    p.part = (float *)((unsigned char *)work + l.part);
    const hipStream_t s = (hipStream_t)stream;
-   if (d.m > 0 || p.dlambda)
+   if (d.m > 0)
    {
       st = d.type == FUSEDMM_TYPE_F32 ? launch_dq_f32(p, dc, d.maps, s) : d.type == FUSEDMM_TYPE_F16 ? launch_dq_f16(p, dc, d.maps, s) : launch_dq_bf16(p, dc, d.maps, s);
       if (st) return st;
    }
-   if (d.n == 0) return kOk;
+   if (d.n == 0 && !p.dlambda) return kOk;
    p.plan = pt.view;
    return d.type == FUSEDMM_TYPE_F32 ? launch_dkv_f32(p, dc, d.maps, s) : d.type == FUSEDMM_TYPE_F16 ? launch_dkv_f16(p, dc, d.maps, s) : launch_dkv_bf16(p, dc, d.maps, s);
 }

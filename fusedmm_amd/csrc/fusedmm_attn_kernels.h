@@ -54,6 +54,7 @@ struct Params {
    float *dlambda;
    float *stats;                      // [m][heads][2 maps]: lse * log2(e) of every map, delta of every map
    float *dlam_units;                 // [unit][wave][heads]: sum over a wave's rows of sum_j P_2 dP
+   int64_t dlam_count;                // units * waves
    float *part;                       // partial sums of split blocks
 };
 
@@ -738,18 +739,16 @@ template <int T, int DC, int MAPS> __global__ __launch_bounds__(256) void attn_d
    if (e < p.d) ((E *)p.dq)[row * p.ldq + head * p.hdq + mp * p.d + e] = (E)Num<T>::from(s * ((mp == 0 ? 1.0f : -p.lambda[head]) * p.scale));
 }
 
-// dlambda_h = - sum of dlam_units: one workgroup per head, in 64 bits, every thread's units and then the threads in order
-template <int T> __global__ __launch_bounds__(256) void attn_dlambda(Params p)
+// dlambda_h = - sum of dlam_units, in 64 bits: every thread's entries and then the threads in order.  The last `heads`
+// workgroups of the dk, dv launch do it: its input is there, and a launch of its own would take longer than the sum.
+template <int THREADS> __device__ inline void dlambda_of(const Params &p, int head, double *s)
 {
-   __shared__ double s[256];
-   const int head = blockIdx.x;
-   const int64_t n = p.m ? (int64_t)p.plan.n_units * (p.plan.block_rows / 16) : 0;
    double x = 0;
 #pragma unroll 4
-   for (int64_t u = threadIdx.x; u < n; u += 256) x += (double)p.dlam_units[u * p.heads + head];
+   for (int64_t u = threadIdx.x; u < p.dlam_count; u += THREADS) x += (double)p.dlam_units[u * p.heads + head];
    s[threadIdx.x] = x;
    __syncthreads();
-   for (int k = 128; k; k >>= 1)
+   for (int k = THREADS / 2; k; k >>= 1)
    {
       if ((int)threadIdx.x < k) s[threadIdx.x] += s[threadIdx.x + k];
       __syncthreads();
@@ -764,6 +763,12 @@ template <int T, int DC, int MAPS, int BR> __global__ __launch_bounds__(BR * 4, 
    typedef Geo<T, DC, MAPS, BR> G;
    typedef typename G::E E;
    ATTN_LDS(G::kStat)
+   const int64_t work_groups = ((int64_t)p.plan.n_units * p.kv_heads + 7) / 8 * 8;
+   if (MAPS == 2 && blockIdx.x >= work_groups)
+   {
+      dlambda_of<G::THREADS>(p, (int)(blockIdx.x - work_groups), (double *)lds);
+      return;
+   }
    const int64_t item = xcd_item(blockIdx.x, (int64_t)p.plan.n_units * p.kv_heads);
    if (item >= (int64_t)p.plan.n_units * p.kv_heads) return;
    const int kvh = (int)(item / p.plan.n_units);

@@ -50,7 +50,7 @@ template <int DC, int MAPS> struct Forward {
    {
       const int64_t n = (int64_t)p.plan.n_units * p.heads;
       if (p.plan.block_rows == 64) hipLaunchKernelGGL((attn_forward<TYPE, DC, MAPS, 64>), dim3(eighths(n)), dim3(256), 0, s, p);
-         else hipLaunchKernelGGL((attn_forward<TYPE, DC, MAPS, 16>), dim3(eighths(n)), dim3(64), 0, s, p);
+      else hipLaunchKernelGGL((attn_forward<TYPE, DC, MAPS, 16>), dim3(eighths(n)), dim3(64), 0, s, p);
       ATTN_HIP(hipGetLastError());
       if (p.plan.n_joins)
       {
@@ -64,21 +64,13 @@ template <int DC, int MAPS> struct Forward {
 template <int DC, int MAPS> struct Dq {
    int operator()(const Params &p, hipStream_t s)
    {
-      if (p.m)
+      const int64_t n = (int64_t)p.plan.n_units * p.heads;
+      if (p.plan.block_rows == 64) hipLaunchKernelGGL((attn_dq<TYPE, DC, MAPS, 64>), dim3(eighths(n)), dim3(256), 0, s, p);
+      else hipLaunchKernelGGL((attn_dq<TYPE, DC, MAPS, 16>), dim3(eighths(n)), dim3(64), 0, s, p);
+      ATTN_HIP(hipGetLastError());
+      if (p.plan.n_joins)
       {
-         const int64_t n = (int64_t)p.plan.n_units * p.heads;
-         if (p.plan.block_rows == 64) hipLaunchKernelGGL((attn_dq<TYPE, DC, MAPS, 64>), dim3(eighths(n)), dim3(256), 0, s, p);
-         else hipLaunchKernelGGL((attn_dq<TYPE, DC, MAPS, 16>), dim3(eighths(n)), dim3(64), 0, s, p);
-         ATTN_HIP(hipGetLastError());
-         if (p.plan.n_joins)
-         {
-            hipLaunchKernelGGL((attn_dq_join<TYPE, DC, MAPS>), dim3((unsigned)((int64_t)p.plan.n_joins * p.heads * p.plan.block_rows / 4 * ((DC * MAPS + 63) / 64))), dim3(256), 0, s, p);
-            ATTN_HIP(hipGetLastError());
-         }
-      }
-      if (MAPS == 2 && p.dlambda)
-      {
-         hipLaunchKernelGGL((attn_dlambda<TYPE>), dim3((unsigned)p.heads), dim3(256), 0, s, p);
+         hipLaunchKernelGGL((attn_dq_join<TYPE, DC, MAPS>), dim3((unsigned)((int64_t)p.plan.n_joins * p.heads * p.plan.block_rows / 4 * ((DC * MAPS + 63) / 64))), dim3(256), 0, s, p);
          ATTN_HIP(hipGetLastError());
       }
       return kOk;
@@ -89,8 +81,9 @@ template <int DC, int MAPS> struct Dkv {
    int operator()(const Params &p, hipStream_t s)
    {
       const int64_t n = (int64_t)p.plan.n_units * p.kv_heads;
-      if (p.plan.block_rows == 64) hipLaunchKernelGGL((attn_dkv<TYPE, DC, MAPS, 64>), dim3(eighths(n)), dim3(256), 0, s, p);
-         else hipLaunchKernelGGL((attn_dkv<TYPE, DC, MAPS, 16>), dim3(eighths(n)), dim3(64), 0, s, p);
+      const dim3 grid(eighths(n) + (p.dlambda ? (unsigned)p.heads : 0u));
+      if (p.plan.block_rows == 64) hipLaunchKernelGGL((attn_dkv<TYPE, DC, MAPS, 64>), grid, dim3(256), 0, s, p);
+      else hipLaunchKernelGGL((attn_dkv<TYPE, DC, MAPS, 16>), grid, dim3(64), 0, s, p);
       ATTN_HIP(hipGetLastError());
       if (p.plan.n_joins)
       {

@@ -761,36 +761,50 @@ template <int T> __device__ inline float code_of(float x, float s, float inv)
    }
 }
 
+constexpr int kKv4Tokens = 8;   // most tokens of a workgroup: it compares their slots, in registers, with all later ones
+
 // A lane per group of 32 values: the 64-bit arithmetic of the step, once per group, then costs less than the codes.
 template <int T> __global__ __launch_bounds__(256) void kv4_write(Kv4Params p)
 {
    typedef typename Num<T>::E E;
-   constexpr int kMost = 32, EPL = Num<T>::EPL;
-   __shared__ int64_t slot[kMost];
-   __shared__ int later[kMost];
+   constexpr int EPL = Num<T>::EPL;
+   __shared__ int32_t slot[kKv4Tokens];
+   __shared__ int later[kKv4Tokens];
    const int tid = threadIdx.x;
    const int64_t t0 = (int64_t)blockIdx.x * p.per_group;
    const int here = (int)(p.tokens - t0 < p.per_group ? p.tokens - t0 : p.per_group);
-   if (tid < kMost)
+   auto slot_at = [&](int64_t t) {   // -1: the token goes nowhere
+      const int64_t c = index_of(p.slots, t, p.index_bytes);
+      return c >= 0 && c < p.n ? (int32_t)c : -1;
+   };
+   if (tid < kKv4Tokens)
    {
       later[tid] = 0;
-      slot[tid] = tid < here ? index_of(p.slots, t0 + tid, p.index_bytes) : -1;
+      slot[tid] = tid < here ? slot_at(t0 + tid) : -1;
    }
    __syncthreads();
    // a slot that is named more than once takes the last token that names it
+   int32_t mine[kKv4Tokens];
+#pragma unroll
+   for (int x = 0; x < kKv4Tokens; x++) mine[x] = slot[x];
+   unsigned dup = 0;
+#pragma unroll 4
    for (int64_t t = t0 + 1 + tid; t < p.tokens; t += 256)
    {
-      const int64_t c = index_of(p.slots, t, p.index_bytes);
-      for (int x = 0; x < here; x++)
-         if (slot[x] == c && t0 + x < t) later[x] = 1;
+      const int32_t c = slot_at(t);
+#pragma unroll
+      for (int x = 0; x < kKv4Tokens; x++) dup |= (unsigned)(mine[x] == c && t0 + x < t) << x;
    }
+#pragma unroll
+   for (int x = 0; x < kKv4Tokens; x++)
+      if (__any((dup >> x) & 1) && (tid & 63) == 0) later[x] = 1;
    __syncthreads();
    const int groups = (p.k_width + p.v_width) / 32, per_token = groups * p.kv_heads;
    for (int x = tid; x < here * per_token; x += 256)
    {
       const int tok = x / per_token, head = x % per_token / groups, grp = x % groups;
       const int64_t c = slot[tok];
-      if (c < 0 || c >= p.n || later[tok]) continue;
+      if (c < 0 || later[tok]) continue;
       const bool is_v = 32 * grp >= p.k_width;
       const int f = is_v ? 32 * grp - p.k_width : 32 * grp;
       const E *from = is_v ? (const E *)p.v + (t0 + tok) * p.ldv + head * p.hdv + f : (const E *)p.k + (t0 + tok) * p.ldk + head * p.hdk + f;
