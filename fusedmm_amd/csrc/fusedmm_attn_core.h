@@ -103,31 +103,28 @@ template <> struct Num<kF32> {
 };
 
 // EPL elements at p, of which the first `valid` exist (the rest read as zero).  vec: p is 16-byte aligned and valid is
-// 0 or EPL.
+// 0 or EPL.  A whole chunk at any other place is one load as well: the hardware takes global addresses as they come.
 template <int T> __device__ inline u4 load_chunk(const typename Num<T>::E *p, int valid, bool vec)
 {
    typedef typename Num<T>::E E;
+   typedef u4 u4_anywhere __attribute__((aligned(2)));
    u4 r = {0, 0, 0, 0};
    if (valid <= 0) return r;
    if (vec) return *reinterpret_cast<const u4 *>(p);
+   if (valid >= Num<T>::EPL) return *reinterpret_cast<const u4_anywhere *>(p);
    if constexpr (sizeof(E) == 2)
    {
 #pragma unroll
-      for (int k = 0; k < 8; k++)
+      for (int k = 0; k < 7; k++)
          if (k < valid) r[k / 2] |= (uint32_t)p[k] << (16 * (k & 1));
    }
    else
    {
 #pragma unroll
-      for (int k = 0; k < 4; k++)
+      for (int k = 0; k < 3; k++)
          if (k < valid) r[k] = __float_as_uint(p[k]);
    }
    return r;
-}
-
-template <int T> __device__ inline bool odd_chunk(u4 v)
-{
-   return Num<T>::odd_word(v[0]) || Num<T>::odd_word(v[1]) || Num<T>::odd_word(v[2]) || Num<T>::odd_word(v[3]);
 }
 
 // scores of 32 gathered rows for one resident row, in the layout of the second product
@@ -141,6 +138,15 @@ template <int T> __device__ inline typename Num<T>::TFrag pack_scores(const floa
       else r[j] = (short)Num<T>::from(p[j / 4][j % 4]);
    }
    return r;
+}
+
+// what rounding took from them, rounded in turn
+template <int T> __device__ inline typename Num<T>::TFrag pack_rest(const float (&p)[2][4], typename Num<T>::TFrag b)
+{
+   float r[2][4];
+#pragma unroll
+   for (int j = 0; j < 8; j++) r[j / 4][j % 4] = T == kF32 ? 0.0f : p[j / 4][j % 4] - Num<T>::to((typename Num<T>::E)b[j]);
+   return pack_scores<T>(r);
 }
 
 // A tile in LDS: 32 rows of W elements.  A row's 16-byte chunks are stored in an order that depends on the row (chunk ^
@@ -265,18 +271,24 @@ __device__ inline void add_odd(f4 (&acc)[NT], const float (&p)[2][4], unsigned m
    }
 }
 
-// acc += (weights of the tile's 32 rows) x (their features f0 .. f0 + 16 NT - 1); CAREFUL: the tile may hold infinities or NaN
-template <int T, int W, bool CAREFUL, int NT>
+// acc += (weights of the tile's 32 rows) x (their features f0 .. f0 + 16 NT - 1); CAREFUL: the tile may hold infinities or
+// NaN; TWICE: 16-bit weights enter as a rounded value and its rounded rest.  One rounding of the weights errs by as much
+// as the rounding of the output does; with the rest, outputs are as exact as their own rounding.
+template <int T, int W, bool CAREFUL, bool TWICE = false, int NT>
 __device__ inline void add_weighted(f4 (&acc)[NT], const float (&p)[2][4], unsigned mine, const unsigned char *tile, int f0, int g, int i, const typename TileView<T, W>::Lane &l)
 {
    typedef TileView<T, W> V;
    const typename Num<T>::TFrag b = pack_scores<T>(p);
+   typename Num<T>::TFrag low;
+   if constexpr (TWICE) low = pack_rest<T>(p, b);
    if constexpr (CAREFUL)
    {
 #pragma unroll
       for (int t = 0; t < NT; t++)
       {
-         acc[t] = Num<T>::mma_t(without_odd<T>(V::transposed(tile, f0 / 16 + t, l)), b, acc[t]);
+         const typename Num<T>::TFrag v = without_odd<T>(V::transposed(tile, f0 / 16 + t, l));
+         acc[t] = Num<T>::mma_t(v, b, acc[t]);
+         if constexpr (TWICE) acc[t] = Num<T>::mma_t(v, low, acc[t]);
          keep_order();
       }
       add_odd<T, W, NT>(acc, p, mine, tile, f0, g, i);
@@ -284,7 +296,12 @@ __device__ inline void add_weighted(f4 (&acc)[NT], const float (&p)[2][4], unsig
    else
    {
 #pragma unroll
-      for (int t = 0; t < NT; t++) acc[t] = Num<T>::mma_t(V::transposed(tile, f0 / 16 + t, l), b, acc[t]);
+      for (int t = 0; t < NT; t++)
+      {
+         const typename Num<T>::TFrag v = V::transposed(tile, f0 / 16 + t, l);
+         acc[t] = Num<T>::mma_t(v, b, acc[t]);
+         if constexpr (TWICE) acc[t] = Num<T>::mma_t(v, low, acc[t]);
+      }
    }
 }
 

@@ -220,22 +220,40 @@ template <class G, int T, int DC, int BR> struct Stream {
 #pragma unroll
       for (int j = 0; j < G::NCH; j++)
       {
+         if (!vec) break;
          const int x = me + G::THREADS * j, r = x / G::CR;
          if (kTile * G::CR < G::THREADS && x >= kTile * G::CR) break;
          const uint32_t col = (uint32_t)c[r];
          const int e = ((x % G::CR) ^ V::twist(r)) * G::N::EPL, f = e % DC;   // this thread's chunk of a gathered row
          const E *fa = (const E *)(a + oa + (uint64_t)col * lda) + (e / DC * d + f);
          const E *fb = (const E *)(b + ob + (uint64_t)col * ldb) + e;
-         if (vec)
+         load_lds16(la + j * (G::THREADS * 16), f < d ? (const void *)fa : (const void *)&zero_chunk);
+         load_lds16(lb + j * (G::THREADS * 16), e < dv ? (const void *)fb : (const void *)&zero_chunk);
+      }
+      if (vec) return;
+      // rows at any place, ends of rows within a chunk: through registers, a few chunks at a time
+      constexpr int B = G::NCH < 4 ? G::NCH : 4;
+#pragma unroll
+      for (int j0 = 0; j0 < G::NCH; j0 += B)
+      {
+         u4 ra[B], rb[B];
+#pragma unroll
+         for (int j = 0; j < B; j++)
          {
-            load_lds16(la + j * (G::THREADS * 16), f < d ? (const void *)fa : (const void *)&zero_chunk);
-            load_lds16(lb + j * (G::THREADS * 16), e < dv ? (const void *)fb : (const void *)&zero_chunk);
+            const int x = me + G::THREADS * (j0 + j), r = x / G::CR;
+            const bool live = kTile * G::CR >= G::THREADS || x < kTile * G::CR;
+            const uint32_t col = (uint32_t)c[live ? r : 0];
+            const int e = ((x % G::CR) ^ V::twist(r)) * G::N::EPL, f = e % DC;
+            ra[j] = load_chunk<T>((const E *)(a + oa + (uint64_t)col * lda) + (e / DC * d + f), !live ? 0 : d - f < G::N::EPL ? d - f : G::N::EPL, false);
+            rb[j] = load_chunk<T>((const E *)(b + ob + (uint64_t)col * ldb) + e, !live ? 0 : dv - e < G::N::EPL ? dv - e : G::N::EPL, false);
          }
-         else
+#pragma unroll
+         for (int j = 0; j < B; j++)
          {
-            // rows at any place, ends of rows within a chunk: element by element through registers
-            *(u4 *)(ta + x * 16) = load_chunk<T>(fa, d - f < G::N::EPL ? d - f : G::N::EPL, false);
-            *(u4 *)(tb + x * 16) = load_chunk<T>(fb, dv - e < G::N::EPL ? dv - e : G::N::EPL, false);
+            const int x = me + G::THREADS * (j0 + j);
+            if (kTile * G::CR < G::THREADS && x >= kTile * G::CR) break;
+            *(u4 *)(ta + x * 16) = ra[j];
+            *(u4 *)(tb + x * 16) = rb[j];
          }
       }
    }
@@ -400,18 +418,26 @@ template <int T, int DC, int MAPS, int BR> __global__ __launch_bounds__(BR * 4, 
             if constexpr (CAREFUL)
             {
 #pragma unroll
-               for (int mp = 0; mp < MAPS; mp++) add_weighted<T, G::W, true>(soft[mp].acc, w[mp], mine, vs, 0, g, i, l);
+               for (int mp = 0; mp < MAPS; mp++) add_weighted<T, G::W, true, T != kF32>(soft[mp].acc, w[mp], mine, vs, 0, g, i, l);
                return;
             }
-            typename G::N::TFrag wf[MAPS];
+            typename G::N::TFrag wf[MAPS], wr[MAPS];   // the weights, and (16-bit) what rounding took from them
 #pragma unroll
-            for (int mp = 0; mp < MAPS; mp++) wf[mp] = pack_scores<T>(w[mp]);
+            for (int mp = 0; mp < MAPS; mp++)
+            {
+               wf[mp] = pack_scores<T>(w[mp]);
+               if constexpr (T != kF32) wr[mp] = pack_rest<T>(w[mp], wf[mp]);
+            }
 #pragma unroll
             for (int x = 0; x < G::NT; x++)
             {
                const typename G::N::TFrag vt = G::V::transposed(vs, x, l);
 #pragma unroll
-               for (int mp = 0; mp < MAPS; mp++) soft[mp].acc[x] = G::N::mma_t(vt, wf[mp], soft[mp].acc[x]);
+               for (int mp = 0; mp < MAPS; mp++)
+               {
+                  soft[mp].acc[x] = G::N::mma_t(vt, wf[mp], soft[mp].acc[x]);
+                  if constexpr (T != kF32) soft[mp].acc[x] = G::N::mma_t(vt, wr[mp], soft[mp].acc[x]);
+               }
             }
          });
       bool odd = odd_sums(soft[0].acc);

@@ -224,7 +224,7 @@ __device__ inline void wave_lds_order()   // this wave's LDS writes before its l
 }
 
 // products of 32 slots with the columns -> weights, and the weighted values
-template <class G, int T, bool CAREFUL>
+template <class G, int T, bool CAREFUL, bool TWICE>
 __device__ inline void row_step(Softmax<G::NT> &r, f4 (&sc)[2], float c2, unsigned mine, bool all, const unsigned char *vs, int g, int i)
 {
    if (!all)
@@ -235,7 +235,7 @@ __device__ inline void row_step(Softmax<G::NT> &r, f4 (&sc)[2], float c2, unsign
    }
    float w[2][4];
    r.weights(w, sc, c2);
-   add_weighted<T, G::W, CAREFUL>(r.acc, w, mine, vs, 0, g, i, G::V::lane(g, i));
+   add_weighted<T, G::W, CAREFUL, TWICE>(r.acc, w, mine, vs, 0, g, i, G::V::lane(g, i));
 }
 
 // The four waves' sums -> the row's output, or its piece of the partial sums.  O: element type of the output.
@@ -513,7 +513,7 @@ __global__ __launch_bounds__(256, (sizeof(typename Num<T>::E) * DC * MAPS >= 512
             sc[0][1] = mp_i ? sc[1][1] : sc[0][1];
          }
          wave_lds_order();
-         row_step<G, T, CAREFUL>(r, sc[0], c2, mine, all, vs, g, i);
+         row_step<G, T, CAREFUL, T != kF32>(r, sc[0], c2, mine, all, vs, g, i);
          wave_lds_order();
       }
       return odd_sums(r.acc);
@@ -711,7 +711,7 @@ __global__ __launch_bounds__(256, (DC * MAPS >= 256 ? 1 : DC * MAPS == 128 && FU
             sc[0][1] = mp_i ? sc[1][1] : sc[0][1];
          }
          wave_lds_order();
-         row_step<G, kF16, CAREFUL>(r, sc[0], c2, mine, all, vs, g, i);
+         row_step<G, kF16, CAREFUL, false>(r, sc[0], c2, mine, all, vs, g, i);
          wave_lds_order();
       };
       // two tiles in turn, so that one is under way while the other is used
