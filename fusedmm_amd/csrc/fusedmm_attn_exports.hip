@@ -197,11 +197,13 @@ bool whole_chunks(const Desc &d)
 
 // ---- serving form ----
 
-// Slots of a piece: about 1024 workgroups over all key heads - a ragged batch is no faster with 2048, two rows of 200k
-// slots are a quarter slower (48 and 62 us with 768 and 2048) - and not under 256 (two tiles per wave), not over 8192.
-int64_t piece_slots(int64_t nnz, int64_t columns)
+// Slots of a piece, over all key heads.  In the tensors' own type about 1024 workgroups, two rounds of the 2 that a CU holds:
+// a ragged batch takes 125 us, with 768 or 2048 workgroups 129 us.  In 4 bits about 768, one round of the 3 that a CU holds: two
+// rows of 200k slots take 37 us, with 1024 workgroups 42 us, a ragged batch 149 and 146 us.  Not under 256 slots (two
+// tiles per wave), not over 8192.
+int64_t piece_slots(int64_t nnz, int64_t columns, bool kv4)
 {
-   const int64_t want = nnz * columns / 1024;
+   const int64_t want = nnz * columns / (kv4 ? 768 : 1024);
    return (std::min<int64_t>(std::max<int64_t>(want, 256), 8192) + 127) / 128 * 128;
 }
 
@@ -210,21 +212,21 @@ struct RowsPlan {
    int64_t piece = 0, cap = 0, table = 0, total = 0;   // table: byte offset behind the partial sums
 };
 
-RowsPlan rows_plan(const Desc &d, int64_t nnz, int dc)
+RowsPlan rows_plan(const Desc &d, int64_t nnz, int dc, bool kv4)
 {
    RowsPlan r;
    const int hp = 16 / d.maps, group = d.heads / d.kv_heads;
    r.passes = (group + hp - 1) / hp;
    const int64_t columns = (int64_t)d.kv_heads * r.passes;
-   r.piece = piece_slots(nnz, columns);
+   r.piece = piece_slots(nnz, columns, kv4);
    if (nnz <= r.piece || d.m == 0) return r;   // no row is cut
    r.cap = nnz / r.piece + d.m;
-   r.table = align256(r.cap * columns * 16 * (dc * d.maps + 2) * 4);
+   r.table = align256(r.cap * columns * 16 * (dc * d.maps + kPartExtra) * 4);
    r.total = r.table + (d.m > kTableRows ? (d.m + 2) * 8 : 0);
    return r;
 }
 
-int rows_common(const char *who, const Desc *d, int64_t nnz, const void *indx, const void *pntrb, const void *pntre, const void *q, const float *lambda,
+int rows_common(const char *who, bool kv4, const Desc *d, int64_t nnz, const void *indx, const void *pntrb, const void *pntre, const void *q, const float *lambda,
                 void *o, void *work, int64_t work_bytes, int *dc, RowsParams *p)
 {
    int st = check_sizes(who, d, dc);
@@ -235,7 +237,7 @@ int rows_common(const char *who, const Desc *d, int64_t nnz, const void *indx, c
    if (d->n > INT32_MAX) return refuse(who, "n is at most 2^31 - 1");
    if (!inputs_ok(*d)) return refuse(who, "a stride is negative or too large");
    if (!apart(d->ldo, d->hdo, d->m, d->heads, d->dv)) return refuse(who, "the rows of o overlap");
-   const RowsPlan r = rows_plan(*d, nnz, *dc);
+   const RowsPlan r = rows_plan(*d, nnz, *dc, kv4);
    if ((std::max<int64_t>(r.cap, d->m) + 8) * d->kv_heads * r.passes > kMaxGrid || d->m * d->heads > kMaxGrid) return refuse(who, "too many rows and heads for one call");
    if (d->m == 0) return kOk;
    if (!q || !o || !pntrb || !pntre || (nnz > 0 && !indx) || (d->maps == 2 && !lambda)) return refuse(who, "a pointer is null");
@@ -507,7 +509,7 @@ int64_t fusedMM_attn_rows_workspace(const fusedMM_attn_desc *desc, const INDEXTY
       (void)refuse(who, "negative nnz");
       return -1;
    }
-   return rows_plan(*desc, nnz, dc).total;
+   return std::max(rows_plan(*desc, nnz, dc, false).total, rows_plan(*desc, nnz, dc, true).total);
 }
 
 int fusedMM_attn_rows(const fusedMM_attn_desc *desc, const INDEXTYPE nnz, const INDEXTYPE *indx, const INDEXTYPE *pntrb, const INDEXTYPE *pntre, const void *q,
@@ -516,7 +518,7 @@ int fusedMM_attn_rows(const fusedMM_attn_desc *desc, const INDEXTYPE nnz, const 
    const char *who = "fusedMM_attn_rows";
    int dc;
    RowsParams p;
-   int st = rows_common(who, desc, nnz, indx, pntrb, pntre, q, lambda, o, work, work_bytes, &dc, &p);
+   int st = rows_common(who, false, desc, nnz, indx, pntrb, pntre, q, lambda, o, work, work_bytes, &dc, &p);
    if (st || desc->m == 0) return st;
    if (desc->n > 0 && (!k || !v)) return refuse(who, "a pointer is null");
    const void *ptrs[] = {indx, pntrb, pntre, q, k, v, lambda, o, work};
@@ -567,7 +569,7 @@ int fusedMM_attn_rows_kv4(const fusedMM_attn_desc *desc, const INDEXTYPE nnz, co
    const char *who = "fusedMM_attn_rows_kv4";
    int dc;
    RowsParams p;
-   int st = rows_common(who, desc, nnz, indx, pntrb, pntre, q, lambda, o, work, work_bytes, &dc, &p);
+   int st = rows_common(who, true, desc, nnz, indx, pntrb, pntre, q, lambda, o, work, work_bytes, &dc, &p);
    if (st) return st;
    if (desc->type == FUSEDMM_TYPE_F32)
    {

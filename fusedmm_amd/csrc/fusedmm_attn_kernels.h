@@ -7,8 +7,8 @@
 // for 64 rows (a tile that no row of a wave names is skipped by that wave); with BR = 16 nothing is shared but nothing
 // is multiplied for the rows of other waves either, which is what rows without common neighbours want.
 //
-// The tiles go from memory straight into LDS (no registers in between), S of them in flight: a gather has several tiles'
-// worth of products to arrive in.  Column ids and masks run ahead of them the same way, in groups of 8 tiles.
+// The tiles go from memory straight into LDS (no registers in between), with BR = 64 one ahead of the one in use.  Column
+// ids and masks run ahead of them the same way, in groups of 8 tiles.
 #pragma once
 #include "fusedmm_attn_core.h"
 
@@ -72,17 +72,20 @@ template <int T, int DC, int MAPS, int BR> struct Geo {
    static constexpr int CV = W / N::KC;
    static constexpr int MC = DC / N::EPL;             // chunks of one map
    static constexpr int NT = W / 16, NTQ = DC / 16;   // 16-feature tiles of v's and of one map's accumulators
-   // Tiles in flight and being used.  More than two cost residency (two tensors' tiles are 4 ... 64 KB of 160): a window
-   // of 512 at 128 bf16 features 55 us with 3 or 4, 44 with 2; a graph's training pass 438 us with 3, 320 with 2.
+   // Tiles of a workgroup, in flight and being used.  A workgroup of one wave is better off with one tile and more company:
+   // training over a graph with 16 neighbours, 4 heads of 128 bf16 (f32) features, 139 us (580) with one, 218 (1069) with
+   // two.  Only where two tensors' tiles are 8 KB two are ahead, 92 us against 97 (64 bf16 features), 158 against 180 (32
+   // f32).  Workgroups of four waves: two are 1 to 3 % ahead of one with 16-bit types and as good with f32; three or four cost
+   // residency (a window of 512 at 128 bf16 features 55 us, 44 with two).
    static constexpr int kPair = 2 * V::kBytes;
-   static constexpr int S = 2;
+   static constexpr int S = BR == 64 || kPair == 8192 ? 2 : 1;
    static constexpr int kMaskBytes = BR * 4;               // of a tile
    static constexpr int kStat = 2 * MAPS * kTile * 4;      // statistics of a tile's rows (dk, dv)
 };
 
-template <int N> __device__ inline void wait_loads()   // all but the N newest loads have arrived, LDS operations are done
+__device__ inline void wait_loads()   // all loads have arrived, LDS operations are done
 {
-   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
+   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
 }
 template <int BR> __device__ inline void tile_barrier()
 {
@@ -320,35 +323,41 @@ template <int M> struct Mode {
    static constexpr int value = M;
 };
 
-// The loop over a unit's tiles that all kernels share: fill the pipeline, then for every step wait, free the oldest
-// buffer, fill it, and use the current one.  steps = tiles * per_tile; load(step, buffer), use(step, buffer).
+// The loop over a unit's tiles that all kernels share.  steps = tiles * per_tile; load(step, buffer), use(step, buffer).
+// The ids of the next group are asked for a group ahead: the waits for the tiles in between include them.
 template <class G, int BR, class S, class Load, class Use> __device__ __forceinline__ void for_tiles(const S &st, int steps, int per_tile, Load load, Use use)
 {
    if (steps > 0)
    {
       st.load_ids(0);
-      wait_loads<0>();
+      wait_loads();
       tile_barrier<BR>();
+      if (G::S == 2) load(0, 0);
    }
-#pragma unroll
-   for (int s = 0; s < G::S - 1; s++)
-      if (s < steps) load(s, s);
-   int buf = 0;
    for (int s = 0; s < steps; s++)
    {
-      // the loads of later steps may still be under way; at the end of the unit there are fewer, and all are waited for
-      if (st.vec && s + G::S - 2 < steps) wait_loads<(G::S - 2) * 2 * G::NCH>();
-      else wait_loads<0>();
-      tile_barrier<BR>();
-      // The ids of the next group are asked for one group ahead: the loads of any tile that a wave waits for before it uses
-      // them were issued later (2 S - 2 <= 8 tiles).
       const int group = s / (kAhead * per_tile) + 1;
-      if (s % (kAhead * per_tile) == 0 && group * (kAhead * per_tile) < steps) st.load_ids(group);
-      if (s + G::S - 1 < steps) load(s + G::S - 1, buf == 0 ? G::S - 1 : buf - 1);
-      use(s, buf);
-      buf = buf == G::S - 1 ? 0 : buf + 1;
+      const bool ids = s % (kAhead * per_tile) == 0 && group * (kAhead * per_tile) < steps;
+      if constexpr (G::S == 1)
+      {
+         if (ids) st.load_ids(group);
+         load(s, 0);
+         wait_loads();
+         tile_barrier<BR>();
+         use(s, 0);
+         wait_loads();   // (LDS: this wave has read the tile)
+         tile_barrier<BR>();
+      }
+      else
+      {
+         wait_loads();
+         tile_barrier<BR>();
+         if (ids) st.load_ids(group);
+         if (s + 1 < steps) load(s + 1, (s + 1) & 1);
+         use(s, s & 1);
+      }
    }
-   wait_loads<0>();   // nothing is under way into LDS when it is used again
+   wait_loads();   // nothing is under way into LDS when it is used again
    tile_barrier<BR>();
 }
 

@@ -107,7 +107,9 @@ int make_table(const RowsParams &p, hipStream_t s)
 template <int O, int DC, int MAPS> int join(const RowsParams &p, hipStream_t s)
 {
    if (!p.cap) return kOk;
-   hipLaunchKernelGGL((attn_rows_join<FMM_ATTN_UNIT, O, DC, MAPS>), dim3((unsigned)(p.m * p.heads)), dim3(256), 0, s, p);
+   const int waves = p.cap > 8 * 4 * (256 / (DC * MAPS)) * p.m ? 16 : 4;   // 4, where they take a row in one batch
+   const size_t lds = (size_t)waves * MAPS * (DC * MAPS + 2) * sizeof(float);
+   hipLaunchKernelGGL((attn_rows_join<FMM_ATTN_UNIT, O, DC, MAPS>), dim3((unsigned)(p.m * p.heads)), dim3(64 * waves), lds, s, p);
    ATTN_HIP(hipGetLastError());
    return kOk;
 }

@@ -20,7 +20,7 @@ struct RowsParams {
    const void *indx, *pntrb, *pntre;
    const void *q, *k, *v;
    int64_t ldq, hdq, ldk, hdk, ldv, hdv, ldo, hdo;
-   int32_t vec_q, vec_kv, vec_o;
+   int32_t vec_q, vec_kv;
    const uint8_t *cache;              // 4-bit records, instead of k and v
    int64_t ldc, hdc;
    const float *lambda;
@@ -28,9 +28,10 @@ struct RowsParams {
    int32_t out_type;                  // 4-bit cache: element type of q and out
    int64_t piece;                     // slots of a piece; doubled on the device while the pieces are more than cap
    int64_t cap;                       // pieces that the workspace has room for; 0: rows are not cut
-   float *part;                       // [piece][kv head][pass][16 columns][W + 2]
+   float *part;                       // [piece][kv head][pass][16 columns][W + kPartExtra]: W features, base, sum of weights
    int64_t *table;                    // m > kTableRows: [0] slots of a piece, [1 + r] pieces of the rows before r
 };
+constexpr int kPartExtra = 4;         // (two are used: columns stay on 16 bytes)
 constexpr int kTableRows = 256;       // up to this many rows, every wave finds its piece from the row pointers itself
 
 struct Kv4Params {
@@ -47,6 +48,8 @@ struct Kv4Params {
    int64_t ldc, hdc;
    int32_t per_group;                    // tokens of a workgroup
 };
+
+typedef float f2 __attribute__((ext_vector_type(2)));
 
 __device__ inline int64_t index_of(const void *a, int64_t i, int bytes)
 {
@@ -254,106 +257,152 @@ __device__ inline void rows_finish(const RowsParams &p, Softmax<G::NT> &r, unsig
       stat[wave][i][1] = r.sum;
    }
    __syncthreads();
+   // four features of a column, and the column's base and sum of weights
    auto column = [&](int c, int f, float &top, float &sum) {
       top = fmaxf(fmaxf(stat[0][c][0], stat[1][c][0]), fmaxf(stat[2][c][0], stat[3][c][0]));
       const float base = top == -INFINITY ? 0.0f : top;
       sum = 0;
-      float x = 0;
+      f4 x = {0, 0, 0, 0};
 #pragma unroll
       for (int w = 0; w < 4; w++)
       {
          const float keep = exp2_fast(stat[w][c][0] - base);
          sum += stat[w][c][1] * keep;
-         x += reinterpret_cast<const float *>(vs_all + w * G::V::kBytes)[c * G::W + f] * keep;
+         x += *reinterpret_cast<const f4 *>(vs_all + w * G::V::kBytes + (c * G::W + f) * 4) * keep;
       }
       return x;
    };
    const int left = p.group - pass * G::HP, heads = left < G::HP ? left : G::HP;
+   constexpr int C4 = G::W / 4;
    if (s.count > 1)
    {
-      float *to = p.part + ((id * p.kv_heads + kvh) * p.passes + pass) * 16 * (G::W + 2);
-      for (int e = tid; e < 16 * G::W; e += 256)
+      float *to = p.part + ((id * p.kv_heads + kvh) * p.passes + pass) * 16 * (G::W + kPartExtra);
+      for (int e = tid; e < 16 * C4; e += 256)
       {
-         const int c = e / G::W, f = e % G::W;
+         const int c = e / C4, f = e % C4 * 4;
          if (c % G::HP >= heads) continue;
          float top, sum;
-         to[c * (G::W + 2) + f] = column(c, f, top, sum);
+         *reinterpret_cast<f4 *>(to + c * (G::W + kPartExtra) + f) = column(c, f, top, sum);
          if (f == 0)
          {
-            to[c * (G::W + 2) + G::W] = top;
-            to[c * (G::W + 2) + G::W + 1] = sum;
+            to[c * (G::W + kPartExtra) + G::W] = top;
+            to[c * (G::W + kPartExtra) + G::W + 1] = sum;
          }
       }
       return;
    }
    typedef typename Num<O>::E EO;
-   for (int e = tid; e < heads * G::W; e += 256)
+   for (int e = tid; e < heads * C4; e += 256)
    {
-      const int hh = e / G::W, f = e % G::W;
+      const int hh = e / C4, f = e % C4 * 4;
       if (f >= p.dv) continue;
       const int head = kvh * p.group + pass * G::HP + hh;
       float top, sum;
-      float x = column(hh, f, top, sum);
-      x = sum == 0.0f ? 0.0f : x / sum;
+      f4 x = column(hh, f, top, sum);
+#pragma unroll
+      for (int j = 0; j < 4; j++) x[j] = sum == 0.0f ? 0.0f : x[j] / sum;
       if constexpr (MAPS == 2)
       {
-         const float y = column(hh + 8, f, top, sum);
-         x -= p.lambda[head] * (sum == 0.0f ? 0.0f : y / sum);
+         const f4 y = column(hh + 8, f, top, sum);
+         const float lambda = p.lambda[head];
+#pragma unroll
+         for (int j = 0; j < 4; j++) x[j] -= lambda * (sum == 0.0f ? 0.0f : y[j] / sum);
       }
-      ((EO *)p.out)[s.row * p.ldo + head * p.hdo + f] = (EO)Num<O>::from(x);
+      store4<O>((EO *)p.out + s.row * p.ldo + head * p.hdo, f, p.dv, x, false);
    }
 }
 
-// rows of several pieces: a workgroup per (row, head), its waves take the pieces in turn
-// (UNIT: the object it is compiled into)
-template <int UNIT, int O, int DC, int MAPS> __global__ __launch_bounds__(256) void attn_rows_join(RowsParams p)
+// Rows of several pieces: a workgroup per (row, head).  W / 4 lanes take a piece, batches of 8 without conditions so that
+// their loads are under way together (places behind the last piece read the last one); the base follows the batches.
+// Bound by the latency of a few dependent loads.  LDS: waves x MAPS x (W + 2) floats.  (UNIT: the object it is compiled into)
+template <int UNIT, int O, int DC, int MAPS> __global__ __launch_bounds__(1024) void attn_rows_join(RowsParams p)
 {
-   constexpr int W = DC * MAPS, HP = 16 / MAPS, PER = (W + 63) / 64;
+   constexpr int W = DC * MAPS, HP = 16 / MAPS, LANES = W / 4, B = 8, kMine = W + 2;
    typedef typename Num<O>::E EO;
-   __shared__ float part[4][MAPS][W + 1];
+   extern __shared__ float part[];
    const int64_t row = blockIdx.x / p.heads;
    const int head = (int)(blockIdx.x % p.heads), kvh = head / p.group, hh = head % p.group, pass = hh / HP;
-   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+   const int f0 = lane % LANES * 4, workers = waves * (64 / LANES), worker = wave * (64 / LANES) + lane / LANES;
    const Spot s = find_piece(p, -1, row);
    if (s.count <= 1) return;
+   const int64_t step = (int64_t)p.kv_heads * p.passes * 16 * (W + kPartExtra);
+   const float *from = p.part + ((s.first * p.kv_heads + kvh) * p.passes + pass) * 16 * (W + kPartExtra) + hh % HP * (W + kPartExtra);
 #pragma unroll
-   for (int mp = 0; mp < MAPS; mp++)
+   for (int mp = 0; mp < MAPS; mp++, from += HP * (W + kPartExtra))
    {
-      const int64_t step = (int64_t)p.kv_heads * p.passes * 16 * (W + 2);
-      const float *from = p.part + ((s.first * p.kv_heads + kvh) * p.passes + pass) * 16 * (W + 2) + (mp * HP + hh % HP) * (W + 2);
-      float top = -INFINITY;
-      for (int64_t u = lane; u < s.count; u += 64) top = fmaxf(top, from[u * step + W]);
-#pragma unroll
-      for (int k = 1; k < 64; k <<= 1) top = fmaxf(top, __shfl_xor(top, k));
-      const float base = top == -INFINITY ? 0.0f : top;
-      float sum = 0, o[PER];
-#pragma unroll
-      for (int x = 0; x < PER; x++) o[x] = 0;
-#pragma unroll 4
-      for (int64_t u = wave; u < s.count; u += 4)
+      float base = -INFINITY, sum = 0;
+      f4 o = {0, 0, 0, 0};
+      auto follow = [&](float to) {   // the base becomes `to`, which is no lower
+         const float keep = to == base ? 1.0f : exp2_fast(base - to);
+         sum *= keep;
+         o *= keep;
+         base = to;
+         return to == -INFINITY ? 0.0f : to;
+      };
+      for (int64_t u0 = 0; u0 < s.count; u0 += B * workers)
       {
-         const float *f = from + u * step;
-         const float keep = exp2_fast(f[W] - base);
-         sum += f[W + 1] * keep;
+         float top = base;
+         f4 x[B];
+         f2 n[B];
 #pragma unroll
-         for (int x = 0; x < PER; x++)
-            if (lane + 64 * x < W) o[x] += f[lane + 64 * x] * keep;
+         for (int b = 0; b < B; b++)
+         {
+            const int64_t u = u0 + worker + b * workers;
+            const float *f = from + (u < s.count ? u : s.count - 1) * step;
+            n[b] = *reinterpret_cast<const f2 *>(f + W);
+            x[b] = *reinterpret_cast<const f4 *>(f + f0);
+         }
+#pragma unroll
+         for (int b = 0; b < B; b++) top = fmaxf(top, n[b][0]);
+         const float at = follow(top);
+#pragma unroll
+         for (int b = 0; b < B; b++)
+         {
+            if (u0 + worker + b * workers >= s.count) break;
+            const float keep = exp2_fast(n[b][0] - at);
+            sum += n[b][1] * keep;
+            o += x[b] * keep;
+         }
       }
 #pragma unroll
-      for (int x = 0; x < PER; x++)
-         if (lane + 64 * x < W) part[wave][mp][lane + 64 * x] = o[x];
-      if (lane == 0) part[wave][mp][W] = sum;
+      for (int k = LANES; k < 64; k <<= 1)   // the pieces of a wave
+      {
+         follow(fmaxf(base, __shfl_xor(base, k)));
+         sum += __shfl_xor(sum, k);
+#pragma unroll
+         for (int j = 0; j < 4; j++) o[j] += __shfl_xor(o[j], k);
+      }
+      float *mine = part + (wave * MAPS + mp) * kMine;
+      if (lane < LANES)
+      {
+#pragma unroll
+         for (int j = 0; j < 4; j++) mine[f0 + j] = o[j];
+      }
+      if (lane == 0)
+      {
+         mine[W] = base;
+         mine[W + 1] = sum;
+      }
    }
    __syncthreads();
    EO *out = (EO *)p.out + row * p.ldo + head * p.hdo;
-   for (int f = threadIdx.x; f < p.dv; f += 256)
+   for (int f = threadIdx.x; f < p.dv; f += blockDim.x)
    {
       float r[MAPS];
 #pragma unroll
       for (int mp = 0; mp < MAPS; mp++)
       {
-         const float sum = part[0][mp][W] + part[1][mp][W] + part[2][mp][W] + part[3][mp][W];
-         const float x = part[0][mp][f] + part[1][mp][f] + part[2][mp][f] + part[3][mp][f];
+         float top = -INFINITY, sum = 0, x = 0;
+         for (int w = 0; w < waves; w++) top = fmaxf(top, part[(w * MAPS + mp) * kMine + W]);
+         const float at = top == -INFINITY ? 0.0f : top;
+         for (int w = 0; w < waves; w++)
+         {
+            const float *of = part + (w * MAPS + mp) * kMine;
+            const float keep = exp2_fast(of[W] - at);
+            sum += of[W + 1] * keep;
+            x += of[f] * keep;
+         }
          r[mp] = sum == 0.0f ? 0.0f : x / sum;
       }
       if constexpr (MAPS == 2) r[0] -= p.lambda[head] * r[1];
@@ -630,19 +679,19 @@ __global__ __launch_bounds__(256, (DC * MAPS >= 256 ? 1 : DC * MAPS == 128 && FU
    float top = 0;
 #pragma unroll
    for (int j = 0; j < WQ; j++)
+   {
+      const int f = code_feature<FULL, WQ>(j, g);
+      const uint16_t *from = (const uint16_t *)p.q + s.row * p.ldq + (col ? (it.kvh * p.group + hh) * p.hdq + mp_i * p.d + f : 0);
+      const u4 x = load_chunk<kF16>(from, col && f < p.d ? 8 : 0, p.vec_q);   // (d is a multiple of 32)
 #pragma unroll
       for (int e = 0; e < 8; e++)
       {
-         const int f = code_feature<FULL, WQ>(j, g) + e;
-         float x = 0;
-         if (col && f < p.d)
-         {
-            const int64_t off = s.row * p.ldq + (it.kvh * p.group + hh) * p.hdq + mp_i * p.d + f;
-            x = p.out_type == kF16 ? Num<kF16>::to(((const uint16_t *)p.q)[off]) : Num<kBF16>::to(((const uint16_t *)p.q)[off]);
-         }
-         qf[j][e] = p.scale < 0 ? -x : x;
-         top = fmaxf(top, fabsf(x));
+         const uint16_t b = (uint16_t)(x[e / 2] >> (16 * (e & 1)));
+         const float y = p.out_type == kF16 ? Num<kF16>::to(b) : Num<kBF16>::to(b);
+         qf[j][e] = p.scale < 0 ? -y : y;
+         top = fmaxf(top, fabsf(y));
       }
+   }
    top = group_max(top);
    const int ex = top > 0 && top < INFINITY ? __builtin_amdgcn_frexp_expf(top) : 0;
    u4 q[WQ];
