@@ -234,8 +234,16 @@ template <class G, int T, int DC, int BR> struct Stream {
          load_lds16(lb + j * (G::THREADS * 16), e < dv ? (const void *)fb : (const void *)&zero_chunk);
       }
       if (vec) return;
-      // rows at any place, ends of rows within a chunk: through registers, a few chunks at a time
-      constexpr int B = G::NCH < 4 ? G::NCH : 4;
+      if (d >= G::N::EPL && dv >= G::N::EPL) load_parts<kShifted>(c, ta, tb, oa, ob);
+      else load_parts<kElements>(c, ta, tb, oa, ob);
+   }
+
+   // rows at any place: through registers, a few chunks at a time
+   template <int MODE> __device__ __forceinline__ void load_parts(const int32_t *c, unsigned char *ta, unsigned char *tb, int64_t oa, int64_t ob) const
+   {
+      constexpr int B = MODE == kElements ? 1 : G::NCH < 4 ? G::NCH : 4;
+      int me = tid;
+      asm volatile("" : "+v"(me));
 #pragma unroll
       for (int j0 = 0; j0 < G::NCH; j0 += B)
       {
@@ -247,8 +255,8 @@ template <class G, int T, int DC, int BR> struct Stream {
             const bool live = kTile * G::CR >= G::THREADS || x < kTile * G::CR;
             const uint32_t col = (uint32_t)c[live ? r : 0];
             const int e = ((x % G::CR) ^ V::twist(r)) * G::N::EPL, f = e % DC;
-            ra[j] = load_chunk<T>((const E *)(a + oa + (uint64_t)col * lda) + (e / DC * d + f), !live ? 0 : d - f < G::N::EPL ? d - f : G::N::EPL, false);
-            rb[j] = load_chunk<T>((const E *)(b + ob + (uint64_t)col * ldb) + e, !live ? 0 : dv - e < G::N::EPL ? dv - e : G::N::EPL, false);
+            ra[j] = load_part<T, MODE>((const E *)(a + oa + (uint64_t)col * lda) + e / DC * d, f, d, live);
+            rb[j] = load_part<T, MODE>((const E *)(b + ob + (uint64_t)col * ldb), e, dv, live);
          }
 #pragma unroll
          for (int j = 0; j < B; j++)
@@ -269,14 +277,18 @@ template <class G, int T, int DC, int BR> struct Stream {
 };
 
 // the resident rows of a wave as the second operand: lane i holds its 16 bytes of every chunk of row i
-template <int T, int CQ> __device__ inline void load_resident(u4 (&r)[CQ], const typename Num<T>::E *row, bool live, int d, int g, bool vec)
+template <int T, int MODE, int CQ> __device__ inline void load_resident_as(u4 (&r)[CQ], const typename Num<T>::E *row, bool live, int d, int g)
 {
 #pragma unroll
-   for (int c = 0; c < CQ; c++)
-   {
-      const int f = c * Num<T>::KC + g * Num<T>::EPL;
-      r[c] = load_chunk<T>(row + f, live ? (d - f < Num<T>::EPL ? d - f : Num<T>::EPL) : 0, vec);
-   }
+   for (int c = 0; c < CQ; c++) r[c] = load_part<T, MODE>(row, c * Num<T>::KC + g * Num<T>::EPL, d, live);
+}
+
+template <int T, int CQ> __device__ inline void load_resident(u4 (&r)[CQ], const typename Num<T>::E *row, bool live, int d, int g, bool vec)
+{
+   const int mode = part_mode<T>(vec, d);
+   if (mode == kAligned) load_resident_as<T, kAligned>(r, row, live, d, g);
+   else if (mode == kShifted) load_resident_as<T, kShifted>(r, row, live, d, g);
+   else load_resident_as<T, kElements>(r, row, live, d, g);
 }
 
 // this lane's part of the product of two resident rows
@@ -319,10 +331,6 @@ template <int BR> __device__ inline bool any_odd(bool odd)
 }
 // How a pass over a unit runs: full 16-byte chunks, any sizes, or any sizes with care for infinities and NaN.
 enum : int { kFull, kAny, kCareful };
-template <int M> struct Mode {
-   static constexpr int value = M;
-};
-
 // The loop over a unit's tiles that all kernels share.  steps = tiles * per_tile; load(step, buffer), use(step, buffer).
 // The ids of the next group are asked for a group ahead: the waits for the tiles in between include them.
 template <class G, int BR, class S, class Load, class Use> __device__ __forceinline__ void for_tiles(const S &st, int steps, int per_tile, Load load, Use use)

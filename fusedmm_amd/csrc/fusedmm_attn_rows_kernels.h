@@ -478,20 +478,26 @@ __global__ __launch_bounds__(256, (sizeof(typename Num<T>::E) * DC * MAPS >= 512
    const int mp_i = i / G::HP, hh = it.pass * G::HP + i % G::HP;
    const bool col = hh < p.group;
    u4 q[G::CQ];
+   auto query = [&](auto mode) __attribute__((always_inline)) {
+      const E *from = (const E *)p.q + s.row * p.ldq + (col ? (it.kvh * p.group + hh) * p.hdq + mp_i * p.d : 0);
 #pragma unroll
-   for (int c = 0; c < G::CQ; c++)
+      for (int c = 0; c < G::CQ; c++) q[c] = load_part<T, decltype(mode)::value>(from, c * G::N::KC + g * G::N::EPL, p.d, col);
+   };
+   const int mode_q = part_mode<T>(p.vec_q, p.d);
+   if (mode_q == kAligned) query(Mode<kAligned>());
+   else if (mode_q == kShifted) query(Mode<kShifted>());
+   else query(Mode<kElements>());
+   if (p.scale < 0)
    {
-      const int f = c * G::N::KC + g * G::N::EPL;
-      const int left = p.d - f;
-      q[c] = load_chunk<T>((const E *)p.q + s.row * p.ldq + (col ? (it.kvh * p.group + hh) * p.hdq + mp_i * p.d + f : 0),
-                           col ? (left < G::N::EPL ? left : G::N::EPL) : 0, p.vec_q);
-      if (p.scale < 0) q[c] = negated<T>(q[c]);
+#pragma unroll
+      for (int c = 0; c < G::CQ; c++) q[c] = negated<T>(q[c]);
    }
    Softmax<G::NT> r;
    const float c2 = score_factor(p.scale);
 
    u4 kf[2][MAPS][G::CQ], vf[G::NV];
-   auto load = [&](int32_t slot) __attribute__((always_inline)) {
+   auto load_as = [&](int32_t slot, auto mode) __attribute__((always_inline)) {
+      constexpr int MODE = decltype(mode)::value;
 #pragma unroll
       for (int a = 0; a < 2; a++)
       {
@@ -502,20 +508,26 @@ __global__ __launch_bounds__(256, (sizeof(typename Num<T>::E) * DC * MAPS >= 512
 #pragma unroll
             for (int x = 0; x < G::CQ; x++)
             {
-               const int f = x * G::N::KC + g * G::N::EPL, left = p.d - f;
+               const int f = x * G::N::KC + g * G::N::EPL;
                if constexpr (FULL) kf[a][mp][x] = *reinterpret_cast<const u4 *>(row + mp * DC + f);
-               else kf[a][mp][x] = load_chunk<T>(row + mp * p.d + f, c < 0 ? 0 : left < G::N::EPL ? left : G::N::EPL, p.vec_kv);
+               else kf[a][mp][x] = load_part<T, MODE>(row + mp * p.d, f, p.d, c >= 0);
             }
       }
 #pragma unroll
       for (int j = 0; j < G::NV; j++)
       {
-         const int e = lane + 64 * j, f = (e % G::CR) * G::N::EPL, left = p.dv - f;
+         const int e = lane + 64 * j, f = (e % G::CR) * G::N::EPL;
          const int32_t c = __shfl(slot, e / G::CR);
-         const E *at = v + (int64_t)(c < 0 ? 0 : c) * p.ldv + f;
-         if constexpr (FULL) vf[j] = *reinterpret_cast<const u4 *>(at);
-         else vf[j] = load_chunk<T>(at, c < 0 ? 0 : left < G::N::EPL ? left : G::N::EPL, p.vec_kv);
+         const E *at = v + (int64_t)(c < 0 ? 0 : c) * p.ldv;
+         if constexpr (FULL) vf[j] = *reinterpret_cast<const u4 *>(at + f);
+         else vf[j] = load_part<T, MODE>(at, f, p.dv, c >= 0);
       }
+   };
+   const int mode_kv = part_mode<T>(p.vec_kv, p.d < p.dv ? p.d : p.dv);
+   auto load = [&](int32_t slot) __attribute__((always_inline)) {
+      if (FULL || mode_kv == kAligned) load_as(slot, Mode<kAligned>());
+      else if (mode_kv == kShifted) load_as(slot, Mode<kShifted>());
+      else load_as(slot, Mode<kElements>());
    };
    constexpr int64_t kStride = 4 * kTile;
    const int64_t end = begin + hi;
@@ -682,7 +694,8 @@ __global__ __launch_bounds__(256, (DC * MAPS >= 256 ? 1 : DC * MAPS == 128 && FU
    {
       const int f = code_feature<FULL, WQ>(j, g);
       const uint16_t *from = (const uint16_t *)p.q + s.row * p.ldq + (col ? (it.kvh * p.group + hh) * p.hdq + mp_i * p.d + f : 0);
-      const u4 x = load_chunk<kF16>(from, col && f < p.d ? 8 : 0, p.vec_q);   // (d is a multiple of 32)
+      u4 x = {0, 0, 0, 0};
+      if (col && f < p.d) x = load_chunk<kF16>(from, p.vec_q);   // (d is a multiple of 32)
 #pragma unroll
       for (int e = 0; e < 8; e++)
       {
@@ -861,7 +874,7 @@ template <int T> __global__ __launch_bounds__(256) void kv4_write(Kv4Params p)
 #pragma unroll
       for (int j = 0; j < 32 / EPL; j++)
       {
-         const u4 a = load_chunk<T>(from + j * EPL, EPL, p.vec);
+         const u4 a = load_chunk<T>(from + j * EPL, p.vec);
 #pragma unroll
          for (int e = 0; e < EPL; e++)
          {
