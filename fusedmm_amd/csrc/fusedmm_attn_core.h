@@ -135,7 +135,7 @@ template <int T, int MODE> __device__ inline u4 load_part(const typename Num<T>:
    else if constexpr (MODE == kElements)
    {
 #pragma unroll
-      for (int k = 0; k < EPL - 1; k++)
+      for (int k = 0; k < EPL; k++)   // (the other tensor may be the one with the short rows)
       {
          if (!live || f + k >= width) continue;
          if constexpr (T == kF32) r[k] = __float_as_uint(row[f + k]);
