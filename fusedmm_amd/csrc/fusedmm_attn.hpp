@@ -74,6 +74,9 @@ inline int64_t dkv_part(int dc, int maps, int br) { return (int64_t)br * (2 * dc
 int launch_forward_f32(const Params &p, int dc, int maps, hipStream_t s);
 int launch_forward_f16(const Params &p, int dc, int maps, hipStream_t s);
 int launch_forward_bf16(const Params &p, int dc, int maps, hipStream_t s);
+int launch_pack_f32(const PackParams &p, hipStream_t s);
+int launch_pack_f16(const PackParams &p, hipStream_t s);
+int launch_pack_bf16(const PackParams &p, hipStream_t s);
 int launch_dq_f32(const Params &p, int dc, int maps, hipStream_t s);      // dq, and the statistics and sums that dkv reads
 int launch_dq_f16(const Params &p, int dc, int maps, hipStream_t s);
 int launch_dq_bf16(const Params &p, int dc, int maps, hipStream_t s);

@@ -124,14 +124,59 @@ int check_device(const char *who, const void *plan)
    return as_plan(plan)->device == dev ? kOk : refuse(who, "the plan belongs to another device than the current one");
 }
 
+bool whole_chunks(const Desc &d)
+{
+   const int epl = 16 / element_bytes(d);
+   return d.d % epl == 0 && d.dv % epl == 0;
+}
+
+// The tensors whose rows a kernel gathers.  Where their sizes or strides keep rows off 16 bytes they are laid out anew in the
+// workspace, once per call: training with 5 columns that all of 1808 rows name, 16 heads, two maps of 38 and 75 bf16
+// features, 185 us instead of 435.  (A pointer alone that is off, which the descriptor does not tell, is not.)
+struct Tensors {
+   const void *a = nullptr, *b = nullptr;
+   int64_t rows = 0, lda = 0, ha = 0, ldb = 0, hb = 0;
+   int heads = 0;
+};
+Tensors keys_values(const Desc &d, const void *k, const void *v) { return {k, v, d.n, d.ldk, d.hdk, d.ldv, d.hdv, d.kv_heads}; }
+Tensors queries_gradients(const Desc &d, const void *q, const void *dout) { return {q, dout, d.m, d.ldq, d.hdq, d.ldo, d.hdo, d.heads}; }
+
+bool packs(const Desc &d, const Tensors &t)
+{
+   const int bytes = element_bytes(d);
+   return t.rows > 0 && (!whole_chunks(d) || (t.lda * bytes) % 16 || (t.ha * bytes) % 16 || (t.ldb * bytes) % 16 || (t.hb * bytes) % 16);
+}
+int64_t pack_bytes(const Desc &d, const Tensors &t, int dc) { return packs(d, t) ? 2 * t.rows * t.heads * dc * d.maps * element_bytes(d) : 0; }
+
+// how the kernels find them; copies them to `to` where they are to be packed
+int gather_from(const char *who, const Desc &d, const Tensors &t, int dc, void *to, hipStream_t s, Gathered *g)
+{
+   const int bytes = element_bytes(d), w = dc * d.maps;
+   if (!packs(d, t))
+   {
+      const bool vec = whole_chunks(d) && lines_up(t.a, t.lda, t.ha, bytes) && lines_up(t.b, t.ldb, t.hb, bytes);
+      *g = Gathered{t.a, t.b, t.ha, t.hb, (int32_t)(t.lda * bytes), (int32_t)(t.ldb * bytes), d.d, d.dv, vec, vec && d.d == dc && d.dv == w};
+      return kOk;
+   }
+   if (2 * (int64_t)t.heads > kMaxGrid) return refuse(who, "too many heads for one call");
+   void *to_b = (unsigned char *)to + t.rows * t.heads * w * bytes;
+   *g = Gathered{to, to_b, t.rows * w, t.rows * w, w * bytes, w * bytes, dc, w, 1, 1};
+   PackParams p{t.a, t.b, to, to_b, t.rows, t.lda, t.ha, t.ldb, t.hb, t.heads, d.d, d.dv, dc, w * bytes / 16, 0};
+   // enough workgroups to fill the GPU, each of a few chunks per thread where there is more
+   const int64_t want = (t.rows * p.chunks + 255) / 256, most = std::max<int64_t>(1, 16384 / (2 * (int64_t)t.heads));
+   p.per_head = (int32_t)std::min(want, most);
+   return d.type == FUSEDMM_TYPE_F32 ? launch_pack_f32(p, s) : d.type == FUSEDMM_TYPE_F16 ? launch_pack_f16(p, s) : launch_pack_bf16(p, s);
+}
+
 struct Layout {   // of a workspace, in bytes
-   int64_t stats = 0, dlam = 0, part = 0, total = 0;
+   int64_t stats = 0, dlam = 0, part = 0, pack = 0, total = 0;
 };
 
 Layout forward_layout(const Desc &d, const Plan &p, int dc)
 {
    Layout l;
-   l.total = p.parts * d.heads * forward_part(dc, d.maps, p.view.block_rows) * 4;
+   l.pack = align256(p.parts * d.heads * forward_part(dc, d.maps, p.view.block_rows) * 4);
+   l.total = l.pack + pack_bytes(d, keys_values(d, nullptr, nullptr), dc);
    return l;
 }
 
@@ -140,7 +185,9 @@ Layout backward_layout(const Desc &d, const Plan &p, const Plan &t, int dc)
    Layout l;
    l.dlam = align256(d.m * d.heads * d.maps * 8);
    l.part = l.dlam + (d.maps == 2 ? align256((int64_t)p.view.n_units * (p.view.block_rows / 16) * d.heads * 4) : 0);
-   l.total = l.part + std::max(p.parts * d.heads * dq_part(dc, d.maps, p.view.block_rows), t.parts * d.kv_heads * dkv_part(dc, d.maps, t.view.block_rows)) * 4;
+   l.pack = l.part + align256(std::max(p.parts * d.heads * dq_part(dc, d.maps, p.view.block_rows), t.parts * d.kv_heads * dkv_part(dc, d.maps, t.view.block_rows)) * 4);
+   // (one after the other)
+   l.total = l.pack + std::max(pack_bytes(d, keys_values(d, nullptr, nullptr), dc), pack_bytes(d, queries_gradients(d, nullptr, nullptr), dc));
    return l;
 }
 
@@ -176,23 +223,12 @@ Params base_params(const Desc &d, const Plan &plan)
    p.hdv = d.hdv;
    p.ldo = d.ldo;
    p.hdo = d.hdo;
-   const int bytes = element_bytes(d);
-   p.ldq_bytes = (int32_t)(d.ldq * bytes);
-   p.ldk_bytes = (int32_t)(d.ldk * bytes);
-   p.ldv_bytes = (int32_t)(d.ldv * bytes);
-   p.ldo_bytes = (int32_t)(d.ldo * bytes);
    return p;
 }
 
 bool inputs_ok(const Desc &d)
 {
    return strides_ok(d.ldq, d.hdq) && strides_ok(d.ldk, d.hdk) && strides_ok(d.ldv, d.hdv) && strides_ok(d.ldo, d.hdo);
-}
-
-bool whole_chunks(const Desc &d)
-{
-   const int epl = 16 / element_bytes(d);
-   return d.d % epl == 0 && d.dv % epl == 0;
 }
 
 // ---- serving form ----
@@ -419,7 +455,8 @@ int fusedMM_attn_forward(const fusedMM_attn_desc *desc, const void *plan, const 
    if (!apart(d.ldo, d.hdo, d.m, d.heads, d.dv)) return refuse(who, "the rows of o overlap");
    if (d.m == 0) return kOk;
    if (!q || !o || (d.n > 0 && (!k || !v)) || (d.maps == 2 && !lambda)) return refuse(who, "a pointer is null");
-   st = check_work(who, work, work_bytes, forward_layout(d, *as_plan(plan), dc).total);
+   const Layout l = forward_layout(d, *as_plan(plan), dc);
+   st = check_work(who, work, work_bytes, l.total);
    if (!st) st = check_device(who, plan);
    const void *ptrs[] = {q, k, v, lambda, o, o2, lse, work};
    if (!st) st = check_pointers(who, ptrs, 8);
@@ -428,7 +465,6 @@ int fusedMM_attn_forward(const fusedMM_attn_desc *desc, const void *plan, const 
    const int bytes = element_bytes(d);
    p.vec = whole_chunks(d) && lines_up(q, d.ldq, d.hdq, bytes) && lines_up(k, d.ldk, d.hdk, bytes) && lines_up(v, d.ldv, d.hdv, bytes) &&
            lines_up(o, d.ldo, d.hdo, bytes) && lines_up(o2, 0, 0, bytes);
-   p.full = p.vec && d.d == dc && d.dv == dc * d.maps;
    p.q = q;
    p.k = k;
    p.v = v;
@@ -438,6 +474,8 @@ int fusedMM_attn_forward(const fusedMM_attn_desc *desc, const void *plan, const 
    p.lse = lse;
    p.part = (float *)work;
    const hipStream_t s = (hipStream_t)stream;
+   st = gather_from(who, d, keys_values(d, k, v), dc, (unsigned char *)work + l.pack, s, &p.gat);
+   if (st) return st;
    return d.type == FUSEDMM_TYPE_F32 ? launch_forward_f32(p, dc, d.maps, s)
           : d.type == FUSEDMM_TYPE_F16 ? launch_forward_f16(p, dc, d.maps, s) : launch_forward_bf16(p, dc, d.maps, s);
 }
@@ -471,7 +509,6 @@ int fusedMM_attn_backward(const fusedMM_attn_desc *desc, const void *plan, const
    p.vec = whole_chunks(d) && lines_up(q, d.ldq, d.hdq, bytes) && lines_up(k, d.ldk, d.hdk, bytes) && lines_up(v, d.ldv, d.hdv, bytes) &&
            lines_up(o, d.ldo, d.hdo, bytes) && lines_up(dout, 0, 0, bytes) && lines_up(dq, 0, 0, bytes) && lines_up(dk, 0, 0, bytes) &&
            lines_up(dv, 0, 0, bytes);
-   p.full = p.vec && d.d == dc && d.dv == dc * d.maps;
    p.q = q;
    p.k = k;
    p.v = v;
@@ -489,13 +526,18 @@ int fusedMM_attn_backward(const fusedMM_attn_desc *desc, const void *plan, const
    p.dlam_units = (float *)((unsigned char *)work + l.dlam);
    p.part = (float *)((unsigned char *)work + l.part);
    const hipStream_t s = (hipStream_t)stream;
+   void *pack = (unsigned char *)work + l.pack;
    if (d.m > 0)
    {
+      st = gather_from(who, d, keys_values(d, k, v), dc, pack, s, &p.gat);
+      if (st) return st;
       st = d.type == FUSEDMM_TYPE_F32 ? launch_dq_f32(p, dc, d.maps, s) : d.type == FUSEDMM_TYPE_F16 ? launch_dq_f16(p, dc, d.maps, s) : launch_dq_bf16(p, dc, d.maps, s);
       if (st) return st;
    }
    if (d.n == 0 && !p.dlambda) return kOk;
    p.plan = pt.view;
+   st = gather_from(who, d, queries_gradients(d, q, dout), dc, pack, s, &p.gat);
+   if (st) return st;
    return d.type == FUSEDMM_TYPE_F32 ? launch_dkv_f32(p, dc, d.maps, s) : d.type == FUSEDMM_TYPE_F16 ? launch_dkv_f16(p, dc, d.maps, s) : launch_dkv_bf16(p, dc, d.maps, s);
 }
 

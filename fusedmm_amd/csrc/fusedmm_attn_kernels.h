@@ -36,15 +36,26 @@ struct PlanView {
    int32_t block_rows;     // BR
 };
 
+// The tensors whose rows are gathered: k and v (forward, dq), or q and do (dkv), as the caller has them or, where their rows
+// are not whole 16-byte chunks, in rows of W elements that attn_pack has laid out: every row is then gathered once per
+// block that names it by direct loads, instead of being shifted into place each time.
+struct Gathered {
+   const void *a, *b;                 // rows of maps pieces of d features, rows of dv features
+   int64_t ha, hb;                    // elements from head to head
+   int32_t lda_bytes, ldb_bytes;      // bytes from row to row
+   int32_t d, dv;
+   int32_t vec;                       // every row is 16-byte aligned and d, dv are multiples of a 16-byte chunk
+   int32_t full;                      // vec, and d and dv fill the instance's width
+};
+
 struct Params {
    PlanView plan;
+   Gathered gat;
    int64_t m, n;                      // query rows, key rows
    int32_t heads, kv_heads, group, d, dv;
    float scale;
    int64_t ldq, hdq, ldk, hdk, ldv, hdv, ldo, hdo;
-   int32_t ldk_bytes, ldv_bytes, ldq_bytes, ldo_bytes;
    int32_t vec;                       // every row of every tensor is 16-byte aligned and d, dv are multiples of a 16-byte chunk
-   int32_t full;                      // vec, and d and dv fill the instance's width
    const void *q, *k, *v, *o, *o2, *dout;
    const float *lambda;
    const float *lse_in;
@@ -125,8 +136,7 @@ template <class G, int T, int DC, int BR> struct Stream {
    static constexpr int NB = BR == 64 ? G::NCH : 1;
    const unsigned char *pa[NB], *pb[NB];   // BR = 64: this thread's chunks of row 0 (more threads would be more registers)
 
-   // a: rows of maps pieces of d features each; b: rows of dv features
-   __device__ inline void set(const unsigned char *t, unsigned char *i, unsigned char *m, const Params &p, const Unit &u, const E *a_, int lda_, const E *b_, int ldb_)
+   __device__ inline void set(const unsigned char *t, unsigned char *i, unsigned char *m, const Params &p, const Unit &u, int64_t head)
    {
       tiles = t;
       ids = i;
@@ -135,13 +145,13 @@ template <class G, int T, int DC, int BR> struct Stream {
       masks = p.plan.masks + (int64_t)u.tile0 * BR;
       tid = threadIdx.x;
       wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-      a = (const unsigned char *)a_;
-      b = (const unsigned char *)b_;
-      lda = lda_;
-      ldb = ldb_;
-      d = p.d;
-      dv = p.dv;
-      vec = p.vec;
+      a = (const unsigned char *)((const E *)p.gat.a + head * p.gat.ha);
+      b = (const unsigned char *)((const E *)p.gat.b + head * p.gat.hb);
+      lda = p.gat.lda_bytes;
+      ldb = p.gat.ldb_bytes;
+      d = p.gat.d;
+      dv = p.gat.dv;
+      vec = p.gat.vec;
       if constexpr (BR == 64)
       {
 #pragma unroll
@@ -276,6 +286,34 @@ template <class G, int T, int DC, int BR> struct Stream {
    }
 };
 
+// Rows at any place -> rows of w elements (maps pieces of w / maps, zeros behind their d features; zeros behind dv), head by
+// head.  A thread per 16-byte chunk; bound by reading and writing the tensors once.
+struct PackParams {
+   const void *a, *b;
+   void *to_a, *to_b;
+   int64_t rows, lda, ha, ldb, hb;    // elements
+   int32_t heads, d, dv, dc, chunks;  // chunks of a row of w
+   int32_t per_head;                  // workgroups
+};
+template <int T> __global__ __launch_bounds__(256) void attn_pack(PackParams p)
+{
+   typedef typename Num<T>::E E;
+   const unsigned z = blockIdx.x / p.per_head;   // heads of a, then of b
+   const bool second = z >= (unsigned)p.heads;
+   const int64_t head = second ? z - p.heads : z;
+   const E *from = second ? (const E *)p.b + head * p.hb : (const E *)p.a + head * p.ha;
+   const int64_t ld = second ? p.ldb : p.lda, total = p.rows * p.chunks;
+   u4 *to = (u4 *)(second ? p.to_b : p.to_a) + head * total;
+   const bool small = p.d < Num<T>::EPL || p.dv < Num<T>::EPL;
+   for (int64_t x = (int64_t)(blockIdx.x % p.per_head) * 256 + threadIdx.x; x < total; x += (int64_t)p.per_head * 256)
+   {
+      const int e = (int)(x & (p.chunks - 1)) * Num<T>::EPL;   // (a power of two of chunks)
+      const E *row = from + (x / p.chunks) * ld + (second ? 0 : e / p.dc * p.d);
+      const int f = second ? e : e % p.dc, width = second ? p.dv : p.d;
+      to[x] = small ? load_part<T, kElements>(row, f, width, true) : load_part<T, kShifted>(row, f, width, true);
+   }
+}
+
 // the resident rows of a wave as the second operand: lane i holds its 16 bytes of every chunk of row i
 template <int T, int MODE, int CQ> __device__ inline void load_resident_as(u4 (&r)[CQ], const typename Num<T>::E *row, bool live, int d, int g)
 {
@@ -390,7 +428,7 @@ template <int T, int DC, int MAPS, int BR> __global__ __launch_bounds__(BR * 4, 
    const int64_t row = (int64_t)u.block * BR + 16 * wave + i;
    const bool live = row < p.m;
    Stream<G, T, DC, BR> st;
-   st.set(lds, lds_ids, lds_bits, p, u, (const E *)p.k + kvh * p.hdk, p.ldk_bytes, (const E *)p.v + kvh * p.hdv, p.ldv_bytes);
+   st.set(lds, lds_ids, lds_bits, p, u, kvh);
 
    u4 qr[MAPS][G::CQ];
 #pragma unroll
@@ -461,7 +499,7 @@ template <int T, int DC, int MAPS, int BR> __global__ __launch_bounds__(BR * 4, 
       if constexpr (MAPS == 2) odd |= odd_sums(soft[1].acc);
       return odd;
    };
-   if (any_odd<BR>(p.full ? pass(Mode<kFull>()) : pass(Mode<kAny>()))) (void)pass(Mode<kCareful>());
+   if (any_odd<BR>(p.gat.full ? pass(Mode<kFull>()) : pass(Mode<kAny>()))) (void)pass(Mode<kCareful>());
 
 #pragma unroll
    for (int mp = 0; mp < MAPS; mp++) soft[mp].sum = group_sum(soft[mp].sum);
@@ -583,7 +621,7 @@ template <int T, int DC, int MAPS, int BR> __global__ __launch_bounds__(BR * 4, 
    const bool live = row < p.m;
    const int64_t srow = live ? row : 0;
    Stream<G, T, DC, BR> st;
-   st.set(lds, lds_ids, lds_bits, p, u, (const E *)p.k + kvh * p.hdk, p.ldk_bytes, (const E *)p.v + kvh * p.hdv, p.ldv_bytes);
+   st.set(lds, lds_ids, lds_bits, p, u, kvh);
 
    u4 qr[MAPS][G::CQ], gr[G::CV];
    float lse2[MAPS], delta[MAPS], sign[MAPS], mean[MAPS];
@@ -686,7 +724,7 @@ template <int T, int DC, int MAPS, int BR> __global__ __launch_bounds__(BR * 4, 
       }
       return odd;
    };
-   if (any_odd<BR>(p.full ? pass(Mode<kFull>()) : pass(Mode<kAny>()))) (void)pass(Mode<kCareful>());
+   if (any_odd<BR>(p.gat.full ? pass(Mode<kFull>()) : pass(Mode<kAny>()))) (void)pass(Mode<kCareful>());
 
 #pragma unroll
    for (int mp = 0; mp < MAPS; mp++) mean[mp] = group_sum(mean[mp]);
@@ -821,7 +859,7 @@ template <int T, int DC, int MAPS, int BR> __global__ __launch_bounds__(BR * 4, 
    const bool live = row < p.n;
    const int64_t srow = live ? row : 0;
    Stream<G, T, DC, BR> st;
-   st.set(lds, lds_ids, lds_bits, p, u, (const E *)p.q, p.ldq_bytes, (const E *)p.dout, p.ldo_bytes);
+   st.set(lds, lds_ids, lds_bits, p, u, 0);
 
    u4 kr[MAPS][G::CQ], vr[G::CV];
 #pragma unroll
@@ -833,7 +871,7 @@ template <int T, int DC, int MAPS, int BR> __global__ __launch_bounds__(BR * 4, 
 
    auto load = [&](int s, int buf, auto full) __attribute__((always_inline)) {
       const int t = s / p.group, head = kvh * p.group + s % p.group;
-      st.template load_tile<decltype(full)::value>(t, buf, head * p.hdq * (int64_t)sizeof(E), head * p.hdo * (int64_t)sizeof(E));
+      st.template load_tile<decltype(full)::value>(t, buf, head * p.gat.ha * (int64_t)sizeof(E), head * p.gat.hb * (int64_t)sizeof(E));
       // the statistics of the tile's rows: [32 rows][2 maps], 8 or 16 bytes of a row each
       if (tid < (MAPS == 2 ? 32 : 64))
       {
@@ -915,7 +953,7 @@ template <int T, int DC, int MAPS, int BR> __global__ __launch_bounds__(BR * 4, 
       for (int mp = 0; mp < MAPS; mp++) odd |= odd_sums(dk[mp]);
       return odd;
    };
-   if (any_odd<BR>(p.full ? pass(Mode<kFull>()) : pass(Mode<kAny>()))) (void)pass(Mode<kCareful>());
+   if (any_odd<BR>(p.gat.full ? pass(Mode<kFull>()) : pass(Mode<kAny>()))) (void)pass(Mode<kCareful>());
 
    constexpr float unscale = 1.0f / G::N::kPScale;
    if (u.part >= 0)

@@ -148,6 +148,13 @@ template <int DC, int MAPS> struct Rows4 {
 
 #if KERNEL == 0
 int NAMED(launch_forward)(const Params &p, int dc, int maps, hipStream_t s) { return choose<Forward>(dc, maps, p, s); }
+
+int NAMED(launch_pack)(const PackParams &p, hipStream_t s)
+{
+   hipLaunchKernelGGL((attn_pack<TYPE>), dim3((unsigned)(2 * (int64_t)p.heads * p.per_head)), dim3(256), 0, s, p);
+   ATTN_HIP(hipGetLastError());
+   return kOk;
+}
 #elif KERNEL == 1
 int NAMED(launch_dq)(const Params &p, int dc, int maps, hipStream_t s) { return choose<Dq>(dc, maps, p, s); }
 #elif KERNEL == 2
