@@ -29,6 +29,7 @@ static_assert(kF32 == FUSEDMM_TYPE_F32 && kF16 == FUSEDMM_TYPE_F16 && kBF16 == F
 
 constexpr int64_t kMaxGrid = ((int64_t)1 << 31) - 8;
 constexpr int64_t kMaxTokens = (int64_t)1 << 20;
+constexpr int64_t kMaxSlots = (int64_t)1 << 44;   // of a serving call
 
 int refuse(const char *who, const char *why)
 {
@@ -111,7 +112,7 @@ int check_plans(const char *who, const Desc &d, const void *plan, const void *pl
    if (p->rows != d.m || p->cols != d.n) return refuse(who, "the plan is of a pattern of another size");
    if (t && (t->rows != d.n || t->cols != d.m)) return refuse(who, "the second plan is not of the transposed pattern's size");
    if (t && t->device != p->device) return refuse(who, "the plans belong to different devices");
-   if ((int64_t)p->view.n_units * d.heads > kMaxGrid || (int64_t)p->view.n_joins * d.heads * (p->view.block_rows / 4) * 8 > kMaxGrid || d.m * d.heads > kMaxGrid ||
+   if ((int64_t)p->view.n_units * d.heads > kMaxGrid || d.n * d.kv_heads > (int64_t)1 << 40 || (int64_t)p->view.n_joins * d.heads * (p->view.block_rows / 4) * 8 > kMaxGrid || d.m * d.heads > kMaxGrid ||
        (t && ((int64_t)t->view.n_units * d.kv_heads > kMaxGrid || (int64_t)t->view.n_joins * d.kv_heads * (t->view.block_rows / 4) * 8 > kMaxGrid || t->tiles * (d.heads / d.kv_heads) > INT32_MAX)))
       return refuse(who, "too many rows and heads for one call");
    return kOk;
@@ -239,11 +240,12 @@ bool inputs_ok(const Desc &d)
 // tiles per wave), not over 8192.
 int64_t piece_slots(int64_t nnz, int64_t columns, bool kv4)
 {
-   const int64_t want = nnz * columns / (kv4 ? 768 : 1024);
+   const int64_t want = std::min<int64_t>(nnz, 8192 * 1024) * columns / (kv4 ? 768 : 1024);   // (longer lists reach 8192 anyhow)
    return (std::min<int64_t>(std::max<int64_t>(want, 256), 8192) + 127) / 128 * 128;
 }
 
 struct RowsPlan {
+   bool fits = false;   // in a launch, and its sizes in 64 bits
    int passes = 0;
    int64_t piece = 0, cap = 0, table = 0, total = 0;   // table: byte offset behind the partial sums
 };
@@ -254,9 +256,13 @@ RowsPlan rows_plan(const Desc &d, int64_t nnz, int dc, bool kv4)
    const int hp = 16 / d.maps, group = d.heads / d.kv_heads;
    r.passes = (group + hp - 1) / hp;
    const int64_t columns = (int64_t)d.kv_heads * r.passes;
+   if (columns > kMaxGrid || d.m > kMaxGrid || nnz > kMaxSlots) return r;
    r.piece = piece_slots(nnz, columns, kv4);
-   if (nnz <= r.piece || d.m == 0) return r;   // no row is cut
-   r.cap = nnz / r.piece + d.m;
+   const bool cut = nnz > r.piece && d.m > 0;
+   const int64_t most = (cut ? nnz / r.piece : 0) + d.m;
+   r.fits = most + 8 <= kMaxGrid / columns && (d.m == 0 || d.heads <= kMaxGrid / d.m);
+   if (!r.fits || !cut) return r;
+   r.cap = most;
    r.table = align256(r.cap * columns * 16 * (dc * d.maps + kPartExtra) * 4);
    r.total = r.table + (d.m > kTableRows ? (d.m + 2) * 8 : 0);
    return r;
@@ -274,7 +280,7 @@ int rows_common(const char *who, bool kv4, const Desc *d, int64_t nnz, const voi
    if (!inputs_ok(*d)) return refuse(who, "a stride is negative or too large");
    if (!apart(d->ldo, d->hdo, d->m, d->heads, d->dv)) return refuse(who, "the rows of o overlap");
    const RowsPlan r = rows_plan(*d, nnz, *dc, kv4);
-   if ((std::max<int64_t>(r.cap, d->m) + 8) * d->kv_heads * r.passes > kMaxGrid || d->m * d->heads > kMaxGrid) return refuse(who, "too many rows and heads for one call");
+   if (!r.fits) return refuse(who, "too many rows, slots and heads for one call");
    if (d->m == 0) return kOk;
    if (!q || !o || !pntrb || !pntre || (nnz > 0 && !indx) || (d->maps == 2 && !lambda)) return refuse(who, "a pointer is null");
    st = check_work(who, work, work_bytes, r.total);
@@ -283,7 +289,6 @@ int rows_common(const char *who, bool kv4, const Desc *d, int64_t nnz, const voi
    *p = RowsParams{};
    p->m = d->m;
    p->n = d->n;
-   p->nnz = nnz;
    p->heads = d->heads;
    p->kv_heads = d->kv_heads;
    p->group = d->heads / d->kv_heads;
@@ -362,7 +367,6 @@ int kv4_common(const char *who, const Desc *d, int64_t tokens, const void *slots
    p->kv_heads = d->kv_heads;
    p->k_width = d->maps * d->d;
    p->v_width = d->dv;
-   p->d = d->d;
    p->index_bytes = (int)sizeof(INDEXTYPE);
    p->slots = slots;
    p->ldk = d->ldk;
@@ -551,7 +555,13 @@ int64_t fusedMM_attn_rows_workspace(const fusedMM_attn_desc *desc, const INDEXTY
       (void)refuse(who, "negative nnz");
       return -1;
    }
-   return std::max(rows_plan(*desc, nnz, dc, false).total, rows_plan(*desc, nnz, dc, true).total);
+   const RowsPlan own = rows_plan(*desc, nnz, dc, false), four = rows_plan(*desc, nnz, dc, true);
+   if (!own.fits || !four.fits)
+   {
+      (void)refuse(who, "too many rows, slots and heads for one call");
+      return -1;
+   }
+   return std::max(own.total, four.total);
 }
 
 int fusedMM_attn_rows(const fusedMM_attn_desc *desc, const INDEXTYPE nnz, const INDEXTYPE *indx, const INDEXTYPE *pntrb, const INDEXTYPE *pntre, const void *q,

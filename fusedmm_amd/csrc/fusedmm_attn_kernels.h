@@ -1,4 +1,5 @@
-// Kernels of attention over a planned pattern: forward, delta, the two backward passes, and the joins of split blocks.
+// Kernels of attention over a planned pattern: forward, the two backward passes, the joins of split blocks, and the packing of
+// rows that are not whole chunks.
 //
 // A plan (fusedmm_attn_plan.hip) lists, for every block of BR = 64 or 16 rows, the columns that any of them names, with
 // one bit per row.  A unit is a run of such columns of one block; a block whose rows are long is several units, whose
@@ -32,7 +33,6 @@ struct PlanView {
    const Unit *units;
    const Join *joins;
    int32_t n_units, n_joins;
-   int64_t rows, cols_n;
    int32_t block_rows;     // BR
 };
 
@@ -414,7 +414,7 @@ template <class G, int BR, class S, class Load, class Use> __device__ __forceinl
 
 // ---- forward ----------------------------------------------------------------------------------------------------------------------
 // One pass over a unit's columns with a running maximum and sum of every row and map.  Scores are kept times log2(e).
-template <int T, int DC, int MAPS, int BR> __global__ __launch_bounds__(BR * 4, (DC * MAPS >= 256 ? 1 : 2)) void attn_forward(Params p)
+template <int T, int DC, int MAPS, int BR> __global__ __launch_bounds__(BR * 4, (DC * MAPS >= 256 || (BR == 16 && T == kF32 && DC * MAPS >= 128) ? 1 : 2)) void attn_forward(Params p)
 {
    typedef Geo<T, DC, MAPS, BR> G;
    typedef typename G::E E;

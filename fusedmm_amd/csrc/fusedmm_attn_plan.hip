@@ -378,7 +378,7 @@ int build(Plan *plan, int br, bool *shared, int64_t m, int64_t n, int64_t nnz, c
    }
    ATTN_HIP(hipStreamSynchronize(stream));
    plan->view = PlanView{(const int32_t *)base, (const uint32_t *)(base + off_masks), (const Unit *)(base + off_units),
-                         (const Join *)(base + off_joins), (int32_t)units.size(), (int32_t)joins.size(), m, n, br};
+                         (const Join *)(base + off_joins), (int32_t)units.size(), (int32_t)joins.size(), br};
    return kOk;
 }
 

@@ -12,7 +12,7 @@
 namespace fmm_attn {
 
 struct RowsParams {
-   int64_t m, n, nnz;
+   int64_t m, n;
    int32_t heads, kv_heads, group, d, dv;
    int32_t passes;                    // runs of 16 / maps query heads within a group
    float scale;
@@ -37,7 +37,6 @@ constexpr int kTableRows = 256;       // up to this many rows, every wave finds 
 struct Kv4Params {
    int64_t tokens, n;
    int32_t kv_heads, k_width, v_width;   // maps * d, dv
-   int32_t d;
    int32_t index_bytes;
    const void *slots;
    const void *k, *v;

@@ -308,7 +308,9 @@ int fusedMM_amd_last_row_order(int *scattered, unsigned int *edges_lower_half, u
 /* Sizes and layout.  Strides count elements: feature c of map p of head h of row i of q is
  * q[i * ldq + h * hdq + p * d + c]; k likewise with kv_heads heads, v and o with dv features and no maps.
  * Packed rows (ld the width of a packed row) and head-major tensors (hd = rows * width) are both described so.
- * heads is a multiple of kv_heads: query head h reads key head h / (heads / kv_heads). */
+ * heads is a multiple of kv_heads: query head h reads key head h / (heads / kv_heads).
+ * d and dv are at least 1, d <= 256 and dv <= 256 with one map, d <= 128 and dv <= 256 with two; ld under 2^29.  Any size
+ * and place is right; packed rows of multiples of 16 bytes on 16-byte addresses are fastest. */
 typedef struct fusedMM_attn_desc {
    int32_t type;               /* FUSEDMM_TYPE_* of q, k, v, o and their gradients */
    int32_t maps;               /* 1 or 2 */
@@ -320,10 +322,10 @@ typedef struct fusedMM_attn_desc {
 } fusedMM_attn_desc;
 
 /*
- * A plan of a pattern that is used many times (a training graph, a prompt's mask): for every block of 64 rows the
- * columns that any of them names, so that a gathered row is loaded once for all of them.  m, n <= 2^26 - 1; nnz at
- * least the sum of the row lengths.  Column ids in ascending order within the rows share best; any order is right.
- * The plan belongs to the current device, holds device memory (12 bytes per distinct (block, column)) and can be used
+ * A plan of a pattern that is used many times (a training graph, a prompt's mask): for every block of 64 rows (16, where
+ * rows share few columns) the columns that any of them names, so that a gathered row is loaded once for all of them.
+ * m, n <= 2^26 - 1; nnz at least the sum of the row lengths.  Column ids in ascending order within the rows share best; any order is right.
+ * The plan belongs to the current device, holds device memory (12 bytes, or 6, per distinct (block, column)) and can be used
  * for any head count, type and feature width.  Waits for the GPU; refused while `stream` is captured.
  * Destroying waits for the device's work and frees the memory; graphs that were captured with the plan end with it.
  */
@@ -332,7 +334,8 @@ int fusedMM_attn_plan_create(const INDEXTYPE m, const INDEXTYPE n, const INDEXTY
 int fusedMM_attn_plan_destroy(void *plan);
 
 /* Bytes of workspace (16-byte aligned) of a forward call, or, with the plan of the transposed pattern, of a forward and
- * of a backward call.  -1: the arguments do not fit together. */
+ * of a backward call: partial sums of long rows, row statistics, and, where sizes or strides keep rows off 16 bytes, room
+ * for the tensors whose rows are gathered.  -1: the arguments do not fit together. */
 int64_t fusedMM_attn_workspace(const fusedMM_attn_desc *desc, const void *plan, const void *plan_t);
 
 /* lambda: fp32 [heads], NULL with one map.  o2 and lse may be NULL where no backward pass follows: o2 (laid out as o)
@@ -374,7 +377,7 @@ int64_t fusedMM_kv4_record_bytes(const int maps, const int d, const int dv);
 
 /* Token t of k and v (ldk, hdk, ldv, hdv and the sizes from desc; m, heads and the other strides are not read) goes to
  * slot slots[t]; tokens whose slot is outside [0, desc->n) are skipped.  Of tokens with the same slot the last one
- * counts.  At most 2^20 tokens.  Bytes of a record behind the last word are left as they are. */
+ * counts.  At most 2^20 tokens, desc->n <= 2^31 - 1.  Bytes of a record behind the last word are left as they are. */
 int fusedMM_kv4_write(const fusedMM_attn_desc *desc, const INDEXTYPE tokens, const INDEXTYPE *slots, const void *k, const void *v,
                       void *cache, int64_t ldc, int64_t hdc, void *stream);
 /* The values of the records of slots[0 .. tokens) in desc->type; slots outside [0, desc->n) read as zeros. */

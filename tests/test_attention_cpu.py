@@ -175,3 +175,24 @@ def test_reference_against_a_loop():
                     o += sign * sum(x * v[c, 0] for x, c in zip(w / w.sum(), cols))
                     assert abs(np.log(w.sum()) - e["lse"][i, h, p]) < 1e-12
             assert np.abs(o - e["o"][i, h]).max() < 1e-12
+
+
+@pytest.mark.parametrize("bits,nnz,change", [
+    (64, 2 ** 62, {}), (64, 2 ** 44, {}), (64, 100, dict(m=2 ** 62)), (64, 100, dict(m=2 ** 20, heads=2 ** 20, ldo=2 ** 26)),
+    (32, 100, dict(m=1, heads=2 ** 31 - 1, kv_heads=2 ** 31 - 1)), (64, 2 ** 40, dict(m=1, heads=2 ** 20, kv_heads=2 ** 20))])
+def test_rows_refuse_sizes_beyond_a_launch(capfd, bits, nnz, change):
+    """No product of sizes wraps round into a small workspace."""
+    d = desc(**change)
+    assert fa.fusedMM_attn_rows_workspace(d, nnz, index_bits=bits) == -1
+    assert "too many rows, slots and heads" in capfd.readouterr().err
+    assert rows(d, nnz=nnz, work=16, size=2 ** 62, index_bits=bits) == fa.FAIL
+    assert "too many rows, slots and heads" in capfd.readouterr().err
+
+
+@pytest.mark.parametrize("n", [2 ** 31, 2 ** 40])
+def test_the_cache_refuses_slots_beyond_32_bits(capfd, n):
+    d = desc(n=n)
+    for call in (lambda: fa.fusedMM_kv4_write(d, 1, 16, 16, 16, 16, 160, 80, stream=0, index_bits=64),
+                 lambda: fa.fusedMM_kv4_read(d, 1, 16, 16, 160, 80, 16, 16, stream=0, index_bits=64)):
+        assert call() == fa.FAIL
+        assert "2^31 - 1" in capfd.readouterr().err
