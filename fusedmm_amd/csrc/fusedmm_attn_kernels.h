@@ -222,7 +222,7 @@ template <class G, int T, int DC, int BR> struct Stream {
       }
    }
 
-   // any sizes and places
+   // any sizes
    __device__ __forceinline__ void load_any(int t, int buf, int64_t oa, int64_t ob) const
    {
       const int32_t *c = tile_ids(t);
@@ -244,16 +244,8 @@ template <class G, int T, int DC, int BR> struct Stream {
          load_lds16(lb + j * (G::THREADS * 16), e < dv ? (const void *)fb : (const void *)&zero_chunk);
       }
       if (vec) return;
-      if (d >= G::N::EPL && dv >= G::N::EPL) load_parts<kShifted>(c, ta, tb, oa, ob);
-      else load_parts<kElements>(c, ta, tb, oa, ob);
-   }
-
-   // rows at any place: through registers, a few chunks at a time
-   template <int MODE> __device__ __forceinline__ void load_parts(const int32_t *c, unsigned char *ta, unsigned char *tb, int64_t oa, int64_t ob) const
-   {
-      constexpr int B = MODE == kElements ? 1 : G::NCH < 4 ? G::NCH : 4;
-      int me = tid;
-      asm volatile("" : "+v"(me));
+      // a tensor that begins off 16 bytes (other rows off them are packed): through registers, a few chunks at a time
+      constexpr int B = G::NCH < 4 ? G::NCH : 4;
 #pragma unroll
       for (int j0 = 0; j0 < G::NCH; j0 += B)
       {
@@ -265,8 +257,8 @@ template <class G, int T, int DC, int BR> struct Stream {
             const bool live = kTile * G::CR >= G::THREADS || x < kTile * G::CR;
             const uint32_t col = (uint32_t)c[live ? r : 0];
             const int e = ((x % G::CR) ^ V::twist(r)) * G::N::EPL, f = e % DC;
-            ra[j] = load_part<T, MODE>((const E *)(a + oa + (uint64_t)col * lda) + e / DC * d, f, d, live);
-            rb[j] = load_part<T, MODE>((const E *)(b + ob + (uint64_t)col * ldb), e, dv, live);
+            ra[j] = load_part<T, kShifted>((const E *)(a + oa + (uint64_t)col * lda) + e / DC * d, f, d, live);
+            rb[j] = load_part<T, kShifted>((const E *)(b + ob + (uint64_t)col * ldb), e, dv, live);
          }
 #pragma unroll
          for (int j = 0; j < B; j++)

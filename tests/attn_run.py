@@ -14,8 +14,8 @@ def dtype(kind):
 
 
 def layout(rows, heads, width, how):
-    """(ld, hd, elements, offset): packed rows, head-major, packed rows inside wider ones (16-byte aligned), or rows and
-    heads at odd places."""
+    """(ld, hd, elements, offset): packed rows, head-major, packed rows inside wider ones (16-byte aligned), the same from an
+    address off 16 bytes, or rows and heads at odd places."""
     if how == "packed":
         return heads * width, width, rows * heads * width, 0
     if how == "heads":
@@ -23,6 +23,9 @@ def layout(rows, heads, width, how):
     if how == "wide":
         ld = heads * width + (-(heads * width)) % 8 + 16
         return ld, width, rows * ld + 8, 8
+    if how == "off":     # strides of whole 16-byte chunks, for widths that are, behind an address that is not
+        ld = heads * width + 8
+        return ld, width, rows * ld + 1, 1
     ld = heads * (width + 3) + 5
     return ld, width + 3, rows * ld + 1, 1
 

@@ -56,6 +56,45 @@ def test_blocks_of_64_and_of_16_rows(kind, d, dv, maps, pattern):
     run_both(Case(kind, maps, m, n, 3, 3, d, dv, indx, pb, pe, seed=d + dv))
 
 
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("d,dv,maps", [(32, 32, 1), (64, 64, 1), (128, 128, 1), (64, 128, 2), (40, 24, 1), (8, 16, 2)])
+@pytest.mark.parametrize("pattern", ["shared", "apart"])
+def test_tensors_that_begin_off_16_bytes(kind, d, dv, maps, pattern):
+    import torch
+    m, n = 70, 1300
+    if pattern == "shared":
+        indx, pb, pe = window_pattern(m, n, 70)
+    else:
+        indx, pb, pe = np.random.default_rng(d).permutation(n)[:m * 18].astype(np.int64), np.arange(m) * 18, np.arange(m) * 18 + 18
+    c = Case(kind, maps, m, n, 4, 2, d, dv, indx, pb, pe, seed=d + dv, how="off")
+    run_both(c, "off")
+    assert c.rows() == 0
+    torch.cuda.synchronize()
+    check_rows(c, c.exact())
+
+
+def test_odd_sizes_are_captured_and_replayed():
+    """Rows that are laid out anew within the call: the graph does so at every replay."""
+    import torch
+    c = Case("bf16", 2, 90, 120, 4, 2, 21, 37, *random_pattern(90, 120, 30, seed=1), seed=2)
+    c.make_plans(True)
+    c.gradients()
+    torch.cuda.synchronize()
+    s, g = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        assert c.forward(stream=s.cuda_stream) == 0 and c.backward(stream=s.cuda_stream) == 0
+    for _ in range(3):
+        for t in (c.q, c.k, c.v, c.do):
+            t.view().copy_(torch.randn(t.view().shape, device="cuda"))
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        e = c.exact(do=True)
+        check_forward(c, e)
+        check_backward(c, e)
+        float(torch.randn(1000, device="cuda").sum())
+
+
 def far(t, ld):
     """The tensor's values in rows `ld` elements apart."""
     import torch
