@@ -1,0 +1,43 @@
+"""Sixteen-bit attention where its roundings count: bounds without a rounding of the weights and without one of the row means
+(tests/attn_tight.py), weights far below the largest, score gradients outside fp16's range, large lambdas."""
+import numpy as np
+import pytest
+
+import fusedmm_amd as fa
+from attn_run import Case, random_pattern, transposed, window_pattern
+from attn_tight import tight
+from test_gpu_attention import check_backward, check_forward
+from test_gpu_attention_rows import CacheCase, check_rows, ragged
+
+pytestmark = pytest.mark.gpu
+
+
+def both(c):
+    import torch
+    c.make_plans(True)
+    c.gradients()
+    assert c.forward() == 0 and c.backward() == 0
+    torch.cuda.synchronize()
+    e = tight(c, do=True)
+    check_forward(c, e)
+    check_backward(c, e)
+    return e
+
+
+def cached(c):
+    return tight(c, k=c.k_values, v=c.v_values, weight_type="f16")
+
+
+# ---- rows over a 4-bit cache -----------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("heads,kv,d,dv,maps", [(8, 2, 32, 32, 1), (2, 1, 64, 96, 1), (4, 2, 32, 64, 2), (20, 1, 64, 128, 2), (3, 3, 128, 128, 1)])
+def test_rows_over_the_cache_round_weights_twice(kind, heads, kv, d, dv, maps):
+    import torch
+    lengths = [1, 40, 700, 0, 1500]
+    c = CacheCase(kind, maps, 5, 1600, heads, kv, d, dv, *ragged(lengths, 1600, seed=1), seed=2)
+    e = cached(c)
+    for nnz in (256, c.nnz):
+        assert c.rows(nnz=nnz) == 0
+        torch.cuda.synchronize()
+        check_rows(c, e)
