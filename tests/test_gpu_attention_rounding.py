@@ -41,3 +41,23 @@ def test_rows_over_the_cache_round_weights_twice(kind, heads, kv, d, dv, maps):
         assert c.rows(nnz=nnz) == 0
         torch.cuda.synchronize()
         check_rows(c, e)
+
+
+# ---- the second rounding and the exact mean --------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("kind", ["bf16"])
+@pytest.mark.parametrize("pattern", ["shared", "apart", "long"])
+@pytest.mark.parametrize("d,dv,maps", [(32, 32, 1), (40, 24, 1), (64, 128, 2), (128, 128, 1), (16, 32, 2), (128, 256, 2)])
+def test_weights_and_gradients_are_rounded_twice(kind, pattern, d, dv, maps):
+    import torch
+    if pattern == "shared":
+        m, n, index = 100, 160, window_pattern(100, 160, 60)
+    elif pattern == "apart":
+        m, n, index = 90, 300, random_pattern(90, 300, 9, seed=2)
+    else:
+        m, n, index = 66, 1100, random_pattern(66, 1100, 9, seed=2, hub=2600)
+    c = Case(kind, maps, m, n, 4, 2, d, dv, *index, seed=d + dv, spread=1.5)
+    e = both(c)
+    assert c.rows() == 0
+    torch.cuda.synchronize()
+    check_rows(c, e)
