@@ -61,8 +61,8 @@ template <> struct Num<kF16> {
    typedef uint16_t E;
    static constexpr int KC = 32, EPL = 8;
    typedef s8 TFrag;
-   // weights of long rows are small: 2^10 keeps them clear of fp16's subnormals (they are at most 1 + |lambda|)
-   static constexpr float kPScale = 1024.0f;
+   // softmax weights of long rows are small: 2^14 keeps them clear of fp16's subnormals (they are at most 1)
+   static constexpr float kPScale = 16384.0f;
    static __device__ inline f4 mma(u4 a, u4 b, f4 c)
    {
       return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
@@ -396,6 +396,45 @@ __device__ inline float group_sum(float x)
 
 // what stands behind this in a branch is not done without it (the compiler would rather select than branch)
 __device__ inline void keep_branch() { asm volatile(""); }
+
+// Sums of weights that have no bound of their own, P1 - lambda P2 or the scores' gradients P (dP - delta): in fp16 they enter the
+// product times 2^up, which follows the largest one of the resident row so far down, 2^14 at most after each step: none of
+// them overflows, and what fp16's smallest step takes is 2^-38 of the largest.  Other types have fp32's range.
+template <int T> struct Range {
+   int up = 100;
+   template <int NT> __device__ inline void fit(float (&w)[2][4], f4 (&acc)[NT])
+   {
+      if constexpr (T == kF16)
+      {
+         float top = 0;
+#pragma unroll
+         for (int j = 0; j < 8; j++) top = fmaxf(top, fabsf(w[j / 4][j % 4]));
+         top = group_max(top);
+         const bool over = ldexpf(top, up) > 32768.0f && top < INFINITY;   // (an infinite weight stays one)
+         if (__any(over))
+         {
+            const int to = over ? 14 - __builtin_amdgcn_frexp_expf(top) : up;
+#pragma unroll
+            for (int t = 0; t < NT; t++)
+#pragma unroll
+               for (int e = 0; e < 4; e++) acc[t][e] = ldexpf(acc[t][e], to - up);
+            up = to;
+         }
+#pragma unroll
+         for (int j = 0; j < 8; j++) w[j / 4][j % 4] = ldexpf(w[j / 4][j % 4], up);
+      }
+   }
+   template <int NT> __device__ inline void undo(f4 (&acc)[NT]) const
+   {
+      if constexpr (T == kF16)
+      {
+#pragma unroll
+         for (int t = 0; t < NT; t++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) acc[t][e] = ldexpf(acc[t][e], -up);
+      }
+   }
+};
 
 // scores whose bit of `mine` is clear -> `other`
 __device__ inline float masked(float x, unsigned mine, int j, float other)

@@ -644,12 +644,14 @@ template <int T, int DC, int MAPS, int BR> __global__ __launch_bounds__(BR * 4, 
 
    const float c2 = p.scale * kLog2e;
    f4 acc[MAPS][G::NTQ], pk[kMend ? MAPS : 1][kMend ? G::NTQ : 1];
+   Range<T> range[MAPS];
    auto pass = [&](auto mode) {
       constexpr bool CAREFUL = decltype(mode)::value == kCareful, FULL = decltype(mode)::value == kFull;
 #pragma unroll
       for (int mp = 0; mp < MAPS; mp++)
       {
          mean[mp] = 0;
+         range[mp] = Range<T>();
 #pragma unroll
          for (int t = 0; t < G::NTQ; t++)
          {
@@ -693,7 +695,9 @@ template <int T, int DC, int MAPS, int BR> __global__ __launch_bounds__(BR * 4, 
                {
                   w[j / 4][j % 4] = pr[j / 4][j % 4] * (dp[j / 4][j % 4] - delta[mp]);   // sign: at the end
                   mean[mp] = fmaf(pr[j / 4][j % 4], dp[j / 4][j % 4], mean[mp]);
+                  if constexpr (G::N::kPScale != 1.0f) pr[j / 4][j % 4] *= G::N::kPScale;
                }
+               range[mp].fit(w, acc[mp]);
                if constexpr (CAREFUL)
                {
                   add_weighted<T, G::W, true, kMend>(acc[mp], w, mine, ks, mp * DC, g, i, l);
@@ -732,7 +736,16 @@ template <int T, int DC, int MAPS, int BR> __global__ __launch_bounds__(BR * 4, 
    if (any_odd<BR>(p.gat.full ? pass(Mode<kFull>()) : pass(Mode<kAny>()))) (void)pass(Mode<kCareful>());
 
 #pragma unroll
-   for (int mp = 0; mp < MAPS; mp++) mean[mp] = group_sum(mean[mp]);
+   for (int mp = 0; mp < MAPS; mp++)
+   {
+      mean[mp] = group_sum(mean[mp]);
+      range[mp].undo(acc[mp]);
+      if constexpr (G::N::kPScale != 1.0f)
+      {
+#pragma unroll
+         for (int t = 0; t < G::NTQ; t++) pk[mp][t] *= 1.0f / G::N::kPScale;
+      }
+   }
    if constexpr (MAPS == 2)
    {
       // (a row behind the last one names nothing: its mean is zero; the units of a split block add up)
@@ -873,6 +886,7 @@ template <int T, int DC, int MAPS, int BR> __global__ __launch_bounds__(BR * 4, 
    load_resident<T, G::CV>(vr, (const E *)p.v + srow * p.ldv + kvh * p.hdv, live, p.dv, g, p.vec);
    const float c2 = p.scale * kLog2e;
    f4 dk[MAPS][G::NTQ], dv[G::NT];
+   Range<T> range_k[MAPS], range_v;
 
    auto load = [&](int s, int buf, auto full) __attribute__((always_inline)) {
       const int t = s / p.group, head = kvh * p.group + s % p.group;
@@ -932,13 +946,10 @@ template <int T, int DC, int MAPS, int BR> __global__ __launch_bounds__(BR * 4, 
 #pragma unroll
             for (int j = 0; j < 8; j++) w[j / 4][j % 4] = masked(w[j / 4][j % 4], mine, j, 0.0f);
          }
+         range_k[mp].fit(w, dk[mp]);
          add_weighted<T, G::W, CAREFUL, T != kF32>(dk[mp], w, mine, qs, mp * DC, g, i, l);
       }
-      if constexpr (G::N::kPScale != 1.0f)
-      {
-#pragma unroll
-         for (int j = 0; j < 8; j++) wv[j / 4][j % 4] *= G::N::kPScale;
-      }
+      range_v.fit(wv, dv);
       add_weighted<T, G::W, CAREFUL, T != kF32>(dv, wv, mine, gs, 0, g, i, l);
    };
    auto pass = [&](auto mode) {
@@ -947,6 +958,9 @@ template <int T, int DC, int MAPS, int BR> __global__ __launch_bounds__(BR * 4, 
       for (int mp = 0; mp < MAPS; mp++)
 #pragma unroll
          for (int t = 0; t < G::NTQ; t++) dk[mp][t] = f4{0, 0, 0, 0};
+#pragma unroll
+      for (int mp = 0; mp < MAPS; mp++) range_k[mp] = Range<T>();
+      range_v = Range<T>();
 #pragma unroll
       for (int t = 0; t < G::NT; t++) dv[t] = f4{0, 0, 0, 0};
       // (steps of one tile, the heads of the group, follow each other: tiles * group < 2^31 is checked by the host)
@@ -960,7 +974,9 @@ template <int T, int DC, int MAPS, int BR> __global__ __launch_bounds__(BR * 4, 
    };
    if (any_odd<BR>(p.gat.full ? pass(Mode<kFull>()) : pass(Mode<kAny>()))) (void)pass(Mode<kCareful>());
 
-   constexpr float unscale = 1.0f / G::N::kPScale;
+#pragma unroll
+   for (int mp = 0; mp < MAPS; mp++) range_k[mp].undo(dk[mp]);
+   range_v.undo(dv);
    if (u.part >= 0)
    {
       // [part][kv head][BR rows][2 W]
@@ -974,7 +990,7 @@ template <int T, int DC, int MAPS, int BR> __global__ __launch_bounds__(BR * 4, 
 #pragma unroll
       for (int x = 0; x < G::NT; x++)
 #pragma unroll
-         for (int e = 0; e < 4; e++) r[G::W + 16 * x + 4 * g + e] = dv[x][e] * unscale;
+         for (int e = 0; e < 4; e++) r[G::W + 16 * x + 4 * g + e] = dv[x][e];
       return;
    }
    if (!live) return;
@@ -985,7 +1001,7 @@ template <int T, int DC, int MAPS, int BR> __global__ __launch_bounds__(BR * 4, 
 #pragma unroll
       for (int x = 0; x < G::NTQ; x++) store4<T>(outk + mp * p.d, 16 * x + 4 * g, p.d, dk[mp][x] * p.scale, p.vec);
 #pragma unroll
-   for (int x = 0; x < G::NT; x++) store4<T>(outv, 16 * x + 4 * g, p.dv, dv[x] * unscale, p.vec);
+   for (int x = 0; x < G::NT; x++) store4<T>(outv, 16 * x + 4 * g, p.dv, dv[x], p.vec);
 }
 
 template <int T, int DC, int MAPS> __global__ __launch_bounds__(256) void attn_dkv_join(Params p)

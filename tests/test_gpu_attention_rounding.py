@@ -43,9 +43,68 @@ def test_rows_over_the_cache_round_weights_twice(kind, heads, kv, d, dv, maps):
         check_rows(c, e)
 
 
+# ---- lambda ----------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("pattern", ["shared", "apart"])
+def test_large_lambdas(kind, pattern):
+    """P1 - lambda P2 of some hundreds is an ordinary weight."""
+    import torch
+    m, n = 90, 120
+    if pattern == "shared":
+        index = window_pattern(m, n, 20)
+    else:
+        index = random_pattern(m, n, 6, seed=3)
+    c = Case(kind, 2, m, n, 4, 2, 32, 64, *index, seed=4)
+    c.lam = torch.tensor([100.0, -300.0, 1000.0, 0.0], device="cuda")
+    c.do.view().mul_(0.125)
+    e = both(c)
+    assert np.abs(e["dv"]).max() > 64 and np.abs(e["o"]).max() < 65504
+
+
+# ---- score gradients -------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("maps", [1, 2])
+@pytest.mark.parametrize("turned", [False, True])
+def test_small_gradients_over_long_rows(maps, turned):
+    """Output gradients of 1e-4 over rows of 4096 columns (and over columns of 4096 rows): each score's gradient is a few of fp16's
+    smallest steps, their sums are not."""
+    m, n = 66, 4096
+    indx, pb, pe = np.tile(np.arange(n), m), np.arange(m) * n, (np.arange(m) + 1) * n
+    if turned:
+        (indx, pb, pe), m, n = transposed(m, n, indx, pb, pe), n, m
+    c = Case("f16", maps, m, n, 2, 1, 32, 32 * maps, indx, pb, pe, seed=1, scale=1.0)
+    c.k.view().mul_(4.0)
+    c.q.view().mul_(0.125)
+    c.do.view().mul_(1e-4 * (4096 / 66 if turned else 1))
+    both(c)
+
+
+def test_large_gradients():
+    """Score gradients beyond 65504 whose products with the scale are ordinary numbers."""
+    c = Case("f16", 1, 80, 300, 4, 2, 32, 64, *random_pattern(80, 300, 4, seed=5, duplicates=False), seed=5, scale=1 / 64)
+    c.v.view().mul_(8.0)
+    c.do.view().mul_(3e3)
+    e = both(c)
+    dP = np.einsum("mhf,nhf->mhn", c.do.numpy(), np.repeat(c.v.numpy(), 2, axis=1))
+    assert np.abs(dP).max() > 3 * 65504 and all(np.abs(e[x]).max() < 65504 for x in ("dq", "dk", "dv"))
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+def test_gradients_of_mixed_sizes(kind):
+    """Rows' gradients from 1e-30 (fp16: 1e-7) to 1e3 next to each other, in one block and under one key: the running range follows."""
+    rng = np.random.default_rng(0)
+    c = Case(kind, 2, 130, 200, 4, 2, 32, 64, *random_pattern(130, 200, 30, seed=7), seed=7)
+    import torch
+    size = 10.0 ** rng.uniform(-7 if kind == "f16" else -30, 3, (130, 1, 1))
+    size[::9] = 0.0
+    c.do.view().mul_(torch.as_tensor(size).to(c.do.buf).to("cuda"))
+    both(c)
+
+
 # ---- the second rounding and the exact mean --------------------------------------------------------------------------------
 
-@pytest.mark.parametrize("kind", ["bf16"])
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
 @pytest.mark.parametrize("pattern", ["shared", "apart", "long"])
 @pytest.mark.parametrize("d,dv,maps", [(32, 32, 1), (40, 24, 1), (64, 128, 2), (128, 128, 1), (16, 32, 2), (128, 256, 2)])
 def test_weights_and_gradients_are_rounded_twice(kind, pattern, d, dv, maps):
