@@ -41,6 +41,7 @@ template <> struct Num<kBF16> {
    static constexpr int KC = 32, EPL = 8;
    typedef s8 TFrag;
    static constexpr float kPScale = 1.0f;
+   static constexpr int kLift = 0;
    static __device__ inline f4 mma(u4 a, u4 b, f4 c)
    {
       return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
@@ -63,6 +64,7 @@ template <> struct Num<kF16> {
    typedef s8 TFrag;
    // softmax weights of long rows are small: 2^14 keeps them clear of fp16's subnormals (they are at most 1)
    static constexpr float kPScale = 16384.0f;
+   static constexpr int kLift = 7;
    static __device__ inline f4 mma(u4 a, u4 b, f4 c)
    {
       return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
@@ -84,6 +86,7 @@ template <> struct Num<kF32> {
    static constexpr int KC = 16, EPL = 4;
    typedef f8 TFrag;
    static constexpr float kPScale = 1.0f;
+   static constexpr int kLift = 0;
    static __device__ inline f4 mma(u4 a, u4 b, f4 c)
    {
       const f4 x = __builtin_bit_cast(f4, a), y = __builtin_bit_cast(f4, b);
@@ -452,10 +455,11 @@ template <int T> __device__ inline u4 negated(u4 v)
    return u4{v[0] ^ m, v[1] ^ m, v[2] ^ m, v[3] ^ m};
 }
 
-// Running softmax of one resident row per lane.  The sums are relative to 2^base; base follows the largest score only when
-// that runs ahead by more than 2^8, so that most tiles rescale nothing: weights are then at most 256, and one of them
-// was 1 when base was set.
-template <int NT> struct Softmax {
+// Running softmax of one resident row per lane.  The sums are relative to 2^(base - LIFT); base follows the largest score only
+// when that runs ahead by more than 2^8, so that most tiles rescale nothing: weights are then at most 2^(8 + LIFT), and one of
+// them was 2^LIFT when base was set.  LIFT is 7 where the weights become fp16: they use its range up to 2^15, and vanish below
+// 2^-32 of the largest instead of 2^-25 - 2^18 slots at 2^-25 of a dominant one are 0.8 % of the row, which their sum has.
+template <int NT, int LIFT> struct Softmax {
    f4 acc[NT];
    float base, sum;
    __device__ inline void clear()
@@ -480,7 +484,7 @@ template <int NT> struct Softmax {
          sum *= keep;
          base = to;
       }
-      const float from = base == -INFINITY ? 0.0f : base;   // nothing named so far: every weight is exp2(-infinity)
+      const float from = base == -INFINITY ? 0.0f : base - LIFT;   // nothing named so far: every weight is exp2(-infinity)
 #pragma unroll
       for (int j = 0; j < 8; j++)
       {

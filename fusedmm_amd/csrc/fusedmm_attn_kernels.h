@@ -434,7 +434,7 @@ template <int T, int DC, int MAPS, int BR> __global__ __launch_bounds__(BR * 4, 
 #pragma unroll
          for (int c = 0; c < G::CQ; c++) qr[mp][c] = negated<T>(qr[mp][c]);
    }
-   Softmax<G::NT> soft[MAPS];
+   Softmax<G::NT, G::N::kLift> soft[MAPS];
    auto pass = [&](auto mode) {
       constexpr bool CAREFUL = decltype(mode)::value == kCareful, FULL = decltype(mode)::value == kFull;
 #pragma unroll
@@ -522,7 +522,7 @@ template <int T, int DC, int MAPS, int BR> __global__ __launch_bounds__(BR * 4, 
    for (int mp = 0; mp < MAPS; mp++)
    {
       inv[mp] = soft[mp].sum == 0.0f ? 0.0f : 1.0f / soft[mp].sum;   // a row without edges is zero
-      if (p.lse && g == 0) p.lse[(row * p.heads + head) * MAPS + mp] = soft[mp].sum == 0.0f ? -INFINITY : (soft[mp].base + log2f(soft[mp].sum)) * kLn2;
+      if (p.lse && g == 0) p.lse[(row * p.heads + head) * MAPS + mp] = soft[mp].sum == 0.0f ? -INFINITY : (soft[mp].base - G::N::kLift + log2f(soft[mp].sum)) * kLn2;
    }
    E *out = (E *)p.out + row * p.ldo + head * p.hdo;
    E *out2 = MAPS == 2 && p.out2 ? (E *)p.out2 + row * p.ldo + head * p.hdo : nullptr;
@@ -578,7 +578,7 @@ template <int T, int DC, int MAPS> __global__ __launch_bounds__(256) void attn_f
          if (live) x += s[f] * keep;
       }
       o[mp] = sum == 0.0f ? 0.0f : x / sum;
-      if (p.lse && lane == 0 && piece == 0) p.lse[(row * p.heads + head) * MAPS + mp] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
+      if (p.lse && lane == 0 && piece == 0) p.lse[(row * p.heads + head) * MAPS + mp] = sum == 0.0f ? -INFINITY : (top - Num<T>::kLift + log2f(sum)) * kLn2;
    }
    if (f >= p.dv) return;
    const int64_t at = row * p.ldo + head * p.hdo + f;

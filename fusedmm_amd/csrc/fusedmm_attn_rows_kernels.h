@@ -227,7 +227,7 @@ __device__ inline void wave_lds_order()   // this wave's LDS writes before its l
 
 // products of 32 slots with the columns -> weights, and the weighted values
 template <class G, int T, bool CAREFUL, bool TWICE>
-__device__ inline void row_step(Softmax<G::NT> &r, f4 (&sc)[2], float c2, unsigned mine, bool all, const unsigned char *vs, int g, int i)
+__device__ inline void row_step(Softmax<G::NT, G::N::kLift> &r, f4 (&sc)[2], float c2, unsigned mine, bool all, const unsigned char *vs, int g, int i)
 {
    if (!all)
    {
@@ -242,7 +242,7 @@ __device__ inline void row_step(Softmax<G::NT> &r, f4 (&sc)[2], float c2, unsign
 
 // The four waves' sums -> the row's output, or its piece of the partial sums.  O: element type of the output.
 template <class G, int MAPS, int O>
-__device__ inline void rows_finish(const RowsParams &p, Softmax<G::NT> &r, unsigned char *vs_all, float (*stat)[16][2], const Spot &s, int64_t id, int kvh, int pass)
+__device__ inline void rows_finish(const RowsParams &p, Softmax<G::NT, G::N::kLift> &r, unsigned char *vs_all, float (*stat)[16][2], const Spot &s, int64_t id, int kvh, int pass)
 {
    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, g = lane >> 4, i = lane & 15;
    r.sum = group_sum(r.sum);
@@ -491,7 +491,7 @@ __global__ __launch_bounds__(256, (sizeof(typename Num<T>::E) * DC * MAPS >= 512
 #pragma unroll
       for (int c = 0; c < G::CQ; c++) q[c] = negated<T>(q[c]);
    }
-   Softmax<G::NT> r;
+   Softmax<G::NT, G::N::kLift> r;
    const float c2 = score_factor(p.scale);
 
    u4 kf[2][MAPS][G::CQ], vf[G::NV];
@@ -719,7 +719,7 @@ __global__ __launch_bounds__(256, (DC * MAPS >= 256 ? 1 : DC * MAPS == 128 && FU
    }
    const float c2 = score_factor(ldexpf(p.scale, ex));
 
-   Softmax<G::NT> r;
+   Softmax<G::NT, G::N::kLift> r;
 
    typedef Record4<DC, MAPS, FULL> Rec;
    auto load = [&](Rec (&to)[2], int32_t slot) __attribute__((always_inline)) {

@@ -102,6 +102,73 @@ def test_gradients_of_mixed_sizes(kind):
     both(c)
 
 
+# ---- weights far below the largest -----------------------------------------------------------------------------------------
+
+def sink(c, depth, value):
+    """Slot 0 scores `depth` log2 units above all others, and its value is zero; the others' values are `value`."""
+    c.q.view().zero_()
+    c.k.view().zero_()
+    c.v.view().fill_(value)
+    c.q.view()[..., 0] = 1.0
+    c.k.view()[0, :, 0] = depth
+    c.v.view()[0] = 0.0
+    if c.maps == 2:
+        c.q.view()[..., c.d] = 1.0
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("maps", [1, 2])
+def test_a_sink_leaves_the_others_their_mass(kind, maps):
+    """One dominant key whose value is zero above 70000 others, each 2^-25.5 of it: the output is their mass."""
+    import torch
+    n = 70000
+    index = (np.tile(np.arange(n), 2), np.array([0, n]), np.array([n, 2 * n]))
+    c = Case(kind, maps, 2, n, 2, 1, 32, 32 * maps, *index, seed=1, scale=float(np.log(2)))
+    sink(c, 25.5, 4.0)
+    e = tight(c)
+    mass = (n - 1) * 2.0 ** -25.5 / (1 + (n - 1) * 2.0 ** -25.5)
+    if maps == 1:
+        assert np.allclose(e["o"], 4 * mass, rtol=1e-6)
+    c.make_plans(False)
+    assert c.forward() == 0
+    torch.cuda.synchronize()
+    check_forward(c, e)
+    for nnz in (100, c.nnz):
+        c.o.view().zero_()
+        assert c.rows(nnz=nnz) == 0
+        torch.cuda.synchronize()
+        check_rows(c, e)
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+def test_a_sink_in_a_cache(kind):
+    import torch
+    n = 60000
+    index = (np.tile(np.arange(n), 2), np.array([0, n]), np.array([n, 2 * n]))
+
+
+    c = Case(kind, 1, 2, n, 2, 1, 32, 32, *index, seed=1, scale=float(np.log(2)))
+    sink(c, 25.5, 4.0)
+    rec = fa.fusedMM_kv4_record_bytes(1, 32, 32)
+    cache = torch.zeros(n * rec, dtype=torch.uint8, device="cuda")
+    every = torch.arange(n, dtype=torch.int32, device="cuda")
+    assert fa.fusedMM_kv4_write(c.desc, n, every, c.k.ptr, c.v.ptr, cache, rec, rec) == 0
+    kx, vx = torch.empty((n, 1, 32), dtype=torch.float32, device="cuda"), torch.empty((n, 1, 32), dtype=torch.float32, device="cuda")
+    c.desc.type = fa.TYPE_F32
+    assert fa.fusedMM_kv4_read(c.desc, n, every, cache, rec, rec, kx, vx) == 0
+    c.desc.type = fa.TYPES[kind]
+    torch.cuda.synchronize()
+    e = tight(c, k=kx.double().cpu().numpy(), v=vx.double().cpu().numpy(), weight_type="f16")
+    assert e["o"].min() > 1e-3
+    for nnz in (100, c.nnz):
+        size = fa.fusedMM_attn_rows_workspace(c.desc, nnz)
+        work = torch.empty(max(size, 16), dtype=torch.uint8, device="cuda")
+        c.o.view().zero_()
+        assert fa.fusedMM_attn_rows_kv4(c.desc, nnz, *c.index, c.q.ptr, cache, rec, rec, None, c.o.ptr, work, size) == 0
+        torch.cuda.synchronize()
+        check_rows(c, e)
+
+
 # ---- the second rounding and the exact mean --------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("kind", ["f16", "bf16"])
