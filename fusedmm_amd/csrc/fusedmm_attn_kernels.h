@@ -399,6 +399,10 @@ template <class G, int BR, class S, class Load, class Use> __device__ __forceinl
    tile_barrier<BR>();
 }
 
+// What a backward pass takes off the scores: lse in units of log2.  A row that weighs nothing (no edges, or all scores minus
+// infinity) has minus infinity there; plus infinity makes all its weights zero, not NaN.
+__device__ inline float row_offset(float lse) { return lse == -INFINITY ? INFINITY : lse * kLog2e; }
+
 #define ATTN_LDS(EXTRA)                                                                                                                        \
    __shared__ __align__(1024) unsigned char lds[G::S * G::kPair + 2 * kAhead * kTile * 4 + 2 * kAhead * G::kMaskBytes + G::S * (EXTRA)];          \
    unsigned char *lds_ids = lds + G::S * G::kPair, *lds_bits = lds_ids + 2 * kAhead * kTile * 4;                                                   \
@@ -626,7 +630,7 @@ template <int T, int DC, int MAPS, int BR> __global__ __launch_bounds__(BR * 4, 
    for (int mp = 0; mp < MAPS; mp++)
    {
       load_resident<T, G::CQ>(qr[mp], (const E *)p.q + srow * p.ldq + head * p.hdq + mp * p.d, live, p.d, g, p.vec);
-      lse2[mp] = p.lse_in[(srow * p.heads + head) * MAPS + mp] * kLog2e;
+      lse2[mp] = row_offset(p.lse_in[(srow * p.heads + head) * MAPS + mp]);
       sign[mp] = mp == 0 ? 1.0f : -p.lambda[head];
    }
    load_resident<T, G::CV>(gr, (const E *)p.dout + srow * p.ldo + head * p.hdo, live, p.dv, g, p.vec);
@@ -820,7 +824,7 @@ template <int T, int DC, int MAPS> __global__ __launch_bounds__(256) void attn_d
       mend[mp] = delta - mean;
       if (lane == 0 && piece == 0)
       {
-         p.stats[(row * p.heads + head) * (2 * MAPS) + mp] = p.lse_in[(row * p.heads + head) * MAPS + mp] * kLog2e;
+         p.stats[(row * p.heads + head) * (2 * MAPS) + mp] = row_offset(p.lse_in[(row * p.heads + head) * MAPS + mp]);
          p.stats[(row * p.heads + head) * (2 * MAPS) + MAPS + mp] = kMend ? mean : delta;
       }
    }

@@ -286,8 +286,9 @@ int fusedMM_amd_last_row_order(int *scattered, unsigned int *edges_lower_half, u
  *    maps = 1   P = softmax_j(scale <q_i, k_j>),               o_i = sum_j P_j v_j
  *    maps = 2   P1, P2 from q1, k1 and q2, k2 (d features each), o_i = sum_j (P1_j - lambda_h P2_j) v_j
  *
- * An edge that a row names twice counts twice; a row without edges gives o = 0 (and lse = -infinity).  Edge ids
- * outside [0, n) are masked places: they are skipped.  There are no edge values.  Sums, maxima and softmax
+ * An edge that a row names twice counts twice; a row without edges gives o = 0 (and lse = -infinity), and so does a
+ * row all of whose scores are -infinity; neither takes part in a gradient.  Edge ids outside [0, n) are masked places: they
+ * are skipped.  There are no edge values.  Sums, maxima and softmax
  * statistics are fp32; fp16/bf16 products run on matrix cores with fp32 accumulation, the softmax weights (and in
  * the backward pass the scores' gradients) rounded to the tensors' type in between.  Results are the same bits
  * from run to run.  Infinities and NaN in rows of k and v reach only the rows that name them.

@@ -1,5 +1,5 @@
 """Infinities and NaN in attention: in blocks that are split and joined, in rows that are laid out anew, in blocks of 16 and of 64
-rows, in records of a 4-bit cache."""
+rows, in records of a 4-bit cache; rows all of whose scores are minus infinity."""
 import numpy as np
 import pytest
 
@@ -84,6 +84,39 @@ def test_only_the_rows_that_name_them(kind, d, dv, maps, pattern, what):
     assert not np.isfinite(b.dvv.numpy()[~other][:, 0, 3]).any()
     keep = np.arange(m) != row
     assert np.array_equal(a.dq.numpy()[keep], b.dq.numpy()[keep])
+
+
+@pytest.mark.parametrize("kind,maps", [("f32", 1), ("f16", 2), ("bf16", 2)])
+@pytest.mark.parametrize("pattern", ["window", "apart", "hub"])
+def test_scores_of_minus_infinity_only(kind, maps, pattern):
+    """A row all of whose scores are minus infinity weighs nothing: zeros and lse = -infinity as for an empty row, and no part in
+    the gradients."""
+    m, n = 90, 700
+    indx, pb, pe = pattern_of(pattern, m, n)
+    a, b = pair(kind, maps, m, n, 2, 1, 32, 32 * maps, (indx, pb, pe))
+    row = int(np.argmax(pe - pb)) if pattern == "hub" else int(np.nonzero(pe - pb > 4)[0][3])
+    cols = np.unique(indx[pb[row]:pe[row]])
+    for c in (a, b):
+        c.k.view()[cols.tolist(), 0, 5] = 1.0            # finite keys that the row's query turns into minus infinity
+        if maps == 2:
+            c.k.view()[cols.tolist(), 0, 32 + 5] = 1.0
+    b.q.view()[row, :, 5] = float("-inf")
+    if maps == 2:
+        b.q.view()[row, :, 32 + 5] = float("-inf")
+    a.do.view()[row] = 0.0                               # (the row gives nothing to dk and dv)
+    train(a, b)
+    assert (b.o.numpy()[row] == 0).all()
+    lse = b.lse[:-1].view(m, 2, maps).cpu().numpy()
+    assert np.isneginf(lse[row]).all() and np.isfinite(lse[[i for i in range(m) if pe[i] > pb[i] and i != row]]).all()
+    assert (b.dq.numpy()[row] == 0).all()
+    keep = np.arange(m) != row
+    for t in ("o", "dq"):
+        assert np.array_equal(getattr(a, t).numpy()[keep], getattr(b, t).numpy()[keep]), t
+    near = lambda x, y: np.abs(x - y).max() <= {"f32": 2.0 ** -22, "f16": 2.0 ** -10, "bf16": 2.0 ** -7}[kind] * np.abs(x).max()
+    rest = np.array([f for f in range(32 * maps) if f % 32 != 5])                 # (0 times an infinite query is NaN)
+    assert near(a.dvv.numpy(), b.dvv.numpy()) and near(a.dk.numpy()[:, :, rest], b.dk.numpy()[:, :, rest])
+    assert b.rows() == 0
+    assert (b.o.numpy()[row] == 0).all()
 
 
 # ---- records of a cache ----------------------------------------------------------------------------------------------------
