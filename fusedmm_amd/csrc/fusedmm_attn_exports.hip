@@ -2,6 +2,7 @@
 // Built once per (INDEXTYPE, VALUETYPE) as the other entry points are; VALUETYPE plays no part, INDEXTYPE is the width of
 // the index arrays.
 #include <algorithm>
+#include <cmath>
 #include <new>
 
 #include "fusedmm_attn.hpp"
@@ -62,6 +63,9 @@ int check_heads(const char *who, const Desc &d)
    if (d.heads < 1 || d.heads % d.kv_heads) return refuse(who, "heads is a positive multiple of kv_heads");
    return kOk;
 }
+
+// (the softmax takes a score factor of NaN or zero for its least positive one)
+int check_scale(const char *who, const Desc &d) { return std::isfinite(d.scale) ? kOk : refuse(who, "scale is not a finite number"); }
 
 bool strides_ok(int64_t ld, int64_t hd)
 {
@@ -274,6 +278,7 @@ int rows_common(const char *who, bool kv4, const Desc *d, int64_t nnz, const voi
    int st = check_sizes(who, d, dc);
    if (st) return st;
    st = check_heads(who, *d);
+   if (!st) st = check_scale(who, *d);
    if (st) return st;
    if (nnz < 0) return refuse(who, "negative nnz");
    if (d->n > INT32_MAX) return refuse(who, "n is at most 2^31 - 1");
@@ -452,6 +457,7 @@ int fusedMM_attn_forward(const fusedMM_attn_desc *desc, const void *plan, const 
    int dc;
    int st = check_sizes(who, desc, &dc);
    if (!st) st = check_heads(who, *desc);
+   if (!st) st = check_scale(who, *desc);
    if (!st) st = check_plans(who, *desc, plan, nullptr, false);
    if (st) return st;
    const Desc &d = *desc;
@@ -492,6 +498,7 @@ int fusedMM_attn_backward(const fusedMM_attn_desc *desc, const void *plan, const
    int dc;
    int st = check_sizes(who, desc, &dc);
    if (!st) st = check_heads(who, *desc);
+   if (!st) st = check_scale(who, *desc);
    if (!st) st = check_plans(who, *desc, plan, plan_t, true);
    if (st) return st;
    const Desc &d = *desc;

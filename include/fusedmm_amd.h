@@ -318,7 +318,7 @@ typedef struct fusedMM_attn_desc {
    int64_t m, n;               /* rows of q and o; rows (cache slots) of k and v */
    int32_t heads, kv_heads;
    int32_t d, dv;              /* features of one map of q and k; of v and o */
-   float scale;
+   float scale;                /* any finite number, negative ones and zero too */
    int64_t ldq, hdq, ldk, hdk, ldv, hdv, ldo, hdo;
 } fusedMM_attn_desc;
 
