@@ -345,10 +345,14 @@ int check_cache(const char *who, const Desc &d, const void *cache, int64_t ldc, 
    return kOk;
 }
 
-int kv4_common(const char *who, const Desc *d, int64_t tokens, const void *slots, const void *k, const void *v, const void *cache, int64_t ldc, int64_t hdc,
+int kv4_common(const char *who, const Desc *desc, int64_t tokens, const void *slots, const void *k, const void *v, const void *cache, int64_t ldc, int64_t hdc,
                bool write, Kv4Params *p)
 {
    int dc;
+   if (!desc) return refuse(who, "no descriptor");
+   Desc own = *desc;
+   own.m = 0;   // not read
+   const Desc *d = &own;
    int st = check_sizes(who, d, &dc);
    if (st) return st;
    st = check_cache(who, *d, cache, ldc, hdc, write);

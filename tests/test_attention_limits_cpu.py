@@ -15,3 +15,13 @@ def test_a_scale_that_is_not_finite(capfd, scale):
                  lambda d: fa.fusedMM_attn_backward(d, None, None, 16, 16, 16, None, 16, None, 16, 16, 16, 16, 16, None, None, 0, stream=0)):
         assert call(desc(scale=scale)) == fa.FAIL
         assert "scale is not a finite number" in capfd.readouterr().err
+
+
+def test_the_cache_does_not_read_rows_and_query_heads():
+    """m, heads and the strides of q and o play no part in writing and reading a cache, whatever they hold."""
+    d = desc(m=-7, heads=-1, ldq=-1, hdq=-1, ldo=-5, hdo=1 << 60, scale=float("nan"))
+    assert fa.fusedMM_kv4_write(d, 0, None, None, None, None, 160, 80, stream=0) == 0
+    assert fa.fusedMM_kv4_read(d, 0, None, None, 160, 80, None, None, stream=0) == 0
+    lib = fa.load(32)
+    assert lib.fusedMM_kv4_write(None, 0, None, None, None, None, 160, 80, None) == fa.FAIL
+    assert lib.fusedMM_kv4_read(None, 0, None, None, 160, 80, None, None, None) == fa.FAIL
