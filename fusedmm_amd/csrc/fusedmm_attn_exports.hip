@@ -72,11 +72,13 @@ bool strides_ok(int64_t ld, int64_t hd)
    return ld >= 0 && hd >= 0 && ld < ((int64_t)1 << 29) && hd < ((int64_t)1 << 48);   // a row's bytes fit 32 bits
 }
 
-// (row, head) pieces of `width` elements that do not overlap: packed rows, or whole heads
+// (row, head) pieces of `width` elements that do not overlap: packed rows, or whole heads.  (In 128 bits: 2^31 heads of a
+// stride of 2^47 are past 64.)
 bool apart(int64_t ld, int64_t hd, int64_t rows, int64_t heads, int64_t width)
 {
-   const bool rows_outer = (heads == 1 || hd >= width) && (rows <= 1 || ld >= (heads - 1) * hd + width);
-   const bool heads_outer = (rows <= 1 || ld >= width) && (heads == 1 || hd >= (rows > 0 ? rows - 1 : 0) * ld + width);
+   typedef __int128 wide;
+   const bool rows_outer = (heads == 1 || hd >= width) && (rows <= 1 || ld >= (wide)(heads - 1) * hd + width);
+   const bool heads_outer = (rows <= 1 || ld >= width) && (heads == 1 || hd >= (wide)(rows > 0 ? rows - 1 : 0) * ld + width);
    return rows_outer || heads_outer;
 }
 

@@ -25,3 +25,10 @@ def test_the_cache_does_not_read_rows_and_query_heads():
     lib = fa.load(32)
     assert lib.fusedMM_kv4_write(None, 0, None, None, None, None, 160, 80, None) == fa.FAIL
     assert lib.fusedMM_kv4_read(None, 0, None, None, 160, 80, None, None, None) == fa.FAIL
+
+
+def test_overlap_is_decided_beyond_64_bits(capfd):
+    """(heads - 1) * hdc of 2^64 bytes is not zero: 2^30 records 2^20 bytes apart under heads 2^44 apart overlap in either order."""
+    d = desc(n=1 << 30, heads=(1 << 20) + 1, kv_heads=(1 << 20) + 1, d=32, dv=32)
+    assert fa.fusedMM_kv4_write(d, 1, 16, 16, 16, 16, 1 << 20, 1 << 44, stream=0) == fa.FAIL
+    assert "records of the cache overlap" in capfd.readouterr().err
