@@ -15,6 +15,7 @@
 
 #include "fusedmm_attn_kernels.h"
 #include "fusedmm_attn_rows_kernels.h"
+#include "fusedmm_attn_sizes.h"
 
 namespace fmm_attn {
 

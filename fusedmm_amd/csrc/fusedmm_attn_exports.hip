@@ -28,7 +28,6 @@ typedef fusedMM_attn_desc Desc;
 static_assert(kOk == FUSEDMM_SUCCESS_RETURN && kFail == FUSEDMM_FAIL_RETURN && kNoMem == FUSEDMM_NOT_ENOUGH_MEM && kNoImpl == FUSEDMM_NO_OPT_IMPL, "");
 static_assert(kF32 == FUSEDMM_TYPE_F32 && kF16 == FUSEDMM_TYPE_F16 && kBF16 == FUSEDMM_TYPE_BF16, "");
 
-constexpr int64_t kMaxGrid = ((int64_t)1 << 31) - 8;
 constexpr int64_t kMaxTokens = (int64_t)1 << 20;
 constexpr int64_t kMaxSlots = (int64_t)1 << 44;   // of a serving call
 
@@ -110,16 +109,18 @@ const Plan *as_plan(const void *p)
    return plan && plan->magic == kPlanMagic ? plan : nullptr;
 }
 
-// plan (and plan_t) against the descriptor
-int check_plans(const char *who, const Desc &d, const void *plan, const void *plan_t, bool need_t)
+PlanSizes sizes_of(const Plan &p) { return {p.view.n_units, p.view.n_joins, p.tiles, p.view.block_rows}; }
+
+// plan (and plan_t, with which a backward pass is asked for) against the descriptor
+int check_plans(const char *who, const Desc &d, int dc, const void *plan, const void *plan_t, bool need_t)
 {
    const Plan *p = as_plan(plan), *t = as_plan(plan_t);
    if (!p || (need_t && !t) || (plan_t && !t)) return refuse(who, "no plan, or one that was destroyed");
    if (p->rows != d.m || p->cols != d.n) return refuse(who, "the plan is of a pattern of another size");
    if (t && (t->rows != d.n || t->cols != d.m)) return refuse(who, "the second plan is not of the transposed pattern's size");
    if (t && t->device != p->device) return refuse(who, "the plans belong to different devices");
-   if ((int64_t)p->view.n_units * d.heads > kMaxGrid || d.n * d.kv_heads > (int64_t)1 << 40 || (int64_t)p->view.n_joins * d.heads * (p->view.block_rows / 4) * 8 > kMaxGrid || d.m * d.heads > kMaxGrid ||
-       (t && ((int64_t)t->view.n_units * d.kv_heads > kMaxGrid || (int64_t)t->view.n_joins * d.kv_heads * (t->view.block_rows / 4) * 8 > kMaxGrid || t->tiles * (d.heads / d.kv_heads) > INT32_MAX)))
+   const int w = dc * d.maps;
+   if (!forward_fits(sizes_of(*p), d.heads, w) || !pack_fits(d.heads) || (t && !backward_fits(sizes_of(*p), sizes_of(*t), d.heads, d.kv_heads, w)))
       return refuse(who, "too many rows and heads for one call");
    return kOk;
 }
@@ -156,7 +157,7 @@ bool packs(const Desc &d, const Tensors &t)
 int64_t pack_bytes(const Desc &d, const Tensors &t, int dc) { return packs(d, t) ? 2 * t.rows * t.heads * dc * d.maps * element_bytes(d) : 0; }
 
 // how the kernels find them; copies them to `to` where they are to be packed
-int gather_from(const char *who, const Desc &d, const Tensors &t, int dc, void *to, hipStream_t s, Gathered *g)
+int gather_from(const Desc &d, const Tensors &t, int dc, void *to, hipStream_t s, Gathered *g)
 {
    const int bytes = element_bytes(d), w = dc * d.maps;
    if (!packs(d, t))
@@ -165,13 +166,10 @@ int gather_from(const char *who, const Desc &d, const Tensors &t, int dc, void *
       *g = Gathered{t.a, t.b, t.ha, t.hb, (int32_t)(t.lda * bytes), (int32_t)(t.ldb * bytes), d.d, d.dv, vec, vec && d.d == dc && d.dv == w};
       return kOk;
    }
-   if (2 * (int64_t)t.heads > kMaxGrid) return refuse(who, "too many heads for one call");
    void *to_b = (unsigned char *)to + t.rows * t.heads * w * bytes;
    *g = Gathered{to, to_b, t.rows * w, t.rows * w, w * bytes, w * bytes, dc, w, 1, 1};
    PackParams p{t.a, t.b, to, to_b, t.rows, t.lda, t.ha, t.ldb, t.hb, t.heads, d.d, d.dv, dc, w * bytes / 16, 0};
-   // enough workgroups to fill the GPU, each of a few chunks per thread where there is more
-   const int64_t want = (t.rows * p.chunks + 255) / 256, most = std::max<int64_t>(1, 16384 / (2 * (int64_t)t.heads));
-   p.per_head = (int32_t)std::min(want, most);
+   p.per_head = (int32_t)pack_per_head(t.rows, t.heads, p.chunks);
    return d.type == FUSEDMM_TYPE_F32 ? launch_pack_f32(p, s) : d.type == FUSEDMM_TYPE_F16 ? launch_pack_f16(p, s) : launch_pack_bf16(p, s);
 }
 
@@ -262,11 +260,11 @@ RowsPlan rows_plan(const Desc &d, int64_t nnz, int dc, bool kv4)
    const int hp = 16 / d.maps, group = d.heads / d.kv_heads;
    r.passes = (group + hp - 1) / hp;
    const int64_t columns = (int64_t)d.kv_heads * r.passes;
-   if (columns > kMaxGrid || d.m > kMaxGrid || nnz > kMaxSlots) return r;
+   if (d.m > INT32_MAX || nnz > kMaxSlots || !rows_fit(d.m, d.m, columns, d.heads)) return r;
    r.piece = piece_slots(nnz, columns, kv4);
    const bool cut = nnz > r.piece && d.m > 0;
    const int64_t most = (cut ? nnz / r.piece : 0) + d.m;
-   r.fits = most + 8 <= kMaxGrid / columns && (d.m == 0 || d.heads <= kMaxGrid / d.m);
+   r.fits = rows_fit(most, d.m, columns, d.heads);
    if (!r.fits || !cut) return r;
    r.cap = most;
    r.table = align256(r.cap * columns * 16 * (dc * d.maps + kPartExtra) * 4);
@@ -450,7 +448,7 @@ int64_t fusedMM_attn_workspace(const fusedMM_attn_desc *desc, const void *plan, 
 {
    const char *who = "fusedMM_attn_workspace";
    int dc;
-   if (check_sizes(who, desc, &dc) || check_heads(who, *desc) || check_plans(who, *desc, plan, plan_t, false)) return -1;
+   if (check_sizes(who, desc, &dc) || check_heads(who, *desc) || check_plans(who, *desc, dc, plan, plan_t, false)) return -1;
    int64_t need = forward_layout(*desc, *as_plan(plan), dc).total;
    if (plan_t) need = std::max(need, backward_layout(*desc, *as_plan(plan), *as_plan(plan_t), dc).total);
    return need;
@@ -464,7 +462,7 @@ int fusedMM_attn_forward(const fusedMM_attn_desc *desc, const void *plan, const 
    int st = check_sizes(who, desc, &dc);
    if (!st) st = check_heads(who, *desc);
    if (!st) st = check_scale(who, *desc);
-   if (!st) st = check_plans(who, *desc, plan, nullptr, false);
+   if (!st) st = check_plans(who, *desc, dc, plan, nullptr, false);
    if (st) return st;
    const Desc &d = *desc;
    if (!inputs_ok(d)) return refuse(who, "a stride is negative or too large");
@@ -490,7 +488,7 @@ int fusedMM_attn_forward(const fusedMM_attn_desc *desc, const void *plan, const 
    p.lse = lse;
    p.part = (float *)work;
    const hipStream_t s = (hipStream_t)stream;
-   st = gather_from(who, d, keys_values(d, k, v), dc, (unsigned char *)work + l.pack, s, &p.gat);
+   st = gather_from(d, keys_values(d, k, v), dc, (unsigned char *)work + l.pack, s, &p.gat);
    if (st) return st;
    return d.type == FUSEDMM_TYPE_F32 ? launch_forward_f32(p, dc, d.maps, s)
           : d.type == FUSEDMM_TYPE_F16 ? launch_forward_f16(p, dc, d.maps, s) : launch_forward_bf16(p, dc, d.maps, s);
@@ -505,7 +503,7 @@ int fusedMM_attn_backward(const fusedMM_attn_desc *desc, const void *plan, const
    int st = check_sizes(who, desc, &dc);
    if (!st) st = check_heads(who, *desc);
    if (!st) st = check_scale(who, *desc);
-   if (!st) st = check_plans(who, *desc, plan, plan_t, true);
+   if (!st) st = check_plans(who, *desc, dc, plan, plan_t, true);
    if (st) return st;
    const Desc &d = *desc;
    if (!inputs_ok(d)) return refuse(who, "a stride is negative or too large");
@@ -546,14 +544,14 @@ int fusedMM_attn_backward(const fusedMM_attn_desc *desc, const void *plan, const
    void *pack = (unsigned char *)work + l.pack;
    if (d.m > 0)
    {
-      st = gather_from(who, d, keys_values(d, k, v), dc, pack, s, &p.gat);
+      st = gather_from(d, keys_values(d, k, v), dc, pack, s, &p.gat);
       if (st) return st;
       st = d.type == FUSEDMM_TYPE_F32 ? launch_dq_f32(p, dc, d.maps, s) : d.type == FUSEDMM_TYPE_F16 ? launch_dq_f16(p, dc, d.maps, s) : launch_dq_bf16(p, dc, d.maps, s);
       if (st) return st;
    }
    if (d.n == 0 && !p.dlambda) return kOk;
    p.plan = pt.view;
-   st = gather_from(who, d, queries_gradients(d, q, dout), dc, pack, s, &p.gat);
+   st = gather_from(d, queries_gradients(d, q, dout), dc, pack, s, &p.gat);
    if (st) return st;
    return d.type == FUSEDMM_TYPE_F32 ? launch_dkv_f32(p, dc, d.maps, s) : d.type == FUSEDMM_TYPE_F16 ? launch_dkv_f16(p, dc, d.maps, s) : launch_dkv_bf16(p, dc, d.maps, s);
 }

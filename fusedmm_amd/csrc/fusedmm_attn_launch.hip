@@ -21,7 +21,8 @@ namespace fmm_attn {
 
 namespace {
 
-[[maybe_unused]] unsigned eighths(int64_t n) { return (unsigned)((n + 7) / 8 * 8); }
+[[maybe_unused]] unsigned unit_groups(const Params &p, int heads) { return (unsigned)eighths((Wide)p.plan.n_units * heads); }
+[[maybe_unused]] dim3 join_grid(const Params &p, int heads, int width) { return dim3((unsigned)join_groups({p.plan.n_units, p.plan.n_joins, 0, p.plan.block_rows}, heads, width)); }
 
 // F<DC, MAPS>()(args) for the instance of (dc, maps)
 template <template <int, int> class F, class... A> int choose(int dc, int maps, A... a)
@@ -48,13 +49,13 @@ template <template <int, int> class F, class... A> int choose(int dc, int maps, 
 template <int DC, int MAPS> struct Forward {
    int operator()(const Params &p, hipStream_t s)
    {
-      const int64_t n = (int64_t)p.plan.n_units * p.heads;
-      if (p.plan.block_rows == 64) hipLaunchKernelGGL((attn_forward<TYPE, DC, MAPS, 64>), dim3(eighths(n)), dim3(256), 0, s, p);
-      else hipLaunchKernelGGL((attn_forward<TYPE, DC, MAPS, 16>), dim3(eighths(n)), dim3(64), 0, s, p);
+      const dim3 grid(unit_groups(p, p.heads));
+      if (p.plan.block_rows == 64) hipLaunchKernelGGL((attn_forward<TYPE, DC, MAPS, 64>), grid, dim3(256), 0, s, p);
+      else hipLaunchKernelGGL((attn_forward<TYPE, DC, MAPS, 16>), grid, dim3(64), 0, s, p);
       ATTN_HIP(hipGetLastError());
       if (p.plan.n_joins)
       {
-         hipLaunchKernelGGL((attn_forward_join<TYPE, DC, MAPS>), dim3((unsigned)((int64_t)p.plan.n_joins * p.heads * p.plan.block_rows / 4 * ((DC * MAPS + 63) / 64))), dim3(256), 0, s, p);
+         hipLaunchKernelGGL((attn_forward_join<TYPE, DC, MAPS>), join_grid(p, p.heads, DC * MAPS), dim3(256), 0, s, p);
          ATTN_HIP(hipGetLastError());
       }
       return kOk;
@@ -64,13 +65,13 @@ template <int DC, int MAPS> struct Forward {
 template <int DC, int MAPS> struct Dq {
    int operator()(const Params &p, hipStream_t s)
    {
-      const int64_t n = (int64_t)p.plan.n_units * p.heads;
-      if (p.plan.block_rows == 64) hipLaunchKernelGGL((attn_dq<TYPE, DC, MAPS, 64>), dim3(eighths(n)), dim3(256), 0, s, p);
-      else hipLaunchKernelGGL((attn_dq<TYPE, DC, MAPS, 16>), dim3(eighths(n)), dim3(64), 0, s, p);
+      const dim3 grid(unit_groups(p, p.heads));
+      if (p.plan.block_rows == 64) hipLaunchKernelGGL((attn_dq<TYPE, DC, MAPS, 64>), grid, dim3(256), 0, s, p);
+      else hipLaunchKernelGGL((attn_dq<TYPE, DC, MAPS, 16>), grid, dim3(64), 0, s, p);
       ATTN_HIP(hipGetLastError());
       if (p.plan.n_joins)
       {
-         hipLaunchKernelGGL((attn_dq_join<TYPE, DC, MAPS>), dim3((unsigned)((int64_t)p.plan.n_joins * p.heads * p.plan.block_rows / 4 * ((DC * MAPS + 63) / 64))), dim3(256), 0, s, p);
+         hipLaunchKernelGGL((attn_dq_join<TYPE, DC, MAPS>), join_grid(p, p.heads, DC * MAPS), dim3(256), 0, s, p);
          ATTN_HIP(hipGetLastError());
       }
       return kOk;
@@ -80,14 +81,13 @@ template <int DC, int MAPS> struct Dq {
 template <int DC, int MAPS> struct Dkv {
    int operator()(const Params &p, hipStream_t s)
    {
-      const int64_t n = (int64_t)p.plan.n_units * p.kv_heads;
-      const dim3 grid(eighths(n) + (p.dlambda ? (unsigned)p.heads : 0u));
+      const dim3 grid(unit_groups(p, p.kv_heads) + (p.dlambda ? (unsigned)p.heads : 0u));
       if (p.plan.block_rows == 64) hipLaunchKernelGGL((attn_dkv<TYPE, DC, MAPS, 64>), grid, dim3(256), 0, s, p);
       else hipLaunchKernelGGL((attn_dkv<TYPE, DC, MAPS, 16>), grid, dim3(64), 0, s, p);
       ATTN_HIP(hipGetLastError());
       if (p.plan.n_joins)
       {
-         hipLaunchKernelGGL((attn_dkv_join<TYPE, DC, MAPS>), dim3((unsigned)((int64_t)p.plan.n_joins * p.kv_heads * p.plan.block_rows / 4 * ((2 * DC * MAPS + 63) / 64))), dim3(256), 0, s, p);
+         hipLaunchKernelGGL((attn_dkv_join<TYPE, DC, MAPS>), join_grid(p, p.kv_heads, 2 * DC * MAPS), dim3(256), 0, s, p);
          ATTN_HIP(hipGetLastError());
       }
       return kOk;
@@ -107,14 +107,14 @@ int make_table(const RowsParams &p, hipStream_t s)
 template <int O, int DC, int MAPS> int join(const RowsParams &p, hipStream_t s)
 {
    if (!p.cap) return kOk;
-   const int waves = p.cap > 8 * 4 * (256 / (DC * MAPS)) * p.m ? 16 : 4;   // 4, where they take a row in one batch
+   const int waves = join_waves(p.cap, p.m, p.heads, DC * MAPS);
    const size_t lds = (size_t)waves * MAPS * (DC * MAPS + 2) * sizeof(float);
    hipLaunchKernelGGL((attn_rows_join<FMM_ATTN_UNIT, O, DC, MAPS>), dim3((unsigned)(p.m * p.heads)), dim3(64 * waves), lds, s, p);
    ATTN_HIP(hipGetLastError());
    return kOk;
 }
 
-unsigned rows_grid(const RowsParams &p) { return eighths(p.cap ? p.cap : p.m) * (unsigned)(p.kv_heads * p.passes); }
+unsigned rows_grid(const RowsParams &p) { return (unsigned)rows_groups(p.cap ? p.cap : p.m, p.kv_heads * p.passes); }
 #endif
 
 #if KERNEL == 3

@@ -212,6 +212,17 @@ struct Memory {   // freed when the building ends, however it does
    int get(size_t bytes) { return hip_code(hipMalloc(&p, bytes ? bytes : 16), "hipMalloc (attention plan)"); }
 };
 
+// launch(first, count) for n items, kPlanSlice at a time
+template <class F> int in_slices(int64_t n, F launch)
+{
+   for (int64_t first = 0; first < n; first += kPlanSlice)
+   {
+      launch(first, std::min(kPlanSlice, n - first));
+      ATTN_HIP(hipGetLastError());
+   }
+   return kOk;
+}
+
 template <class X> int upload(Memory &to, const std::vector<X> &v)
 {
    const int st = to.get(v.size() * sizeof(X));
@@ -273,9 +284,10 @@ int build(Plan *plan, int br, bool *shared, int64_t m, int64_t n, int64_t nnz, c
    {
       int st = upload(d_chunks, chunks);
       if (st) return st;
-      hipLaunchKernelGGL(plan_chunk_edges, dim3((unsigned)((chunks.size() + 3) / 4)), dim3(256), 0, stream, (Chunk *)d_chunks.p,
-                         (int64_t)chunks.size(), m, br, pb, pe, ib);
-      ATTN_HIP(hipGetLastError());
+      st = in_slices((int64_t)chunks.size(), [&](int64_t first, int64_t count) {
+         hipLaunchKernelGGL(plan_chunk_edges, dim3((unsigned)((count + 3) / 4)), dim3(256), 0, stream, (Chunk *)d_chunks.p + first, count, m, br, pb, pe, ib);
+      });
+      if (st) return st;
       ATTN_HIP(hipMemcpyAsync(chunks.data(), d_chunks.p, chunks.size() * sizeof(Chunk), hipMemcpyDeviceToHost, stream));
       ATTN_HIP(hipStreamSynchronize(stream));
       for (Chunk &c : chunks)
@@ -289,14 +301,17 @@ int build(Plan *plan, int br, bool *shared, int64_t m, int64_t n, int64_t nnz, c
       if (!st) st = d_masks.get((size_t)at * 8);
       if (!st) st = d_counts.get(chunks.size() * sizeof(int2));
       if (st) return st;
-      const dim3 grid((unsigned)chunks.size());
-      if (small)
-         hipLaunchKernelGGL((plan_fill<4096, 256>), grid, dim3(256), 0, stream, (const Chunk *)d_chunks.p, (int64_t)chunks.size(), m, br, n, indx, pb, pe, ib,
-                            (int32_t *)d_cols.p, (uint64_t *)d_masks.p, (int2 *)d_counts.p);
-      if (large)
-         hipLaunchKernelGGL((plan_fill<kMostRows * kChunkSlots, 1024>), grid, dim3(1024), 0, stream, (const Chunk *)d_chunks.p,
-                            (int64_t)chunks.size(), m, br, n, indx, pb, pe, ib, (int32_t *)d_cols.p, (uint64_t *)d_masks.p, (int2 *)d_counts.p);
-      ATTN_HIP(hipGetLastError());
+      st = in_slices((int64_t)chunks.size(), [&](int64_t first, int64_t count) {
+         const Chunk *of = (const Chunk *)d_chunks.p + first;
+         int2 *to = (int2 *)d_counts.p + first;
+         if (small)
+            hipLaunchKernelGGL((plan_fill<4096, 256>), dim3((unsigned)count), dim3(256), 0, stream, of, count, m, br, n, indx, pb, pe, ib, (int32_t *)d_cols.p,
+                               (uint64_t *)d_masks.p, to);
+         if (large)
+            hipLaunchKernelGGL((plan_fill<kMostRows * kChunkSlots, 1024>), dim3((unsigned)count), dim3(1024), 0, stream, of, count, m, br, n, indx, pb, pe, ib,
+                               (int32_t *)d_cols.p, (uint64_t *)d_masks.p, to);
+      });
+      if (st) return st;
       ATTN_HIP(hipMemcpyAsync(counts.data(), d_counts.p, chunks.size() * sizeof(int2), hipMemcpyDeviceToHost, stream));
       ATTN_HIP(hipStreamSynchronize(stream));
       if (br == 64)
@@ -369,8 +384,11 @@ int build(Plan *plan, int br, bool *shared, int64_t m, int64_t n, int64_t nnz, c
       Memory by_column;
       st = by_column.get((size_t)to * 8);
       if (st) return st;
-      hipLaunchKernelGGL(plan_pack, dim3((unsigned)pieces.size()), dim3(256), 0, stream, (const Piece *)d_pieces.p, (const int32_t *)d_cols.p,
-                         (const uint64_t *)d_masks.p, (int32_t *)base, (uint64_t *)by_column.p);
+      st = in_slices((int64_t)pieces.size(), [&](int64_t first, int64_t count) {
+         hipLaunchKernelGGL(plan_pack, dim3((unsigned)count), dim3(256), 0, stream, (const Piece *)d_pieces.p + first, (const int32_t *)d_cols.p,
+                            (const uint64_t *)d_masks.p, (int32_t *)base, (uint64_t *)by_column.p);
+      });
+      if (st) return st;
       hipLaunchKernelGGL(plan_masks, dim3((unsigned)std::min<int64_t>((to / kTile * br + 255) / 256, 1 << 16)), dim3(256), 0, stream,
                          (const uint64_t *)by_column.p, to / kTile, br, (uint32_t *)(base + off_masks));
       ATTN_HIP(hipGetLastError());

@@ -298,7 +298,8 @@ int fusedMM_amd_last_row_order(int *scattered, unsigned int *edges_lower_half, u
  * calls may run side by side on different streams and in different threads, and may be captured into graphs,
  * as long as calls that can overlap have workspaces and outputs of their own.  Rows behind the last
  * one and columns between the heads are left as they are.  Return values are fusedMM status codes:
- * FUSEDMM_FAIL_RETURN for arguments that do not fit together (with a line on stderr), FUSEDMM_NOT_ENOUGH_MEM for
+ * FUSEDMM_FAIL_RETURN for arguments that do not fit together (with a line on stderr; also for sizes whose launches would hold
+ * 2^32 threads or more: over a plan, about 2^30 rows x heads, in the serving form 2^24), FUSEDMM_NOT_ENOUGH_MEM for
  * a workspace that is too small, FUSEDMM_NO_OPT_IMPL for sizes without a kernel: d <= 256 and dv <= 256 with one
  * map, d <= 128 and dv <= 256 with two.
  */
