@@ -104,16 +104,20 @@ template <int BR> __device__ inline void tile_barrier()
 }
 
 // 16 (4) bytes per lane, memory -> LDS at base + 16 (4) * lane.  The address registers are read when the load issues, it
-// writes no register, and the waits are wait_loads(): the compiler's own waits for its own loads count these as later
-// or earlier ones and only get stricter.
+// writes no register but m0, which is named so that the compiler keeps nothing in it across (it warns that it would not save
+// a reserved register; none is wanted back).  The waits are wait_loads(): the compiler's own waits for its own loads
+// count these as later or earlier ones and only get stricter.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 __device__ inline void load_lds16(uint32_t base, const void *from)
 {
-   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(__builtin_amdgcn_readfirstlane(base)), "v"(from) : "memory");
+   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(__builtin_amdgcn_readfirstlane(base)), "v"(from) : "memory", "m0");
 }
 __device__ inline void load_lds4(uint32_t base, const void *from)
 {
-   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(__builtin_amdgcn_readfirstlane(base)), "v"(from) : "memory");
+   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(__builtin_amdgcn_readfirstlane(base)), "v"(from) : "memory", "m0");
 }
+#pragma clang diagnostic pop
 __device__ inline uint32_t lds_address(const void *p)
 {
    return __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void *)p);

@@ -100,3 +100,17 @@ def test_rows_beyond_a_launch_are_refused_beforehand(capfd, bits):
         assert "too many rows" in capfd.readouterr().err
         assert rows(d, index_bits=bits) == fa.FAIL and "too many rows" in capfd.readouterr().err
     assert fa.fusedMM_attn_rows_workspace(desc(m=(1 << 20) - 8, heads=16, kv_heads=16, ldo=1024), 100, index_bits=bits) == 0
+
+
+def test_inline_assembly_names_m0_where_it_writes_it():
+    import os
+    import re
+    csrc = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "fusedmm_amd", "csrc")
+    seen = 0
+    for name in sorted(os.listdir(csrc)):
+        if name.startswith("fusedmm_attn"):
+            for asm in re.findall(r"asm volatile\((.*?)\);", open(os.path.join(csrc, name)).read(), re.S):
+                if "s_mov_b32 m0" in asm:
+                    seen += 1
+                    assert asm.rstrip().endswith('"m0"'), (name, asm)
+    assert seen == 2
