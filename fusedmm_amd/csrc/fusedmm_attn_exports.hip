@@ -386,8 +386,6 @@ int kv4_common(const char *who, const Desc *desc, int64_t tokens, const void *sl
    p->vec = lines_up(k, d->ldk, d->hdk, bytes) && lines_up(v, d->ldv, d->hdv, bytes);
    p->ldc = ldc;
    p->hdc = hdc;
-   // Tokens of a workgroup: it walks over all later slots, so tokens share that walk as soon as there are enough of them.
-   p->per_group = (int)std::min<int64_t>(kKv4Tokens, std::max<int64_t>(1, tokens / 2048));
    return kOk;
 }
 

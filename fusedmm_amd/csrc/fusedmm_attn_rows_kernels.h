@@ -45,7 +45,7 @@ struct Kv4Params {
    int32_t vec;
    uint8_t *cache;
    int64_t ldc, hdc;
-   int32_t per_group;                    // tokens of a workgroup
+   int32_t per_group;                    // tokens of a workgroup (writing)
 };
 
 typedef float f2 __attribute__((ext_vector_type(2)));
