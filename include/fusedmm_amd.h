@@ -374,6 +374,8 @@ int fusedMM_attn_rows(const fusedMM_attn_desc *desc, const INDEXTYPE nnz, const 
  * exact in fp16.  With lo = min(0, values), hi = max(0, values), s is (hi - lo) / 15 rounded up to 7 significant bits
  * and to a multiple of 2^-20, z = rint(-lo / s), code = clamp(rint(x / s) + z, 0, 15), ties to even.  Magnitudes above
  * 32768 saturate; a NaN makes its group of 32 NaN.  d and dv are multiples of 32.
+ * Records of any such d and dv (up to 256; d to 128 with two maps) are written and read back, but fusedMM_attn_rows_kv4 attends only over
+ * those it lists below: not with d or dv over 128 (two maps: d over 64 or dv over 128), d = dv = 256 (128 and 256) apart.
  */
 int64_t fusedMM_kv4_record_bytes(const int maps, const int d, const int dv);
 
