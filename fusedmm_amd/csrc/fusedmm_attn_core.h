@@ -311,7 +311,8 @@ __device__ inline void add_odd(f4 (&acc)[NT], const float (&p)[2][4], unsigned m
 
 // acc += (weights of the tile's 32 rows) x (their features f0 .. f0 + 16 NT - 1); CAREFUL: the tile may hold infinities or
 // NaN; TWICE: 16-bit weights enter as a rounded value and its rounded rest.  One rounding of the weights errs by as much
-// as the rounding of the output does; with the rest, outputs are as exact as their own rounding.
+// as the rounding of the output does; with the rest, outputs are as exact as their own rounding.  (Once is enough for the
+// sum in dq that only multiplies what a rounded delta is off by.)
 template <int T, int W, bool CAREFUL, bool TWICE = false, int NT>
 __device__ inline void add_weighted(f4 (&acc)[NT], const float (&p)[2][4], unsigned mine, const unsigned char *tile, int f0, int g, int i, const typename TileView<T, W>::Lane &l)
 {

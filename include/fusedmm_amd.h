@@ -288,16 +288,17 @@ int fusedMM_amd_last_row_order(int *scattered, unsigned int *edges_lower_half, u
  *
  * An edge that a row names twice counts twice; a row without edges gives o = 0 (and lse = -infinity), and so does a
  * row all of whose scores are -infinity; neither takes part in a gradient.  Edge ids outside [0, n) are masked places: they
- * are skipped.  There are no edge values.  Sums, maxima and softmax
- * statistics are fp32; fp16/bf16 products run on matrix cores with fp32 accumulation, the softmax weights (and in
- * the backward pass the scores' gradients) rounded to the tensors' type in between.  Results are the same bits
- * from run to run.  Infinities and NaN in rows of k and v reach only the rows that name them.
+ * are skipped.  There are no edge values.  Sums, maxima and softmax statistics are fp32.  fp16/bf16 products run on matrix
+ * cores with fp32 accumulation; the softmax weights, and in the backward pass the scores' gradients, enter them as a value
+ * rounded to the tensors' type and the rounded rest of it, in fp16 scaled into its range (weights below 2^-32 of a row's
+ * largest vanish), so that results are as exact as their own rounding.  Results are the same bits from run to run.
+ * Infinities and NaN in rows of k and v reach only the rows that name them.
  *
  * All pointers are device memory of the current device, all work is enqueued on `stream` (a hipStream_t), nothing
  * is allocated, no state is kept and nothing waits for the GPU (fusedMM_attn_plan_create and _destroy apart): the
  * calls may run side by side on different streams and in different threads, and may be captured into graphs,
- * as long as calls that can overlap have workspaces and outputs of their own.  Rows behind the last
- * one and columns between the heads are left as they are.  Return values are fusedMM status codes:
+ * as long as calls that can overlap have workspaces and outputs of their own.  Outputs and workspace share no memory with
+ * operands.  Rows behind the last one and columns between the heads are left as they are.  Return values are fusedMM status codes:
  * FUSEDMM_FAIL_RETURN for arguments that do not fit together (with a line on stderr; also for sizes whose launches would hold
  * 2^32 threads or more: over a plan, about 2^30 rows x heads, in the serving form 2^24), FUSEDMM_NOT_ENOUGH_MEM for
  * a workspace that is too small, FUSEDMM_NO_OPT_IMPL for sizes without a kernel: d <= 256 and dv <= 256 with one
@@ -328,7 +329,9 @@ typedef struct fusedMM_attn_desc {
  * rows share few columns) the columns that any of them names, so that a gathered row is loaded once for all of them.
  * m, n <= 2^26 - 1; nnz at least the sum of the row lengths.  Column ids in ascending order within the rows share best; any order is right.
  * The plan belongs to the current device, holds device memory (12 bytes, or 6, per distinct (block, column)) and can be used
- * for any head count, type and feature width.  Waits for the GPU; refused while `stream` is captured.
+ * for any head count, type and feature width.  Waits for the GPU; refused while `stream` is captured.  It allocates and copies:
+ * no other stream should be under a capture that forbids that to all threads, then or when a plan is destroyed.
+ * Making one takes 0.4 to 3 ms, as long as several calls of small patterns: keep it for all layers and steps of a pattern.
  * Destroying waits for the device's work and frees the memory; graphs that were captured with the plan end with it.
  */
 int fusedMM_attn_plan_create(const INDEXTYPE m, const INDEXTYPE n, const INDEXTYPE nnz, const INDEXTYPE *indx,
@@ -381,7 +384,7 @@ int64_t fusedMM_kv4_record_bytes(const int maps, const int d, const int dv);
 
 /* Token t of k and v (ldk, hdk, ldv, hdv and the sizes from desc; m, heads and the other strides are not read) goes to
  * slot slots[t]; tokens whose slot is outside [0, desc->n) are skipped.  Of tokens with the same slot the last one
- * counts.  At most 2^20 tokens, desc->n <= 2^31 - 1.  Bytes of a record behind the last word are left as they are. */
+ * counts.  At most 2^20 tokens (8192 to a launch), desc->n <= 2^31 - 1.  Bytes of a record behind the last word are left as they are. */
 int fusedMM_kv4_write(const fusedMM_attn_desc *desc, const INDEXTYPE tokens, const INDEXTYPE *slots, const void *k, const void *v,
                       void *cache, int64_t ldc, int64_t hdc, void *stream);
 /* The values of the records of slots[0 .. tokens) in desc->type; slots outside [0, desc->n) read as zeros. */
@@ -389,7 +392,7 @@ int fusedMM_kv4_read(const fusedMM_attn_desc *desc, const INDEXTYPE tokens, cons
                      int64_t hdc, void *k, void *v, void *stream);
 /* fusedMM_attn_rows over such a cache; desc->type (of q and o) is fp16 or bf16.  d and dv are any multiples of 32 up
  * to 128 (d to 64 with two maps), or d = dv = 256 (d = 128, dv = 256 with two maps).  Products run on fp16 operands: the
- * cache's values are exact in it, each head's query is scaled by a power of two into its range. */
+ * cache's values are exact in it, each head's query is scaled by a power of two into its range, weights enter as above. */
 int fusedMM_attn_rows_kv4(const fusedMM_attn_desc *desc, const INDEXTYPE nnz, const INDEXTYPE *indx, const INDEXTYPE *pntrb,
                           const INDEXTYPE *pntre, const void *q, const void *cache, int64_t ldc, int64_t hdc, const float *lambda,
                           void *o, void *work, int64_t work_bytes, void *stream);
