@@ -68,7 +68,7 @@ inline int width_class(int d, int dv, int maps)
 
 // floats of partial sums that one split unit of one head leaves
 inline int64_t forward_part(int dc, int maps, int br) { return (int64_t)maps * br * (dc * maps + 2); }
-inline int64_t dq_part(int dc, int maps, int br) { return (int64_t)br * (2 * dc * maps + 4); }
+inline int64_t dq_part(int dc, int maps, int br) { return (int64_t)br * (2 * dc * maps + 6); }
 inline int64_t dkv_part(int dc, int maps, int br) { return (int64_t)br * (2 * dc * maps); }
 
 // one function per (type, kernel) object; dc and maps choose the instance

@@ -406,6 +406,10 @@ template <class G, int BR, class S, class Load, class Use> __device__ __forceinl
 // What a backward pass takes off the scores: lse in units of log2.  A row that weighs nothing (no edges, or all scores minus
 // infinity) has minus infinity there; plus infinity makes all its weights zero, not NaN.
 __device__ inline float row_offset(float lse) { return lse == -INFINITY ? INFINITY : lse * kLog2e; }
+// lse is off by up to |lse| 2^-24 and is turned between logarithms twice: all weights of a row are then off alike, by some 1e-7.
+// Their sum tells by how much.  dq and the means are divided by it; the offset that dkv takes off is moved by its logarithm.
+__device__ inline float row_share(float total) { return total == 0.0f ? 0.0f : 1.0f / total; }
+__device__ inline float row_offset(float lse2, float total) { return total > 0.0f ? lse2 + log2f(total) : lse2; }
 
 #define ATTN_LDS(EXTRA)                                                                                                                        \
    __shared__ __align__(1024) unsigned char lds[G::S * G::kPair + 2 * kAhead * kTile * 4 + 2 * kAhead * G::kMaskBytes + G::S * (EXTRA)];          \
@@ -605,12 +609,12 @@ template <int T, int DC, int MAPS> __global__ __launch_bounds__(256) void attn_f
 // It comes from o as it was rounded to 16 bits, which a row of few edges feels: with mean = sum_j P dP, formed here in
 // fp32, dq = sum_j P (dP - delta) k + (delta - mean) sum_j P k.  The second sum is small where it counts, so its own rounding
 // does not matter; the exact mean replaces delta for dk.  fp32 needs none of it: there delta is off by what o's own
-// rounding is, and P by |lse| 2^-24 through lse's, 2.6e-7 of the gradients in all where sums of exact terms are 1.6e-7 off.
+// rounding is.
 //
 // The 16-bit weights and scores' gradients enter dq, dk and dv as a rounded value and its rounded rest, as the forward pass's
 // do: rounded once they left bf16 gradients 0.0024 off in two norms, where their own rounding is 0.0017.  A window of 256
 // and 16 first columns, 16384 rows, 8 heads, two maps of 64 x 128: 316 us a training pass instead of 286; in fp16, with
-// Range, 351 instead of 293.
+// Range, 351 instead of 293.  The weights' sum takes another 1 %.
 template <int T, int DC, int MAPS, int BR> __global__ __launch_bounds__(BR * 4, (DC * MAPS >= 256 || T == kF32 ? 1 : 2)) void attn_dq(Params p)
 {
    typedef Geo<T, DC, MAPS, BR> G;
@@ -630,7 +634,7 @@ template <int T, int DC, int MAPS, int BR> __global__ __launch_bounds__(BR * 4, 
    st.set(lds, lds_ids, lds_bits, p, u, kvh);
 
    u4 qr[MAPS][G::CQ], gr[G::CV];
-   float lse2[MAPS], delta[MAPS], sign[MAPS], mean[MAPS];
+   float lse2[MAPS], delta[MAPS], sign[MAPS], mean[MAPS], total[MAPS];
 #pragma unroll
    for (int mp = 0; mp < MAPS; mp++)
    {
@@ -659,7 +663,7 @@ template <int T, int DC, int MAPS, int BR> __global__ __launch_bounds__(BR * 4, 
 #pragma unroll
       for (int mp = 0; mp < MAPS; mp++)
       {
-         mean[mp] = 0;
+         mean[mp] = total[mp] = 0;
          range[mp] = Range<T>();
 #pragma unroll
          for (int t = 0; t < G::NTQ; t++)
@@ -704,6 +708,7 @@ template <int T, int DC, int MAPS, int BR> __global__ __launch_bounds__(BR * 4, 
                {
                   w[j / 4][j % 4] = pr[j / 4][j % 4] * (dp[j / 4][j % 4] - delta[mp]);   // sign: at the end
                   mean[mp] = fmaf(pr[j / 4][j % 4], dp[j / 4][j % 4], mean[mp]);
+                  total[mp] += pr[j / 4][j % 4];
                   if constexpr (G::N::kPScale != 1.0f) pr[j / 4][j % 4] *= G::N::kPScale;
                }
                range[mp].fit(w, acc[mp]);
@@ -748,6 +753,8 @@ template <int T, int DC, int MAPS, int BR> __global__ __launch_bounds__(BR * 4, 
    for (int mp = 0; mp < MAPS; mp++)
    {
       mean[mp] = group_sum(mean[mp]);
+      total[mp] = group_sum(total[mp]);
+      if (u.part < 0) mean[mp] *= row_share(total[mp]);
       range[mp].undo(acc[mp]);
       if constexpr (G::N::kPScale != 1.0f)
       {
@@ -757,7 +764,7 @@ template <int T, int DC, int MAPS, int BR> __global__ __launch_bounds__(BR * 4, 
    }
    if constexpr (MAPS == 2)
    {
-      // (a row behind the last one names nothing: its mean is zero; the units of a split block add up)
+      // (a row behind the last one names nothing: its mean is zero; the units of a split block add up, without the share)
       float x = mean[1];
 #pragma unroll
       for (int k = 8; k; k >>= 1) x += __shfl_xor(x, k);
@@ -765,8 +772,8 @@ template <int T, int DC, int MAPS, int BR> __global__ __launch_bounds__(BR * 4, 
    }
    if (u.part >= 0)
    {
-      // [part][head][BR rows][W + W + 4]: the two sums, the means, the deltas
-      float *r = p.part + (((int64_t)u.part * p.heads + head) * BR + 16 * wave + i) * (2 * G::W + 4);
+      // [part][head][BR rows][W + W + 6]: the two sums, the means, the deltas, the weights
+      float *r = p.part + (((int64_t)u.part * p.heads + head) * BR + 16 * wave + i) * (2 * G::W + 6);
 #pragma unroll
       for (int mp = 0; mp < MAPS; mp++)
       {
@@ -782,6 +789,7 @@ template <int T, int DC, int MAPS, int BR> __global__ __launch_bounds__(BR * 4, 
          {
             r[2 * G::W + mp] = mean[mp];
             r[2 * G::W + 2 + mp] = delta[mp];
+            r[2 * G::W + 4 + mp] = total[mp];
          }
       }
       return;
@@ -792,7 +800,7 @@ template <int T, int DC, int MAPS, int BR> __global__ __launch_bounds__(BR * 4, 
 #pragma unroll
       for (int mp = 0; mp < MAPS; mp++)
       {
-         p.stats[(row * p.heads + head) * (2 * MAPS) + mp] = lse2[mp];
+         p.stats[(row * p.heads + head) * (2 * MAPS) + mp] = row_offset(lse2[mp], total[mp]);
          p.stats[(row * p.heads + head) * (2 * MAPS) + MAPS + mp] = kMend ? mean[mp] : delta[mp];
       }
    }
@@ -804,7 +812,7 @@ template <int T, int DC, int MAPS, int BR> __global__ __launch_bounds__(BR * 4, 
       {
          f4 r = acc[mp][x];
          if constexpr (kMend) r += (delta[mp] - mean[mp]) * pk[mp][x];
-         store4<T>(out + mp * p.d, 16 * x + 4 * g, p.d, r * (sign[mp] * p.scale), p.vec);
+         store4<T>(out + mp * p.d, 16 * x + 4 * g, p.d, r * (sign[mp] * p.scale * row_share(total[mp])), p.vec);
       }
 }
 
@@ -816,20 +824,26 @@ template <int T, int DC, int MAPS> __global__ __launch_bounds__(256) void attn_d
    JOIN_WHERE(p.heads, (W + 63) / 64)
    const int64_t row = (int64_t)j.block * br + r;
    if (row >= p.m) return;
-   const int64_t step = (int64_t)p.heads * br * (2 * W + 4);
-   const float *from = p.part + (((int64_t)j.part0 * p.heads + head) * br + r) * (2 * W + 4);
-   float mend[MAPS];
+   const int64_t step = (int64_t)p.heads * br * (2 * W + 6);
+   const float *from = p.part + (((int64_t)j.part0 * p.heads + head) * br + r) * (2 * W + 6);
+   float mend[MAPS], share[MAPS];
 #pragma unroll
    for (int mp = 0; mp < MAPS; mp++)
    {
-      float mean = 0;
+      float mean = 0, total = 0;
 #pragma unroll 8
-      for (int u = 0; u < j.parts; u++) mean += from[u * step + 2 * W + mp];
+      for (int u = 0; u < j.parts; u++)
+      {
+         mean += from[u * step + 2 * W + mp];
+         total += from[u * step + 2 * W + 4 + mp];
+      }
+      share[mp] = row_share(total);
+      mean *= share[mp];
       const float delta = from[2 * W + 2 + mp];
       mend[mp] = delta - mean;
       if (lane == 0 && piece == 0)
       {
-         p.stats[(row * p.heads + head) * (2 * MAPS) + mp] = row_offset(p.lse_in[(row * p.heads + head) * MAPS + mp]);
+         p.stats[(row * p.heads + head) * (2 * MAPS) + mp] = row_offset(row_offset(p.lse_in[(row * p.heads + head) * MAPS + mp]), total);
          p.stats[(row * p.heads + head) * (2 * MAPS) + MAPS + mp] = kMend ? mean : delta;
       }
    }
@@ -844,7 +858,7 @@ template <int T, int DC, int MAPS> __global__ __launch_bounds__(256) void attn_d
    }
    const int mp = f / DC, e = f - mp * DC;
    if (kMend) s += (mp == 0 ? mend[0] : mend[MAPS - 1]) * s2;
-   if (e < p.d) ((E *)p.dq)[row * p.ldq + head * p.hdq + mp * p.d + e] = (E)Num<T>::from(s * ((mp == 0 ? 1.0f : -p.lambda[head]) * p.scale));
+   if (e < p.d) ((E *)p.dq)[row * p.ldq + head * p.hdq + mp * p.d + e] = (E)Num<T>::from(s * ((mp == 0 ? share[0] : -p.lambda[head] * share[MAPS - 1]) * p.scale));
 }
 
 // dlambda_h = - sum of dlam_units, in 64 bits: every thread's entries and then the threads in order.  The last `heads`

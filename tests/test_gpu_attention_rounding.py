@@ -187,3 +187,30 @@ def test_weights_and_gradients_are_rounded_twice(kind, pattern, d, dv, maps):
     assert c.rows() == 0
     torch.cuda.synchronize()
     check_rows(c, e)
+
+
+# ---- the weights' sum ------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("window", [37, 100, 300])
+def test_weights_of_the_backward_pass_add_up_to_one(kind, window):
+    """One value and one output gradient for all: every row's mean is 1, whatever its scores, and dlambda the number of rows.  The
+    weights come from lse, which scores of 30 to 60 leave off by up to 2^-19; their sum takes that off again."""
+    import torch
+    m, n = 128, 500
+    c = Case(kind, 2, m, n, 2, 1, 16, 16, *window_pattern(m, n, window), seed=3)
+    for t in (c.q, c.v, c.do):
+        t.view().zero_()
+    c.q.view()[..., 0] = 1.0
+    c.q.view()[..., 16] = 1.0
+    c.v.view()[..., 0] = 1.0
+    c.do.view()[..., 0] = 1.0
+    c.k.view()[..., 0] += 120.0
+    c.k.view()[..., 16] += 200.0
+    c.make_plans(True)
+    c.gradients()
+    assert c.forward() == 0 and c.backward() == 0
+    torch.cuda.synchronize()
+    # mean and sum are the same additions: their quotient is off by a reciprocal and a product (2 * 2^-24), a wave's sum by four
+    # additions and dlambda by its own rounding
+    assert np.abs(c.dlam.double().cpu().numpy() + m).max() <= m * 7 * 2.0 ** -24
